@@ -353,6 +353,97 @@ int vx_qkv_pack(const void* qkv, int64_t ld_qkv, const void* p0, int64_t ld_p0, 
                 const void* pos_v, float scale, int64_t T, int heads, int head_dim, void* q2, void* k2,
                 void* v2, void* stream);
 
+/* Paged cache of keys and values of an autoregressive decoder over encoder frames: what attention rescoring and token-by-token
+ * decoding of n-best hypotheses read.  (No counterpart in the reference, which rescores whole hypotheses,
+ * veloxvoice/models/wenet/attention_decoder.py:192-240.)
+ *   k, v   bf16; element (page, token in the page, head, c) at page * k_page + token * k_token + head * k_head + c: any order of the
+ *          dimensions, strides in elements (multiples of 8), addresses 16-byte aligned, head_dim contiguous. */
+typedef struct {
+  int32_t struct_size; /* sizeof(vx_kv_cache) */
+  int32_t page_size;   /* tokens per page, any number >= 1 */
+  int64_t pages;
+  int32_t kv_heads, head_dim;
+  void* k;
+  void* v;
+  int64_t k_page, k_token, k_head;
+  int64_t v_page, v_token, v_head;
+} vx_kv_cache;
+
+/* The rows of a call and the sequences that they continue.
+ *   lengths      i32 [sequences]: own tokens of a sequence that the cache holds BEFORE the rows of this call (the same numbers for
+ *                vx_kv_append and the vx_prefix_attention behind it); negative: the sequence takes no part
+ *   row_offsets  i32 [sequences + 1], ascending: rows [o_s, o_{s+1}) are the next tokens of sequence s; NULL: one row each.  Rows
+ *                outside [o_0, o_sequences) belong to no sequence
+ *   page_table   i32 [sequences][table_pages], row stride ld_table: entry j is the page of the sequence's own tokens
+ *                [j page_size, (j + 1) page_size).  An entry outside [0, pages) is a page that is not there.
+ * All of it is device memory that is checked where it is read: no value of an entry makes a kernel leave the cache. */
+typedef struct {
+  int32_t struct_size; /* sizeof(vx_kv_rows) */
+  int32_t reserved;    /* 0 */
+  int64_t rows, sequences;
+  const int32_t* lengths;
+  const int32_t* row_offsets;
+  const int32_t* page_table;
+  int64_t ld_table, table_pages;
+} vx_kv_rows;
+
+/* Keys and values of new tokens into their pages, rotated by position on the way, and the queries rotated with them: one launch.
+ * Row r, the i-th new token of sequence s, is own token t = lengths[s] + i at position starts[s] + t:
+ *   k page(s, t) = bf16(rotate(k[r])),  v page(s, t) = bf16(v[r]),  q_out[r] = bf16(rotate(q[r]))
+ * The first rot_dim of the head_dim values are rotated by the angle whose cosine and sine are in row `position` of
+ * rotary f32 [positions][rot_dim] = cos of rot_dim / 2 angles | sin: pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) when
+ * `interleaved`.  Products and sums in fp32, rounded once.
+ * A row of no sequence, of one that takes no part, or at a position outside [0, positions) is left out: nothing is stored, its
+ * q_out is zero.  A row whose page is not there or beyond the table is not stored.  Two rows must not go to one place. */
+typedef struct {
+  int32_t struct_size; /* sizeof(vx_kv_append_desc) */
+  int32_t dtype;       /* of q, k, v: VX_F32 or VX_BF16 */
+  const void* k;       /* [rows, kv_heads, head_dim]: strides in elements, 16-byte aligned rows and heads */
+  const void* v;
+  const void* q;       /* [rows, q_heads, head_dim] or NULL */
+  int64_t k_row, k_head, v_row, v_head, q_row, q_head;
+  void* q_out;         /* bf16 [rows, q_heads, head_dim], must be given with q; may be q where q is bf16 */
+  int64_t qo_row, qo_head;
+  const float* rotary; /* NULL: no rotation */
+  int64_t positions, ld_rotary;
+  const int32_t* starts; /* i32 [sequences]: position of a sequence's first own token; NULL: 0 */
+  int32_t q_heads, rot_dim; /* rot_dim: a multiple of 16, at most head_dim */
+  int32_t interleaved, reserved; /* reserved: 0 */
+} vx_kv_append_desc;
+/* head_dim: a multiple of 16, at most 256 */
+int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_kv_append_desc* desc, void* stream);
+
+/* Attention of new tokens over a prefix that the sequences of a group share and over their own tokens:
+ *   out[r, h] = sum_j softmax_j(scale q[r, h] . k_j) v_j,  key head h / (q_heads / kv_heads),
+ * j over the keys [0, prefix_lengths[g]) of the pages prefix_table[g] and over own tokens t <= lengths[s] + i of the sequence
+ * (row r is its i-th new token, which vx_kv_append has stored), both without the pages that are not there.  The prefix is read once for all
+ * rows of its group.  A row without any key, of no sequence or of one that takes no part: zeros.
+ *   groups         sequences [group_offsets[g], group_offsets[g + 1]) belong to group g (i32 [groups + 1], ascending); NULL: groups of
+ *                  sequences / groups each.  0 groups: no prefix
+ *   out            bf16 [rows, q_heads, head_dim]
+ *   scratch        vx_prefix_attention_scratch(cache, rows, desc) bytes, 16-byte aligned
+ * bf16 operands, fp32 scores, softmax statistics and sums; probabilities are rounded to bf16 for the second product.  What lies in unread places
+ * of the cache (NaN included) does not reach a result.  head_dim 64 or 128. */
+typedef struct {
+  int32_t struct_size; /* sizeof(vx_prefix_attention_desc) */
+  int32_t q_heads;
+  const void* q;       /* bf16 [rows, q_heads, head_dim], strides in elements, 16-byte aligned rows and heads */
+  int64_t q_row, q_head;
+  void* out;
+  int64_t o_row, o_head;
+  int64_t groups;
+  const int32_t* group_offsets;
+  const int32_t* prefix_table; /* i32 [groups][prefix_pages], row stride ld_prefix */
+  int64_t ld_prefix, prefix_pages;
+  const int32_t* prefix_lengths; /* i32 [groups] */
+  float scale;
+  int32_t reserved; /* 0 */
+  void* scratch;
+  int64_t scratch_bytes;
+} vx_prefix_attention_desc;
+int64_t vx_prefix_attention_scratch(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
+int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc, void* stream);
+
 /* Block-scaled FP4 GEMM for callers that cannot allocate device memory.  (No counterpart in
  * the reference: its Python wrappers allocate through torch.)
  *

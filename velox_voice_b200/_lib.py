@@ -74,6 +74,9 @@ EXPORTS = (
     "vx_conformer_pass_frames",
     "vx_conformer_pass_scratch",
     "vx_conformer_pass",
+    "vx_kv_append",
+    "vx_prefix_attention",
+    "vx_prefix_attention_scratch",
 )
 
 
@@ -120,6 +123,96 @@ class GemmDesc(C.Structure):
         ("topk_count", C.c_void_p),
         ("topk_capacity", C.c_int32),
         ("quant_col0", C.c_int32),
+    ]
+
+
+class KvCache(C.Structure):
+    """``vx_kv_cache``."""
+
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("page_size", C.c_int32),
+        ("pages", C.c_int64),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_page", C.c_int64),
+        ("k_token", C.c_int64),
+        ("k_head", C.c_int64),
+        ("v_page", C.c_int64),
+        ("v_token", C.c_int64),
+        ("v_head", C.c_int64),
+    ]
+
+
+class KvRows(C.Structure):
+    """``vx_kv_rows``."""
+
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("reserved", C.c_int32),
+        ("rows", C.c_int64),
+        ("sequences", C.c_int64),
+        ("lengths", C.c_void_p),
+        ("row_offsets", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("ld_table", C.c_int64),
+        ("table_pages", C.c_int64),
+    ]
+
+
+class KvAppendDesc(C.Structure):
+    """``vx_kv_append_desc``."""
+
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("dtype", C.c_int32),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q", C.c_void_p),
+        ("k_row", C.c_int64),
+        ("k_head", C.c_int64),
+        ("v_row", C.c_int64),
+        ("v_head", C.c_int64),
+        ("q_row", C.c_int64),
+        ("q_head", C.c_int64),
+        ("q_out", C.c_void_p),
+        ("qo_row", C.c_int64),
+        ("qo_head", C.c_int64),
+        ("rotary", C.c_void_p),
+        ("positions", C.c_int64),
+        ("ld_rotary", C.c_int64),
+        ("starts", C.c_void_p),
+        ("q_heads", C.c_int32),
+        ("rot_dim", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class PrefixAttentionDesc(C.Structure):
+    """``vx_prefix_attention_desc``."""
+
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("q_heads", C.c_int32),
+        ("q", C.c_void_p),
+        ("q_row", C.c_int64),
+        ("q_head", C.c_int64),
+        ("out", C.c_void_p),
+        ("o_row", C.c_int64),
+        ("o_head", C.c_int64),
+        ("groups", C.c_int64),
+        ("group_offsets", C.c_void_p),
+        ("prefix_table", C.c_void_p),
+        ("ld_prefix", C.c_int64),
+        ("prefix_pages", C.c_int64),
+        ("prefix_lengths", C.c_void_p),
+        ("scale", C.c_float),
+        ("reserved", C.c_int32),
+        ("scratch", C.c_void_p),
+        ("scratch_bytes", C.c_int64),
     ]
 
 
@@ -216,6 +309,12 @@ def load(build_if_missing: bool = True) -> C.CDLL:
         lib.vx_conformer_pass_scratch.argtypes = [i64, i64]
         lib.vx_conformer_pass.restype = i32
         lib.vx_conformer_pass.argtypes = [vp, vp]
+        lib.vx_kv_append.restype = i32
+        lib.vx_kv_append.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(KvAppendDesc), vp]
+        lib.vx_prefix_attention_scratch.restype = i64
+        lib.vx_prefix_attention_scratch.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc)]
+        lib.vx_prefix_attention.restype = i32
+        lib.vx_prefix_attention.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc), vp]
         lib.vx_ctc_topk_threshold.restype = i32
         lib.vx_ctc_topk_threshold.argtypes = [vp, i64, i64, i32, vp, vp]
         lib.vx_ctc_topk_finish.restype = i32

@@ -3,7 +3,8 @@
 Two layers:
 
 * the library's own operators -- :func:`quantize`, :func:`ln_quantize`, :func:`layernorm`,
-  :func:`bsgemm` -- which carry every format and fused epilogue;
+  :func:`bsgemm` -- which carry every format and fused epilogue, and the paged cache of a decoder behind the
+  encoder -- :func:`kv_append`, :func:`prefix_attention`;
 * the reference's operator names with the reference's signatures
   (``veloxvoice/kernels/ops/triton_ops.py`` and ``veloxvoice/kernels/ops/cuda_ops.py``):
   :func:`per_row_col_quantize`, :func:`triton_quantize_w`, :func:`mxfp4_block_quantize`,
@@ -722,6 +723,205 @@ def mma_peak_tflops(kind: str = "fp4", n_tile: int = 256, iters: int = 4096) -> 
     rc = _lib.load().vx_mma_peak_probe(0 if kind == "fp4" else 1, n_tile, iters, C.byref(out))
     _lib.check(rc, "vx_mma_peak_probe")
     return float(out.value)
+
+
+# ======================================================================================
+# Paged cache of keys and values, and the attention that reads it.
+# ======================================================================================
+
+
+def rotary_table(positions: int, rot_dim: int, base: float = 10000.0, *, device="cuda") -> torch.Tensor:
+    """Cosines and sines for :func:`kv_append`: f32 [positions, rot_dim], row p = cos(p w_i) | sin(p w_i) with
+    w_i = base^(-2 i / rot_dim), i < rot_dim / 2; angles and functions in fp64, rounded once."""
+    if rot_dim < 16 or rot_dim % 16 != 0:
+        raise ValueError(f"rot_dim must be a positive multiple of 16, got {rot_dim}")
+    w = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    a = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * w
+    return torch.cat([a.cos(), a.sin()], dim=1).float()
+
+
+def _int32_on(t, name: str, shape, dev) -> torch.Tensor:
+    """int32 tensor of the given shape (None: any size) on the cache's device, rows contiguous."""
+    _require_cuda(t, name)
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("n" if n is None else str(n) for n in shape)
+        raise ValueError(f"{name} must be int32 [{want}], got {t.dtype} {tuple(t.shape)}")
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _step(t: torch.Tensor, dim: int) -> int:
+    """Stride of a dimension that is walked; that of a single entry says nothing."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _in_pieces(t: torch.Tensor) -> bool:
+    """Rows and heads at 16-byte addresses, values of a head in a row."""
+    e = t.element_size()
+    return (t.data_ptr() % 16 == 0 and (t.shape[-1] <= 1 or t.stride(-1) == 1)
+            and all(_step(t, i) * e % 16 == 0 for i in range(t.dim() - 1)))
+
+
+def _kv_cache(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        _require_cuda(t, n)
+        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape != k_pages.shape or t.device != k_pages.device:
+            raise ValueError("k_pages and v_pages must be bfloat16 [pages, page_size, kv_heads, head_dim] tensors of one shape on one device")
+        if not _in_pieces(t):
+            raise ValueError(f"{n} must have contiguous heads at 16-byte aligned addresses (strides {t.stride()})")
+    pages, size, heads, dim = k_pages.shape
+    if size < 1 or heads < 1:
+        raise ValueError(f"pages hold at least one token of one head, got {tuple(k_pages.shape)}")
+    return _lib.KvCache(C.sizeof(_lib.KvCache), size, pages, heads, dim, k_pages.data_ptr(), v_pages.data_ptr(),
+                        *(_step(k_pages, i) for i in range(3)), *(_step(v_pages, i) for i in range(3)))
+
+
+def _kv_rows(rows: int, page_table, lengths, row_offsets, dev):
+    """The descriptor and the tensors that it points to."""
+    page_table = _int32_on(page_table, "page_table", (None, None), dev)
+    n = page_table.shape[0]
+    lengths = _int32_on(lengths, "lengths", (n,), dev)
+    if row_offsets is not None:
+        row_offsets = _int32_on(row_offsets, "row_offsets", (n + 1,), dev)
+    elif rows != n:
+        raise ValueError(f"without row_offsets every sequence has one row, got {rows} rows of {n} sequences")
+    width = page_table.shape[1]
+    d = _lib.KvRows(C.sizeof(_lib.KvRows), 0, rows, n, lengths.data_ptr(), _ptr(row_offsets), page_table.data_ptr(),
+                    page_table.stride(0) if n > 1 else width, width)
+    return d, (page_table, lengths, row_offsets)
+
+
+def _heads3d(t, name: str, rows, heads, k_pages, dtypes) -> torch.Tensor:
+    """[rows, heads, head_dim] operand on the cache's device; copied where its rows are not at 16-byte addresses."""
+    _require_cuda(t, name)
+    if t.device != k_pages.device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {k_pages.device}")
+    if t.dim() != 3 or t.shape[2] != k_pages.shape[3] or (rows is not None and t.shape[0] != rows) or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {k_pages.shape[3]}], got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    return t if _in_pieces(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+              lengths: torch.Tensor, *, q: Optional[torch.Tensor] = None, rotary: Optional[torch.Tensor] = None,
+              interleaved: bool = False, row_offsets: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+              q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Keys and values of new tokens into their pages, rotated by position on the way, and the queries rotated with them
+    (``vx_kv_append``, one launch).  Returns the rotated queries bf16 [rows, heads, head_dim] (None without ``q``).
+
+    k, v [rows, kv_heads, head_dim], q [rows, heads, head_dim], all f32 or all bf16, any row and head strides (views of a fused
+    projection's output); k_pages, v_pages bf16 [pages, page_size, kv_heads, head_dim], written in place.  Row r, the i-th new token
+    of sequence s, is own token ``t = lengths[s] + i``: it goes to ``page_table[s, t // page_size]``, place ``t % page_size``, rotated
+    for position ``starts[s] + t``.  ``row_offsets`` int32 [sequences + 1]: rows [o_s, o_{s+1}) belong to sequence s; without it each
+    sequence has one row.  ``rotary`` f32 [positions, rot_dim] (:func:`rotary_table`): the first rot_dim values of a head are rotated in
+    pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) when ``interleaved``; None: no rotation.
+
+    Left out, with zero queries: rows of no sequence, of one of negative length, at a position that the table does not have.  Not
+    stored: tokens whose page is not there (an entry outside [0, pages), or none).  ``lengths`` stays as it is: the same call of
+    :func:`prefix_attention` takes it, and the program then moves it on."""
+    cache = _kv_cache(k_pages, v_pages)
+    dev, kv = k_pages.device, k_pages.shape[2]
+    kinds = (torch.float32, torch.bfloat16)
+    k = _heads3d(k, "k", None, kv, k_pages, kinds)
+    rows = k.shape[0]
+    v = _heads3d(v, "v", rows, kv, k_pages, (k.dtype,))
+    d = _lib.KvAppendDesc(struct_size=C.sizeof(_lib.KvAppendDesc), dtype=_dt(k, "k"))
+    d.k, d.k_row, d.k_head = k.data_ptr(), _step(k, 0), _step(k, 1)
+    d.v, d.v_row, d.v_head = v.data_ptr(), _step(v, 0), _step(v, 1)
+    if q is not None:
+        given = q
+        q = _heads3d(q, "q", rows, None, k_pages, (k.dtype,))
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+        else:
+            _require_cuda(q_out, "q_out")
+            if q_out.dtype != torch.bfloat16 or q_out.shape != q.shape or q_out.device != dev or not _in_pieces(q_out):
+                raise ValueError("q_out must be bfloat16 of q's shape with contiguous heads at 16-byte aligned addresses")
+            if q_out is given:
+                q = q_out
+        d.q, d.q_row, d.q_head, d.q_heads = q.data_ptr(), _step(q, 0), _step(q, 1), q.shape[1]
+        d.q_out, d.qo_row, d.qo_head = q_out.data_ptr(), _step(q_out, 0), _step(q_out, 1)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if rotary is not None:
+        _require_cuda(rotary, "rotary")
+        if rotary.dtype != torch.float32 or rotary.dim() != 2 or rotary.device != dev:
+            raise ValueError("rotary must be float32 [positions, rot_dim] on the cache's device")
+        if rotary.shape[1] % 16 != 0 or not 16 <= rotary.shape[1] <= k.shape[2]:
+            raise ValueError(f"rot_dim must be a multiple of 16 up to head_dim {k.shape[2]}, got {rotary.shape[1]}")
+        if not _in_pieces(rotary):
+            rotary = rotary.clone(memory_format=torch.contiguous_format)
+        d.rotary, d.positions, d.rot_dim = rotary.data_ptr(), rotary.shape[0], rotary.shape[1]
+        d.ld_rotary = rotary.stride(0) if rotary.shape[0] > 1 else rotary.shape[1]
+        d.interleaved = int(interleaved)
+    r, keep = _kv_rows(rows, page_table, lengths, row_offsets, dev)
+    if starts is not None:
+        starts = _int32_on(starts, "starts", (r.sequences,), dev)
+        d.starts = starts.data_ptr()
+    _lib.check(_lib.load().vx_kv_append(C.byref(cache), C.byref(r), C.byref(d), _stream()), "vx_kv_append")
+    _count()
+    del keep
+    return q_out
+
+
+def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                     prefix_table: Optional[torch.Tensor] = None, prefix_lengths: Optional[torch.Tensor] = None, *,
+                     row_offsets: Optional[torch.Tensor] = None, group_offsets: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of new tokens over a prefix that the sequences of a group share, read once for all of them, and over their own
+    tokens (``vx_prefix_attention``).  q bf16 [rows, heads, head_dim] -> bf16 [rows, heads, head_dim]; heads a multiple of kv_heads,
+    head_dim 64 or 128.
+
+    Row r, the i-th new token of sequence s (``row_offsets``, ``lengths``, ``page_table`` as for :func:`kv_append`, called before
+    with the same ``lengths``), attends to own tokens t <= lengths[s] + i and to the prefix of its group: keys
+    [0, prefix_lengths[g]) of the pages ``prefix_table[g]`` (int32 [groups, pages]).  ``group_offsets`` int32 [groups + 1]: sequences
+    [o_g, o_{g+1}) are group g; without it the groups are of one size.  Without ``prefix_table`` there is no prefix.  Keys on pages
+    that are not there (entries outside [0, pages)) are not attended; a row that has no key, or whose sequence has a negative
+    length, gets zeros.  ``scale``: head_dim ** -0.5 unless given."""
+    cache = _kv_cache(k_pages, v_pages)
+    dev, kv, dim = k_pages.device, k_pages.shape[2], k_pages.shape[3]
+    q = _heads3d(q, "q", None, None, k_pages, (torch.bfloat16,))
+    if dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {dim}")
+    rows, heads = q.shape[0], q.shape[1]
+    if heads < 1 or heads % kv != 0:
+        raise ValueError(f"q has {heads} heads, not a multiple of the cache's {kv}")
+    r, keep = _kv_rows(rows, page_table, lengths, row_offsets, dev)
+    d = _lib.PrefixAttentionDesc(struct_size=C.sizeof(_lib.PrefixAttentionDesc), q_heads=heads)
+    d.q, d.q_row, d.q_head = q.data_ptr(), _step(q, 0), _step(q, 1)
+    if (prefix_table is None) != (prefix_lengths is None):
+        raise ValueError("prefix_table and prefix_lengths go together")
+    if prefix_table is not None:
+        prefix_table = _int32_on(prefix_table, "prefix_table", (None, None), dev)
+        groups, width = prefix_table.shape
+        prefix_lengths = _int32_on(prefix_lengths, "prefix_lengths", (groups,), dev)
+        if group_offsets is not None:
+            group_offsets = _int32_on(group_offsets, "group_offsets", (groups + 1,), dev)
+        elif groups == 0 or r.sequences % groups != 0:
+            raise ValueError(f"without group_offsets the groups are of one size, got {r.sequences} sequences and {groups} groups")
+        d.groups, d.group_offsets = groups, _ptr(group_offsets)
+        d.prefix_table, d.ld_prefix, d.prefix_pages = prefix_table.data_ptr(), prefix_table.stride(0) if groups > 1 else width, width
+        d.prefix_lengths = prefix_lengths.data_ptr()
+    d.scale = dim ** -0.5 if scale is None else float(scale)
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=torch.bfloat16, device=dev)
+    else:
+        _require_cuda(out, "out")
+        if out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != dev or not _in_pieces(out):
+            raise ValueError("out must be bfloat16 of q's shape with contiguous heads at 16-byte aligned addresses")
+    d.out, d.o_row, d.o_head = out.data_ptr(), _step(out, 0), _step(out, 1)
+    lib = _lib.load()
+    size = int(lib.vx_prefix_attention_scratch(C.byref(cache), C.byref(r), C.byref(d)))
+    if size < 0:
+        _lib.check(size, "vx_prefix_attention")
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    d.scratch, d.scratch_bytes = _ptr(scratch), size
+    _lib.check(lib.vx_prefix_attention(C.byref(cache), C.byref(r), C.byref(d), _stream()), "vx_prefix_attention")
+    _count()
+    del keep, prefix_table, prefix_lengths, group_offsets
+    return out
 
 
 # ======================================================================================
