@@ -3,114 +3,378 @@
 //   out[r, h] = sum_j softmax_j(scale q[r, h] . k_j) v_j
 //   keys: tokens [0, prefix_lengths[g]) of the group's pages, own tokens t <= lengths[s] + i of the sequence
 //
-// One warp per row and head.  32 keys a step: a lane takes the score of one key, the maximum and the sum of the softmax run along
-// (m, l), and every lane sums its share of the 32 weighted values.
-// What bounds it: L1 and L2; every row and head reads its keys and values for itself.
+// How the work is cut: vx_prefix.cuh.  This file has the kernel for few rows per owner and key head, the kernel that joins the parts, and
+// the entry points.
+//
+// prefix_rows_kernel: up to 16 rows against one chunk of keys per CTA of four warps, which take 16 (head_dim 128) or 32 (64) keys in turn.
+// Every key and value is read once, by one lane, straight into the registers that the tensor cores take it from; shared memory holds only
+// what the four warps join at the end.  Keys and values are the m16 side of m16n8k16 products, so that eight rows fill one and
+// nothing is computed for rows that do not exist.  With lane = 4 g + c:
+//   S^T = K Q^T: the order of the terms of a sum over head_dim is free.  A lane reads 16 bytes = 8 values of keys g and g + 8 at 8 (c + 4 i);
+//     the registers are the A fragments of two products whose 16 "k" are the values 8 (c + 4 i) + {0, 1, 2, 3} (then {4, ..., 7}) of the
+//     four c; Q is read in the same order.
+//   O^T += V^T P^T: the accumulators hold P^T by keys; transposed in 8 x 8 blocks (movmatrix) they are the B fragment.  A lane reads 8 values
+//     of each of the keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 at 64 b + 8 g and pairs two keys' values with byte permutes; product j of block b has
+//     columns 64 b + 8 g + 2 j (rows g of its A) and 64 b + 8 g + 2 j + 1 (rows g + 8).
+// The reference maximum of a row moves only when a score exceeds it by more than 8 (probabilities stay below 2^8), so most steps
+// need a vote and no shuffles; sums are kept per lane until the end.  K of the next step is requested when S is formed, V when O is.
+// What bounds it: HBM, each chunk read once; a step's products cost a tenth of the time that its bytes take.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "vx_common.cuh"
-#include "vx_paged.cuh"
-#include "vx_ptx.cuh"
+#include "vx_prefix.cuh"
 
 namespace vx {
 namespace {
 
-constexpr int PA_WARPS = 4;
+constexpr int PR_WARPS = 4;
 
-struct PrefixParams {
-  PagedCache cache;
-  KvRows rows;
-  const __nv_bfloat16* q;
-  int64_t q_row, q_head;
-  __nv_bfloat16* out;
-  int64_t o_row, o_head;
-  int32_t q_heads, per_kv;
-  int32_t groups, group_size;
-  const int32_t* group_offsets;
-  PagedTable prefix;
-  const int32_t* prefix_lengths;
-  float scale;
+struct RowsParams {
+  PrefixParams p;
+  Span span[2];
+  int32_t first_items;  // items of span[0]; those of span[1] follow
 };
 
-// group of a sequence, -1: none
-__device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
-  if (p.groups == 0) return -1;
-  if (!p.group_offsets) return s / p.group_size;
-  const int g = find_owner(p.group_offsets, p.groups, s);
-  return s >= p.group_offsets[g] && s < p.group_offsets[g + 1] ? g : -1;
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// 16 bytes that no one else of the SM will read
+__device__ __forceinline__ uint4 load_once(const __nv_bfloat16* p) {
+  uint4 u;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
 }
 
-template <int D>
-__global__ void __launch_bounds__(PA_WARPS * 32) prefix_attention_kernel(const PrefixParams p) {
+// 8 x 8 block of 16-bit values, lane 4 g + c holding (g, 2 c) and (g, 2 c + 1): the same of its transpose
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// RB blocks of eight rows.
+template <int D, int RB>
+__global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_kernel(const __grid_constant__ RowsParams rp) {
   pdl_launch_dependents();
-  __shared__ float q_s[PA_WARPS][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * PA_WARPS + warp;
+  constexpr int NT = D == 64 ? 2 : 1;      // blocks of 16 keys per step
+  constexpr int KC = D / 32;               // 16-byte pieces of a key per lane
+  constexpr int VB = D / 64;               // and of a value
+  constexpr int TM = 8 * RB;
+  __shared__ float o_s[PR_WARPS][TM][D + 4];
+  __shared__ float2 ml_s[PR_WARPS][TM];
+  const PrefixParams& p = rp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   pdl_wait();
-  if (item >= static_cast<int64_t>(p.rows.rows) * p.q_heads) return;
-  const int row = static_cast<int>(item / p.q_heads), head = static_cast<int>(item % p.q_heads), kv = head / p.per_kv;
-  constexpr int VL = D / 32;
-  for (int c = 0; c < VL; ++c) {
-    const int i = c * 32 + lane;
-    q_s[warp][i] = __bfloat162float(p.q[row * p.q_row + head * p.q_head + i]) * p.scale;
+  int n = static_cast<int>(blockIdx.x);
+  const bool second = n >= rp.first_items;
+  if (second) n -= rp.first_items;
+  const Span& sp = rp.span[second];
+  const int head = n % p.kv_heads;  // heads of a token lie next to each other
+  n /= p.kv_heads;
+  const int chunk = n / sp.slots;
+  Item it;
+  if (!find_item<TM>(p, sp, n - chunk * sp.slots, chunk, it)) return;
+  const PagedTable& table = sp.own ? p.rows.table : p.prefix;
+  const __nv_bfloat16* const kb = p.cache.k.p + head * p.cache.k.head;
+  const __nv_bfloat16* const vb = p.cache.v.p + head * p.cache.v.head;
+
+  // queries: row 8 r + g, the pieces of this lane
+  uint32_t q[RB][KC][4];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const int rho = it.rho0 + 8 * r + g;
+    uint32_t tok, hq;
+    p.per_kv.divmod(static_cast<uint32_t>(rho), tok, hq);
+    const __nv_bfloat16* src = p.q + static_cast<int64_t>(it.row0 + static_cast<int>(tok)) * p.q_row + (head * static_cast<int64_t>(p.per_kv.d) + hq) * p.q_head;
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (rho < it.rows) u = *reinterpret_cast<const uint4*>(src + 8 * (c + 4 * i));
+      q[r][i][0] = u.x; q[r][i][1] = u.y; q[r][i][2] = u.z; q[r][i][3] = u.w;
+    }
   }
-  __syncwarp();
-  float m = -INFINITY, l = 0.0f, o[VL] = {};
-  auto run = [&](const PagedTable& table, int owner, int64_t n) {
-    n = min(n, static_cast<int64_t>(table.pages) * p.cache.page_size.d);
-    for (int64_t j0 = 0; j0 < n; j0 += 32) {
-      const int64_t j = j0 + lane;
+  // keys that row 8 r + 2 c + e sees; the first row of the tile sees fewest
+  int limit[RB][2], min_limit = it.keys;
+#pragma unroll
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      limit[r][e] = sp.own ? own_keys(p, it.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0 + 8 * r + 2 * c + e)))) : it.keys;
+  if (sp.own) min_limit = own_keys(p, it.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0))));
+
+  constexpr int STEP = 16 * NT * PR_WARPS;
+  int j0 = it.key0 + warp * 16 * NT;
+  // lane l holds where key j0 + l (l < 16 NT) is, in elements of the two tensors; -1: not there
+  int64_t k_off, v_off;
+  auto locate = [&](int j) {
+    k_off = v_off = -1;
+    if (lane < 16 * NT && j + lane < it.keys) {
       uint32_t index, slot;
-      p.cache.page_size.divmod(static_cast<uint32_t>(j), index, slot);
-      const int page = j < n ? page_of(table, owner, index, p.cache.pages) : -1;
-      float s = -INFINITY;
+      p.cache.page_size.divmod(static_cast<uint32_t>(j + lane), index, slot);
+      const int page = page_of(table, it.owner, index, p.cache.pages);
       if (page >= 0) {
-        const uint4* k = reinterpret_cast<const uint4*>(p.cache.k.p + page * p.cache.k.page + slot * p.cache.k.token + kv * p.cache.k.head);
-        s = 0.0f;
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 u = k[c];
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s += __uint_as_float(w[e] << 16) * q_s[warp][c * 8 + 2 * e] + __uint_as_float(w[e] & 0xffff0000u) * q_s[warp][c * 8 + 2 * e + 1];
-        }
-      }
-      float mx = s;
-      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float m_new = fmaxf(m, mx);
-      const float ref = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = expf(m - ref), w = page >= 0 ? expf(s - ref) : 0.0f;
-      float sum = w;
-      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      l = l * alpha + sum;
-      m = m_new;
-#pragma unroll
-      for (int c = 0; c < VL; ++c) o[c] *= alpha;
-      for (int x = 0; x < 32; ++x) {
-        const int pg = __shfl_sync(0xffffffffu, page, x);
-        const uint32_t sl = __shfl_sync(0xffffffffu, slot, x);
-        const float wx = __shfl_sync(0xffffffffu, w, x);
-        if (pg < 0) continue;
-        const __nv_bfloat16* v = p.cache.v.p + pg * p.cache.v.page + sl * p.cache.v.token + kv * p.cache.v.head;
-#pragma unroll
-        for (int c = 0; c < VL; ++c) o[c] += wx * __bfloat162float(v[c * 32 + lane]);
+        k_off = page * p.cache.k.page + slot * p.cache.k.token;
+        v_off = page * p.cache.v.page + slot * p.cache.v.token;
       }
     }
   };
-  int s, i;
-  if (row_sequence(p.rows, row, s, i)) {
-    const int g = group_of(p, s);
-    if (g >= 0) run(p.prefix, g, p.prefix_lengths[g]);
-    run(p.rows.table, s, static_cast<int64_t>(p.rows.lengths[s]) + i + 1);
+  uint32_t kr[NT][2][KC][4], vr[NT][4][VB][4];
+  uint32_t there = 0;  // bit 2 t + b: key 16 t + 8 b + g
+  auto load_k = [&]() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int64_t off = __shfl_sync(0xffffffffu, k_off, t * 16 + b * 8 + g);
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (off >= 0) u = load_once(kb + off + 8 * (c + 4 * i));
+          kr[t][b][i][0] = u.x; kr[t][b][i][1] = u.y; kr[t][b][i][2] = u.z; kr[t][b][i][3] = u.w;
+        }
+      }
+  };
+  auto load_v = [&]() {
+    there = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        if (__shfl_sync(0xffffffffu, v_off, t * 16 + b * 8 + g) >= 0) there |= 1u << (2 * t + b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t off = __shfl_sync(0xffffffffu, v_off, t * 16 + 2 * c + (e & 1) + 8 * (e >> 1));
+#pragma unroll
+        for (int b = 0; b < VB; ++b) {
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (off >= 0) u = load_once(vb + off + 64 * b + 8 * g);
+          vr[t][e][b][0] = u.x; vr[t][e][b][1] = u.y; vr[t][e][b][2] = u.z; vr[t][e][b][3] = u.w;
+        }
+      }
+    }
+  };
+
+  const float NEG_INF = __int_as_float(0xff800000);
+  float m_ref[RB][2], l[RB][2], o[RB][VB][4][4];  // of rows 8 r + 2 c + e
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    m_ref[r][0] = m_ref[r][1] = NEG_INF;
+    l[r][0] = l[r][1] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < VB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[r][b][j][0] = o[r][b][j][1] = o[r][b][j][2] = o[r][b][j][3] = 0.0f;
   }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  for (int c = 0; c < VL; ++c) p.out[row * p.o_row + head * p.o_head + c * 32 + lane] = __float2bfloat16_rn(o[c] * inv);
+
+  if (j0 < it.keys) {
+    locate(j0);
+    load_k();
+    load_v();
+  }
+  for (; j0 < it.keys; j0 += STEP) {
+    float s[RB][NT][4];  // [2 b + e]: key 16 t + 8 b + g, row 8 r + 2 c + e
+    const bool more = j0 + STEP < it.keys;
+    if (more) locate(j0 + STEP);
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        s[r][t][0] = s[r][t][1] = s[r][t][2] = s[r][t][3] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            mma_bf16_16816(s[r][t], kr[t][0][i][2 * h], kr[t][1][i][2 * h], kr[t][0][i][2 * h + 1], kr[t][1][i][2 * h + 1], q[r][i][2 * h], q[r][i][2 * h + 1]);
+      }
+    if (more) load_k();
+    // scores in units of log2; keys that are not there or that the row does not see count as -inf
+    const bool edge = j0 + 16 * NT > min_limit;
+    bool moves = false;
+    float mx[RB][2];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mx[r][e] = NEG_INF;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            bool seen = (there >> (2 * t + b)) & 1;
+            if (edge) seen = seen && j0 + 16 * t + 8 * b + g < limit[r][e];
+            const float x = seen ? s[r][t][2 * b + e] * p.scale2 : NEG_INF;
+            s[r][t][2 * b + e] = x;
+            mx[r][e] = fmaxf(mx[r][e], x);
+          }
+        moves = moves || mx[r][e] > m_ref[r][e] + 8.0f;
+      }
+    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx[r][e] = fmaxf(mx[r][e], __shfl_xor_sync(0xffffffffu, mx[r][e], x));
+          const float m_new = fmaxf(m_ref[r][e], mx[r][e]);
+          const float alpha = m_new == NEG_INF ? 1.0f : ex2(m_ref[r][e] - m_new);
+          m_ref[r][e] = m_new;
+          l[r][e] *= alpha;
+#pragma unroll
+          for (int b = 0; b < VB; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[r][b][j][e] *= alpha;
+              o[r][b][j][2 + e] *= alpha;
+            }
+        }
+    }
+    uint32_t pt[RB][NT][2];  // P^T as B fragments
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const float ref0 = m_ref[r][0] == NEG_INF ? 0.0f : m_ref[r][0], ref1 = m_ref[r][1] == NEG_INF ? 0.0f : m_ref[r][1];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float x0 = ex2(s[r][t][2 * b] - ref0), x1 = ex2(s[r][t][2 * b + 1] - ref1);
+          l[r][0] += x0;
+          l[r][1] += x1;
+          pt[r][t][b] = transpose8x8(pack_bf16(x0, x1));
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int b = 0; b < VB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a0 = __byte_perm(vr[t][0][b][j], vr[t][1][b][j], 0x5410), a1 = __byte_perm(vr[t][0][b][j], vr[t][1][b][j], 0x7632);
+          const uint32_t a2 = __byte_perm(vr[t][2][b][j], vr[t][3][b][j], 0x5410), a3 = __byte_perm(vr[t][2][b][j], vr[t][3][b][j], 0x7632);
+#pragma unroll
+          for (int r = 0; r < RB; ++r) mma_bf16_16816(o[r][b][j], a0, a1, a2, a3, pt[r][t][0], pt[r][t][1]);
+        }
+    if (more) load_v();
+  }
+
+  // the four warps' parts of a row
+#pragma unroll
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], x);
+      const int lr = 8 * r + 2 * c + e;
+      if (g == 0) ml_s[warp][lr] = make_float2(m_ref[r][e], l[r][e]);
+#pragma unroll
+      for (int b = 0; b < VB; ++b) {  // columns 64 b + 8 g + 2 j + {0, 1}
+        float* dst = &o_s[warp][lr][64 * b + 8 * g];
+        reinterpret_cast<float4*>(dst)[0] = make_float4(o[r][b][0][e], o[r][b][0][2 + e], o[r][b][1][e], o[r][b][1][2 + e]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(o[r][b][2][e], o[r][b][2][2 + e], o[r][b][3][e], o[r][b][3][2 + e]);
+      }
+    }
+  __syncthreads();
+  constexpr int PIECES = D / 4;
+  for (int i = threadIdx.x; i < TM * PIECES; i += PR_WARPS * 32) {
+    const int lr = i / PIECES, col = (i % PIECES) * 4, rho = it.rho0 + lr;
+    if (rho >= it.rows) break;
+    float m = NEG_INF, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < PR_WARPS; ++w) m = fmaxf(m, ml_s[w][lr].x);
+    const float ref = m == NEG_INF ? 0.0f : m;
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < PR_WARPS; ++w) {
+      const float a = ex2(ml_s[w][lr].x - ref);
+      const float4 x = *reinterpret_cast<const float4*>(&o_s[w][lr][col]);
+      sum += a * ml_s[w][lr].y;
+      acc.x += a * x.x; acc.y += a * x.y; acc.z += a * x.z; acc.w += a * x.w;
+    }
+    uint32_t tok, hq;
+    p.per_kv.divmod(static_cast<uint32_t>(rho), tok, hq);
+    const int64_t row = it.row0 + static_cast<int>(tok), qh = head * static_cast<int64_t>(p.per_kv.d) + hq;
+    const int64_t at = (static_cast<int64_t>(sp.part0 + chunk) * p.rows.rows + row) * p.q_heads + qh;
+    if (col == 0) p.part_ml[at] = make_float2(m, sum);
+    *reinterpret_cast<float4*>(p.part_o + at * D + col) = acc;
+  }
 }
 
-int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, PrefixParams& p) {
+// The parts of every row joined, and zeros for the rows that have none.  One block per row and 1,024 values of it.
+struct JoinParams {
+  PrefixParams p;
+  Span span[2];  // prefix, own
+};
+template <int D>
+__global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant__ JoinParams jp) {
+  pdl_launch_dependents();
+  const PrefixParams& p = jp.p;
+  const int row = static_cast<int>(blockIdx.x);
+  const int col = (static_cast<int>(blockIdx.y) * 256 + static_cast<int>(threadIdx.x)) * 4;
+  pdl_wait();
+  if (col >= p.q_heads * D) return;
+  const int h = col / D, d = col % D;
+  int parts[2] = {0, 0}, s, i;
+  if (row_sequence(p.rows, row, s, i)) {
+    const int g = group_of(p, s);
+    if (g >= 0 && jp.span[0].chunks) parts[0] = (prefix_keys(p, g) + jp.span[0].chunk - 1) / jp.span[0].chunk;
+    if (jp.span[1].chunks) parts[1] = (own_keys(p, p.rows.lengths[s], i) + jp.span[1].chunk - 1) / jp.span[1].chunk;
+  }
+  const int64_t at = static_cast<int64_t>(row) * p.q_heads + h, step = static_cast<int64_t>(p.rows.rows) * p.q_heads;
+  const float NEG_INF = __int_as_float(0xff800000);
+  float m = NEG_INF;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    for (int c = 0; c < parts[e]; ++c) m = fmaxf(m, p.part_ml[at + (jp.span[e].part0 + c) * step].x);
+  const float ref = m == NEG_INF ? 0.0f : m;
+  float sum = 0.0f;
+  float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll 4
+    for (int c = 0; c < parts[e]; ++c) {
+      const int64_t a = at + (jp.span[e].part0 + c) * step;
+      const float2 ml = p.part_ml[a];
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + a * D + d);
+      const float w = ex2(ml.x - ref);
+      sum += w * ml.y;
+      acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+    }
+  }
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  *reinterpret_cast<uint2*>(p.out + row * p.o_row + h * p.o_head + d) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+}
+
+struct Plan {
+  Span prefix, own;
+  bool full_tile;
+  int parts;
+  int64_t ml_bytes, bytes;
+};
+
+// keys per chunk: enough CTAs for all SMs, and for long runs several rounds of them so that the last round costs little
+int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int unit) {
+  const int64_t one_round = capacity * items / resident;
+  int64_t c = one_round <= 4 * unit ? one_round : (one_round / 8 > 4 * unit ? one_round / 8 : 4 * unit);
+  c = (c + unit - 1) / unit * unit;
+  if (c < unit) c = unit;
+  const int64_t all = (capacity + unit - 1) / unit * unit;
+  return static_cast<int>(c < all ? c : (all > 0 ? all : unit));
+}
+
+int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, PrefixParams& p, Plan& plan) {
   const int rc = check_paged(cache, rows, p.cache, p.rows);
   if (rc) return rc;
   if (!d || d->struct_size != static_cast<int32_t>(sizeof(vx_prefix_attention_desc))) return fail(-1, "vx_prefix_attention_desc: struct_size");
@@ -127,14 +391,42 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     if (!d->prefix_lengths || (d->prefix_pages > 0 && (!d->prefix_table || d->ld_prefix < d->prefix_pages)))
       return fail(-1, "prefix_lengths or prefix_table is NULL, or its rows are too short");
   }
+  const int per = d->q_heads / cache->kv_heads;
   p.q_heads = d->q_heads;
-  p.per_kv = d->q_heads / cache->kv_heads;
+  p.kv_heads = cache->kv_heads;
+  p.per_kv = FastDiv(static_cast<uint32_t>(per));
   p.groups = static_cast<int32_t>(d->groups);
   p.group_offsets = d->group_offsets;
   p.group_size = p.groups > 0 && !p.group_offsets ? static_cast<int32_t>(rows->sequences / d->groups) : 0;
   p.prefix = {d->prefix_table, d->ld_prefix, static_cast<int32_t>(d->prefix_pages)};
   p.prefix_lengths = d->prefix_lengths;
-  p.scale = d->scale;
+  p.scale2 = d->scale * 1.4426950408889634f;
+
+  plan = Plan{};
+  const int64_t R = rows->rows, S = rows->sequences, G = d->groups;
+  if (R == 0 || S == 0) return 0;
+  const int64_t cap_p = G > 0 ? d->prefix_pages * cache->page_size : 0, cap_o = rows->table_pages * cache->page_size;
+  // rows per owner and key head, on the average
+  const bool single = !rows->row_offsets;
+  plan.full_tile = (cap_p > 0 && R * per > 8 * G) || (cap_o > 0 && R * per > 8 * S);
+  const int tm = plan.full_tile ? 16 : 8;
+  const int unit = cache->head_dim == 64 ? 128 : 64;
+  const int64_t resident = static_cast<int64_t>(sm_count()) * (plan.full_tile ? 2 : 3);
+  auto cut = [&](Span& sp, int own, int64_t owners, int64_t cap, int64_t equal_rows) {
+    if (cap <= 0 || owners <= 0) return;
+    sp.own = own;
+    sp.equal = equal_rows > 0 ? static_cast<int32_t>((equal_rows + tm - 1) / tm) : 0;
+    sp.slots = static_cast<int32_t>(sp.equal ? owners * sp.equal : R * per / tm + owners);
+    sp.chunk = chunk_keys(cap, static_cast<int64_t>(sp.slots) * p.kv_heads, resident, unit);
+    sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
+  };
+  cut(plan.prefix, 0, G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
+  cut(plan.own, 1, S, cap_o, single ? per : 0);
+  plan.own.part0 = plan.prefix.chunks;
+  plan.parts = plan.prefix.chunks + plan.own.chunks;
+  const int64_t cells = R * d->q_heads;
+  plan.ml_bytes = (plan.parts * cells * 8 + 15) / 16 * 16;
+  plan.bytes = plan.ml_bytes + plan.parts * cells * cache->head_dim * 4;
   return 0;
 }
 
@@ -144,24 +436,43 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
 extern "C" int64_t vx_prefix_attention_scratch(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
   using namespace vx;
   PrefixParams p{};
-  const int rc = check_prefix(cache, rows, d, p);
-  return rc ? rc : 0;
+  Plan plan;
+  const int rc = check_prefix(cache, rows, d, p, plan);
+  return rc ? rc : plan.bytes;
 }
 
 extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, void* stream) {
   using namespace vx;
   PrefixParams p{};
-  const int rc = check_prefix(cache, rows, d, p);
+  Plan plan;
+  const int rc = check_prefix(cache, rows, d, p, plan);
   if (rc) return rc;
   if (p.rows.rows == 0) return 0;
   if (!d->q || !d->out) return fail(-1, "q and out must not be NULL");
   if (!pieces_ok(d->q, d->q_row, d->q_head, 2) || !pieces_ok(d->out, d->o_row, d->o_head, 2)) return fail(-1, "rows and heads of q and out must be 16-byte aligned");
+  if (plan.bytes > 0 && (!d->scratch || !aligned16(d->scratch) || d->scratch_bytes < plan.bytes))
+    return fail(-1, "scratch must be %lld bytes, 16-byte aligned", (long long)plan.bytes);
   p.q = static_cast<const __nv_bfloat16*>(d->q); p.q_row = d->q_row; p.q_head = d->q_head;
   p.out = static_cast<__nv_bfloat16*>(d->out); p.o_row = d->o_row; p.o_head = d->o_head;
-  const int64_t items = static_cast<int64_t>(p.rows.rows) * p.q_heads;
-  const dim3 grid(static_cast<unsigned>((items + PA_WARPS - 1) / PA_WARPS));
+  p.part_ml = static_cast<float2*>(d->scratch);
+  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d->scratch) + plan.ml_bytes);
   const auto st = static_cast<cudaStream_t>(stream);
-  if (cache->head_dim == 64) VX_CUDA_OK(launch_dependent(prefix_attention_kernel<64>, grid, dim3(PA_WARPS * 32), 0, st, p));
-  else VX_CUDA_OK(launch_dependent(prefix_attention_kernel<128>, grid, dim3(PA_WARPS * 32), 0, st, p));
+  const bool d64 = cache->head_dim == 64;
+  if (plan.parts > 0) {
+    RowsParams rp{p, {plan.prefix, plan.own}, 0};
+    const int64_t first = static_cast<int64_t>(plan.prefix.slots) * plan.prefix.chunks * p.kv_heads;
+    const int64_t items = first + static_cast<int64_t>(plan.own.slots) * plan.own.chunks * p.kv_heads;
+    if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
+    rp.first_items = static_cast<int32_t>(first);
+    const dim3 grid(static_cast<unsigned>(items)), block(PR_WARPS * 32);
+    auto kernel = d64 ? (plan.full_tile ? prefix_rows_kernel<64, 2> : prefix_rows_kernel<64, 1>)
+                      : (plan.full_tile ? prefix_rows_kernel<128, 2> : prefix_rows_kernel<128, 1>);
+    VX_CUDA_OK(launch_dependent(kernel, grid, block, 0, st, rp));
+  }
+  JoinParams jp{p, {plan.prefix, plan.own}};
+  const dim3 grid(static_cast<unsigned>(p.rows.rows), static_cast<unsigned>((p.q_heads * cache->head_dim + 1023) / 1024));
+  const int threads = p.q_heads * cache->head_dim >= 1024 ? 256 : (p.q_heads * cache->head_dim / 4 + 31) / 32 * 32;
+  auto join = d64 ? prefix_join_kernel<64> : prefix_join_kernel<128>;
+  VX_CUDA_OK(launch_dependent(join, grid, dim3(threads), 0, st, jp));
   return 0;
 }
