@@ -544,3 +544,41 @@ def test_refusals(ops):
         with pytest.raises(err):
             attend(*a, **kw)
     assert ops._lib.device_status() == 0
+
+
+def test_native_and_general_routes_agree(ops, monkeypatch):
+    """The native host path and the Python code behind it pass the same descriptors on."""
+    class Declines:
+        @staticmethod
+        def kv_append(*a):
+            return None
+
+        prefix_attention = kv_append
+
+        @staticmethod
+        def launches():
+            return 0
+
+    def results():
+        out = []
+        for kw in (dict(heads=8, kv=8, d=64, n=10), dict(heads=8, kv=2, d=128, n=5, tokens=20)):
+            out += [t for pair in _decode(ops, 3, prefix=100, **kw)[0] for t in pair]
+        k_pages, v_pages = make_cache(6, 16, 2, 64, "heads")
+        x = torch.randn(4, 3, 2, 64, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+        rot = ops.rotary_table(99, 32)
+        q_out = torch.zeros(4, 2, 64, device="cuda", dtype=torch.bfloat16)
+        t, n, off = ints([[0, 1, 2], [3, 4, 5]]), ints([5, 17]), ints([0, 3, 4])
+        got = ops.kv_append(x[:, 0], x[:, 1], k_pages, v_pages, t, n, q=x[:, 2], rotary=rot, interleaved=True, row_offsets=off, starts=ints([9, 1]), q_out=q_out)
+        assert got is q_out and ops.kv_append(x[:, 0], x[:, 1], k_pages, v_pages, t, n, row_offsets=off) is None
+        o = torch.zeros_like(q_out)
+        assert ops.prefix_attention(q_out, k_pages, v_pages, t, n, ints([[0], [3]]), ints([9, 16]), row_offsets=off, group_offsets=ints([0, 1, 2]), scale=0.3, out=o) is o
+        return out + [q_out, o, k_pages, v_pages]
+
+    before = ops.launch_count()
+    first = results()
+    assert ops.launch_count() > before
+    assert ops._native is not None
+    monkeypatch.setattr(ops, "_native", Declines)
+    second = results()
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)

@@ -31,7 +31,7 @@ namespace {
   X(vx_last_error) X(vx_quantize_pack) X(vx_ln_quantize_pack) X(vx_ln2_quantize_pack) X(vx_amax) X(vx_bsgemm)        \
   X(vx_bsgemm_natural_sf_supported) X(vx_bsgemm_residual_ln_supported) X(vx_bsgemm_residual_ln) X(vx_bsgemm_residual_ln2) X(vx_argmax_ids) X(vx_relpos_attention)   \
   X(vx_power_mel_log) X(vx_power_mel_log_supported) X(vx_sf_from_natural_pair) X(vx_rowscale_linear) X(vx_rowscale_linear_scratch) X(vx_ctc_topk_rows) X(vx_ctc_topk)        \
-  X(vx_conformer_pass_supported) X(vx_conformer_pass_scratch) X(vx_conformer_pass)
+  X(vx_conformer_pass_supported) X(vx_conformer_pass_scratch) X(vx_conformer_pass) X(vx_kv_append) X(vx_prefix_attention) X(vx_prefix_attention_scratch)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   VX_FUNCS(X)
@@ -1178,6 +1178,157 @@ PyObject* py_reset(PyObject*, PyObject*) {
   Py_RETURN_NONE;
 }
 
+// ---------------------------------------------------------------- paged cache
+// stride of a dimension that is walked; that of a single entry says nothing
+int64_t step(const at::Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+// rows and heads at 16-byte addresses, values of a head in a row
+bool in_pieces(const at::Tensor& t) {
+  const int64_t last = t.dim() - 1, es = t.element_size();
+  if ((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0 || (t.size(last) > 1 && t.stride(last) != 1)) return false;
+  for (int64_t i = 0; i < last; ++i)
+    if (step(t, static_cast<int>(i)) * es % 16 != 0) return false;
+  return true;
+}
+// int32 [n] or [n, m] (n, m < 0: any) on `dev`, rows contiguous
+bool int32_arg(PyObject* o, int64_t n, int64_t m, int dims, const at::Device& dev, const at::Tensor** t) {
+  if (!is_cuda_tensor(o)) return false;
+  const at::Tensor& x = THPVariable_Unpack(o);
+  *t = &x;
+  if (x.scalar_type() != at::kInt || x.dim() != dims || x.device() != dev || (n >= 0 && x.size(0) != n)) return false;
+  if (dims == 2 && m >= 0 && x.size(1) != m) return false;
+  return x.size(dims - 1) <= 1 || x.stride(dims - 1) == 1;
+}
+const int32_t* int32_ptr(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+
+bool paged_cache(PyObject* ko, PyObject* vo, vx_kv_cache& c, at::Device& dev) {
+  if (!is_cuda_tensor(ko) || !is_cuda_tensor(vo)) return false;
+  const at::Tensor &k = THPVariable_Unpack(ko), &v = THPVariable_Unpack(vo);
+  if (k.scalar_type() != at::kBFloat16 || v.scalar_type() != at::kBFloat16 || k.dim() != 4 || k.sizes() != v.sizes() || k.device() != v.device() ||
+      k.size(1) < 1 || k.size(2) < 1 || k.size(1) > 0x7fffffff || k.size(2) > 0x7fffffff || !in_pieces(k) || !in_pieces(v))
+    return false;
+  dev = k.device();
+  c = {static_cast<int32_t>(sizeof(vx_kv_cache)), static_cast<int32_t>(k.size(1)), k.size(0), static_cast<int32_t>(k.size(2)), static_cast<int32_t>(k.size(3)),
+       k.data_ptr(), v.data_ptr(), step(k, 0), step(k, 1), step(k, 2), step(v, 0), step(v, 1), step(v, 2)};
+  return true;
+}
+bool paged_rows(int64_t rows, PyObject* table, PyObject* lengths, PyObject* offsets, const at::Device& dev, vx_kv_rows& r) {
+  const at::Tensor *t, *n, *o = nullptr;
+  if (!int32_arg(table, -1, -1, 2, dev, &t) || !int32_arg(lengths, t->size(0), -1, 1, dev, &n)) return false;
+  if (offsets == Py_None ? rows != t->size(0) : !int32_arg(offsets, t->size(0) + 1, -1, 1, dev, &o)) return false;
+  r = {static_cast<int32_t>(sizeof(vx_kv_rows)), 0, rows, t->size(0), int32_ptr(*n), o ? int32_ptr(*o) : nullptr, int32_ptr(*t),
+       t->size(0) > 1 ? t->stride(0) : t->size(1), t->size(1)};
+  return true;
+}
+// [rows, heads, head_dim] operand (rows, heads < 0: any)
+bool heads3d(PyObject* o, int64_t rows, int64_t heads, int64_t dim, const at::Device& dev, const at::Tensor** t) {
+  if (!is_cuda_tensor(o)) return false;
+  const at::Tensor& x = THPVariable_Unpack(o);
+  *t = &x;
+  return x.dim() == 3 && x.device() == dev && x.size(2) == dim && (rows < 0 || x.size(0) == rows) && (heads < 0 || x.size(1) == heads) && in_pieces(x);
+}
+
+// kv_append(k, v, k_pages, v_pages, page_table, lengths, q | None, rotary | None, interleaved, row_offsets | None, starts | None, q_out | None)
+//   -> q_out | True (no queries) | None
+PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
+  VX_BEGIN
+  VX_ARGS(12)
+  vx_kv_cache cache;
+  vx_kv_rows rows;
+  vx_kv_append_desc d{};
+  at::Device dev(at::kCUDA);
+  const at::Tensor *k, *v, *q = nullptr, *t;
+  if (!paged_cache(p[2], p[3], cache, dev) || !heads3d(p[0], -1, cache.kv_heads, cache.head_dim, dev, &k) ||
+      !heads3d(p[1], k->size(0), cache.kv_heads, cache.head_dim, dev, &v) || !paged_rows(k->size(0), p[4], p[5], p[9], dev, rows))
+    Py_RETURN_NONE;
+  d.struct_size = sizeof(vx_kv_append_desc);
+  d.dtype = dtype_code(*k);
+  if (d.dtype < 0 || v->scalar_type() != k->scalar_type()) Py_RETURN_NONE;
+  d.k = k->data_ptr(); d.k_row = step(*k, 0); d.k_head = step(*k, 1);
+  d.v = v->data_ptr(); d.v_row = step(*v, 0); d.v_head = step(*v, 1);
+  if (p[6] != Py_None) {
+    if (!heads3d(p[6], rows.rows, -1, cache.head_dim, dev, &q) || q->scalar_type() != k->scalar_type()) Py_RETURN_NONE;
+    d.q = q->data_ptr(); d.q_row = step(*q, 0); d.q_head = step(*q, 1); d.q_heads = static_cast<int>(q->size(1));
+  }
+  at::Tensor out;
+  if (p[11] != Py_None) {
+    if (!q || !heads3d(p[11], rows.rows, d.q_heads, cache.head_dim, dev, &t) || t->scalar_type() != at::kBFloat16) Py_RETURN_NONE;
+    out = *t;
+  }
+  if (p[7] != Py_None) {
+    if (!is_cuda_tensor(p[7])) Py_RETURN_NONE;
+    const at::Tensor& r = THPVariable_Unpack(p[7]);
+    if (r.scalar_type() != at::kFloat || r.dim() != 2 || r.device() != dev || r.size(1) % 16 != 0 || r.size(1) < 16 || r.size(1) > cache.head_dim || !in_pieces(r)) Py_RETURN_NONE;
+    d.rotary = static_cast<const float*>(r.data_ptr());
+    d.positions = r.size(0); d.rot_dim = static_cast<int>(r.size(1)); d.ld_rotary = r.size(0) > 1 ? r.stride(0) : r.size(1);
+    d.interleaved = as_bool(p[8]);
+  }
+  if (p[10] != Py_None) {
+    if (!int32_arg(p[10], rows.sequences, -1, 1, dev, &t)) Py_RETURN_NONE;
+    d.starts = int32_ptr(*t);
+  }
+  {
+    NoGil nogil;
+    if (q && !out.defined()) out = empty(q->sizes(), at::kBFloat16, dev);
+    if (q) { d.q_out = out.data_ptr(); d.qo_row = step(out, 0); d.qo_head = step(out, 1); }
+    check(g.vx_kv_append(&cache, &rows, &d, stream()), "vx_kv_append");
+    count();
+  }
+  if (!q) Py_RETURN_TRUE;
+  return p[11] != Py_None ? Py_NewRef(p[11]) : wrap(out);
+  VX_END
+}
+
+// prefix_attention(q, k_pages, v_pages, page_table, lengths, prefix_table | None, prefix_lengths | None, row_offsets | None, group_offsets | None,
+//   scale | None, out | None) -> out | None
+PyObject* py_prefix_attention(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
+  VX_BEGIN
+  VX_ARGS(11)
+  vx_kv_cache cache;
+  vx_kv_rows rows;
+  vx_prefix_attention_desc d{};
+  at::Device dev(at::kCUDA);
+  const at::Tensor *q, *t, *n, *o;
+  if (!paged_cache(p[1], p[2], cache, dev) || !heads3d(p[0], -1, -1, cache.head_dim, dev, &q) || q->scalar_type() != at::kBFloat16 ||
+      (cache.head_dim != 64 && cache.head_dim != 128) || q->size(1) < 1 || q->size(1) % cache.kv_heads != 0 || !paged_rows(q->size(0), p[3], p[4], p[7], dev, rows))
+    Py_RETURN_NONE;
+  d.struct_size = sizeof(vx_prefix_attention_desc);
+  d.q = q->data_ptr(); d.q_row = step(*q, 0); d.q_head = step(*q, 1); d.q_heads = static_cast<int>(q->size(1));
+  if ((p[5] == Py_None) != (p[6] == Py_None)) Py_RETURN_NONE;
+  if (p[5] != Py_None) {
+    if (!int32_arg(p[5], -1, -1, 2, dev, &t) || !int32_arg(p[6], t->size(0), -1, 1, dev, &n)) Py_RETURN_NONE;
+    d.groups = t->size(0);
+    if (p[8] != Py_None) {
+      if (!int32_arg(p[8], d.groups + 1, -1, 1, dev, &o)) Py_RETURN_NONE;
+      d.group_offsets = int32_ptr(*o);
+    } else if (d.groups == 0 || rows.sequences % d.groups != 0) {
+      Py_RETURN_NONE;
+    }
+    d.prefix_table = int32_ptr(*t); d.ld_prefix = d.groups > 1 ? t->stride(0) : t->size(1); d.prefix_pages = t->size(1);
+    d.prefix_lengths = int32_ptr(*n);
+  }
+  d.scale = p[9] == Py_None ? (cache.head_dim == 64 ? 0.125f : 0.08838834764831845f) : static_cast<float>(as_double(p[9]));
+  at::Tensor out, scratch;
+  if (p[10] != Py_None) {
+    if (!heads3d(p[10], q->size(0), q->size(1), cache.head_dim, dev, &t) || t->scalar_type() != at::kBFloat16) Py_RETURN_NONE;
+    out = *t;
+  }
+  {
+    NoGil nogil;
+    if (!out.defined()) out = empty(q->sizes(), at::kBFloat16, dev);
+    d.out = out.data_ptr(); d.o_row = step(out, 0); d.o_head = step(out, 1);
+    const int64_t size = g.vx_prefix_attention_scratch(&cache, &rows, &d);
+    if (size < 0) check(static_cast<int>(size), "vx_prefix_attention");
+    if (size > 0) {
+      scratch = empty({size}, at::kByte, dev);
+      d.scratch = scratch.data_ptr(); d.scratch_bytes = size;
+    }
+    check(g.vx_prefix_attention(&cache, &rows, &d, stream()), "vx_prefix_attention");
+    count(2);
+  }
+  return p[10] != Py_None ? Py_NewRef(p[10]) : wrap(out);
+  VX_END
+}
+
 // init(library path, VeloxError, Quantized)
 PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   VX_ARGS(3)
@@ -1215,6 +1366,8 @@ PyMethodDef kMethods[] = {
     VX_METHOD("qkv_pack_gemm", py_qkv_pack_gemm),
     VX_METHOD("heads_gemm", py_heads_gemm),
     VX_METHOD("power_mel_log", py_power_mel_log),
+    VX_METHOD("kv_append", py_kv_append),
+    VX_METHOD("prefix_attention", py_prefix_attention),
     VX_METHOD("stack_plan", py_stack_plan),
     VX_METHOD("stack_plan_current", py_stack_plan_current),
     VX_METHOD("stack_forward", py_stack_forward),

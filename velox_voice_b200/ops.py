@@ -821,6 +821,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     Left out, with zero queries: rows of no sequence, of one of negative length, at a position that the table does not have.  Not
     stored: tokens whose page is not there (an entry outside [0, pages), or none).  ``lengths`` stays as it is: the same call of
     :func:`prefix_attention` takes it, and the program then moves it on."""
+    r = (_native or _host()).kv_append(k, v, k_pages, v_pages, page_table, lengths, q, rotary, interleaved, row_offsets, starts, q_out)
+    if r is not None:
+        return None if r is True else r
     cache = _kv_cache(k_pages, v_pages)
     dev, kv = k_pages.device, k_pages.shape[2]
     kinds = (torch.float32, torch.bfloat16)
@@ -880,6 +883,10 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     [o_g, o_{g+1}) are group g; without it the groups are of one size.  Without ``prefix_table`` there is no prefix.  Keys on pages
     that are not there (entries outside [0, pages)) are not attended; a row that has no key, or whose sequence has a negative
     length, gets zeros.  ``scale``: head_dim ** -0.5 unless given."""
+    r = (_native or _host()).prefix_attention(q, k_pages, v_pages, page_table, lengths, prefix_table, prefix_lengths, row_offsets, group_offsets,
+                                              scale, out)
+    if r is not None:
+        return r
     cache = _kv_cache(k_pages, v_pages)
     dev, kv, dim = k_pages.device, k_pages.shape[2], k_pages.shape[3]
     q = _heads3d(q, "q", None, None, k_pages, (torch.bfloat16,))
@@ -919,7 +926,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     d.scratch, d.scratch_bytes = _ptr(scratch), size
     _lib.check(lib.vx_prefix_attention(C.byref(cache), C.byref(r), C.byref(d), _stream()), "vx_prefix_attention")
-    _count()
+    _count(2)
     del keep, prefix_table, prefix_lengths, group_offsets
     return out
 
