@@ -12,7 +12,6 @@
 #pragma once
 
 #include "vx_paged.cuh"
-#include "vx_ptx.cuh"
 
 namespace vx {
 
@@ -131,7 +130,9 @@ __device__ __forceinline__ bool find_item(const PrefixParams& p, const Span& sp,
   return true;
 }
 
-// Work of the tile kernel (128 rows and more per owner and key head), launched by vx_prefix_attention.
+constexpr int kTileRows = 256;  // rows that a CTA of prefix_tiles_kernel takes
+
+// Launches prefix_tiles_kernel on the spans that have chunks.
 int launch_prefix_tiles(const PrefixParams& p, int head_dim, const Span& prefix, const Span& own, void* stream);
 
 }  // namespace vx

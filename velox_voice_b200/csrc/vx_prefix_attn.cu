@@ -26,11 +26,13 @@
 
 #include "vx_common.cuh"
 #include "vx_prefix.cuh"
+#include "vx_ptx.cuh"
 
 namespace vx {
 namespace {
 
 constexpr int PR_WARPS = 4;
+constexpr int kRowsKernel = 16;  // rows per owner and key head up to which prefix_rows_kernel takes a span
 
 struct RowsParams {
   PrefixParams p;
@@ -359,19 +361,27 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant_
 
 struct Plan {
   Span prefix, own;
-  bool full_tile;
+  bool prefix_tiles, own_tiles;  // which kernel walks the span
+  int blocks;                    // of eight rows, of the kernel for few rows
   int parts;
   int64_t ml_bytes, bytes;
 };
 
-// keys per chunk: enough CTAs for all SMs, and for long runs several rounds of them so that the last round costs little
-int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int unit) {
-  const int64_t one_round = capacity * items / resident;
-  int64_t c = one_round <= 4 * unit ? one_round : (one_round / 8 > 4 * unit ? one_round / 8 : 4 * unit);
-  c = (c + unit - 1) / unit * unit;
-  if (c < unit) c = unit;
-  const int64_t all = (capacity + unit - 1) / unit * unit;
-  return static_cast<int>(c < all ? c : (all > 0 ? all : unit));
+int64_t round_up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+
+// Keys per chunk for a span of `items` tiles times key heads.  Short runs are cut so that one round of CTAs (`resident`) takes them all;
+// long ones into several rounds, since owners differ in length and the last round should cost little.  Each part costs its sums in
+// scratch, so no chunk is below `least` keys there.
+int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int64_t unit, int64_t least, int64_t rounds) {
+  const int64_t one_round = (capacity * items + resident - 1) / resident;
+  int64_t c = one_round;
+  if (one_round > least) {
+    const int64_t cuts = (rounds * resident + items - 1) / items;
+    c = capacity / cuts > least ? (capacity + cuts - 1) / cuts : least;
+  }
+  c = round_up(c > unit ? c : unit, unit);
+  const int64_t all = round_up(capacity, unit);
+  return static_cast<int>(c < all ? c : all);
 }
 
 int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, PrefixParams& p, Plan& plan) {
@@ -391,6 +401,7 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     if (!d->prefix_lengths || (d->prefix_pages > 0 && (!d->prefix_table || d->ld_prefix < d->prefix_pages)))
       return fail(-1, "prefix_lengths or prefix_table is NULL, or its rows are too short");
   }
+  if (!(d->scale > 0.0f) || d->scale > 3.0e38f) return fail(-1, "scale must be positive and finite");
   const int per = d->q_heads / cache->kv_heads;
   p.q_heads = d->q_heads;
   p.kv_heads = cache->kv_heads;
@@ -406,22 +417,25 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
   const int64_t R = rows->rows, S = rows->sequences, G = d->groups;
   if (R == 0 || S == 0) return 0;
   const int64_t cap_p = G > 0 ? d->prefix_pages * cache->page_size : 0, cap_o = rows->table_pages * cache->page_size;
-  // rows per owner and key head, on the average
+  // The kernel of a span goes by its rows per owner and key head, on the average (which kernel takes a row changes no result beyond rounding).
   const bool single = !rows->row_offsets;
-  plan.full_tile = (cap_p > 0 && R * per > 8 * G) || (cap_o > 0 && R * per > 8 * S);
-  const int tm = plan.full_tile ? 16 : 8;
-  const int unit = cache->head_dim == 64 ? 128 : 64;
-  const int64_t resident = static_cast<int64_t>(sm_count()) * (plan.full_tile ? 2 : 3);
-  auto cut = [&](Span& sp, int own, int64_t owners, int64_t cap, int64_t equal_rows) {
+  const int64_t rows_p = cap_p > 0 ? R * per / G : 0, rows_o = cap_o > 0 ? R * per / S : 0;
+  plan.prefix_tiles = rows_p > kRowsKernel;
+  plan.own_tiles = rows_o > kRowsKernel;
+  plan.blocks = (!plan.prefix_tiles && rows_p > 8) || (!plan.own_tiles && rows_o > 8) ? 2 : 1;
+  auto cut = [&](Span& sp, int own, bool tiles, int64_t owners, int64_t cap, int64_t equal_rows) {
     if (cap <= 0 || owners <= 0) return;
+    const int tm = tiles ? kTileRows : 8 * plan.blocks;
     sp.own = own;
     sp.equal = equal_rows > 0 ? static_cast<int32_t>((equal_rows + tm - 1) / tm) : 0;
     sp.slots = static_cast<int32_t>(sp.equal ? owners * sp.equal : R * per / tm + owners);
-    sp.chunk = chunk_keys(cap, static_cast<int64_t>(sp.slots) * p.kv_heads, resident, unit);
+    const int64_t items = static_cast<int64_t>(sp.slots) * p.kv_heads;
+    if (tiles) sp.chunk = chunk_keys(cap, items, sm_count(), 256, 1024, 4);
+    else sp.chunk = chunk_keys(cap, items, static_cast<int64_t>(sm_count()) * (plan.blocks == 1 ? 3 : 2), cache->head_dim == 64 ? 128 : 64, 256, 8);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
-  cut(plan.prefix, 0, G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
-  cut(plan.own, 1, S, cap_o, single ? per : 0);
+  cut(plan.prefix, 0, plan.prefix_tiles, G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
+  cut(plan.own, 1, plan.own_tiles, S, cap_o, single ? per : 0);
   plan.own.part0 = plan.prefix.chunks;
   plan.parts = plan.prefix.chunks + plan.own.chunks;
   const int64_t cells = R * d->q_heads;
@@ -458,15 +472,21 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
   p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d->scratch) + plan.ml_bytes);
   const auto st = static_cast<cudaStream_t>(stream);
   const bool d64 = cache->head_dim == 64;
-  if (plan.parts > 0) {
-    RowsParams rp{p, {plan.prefix, plan.own}, 0};
-    const int64_t first = static_cast<int64_t>(plan.prefix.slots) * plan.prefix.chunks * p.kv_heads;
-    const int64_t items = first + static_cast<int64_t>(plan.own.slots) * plan.own.chunks * p.kv_heads;
+  const Span none{0, 1, 1, 1, 0, 0};
+  p.status = device_status_ptr();
+  if (plan.prefix_tiles || plan.own_tiles) {
+    const int e = launch_prefix_tiles(p, cache->head_dim, plan.prefix_tiles ? plan.prefix : none, plan.own_tiles ? plan.own : none, stream);
+    if (e) return e;
+  }
+  if ((!plan.prefix_tiles && plan.prefix.chunks > 0) || (!plan.own_tiles && plan.own.chunks > 0)) {
+    RowsParams rp{p, {plan.prefix_tiles ? none : plan.prefix, plan.own_tiles ? none : plan.own}, 0};
+    const int64_t first = static_cast<int64_t>(rp.span[0].slots) * rp.span[0].chunks * p.kv_heads;
+    const int64_t items = first + static_cast<int64_t>(rp.span[1].slots) * rp.span[1].chunks * p.kv_heads;
     if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
     rp.first_items = static_cast<int32_t>(first);
     const dim3 grid(static_cast<unsigned>(items)), block(PR_WARPS * 32);
-    auto kernel = d64 ? (plan.full_tile ? prefix_rows_kernel<64, 2> : prefix_rows_kernel<64, 1>)
-                      : (plan.full_tile ? prefix_rows_kernel<128, 2> : prefix_rows_kernel<128, 1>);
+    auto kernel = d64 ? (plan.blocks == 2 ? prefix_rows_kernel<64, 2> : prefix_rows_kernel<64, 1>)
+                      : (plan.blocks == 2 ? prefix_rows_kernel<128, 2> : prefix_rows_kernel<128, 1>);
     VX_CUDA_OK(launch_dependent(kernel, grid, block, 0, st, rp));
   }
   JoinParams jp{p, {plan.prefix, plan.own}};

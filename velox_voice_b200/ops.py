@@ -882,7 +882,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     [0, prefix_lengths[g]) of the pages ``prefix_table[g]`` (int32 [groups, pages]).  ``group_offsets`` int32 [groups + 1]: sequences
     [o_g, o_{g+1}) are group g; without it the groups are of one size.  Without ``prefix_table`` there is no prefix.  Keys on pages
     that are not there (entries outside [0, pages)) are not attended; a row that has no key, or whose sequence has a negative
-    length, gets zeros.  ``scale``: head_dim ** -0.5 unless given."""
+    length, gets zeros.  ``scale``: positive, head_dim ** -0.5 unless given."""
     r = (_native or _host()).prefix_attention(q, k_pages, v_pages, page_table, lengths, prefix_table, prefix_lengths, row_offsets, group_offsets,
                                               scale, out)
     if r is not None:
