@@ -31,7 +31,7 @@ namespace {
 
 constexpr int PT_BN = 128;                 // keys per tile
 constexpr int PT_PANEL = 128 * 128;        // 128 rows of 64 bf16
-constexpr int PT_THREADS = 13 * 32;
+constexpr int PT_THREADS = 16 * 32;         // (warps 13..15 only fill the fourth warpgroup)
 constexpr int PT_MASKS = 8;                // tiles whose masks are kept
 constexpr uint32_t PT_TM_SLOT = 256, PT_TM_O = 128, PT_TM_COLS = 512;
 
@@ -40,7 +40,6 @@ struct TileShape {
   static constexpr int kPanels = D / 64;
   static constexpr int kTile = kPanels * PT_PANEL;   // bytes of a K or V tile and of a slot's Q
   static constexpr int kStages = D == 128 ? 5 : 10;
-  static constexpr int kLag = 3;                     // tiles a loader has in flight before it waits for the oldest
   static constexpr int kSmem = (2 + kStages) * kTile + 1024;
 };
 
@@ -79,11 +78,9 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// The barrier is arrived at once for this thread when its copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -137,7 +134,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_full, dual ? 8 : 4);
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&bar.full[s], 4);
+      mbar_init(&bar.full[s], 128);  // the loaders' threads
       mbar_init(&bar.empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -156,9 +153,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bar.tmem_base;
+  // Registers: 128 a thread at launch, 512 for a thread of each of the four warpgroups.  The softmax, which holds a row of S, takes 192 in
+  // two of them, the other two leave 64 each (2 x 192 + 2 x 64 = 512); every warp of a warpgroup passes the same setmaxnreg.
 
   if (warp >= 8 && warp < 12) {
     // =========================== loaders ===========================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // Order: K0, K1, V0, K2, V1, ..., V(tiles - 1), each into the next stage of the ring.
     const int w = warp - 8;
     const PagedTable& table = sp.own ? p.rows.table : p.prefix;
@@ -168,16 +168,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     constexpr int KEYS = 32 / LANES;       // keys per instruction
     const int piece = lane % LANES, sub = lane / LANES;
     const uint32_t ring_u = smem_u32(ring) + (piece >> 3) * PT_PANEL;
-    int stage = 0, issued = 0;
+    int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    auto signal = [&](int s) {  // this warp's part of a stage has landed
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.full[s]);
-    };
     auto load = [&](const __nv_bfloat16* base, int64_t off) {
-      ok = __all_sync(0xffffffffu, mbar_wait<true>(&bar.empty[stage], phase ^ 1, p.status, 40));
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar.empty[stage], phase ^ 1, p.status, 40));
       if (!ok) return;
       const uint32_t dst = ring_u + stage * Shape::kTile;
 #pragma unroll
@@ -186,12 +181,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         const int64_t o = __shfl_sync(0xffffffffu, off, key);
         cp_async16(dst + (w * 32 + key) * 128 + (((piece & 7) ^ (key & 7)) << 4), base + (o < 0 ? 0 : o) + piece * 8, o >= 0);
       }
-      cp_async_commit();
+      cp_async_arrive(&bar.full[stage]);
       if (++stage == NS) { stage = 0; phase ^= 1; }
-      if (++issued > Shape::kLag) {
-        cp_async_wait<Shape::kLag>();
-        signal((stage + NS - 1 - Shape::kLag) % NS);
-      }
     };
     int64_t v_prev = -1;  // the tile before
     for (int t = 0; t <= tiles && ok; ++t) {
@@ -219,21 +210,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       if (t > 0) load(vb, v_prev);
       v_prev = v_off;
     }
-    cp_async_wait<0>();
-    if (ok)
-      for (int i = issued < Shape::kLag ? issued : Shape::kLag; i > 0; --i) signal((stage + NS - i) % NS);
-  } else if (warp == 12) {
+    cp_async_wait_all();
+  } else if (warp >= 12) {
     // =========================== MMA issuer ===========================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 12) {
     const bool leader = elect_one();
     const uint32_t idesc_s = idesc_bf16(128, PT_BN, false), idesc_o = idesc_bf16(128, 64, true);
     const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
     auto desc = [&](uint32_t lo) { return (static_cast<uint64_t>(desc_hi) << 32) | lo; };
     const uint32_t q_lo = smem_u32(q_s) >> 4, ring_lo = smem_u32(ring) >> 4;
-    bool ok = mbar_wait_spin<true>(&bar.q_full, 0, p.status, 41);
+    bool ok = mbar_wait_spin(&bar.q_full, 0, p.status, 41);
     tc_fence_after();
     auto k_stage = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
     auto v_stage = [&](int j) { return j < tiles - 1 ? 2 * j + 2 : 2 * j + 1; };
-    auto landed = [&](int i) { return mbar_wait_spin<true>(&bar.full[i % NS], (i / NS) & 1, p.status, 42); };
+    // (the copies are writes of the generic proxy: the fence orders them before the products that read them)
+    auto landed = [&](int i) {
+      const bool there = mbar_wait_spin(&bar.full[i % NS], (i / NS) & 1, p.status, 42);
+      fence_proxy_async_smem();
+      return there;
+    };
     auto issue_s = [&](int slot, int j) {
       const uint32_t qa = q_lo + (dual ? slot : 0) * (Shape::kTile >> 4), kt = ring_lo + (k_stage(j) % NS) * (Shape::kTile >> 4);
 #pragma unroll
@@ -266,7 +262,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         ok = landed(v_stage(j));
         for (int slot = 0; slot < 2 && ok; ++slot) {
           if (j >= n_slot[slot]) continue;
-          ok = mbar_wait_spin<true>(&bar.p_full[slot], j & 1, p.status, 43);
+          ok = mbar_wait_spin(&bar.p_full[slot], j & 1, p.status, 43);
           if (!ok) break;
           tc_fence_after();
           issue_o(slot, j, j == 0);
@@ -292,7 +288,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       }
       for (int j = 0; j < tiles && ok; ++j) {
         const int slot = j & 1;
-        ok = landed(v_stage(j)) && mbar_wait_spin<true>(&bar.p_full[slot], (j >> 1) & 1, p.status, 43);
+        ok = landed(v_stage(j)) && mbar_wait_spin(&bar.p_full[slot], (j >> 1) & 1, p.status, 43);
         if (!ok) break;
         tc_fence_after();
         issue_o(slot, j, j < 2);
@@ -308,8 +304,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         }
       }
     }
-  } else if (warp < 8) {
+    }
+  } else {
     // =========================== softmax: a row per thread ===========================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int slot = warp >> 2, quad = warp & 3, local = quad * 32 + lane;
     const uint32_t tm = tmem_base + slot * PT_TM_SLOT + (static_cast<uint32_t>(quad * 32) << 16);
     const int rho = it.rho0 + (dual ? slot * 128 : 0) + local;
@@ -339,13 +337,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     for (int u = 0; u < mine; ++u) {
       const int t = dual ? u : 2 * u + slot;
       if (idle) {
-        ok = __all_sync(0xffffffffu, mbar_wait_spin<true>(&bar.s_full[slot], u & 1, p.status, 47));
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.s_full[slot], u & 1, p.status, 47));
         if (!ok) break;
         if (lane == 0) mbar_arrive(&bar.p_full[slot]);
         continue;
       }
       // which keys of the tile this row sees
-      ok = __all_sync(0xffffffffu, mbar_wait_spin<true>(&bar.mask_full[t % PT_MASKS], (t / PT_MASKS) & 1, p.status, 44));
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.mask_full[t % PT_MASKS], (t / PT_MASKS) & 1, p.status, 44));
       if (!ok) break;
       uint32_t seen[4];
       bool all = true;
@@ -355,23 +353,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         all = all && seen[i] == 0xffffffffu;
       }
       const bool masked = __any_sync(0xffffffffu, !all);
-      ok = __all_sync(0xffffffffu, mbar_wait_spin<true>(&bar.s_full[slot], u & 1, p.status, 45));
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.s_full[slot], u & 1, p.status, 45));
       if (!ok) break;
       tc_fence_after();
-      float mx = NEG_INF;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t s[32];
-        tc_ld_32x32b_x32(tm + 32 * i, s);
-        tc_wait_ld();
+      uint32_t sc[4][32];
+      tc_ld_32x32b_x32(tm, sc[0]);
+      tc_ld_32x32b_x32(tm + 32, sc[1]);
+      tc_wait_ld();
+      tc_ld_32x32b_x32(tm + 64, sc[2]);
+      tc_ld_32x32b_x32(tm + 96, sc[3]);
+      float m4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+      auto largest = [&](int i) {
         if (masked) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (!((seen[i] >> e) & 1)) s[e] = 0xff800000u;
+            if (!((seen[i] >> e) & 1)) sc[i][e] = 0xff800000u;
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) mx = max3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-      }
+        for (int e = 0; e < 32; e += 2) m4[(e >> 1) & 3] = max3(m4[(e >> 1) & 3], __uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1]));
+      };
+      largest(0);
+      largest(1);
+      tc_wait_ld();
+      largest(2);
+      largest(3);
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       const float m_tile = mx * p.scale2;
       const bool moves = m_tile > m_ref + 8.0f;
       if (__any_sync(0xffffffffu, moves)) {
@@ -396,24 +402,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t s[32], pk[16];
-        tc_ld_32x32b_x32(tm + 32 * i, s);
-        tc_wait_ld();
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((seen[i] >> e) & 1)) s[e] = 0xff800000u;
-        }
+        uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           float x0, x1;
-          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), k2, n2), x0, x1);
+          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1])), k2, n2), x0, x1);
           x0 = ex2(x0);
           x1 = ex2(x1);
           sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], pack_f32x2(x0, x1));
           pk[e >> 1] = pack_bf16(x0, x1);
         }
-        tc_st_x16(tm + 16 * i, pk);  // over columns that have been read
+        tc_st_x16(tm + 16 * i, pk);  // over S, which is in registers
       }
       float a0, a1, b0, b1;
       unpack_f32x2(sum[0], a0, a1);
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.p_full[slot]);
     }
-    if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_spin<true>(&bar.o_full[slot], 0, p.status, 46));
+    if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.o_full[slot], 0, p.status, 46));
     tc_fence_after();
     const int64_t at = (static_cast<int64_t>(sp.part0 + chunk) * p.rows.rows + row) * p.q_heads + qh;
     if (dual) {
