@@ -24,6 +24,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "vx_common.cuh"
 #include "vx_prefix.cuh"
 #include "vx_ptx.cuh"
@@ -54,13 +56,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// 16 bytes that no one else of the SM will read
-__device__ __forceinline__ uint4 load_once(const __nv_bfloat16* p) {
-  uint4 u;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
-  return u;
-}
-
 // 8 x 8 block of 16-bit values, lane 4 g + c holding (g, 2 c) and (g, 2 c + 1): the same of its transpose
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -68,15 +63,37 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ld_shared16(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// 16 keys and their values per stage of a warp's ring.
+template <int D>
+struct RowsShape {
+  static constexpr int kHalf = 16 * D * 2;                       // bytes of the keys of a stage
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kRing = kStages * 2 * kHalf;              // of a warp
+  static constexpr int kSmem = PR_WARPS * kRing;
+};
+
 // RB blocks of eight rows.
 template <int D, int RB>
-__global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_kernel(const __grid_constant__ RowsParams rp) {
+__global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __grid_constant__ RowsParams rp) {
   pdl_launch_dependents();
-  constexpr int NT = D == 64 ? 2 : 1;      // blocks of 16 keys per step
+  using Shape = RowsShape<D>;
+  constexpr int NS = Shape::kStages;
   constexpr int KC = D / 32;               // 16-byte pieces of a key per lane
   constexpr int VB = D / 64;               // and of a value
   constexpr int TM = 8 * RB;
-  __shared__ float o_s[PR_WARPS][TM][D + 4];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 ml_s[PR_WARPS][TM];
   const PrefixParams& p = rp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -93,6 +110,52 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
   const PagedTable& table = sp.own ? p.rows.table : p.prefix;
   const __nv_bfloat16* const kb = p.cache.k.p + head * p.cache.k.head;
   const __nv_bfloat16* const vb = p.cache.v.p + head * p.cache.v.head;
+  const int blocks = it.rows - it.rho0 > 8 ? RB : 1;  // that have rows
+
+  // The ring: the copies of a step are one group, a warp waits for its own.
+  constexpr int STEP = 16 * PR_WARPS;
+  constexpr int LANES = D / 8, KEYS = 32 / LANES;  // lanes per key, keys per copy instruction
+  const int piece = lane % LANES, sub = lane / LANES;
+  const uint32_t ring = smem_u32(smem) + warp * Shape::kRing;
+  int j_load = it.key0 + warp * 16, s_load = 0;
+  uint32_t there_ring[NS];  // of each stage: bit k: key k is there
+  auto fetch = [&](uint32_t& there) {  // the next 16 keys of this warp into stage s_load
+    int64_t k_off = -1, v_off = -1;
+    const int j = j_load + lane;
+    if (lane < 16 && j < it.keys) {
+      uint32_t index, slot;
+      p.cache.page_size.divmod(static_cast<uint32_t>(j), index, slot);
+      const int page = page_of(table, it.owner, index, p.cache.pages);
+      if (page >= 0) {
+        k_off = page * p.cache.k.page + slot * p.cache.k.token;
+        v_off = page * p.cache.v.page + slot * p.cache.v.token;
+      }
+    }
+    there = __ballot_sync(0xffffffffu, k_off >= 0);
+    const uint32_t dst = ring + s_load * 2 * Shape::kHalf;
+#pragma unroll
+    for (int i = 0; i < 16 / KEYS; ++i) {
+      const int key = i * KEYS + sub;
+      const int64_t o = __shfl_sync(0xffffffffu, k_off, key);
+      cp_async16(dst + key * (D * 2) + ((piece ^ ((key & 1) << 2)) << 4), kb + (o < 0 ? 0 : o) + piece * 8, o >= 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / KEYS; ++i) {
+      const int key = i * KEYS + sub;
+      const int64_t o = __shfl_sync(0xffffffffu, v_off, key);
+      cp_async16(dst + Shape::kHalf + key * (D * 2) + ((piece ^ (((key >> 1) & 3) << 1)) << 4), vb + (o < 0 ? 0 : o) + piece * 8, o >= 0);
+    }
+    j_load += STEP;
+    if (++s_load == NS) s_load = 0;
+  };
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    there_ring[i] = 0;
+    if (i < NS - 1) {
+      if (j_load < it.keys) fetch(there_ring[i]);
+      cp_async_commit();
+    }
+  }
 
   // queries: row 8 r + g, the pieces of this lane
   uint32_t q[RB][KC][4];
@@ -118,58 +181,6 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
       limit[r][e] = sp.own ? own_keys(p, it.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0 + 8 * r + 2 * c + e)))) : it.keys;
   if (sp.own) min_limit = own_keys(p, it.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0))));
 
-  constexpr int STEP = 16 * NT * PR_WARPS;
-  int j0 = it.key0 + warp * 16 * NT;
-  // lane l holds where key j0 + l (l < 16 NT) is, in elements of the two tensors; -1: not there
-  int64_t k_off, v_off;
-  auto locate = [&](int j) {
-    k_off = v_off = -1;
-    if (lane < 16 * NT && j + lane < it.keys) {
-      uint32_t index, slot;
-      p.cache.page_size.divmod(static_cast<uint32_t>(j + lane), index, slot);
-      const int page = page_of(table, it.owner, index, p.cache.pages);
-      if (page >= 0) {
-        k_off = page * p.cache.k.page + slot * p.cache.k.token;
-        v_off = page * p.cache.v.page + slot * p.cache.v.token;
-      }
-    }
-  };
-  uint32_t kr[NT][2][KC][4], vr[NT][4][VB][4];
-  uint32_t there = 0;  // bit 2 t + b: key 16 t + 8 b + g
-  auto load_k = [&]() {
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int64_t off = __shfl_sync(0xffffffffu, k_off, t * 16 + b * 8 + g);
-#pragma unroll
-        for (int i = 0; i < KC; ++i) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (off >= 0) u = load_once(kb + off + 8 * (c + 4 * i));
-          kr[t][b][i][0] = u.x; kr[t][b][i][1] = u.y; kr[t][b][i][2] = u.z; kr[t][b][i][3] = u.w;
-        }
-      }
-  };
-  auto load_v = [&]() {
-    there = 0;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-        if (__shfl_sync(0xffffffffu, v_off, t * 16 + b * 8 + g) >= 0) there |= 1u << (2 * t + b);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t off = __shfl_sync(0xffffffffu, v_off, t * 16 + 2 * c + (e & 1) + 8 * (e >> 1));
-#pragma unroll
-        for (int b = 0; b < VB; ++b) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (off >= 0) u = load_once(vb + off + 64 * b + 8 * g);
-          vr[t][e][b][0] = u.x; vr[t][e][b][1] = u.y; vr[t][e][b][2] = u.z; vr[t][e][b][3] = u.w;
-        }
-      }
-    }
-  };
-
   const float NEG_INF = __int_as_float(0xff800000);
   float m_ref[RB][2], l[RB][2], o[RB][VB][4][4];  // of rows 8 r + 2 c + e
 #pragma unroll
@@ -182,29 +193,27 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
       for (int j = 0; j < 4; ++j) o[r][b][j][0] = o[r][b][j][1] = o[r][b][j][2] = o[r][b][j][3] = 0.0f;
   }
 
-  if (j0 < it.keys) {
-    locate(j0);
-    load_k();
-    load_v();
-  }
-  for (; j0 < it.keys; j0 += STEP) {
-    float s[RB][NT][4];  // [2 b + e]: key 16 t + 8 b + g, row 8 r + 2 c + e
-    const bool more = j0 + STEP < it.keys;
-    if (more) locate(j0 + STEP);
+  // where this lane reads its fragments in a stage
+  const uint32_t k_at = g * (D * 2) + ((c ^ ((g & 1) << 2)) << 4);                                // keys g, g + 8: pieces c + 4 i
+  const uint32_t v_at = Shape::kHalf + 2 * c * (D * 2) + ((g ^ (c << 1)) << 4);                   // keys 2 c + e + 8 f: pieces g + 8 b
+  auto step = [&](const uint32_t there, const uint32_t at, const int j0) {
+    float s[RB][4];  // [2 b + e]: key 8 b + g, row 8 r + 2 c + e
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int r = 0; r < RB; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.0f;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        s[r][t][0] = s[r][t][1] = s[r][t][2] = s[r][t][3] = 0.0f;
+    for (int i = 0; i < KC; ++i) {
+      uint32_t k0[4], k1[4];
+      ld_shared16(at + (k_at ^ ((i & 1) << 6)) + (i >> 1) * 128, k0);
+      ld_shared16(at + (k_at ^ ((i & 1) << 6)) + (i >> 1) * 128 + 8 * (D * 2), k1);
 #pragma unroll
-        for (int i = 0; i < KC; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            mma_bf16_16816(s[r][t], kr[t][0][i][2 * h], kr[t][1][i][2 * h], kr[t][0][i][2 * h + 1], kr[t][1][i][2 * h + 1], q[r][i][2 * h], q[r][i][2 * h + 1]);
-      }
-    if (more) load_k();
+      for (int r = 0; r < RB; ++r)
+        if (r < blocks) {
+          mma_bf16_16816(s[r], k0[0], k1[0], k0[1], k1[1], q[r][i][0], q[r][i][1]);
+          mma_bf16_16816(s[r], k0[2], k1[2], k0[3], k1[3], q[r][i][2], q[r][i][3]);
+        }
+    }
     // scores in units of log2; keys that are not there or that the row does not see count as -inf
-    const bool edge = j0 + 16 * NT > min_limit;
+    const bool edge = j0 + 16 > min_limit;
     bool moves = false;
     float mx[RB][2];
 #pragma unroll
@@ -213,15 +222,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
       for (int e = 0; e < 2; ++e) {
         mx[r][e] = NEG_INF;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            bool seen = (there >> (2 * t + b)) & 1;
-            if (edge) seen = seen && j0 + 16 * t + 8 * b + g < limit[r][e];
-            const float x = seen ? s[r][t][2 * b + e] * p.scale2 : NEG_INF;
-            s[r][t][2 * b + e] = x;
-            mx[r][e] = fmaxf(mx[r][e], x);
-          }
+        for (int b = 0; b < 2; ++b) {
+          bool seen = (there >> (8 * b + g)) & 1;
+          if (edge) seen = seen && j0 + 8 * b + g < limit[r][e];
+          const float x = seen ? s[r][2 * b + e] * p.scale2 : NEG_INF;
+          s[r][2 * b + e] = x;
+          mx[r][e] = fmaxf(mx[r][e], x);
+        }
         moves = moves || mx[r][e] > m_ref[r][e] + 8.0f;
       }
     if (__any_sync(0xffffffffu, moves)) {
@@ -244,35 +251,55 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
             }
         }
     }
-    uint32_t pt[RB][NT][2];  // P^T as B fragments
+    uint32_t pt[RB][2];  // P^T as B fragments
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const float ref0 = m_ref[r][0] == NEG_INF ? 0.0f : m_ref[r][0], ref1 = m_ref[r][1] == NEG_INF ? 0.0f : m_ref[r][1];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float x0 = ex2(s[r][t][2 * b] - ref0), x1 = ex2(s[r][t][2 * b + 1] - ref1);
-          l[r][0] += x0;
-          l[r][1] += x1;
-          pt[r][t][b] = transpose8x8(pack_bf16(x0, x1));
-        }
+      for (int b = 0; b < 2; ++b) {
+        const float x0 = ex2(s[r][2 * b] - ref0), x1 = ex2(s[r][2 * b + 1] - ref1);
+        l[r][0] += x0;
+        l[r][1] += x1;
+        pt[r][b] = transpose8x8(pack_bf16(x0, x1));
+      }
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int b = 0; b < VB; ++b) {
+      uint32_t v[4][4];
 #pragma unroll
-      for (int b = 0; b < VB; ++b)
+      for (int e = 0; e < 4; ++e) ld_shared16(at + v_at + b * 128 + ((e & 1) + 8 * (e >> 1)) * (D * 2), v[e]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t a0 = __byte_perm(vr[t][0][b][j], vr[t][1][b][j], 0x5410), a1 = __byte_perm(vr[t][0][b][j], vr[t][1][b][j], 0x7632);
-          const uint32_t a2 = __byte_perm(vr[t][2][b][j], vr[t][3][b][j], 0x5410), a3 = __byte_perm(vr[t][2][b][j], vr[t][3][b][j], 0x7632);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5410), a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
+        const uint32_t a2 = __byte_perm(v[2][j], v[3][j], 0x5410), a3 = __byte_perm(v[2][j], v[3][j], 0x7632);
 #pragma unroll
-          for (int r = 0; r < RB; ++r) mma_bf16_16816(o[r][b][j], a0, a1, a2, a3, pt[r][t][0], pt[r][t][1]);
-        }
-    if (more) load_v();
+        for (int r = 0; r < RB; ++r)
+          if (r < blocks) mma_bf16_16816(o[r][b][j], a0, a1, a2, a3, pt[r][0], pt[r][1]);
+      }
+    }
+  };
+  int j0 = it.key0 + warp * 16;
+  for (;;) {
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if (j0 >= it.keys) { done = true; break; }
+      cp_async_wait<NS - 2>();
+      __syncwarp();
+      // the stage behind (that of the step before, which every lane has read) is filled again
+      if (j_load < it.keys) fetch(there_ring[(i + NS - 1) % NS]);
+      cp_async_commit();
+      step(there_ring[i], ring + i * 2 * Shape::kHalf, j0);
+      j0 += STEP;
+    }
+    if (done) break;
   }
+  __syncthreads();  // every warp is done with its ring: the sums go there
 
   // the four warps' parts of a row
+  constexpr int PITCH = D + 4;
+  static_assert(PR_WARPS * TM * PITCH * 4 <= Shape::kSmem, "the sums fit in the rings");
+  float* const o_s = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int r = 0; r < RB; ++r)
 #pragma unroll
@@ -283,7 +310,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
       if (g == 0) ml_s[warp][lr] = make_float2(m_ref[r][e], l[r][e]);
 #pragma unroll
       for (int b = 0; b < VB; ++b) {  // columns 64 b + 8 g + 2 j + {0, 1}
-        float* dst = &o_s[warp][lr][64 * b + 8 * g];
+        float* dst = o_s + (warp * TM + lr) * PITCH + 64 * b + 8 * g;
         reinterpret_cast<float4*>(dst)[0] = make_float4(o[r][b][0][e], o[r][b][0][2 + e], o[r][b][1][e], o[r][b][1][2 + e]);
         reinterpret_cast<float4*>(dst)[1] = make_float4(o[r][b][2][e], o[r][b][2][2 + e], o[r][b][3][e], o[r][b][3][2 + e]);
       }
@@ -301,7 +328,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
 #pragma unroll
     for (int w = 0; w < PR_WARPS; ++w) {
       const float a = ex2(ml_s[w][lr].x - ref);
-      const float4 x = *reinterpret_cast<const float4*>(&o_s[w][lr][col]);
+      const float4 x = *reinterpret_cast<const float4*>(o_s + (w * TM + lr) * PITCH + col);
       sum += a * ml_s[w][lr].y;
       acc.x += a * x.x; acc.y += a * x.y; acc.z += a * x.z; acc.w += a * x.w;
     }
@@ -312,6 +339,20 @@ __global__ void __launch_bounds__(PR_WARPS * 32, RB == 1 ? 3 : 2) prefix_rows_ke
     if (col == 0) p.part_ml[at] = make_float2(m, sum);
     *reinterpret_cast<float4*>(p.part_o + at * D + col) = acc;
   }
+}
+
+template <int D, int RB>
+int launch_rows(const RowsParams& rp, int64_t items, cudaStream_t st) {
+  int dev = 0;
+  VX_CUDA_OK(cudaGetDevice(&dev));
+  static std::atomic<uint64_t> attr_done{0};
+  const bool cached = dev >= 0 && dev < 64;
+  if (!cached || !(attr_done.load(std::memory_order_acquire) & (1ull << dev))) {
+    VX_CUDA_OK(cudaFuncSetAttribute(prefix_rows_kernel<D, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsShape<D>::kSmem));
+    if (cached) attr_done.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  VX_CUDA_OK(launch_dependent(prefix_rows_kernel<D, RB>, dim3(static_cast<unsigned>(items)), dim3(PR_WARPS * 32), RowsShape<D>::kSmem, st, rp));
+  return 0;
 }
 
 // The parts of every row joined, and zeros for the rows that have none.  One block per row and 1,024 values of it.
@@ -431,7 +472,7 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     sp.slots = static_cast<int32_t>(sp.equal ? owners * sp.equal : R * per / tm + owners);
     const int64_t items = static_cast<int64_t>(sp.slots) * p.kv_heads;
     if (tiles) sp.chunk = chunk_keys(cap, items, sm_count(), 256, 1024, 4);
-    else sp.chunk = chunk_keys(cap, items, static_cast<int64_t>(sm_count()) * (plan.blocks == 1 ? 3 : 2), cache->head_dim == 64 ? 128 : 64, 256, 8);
+    else sp.chunk = chunk_keys(cap, items, 2 * static_cast<int64_t>(sm_count()), 16 * PR_WARPS, cache->head_dim == 64 ? 512 : 256, 8);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
   cut(plan.prefix, 0, plan.prefix_tiles, G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
@@ -484,10 +525,9 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
     const int64_t items = first + static_cast<int64_t>(rp.span[1].slots) * rp.span[1].chunks * p.kv_heads;
     if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
     rp.first_items = static_cast<int32_t>(first);
-    const dim3 grid(static_cast<unsigned>(items)), block(PR_WARPS * 32);
-    auto kernel = d64 ? (plan.blocks == 2 ? prefix_rows_kernel<64, 2> : prefix_rows_kernel<64, 1>)
-                      : (plan.blocks == 2 ? prefix_rows_kernel<128, 2> : prefix_rows_kernel<128, 1>);
-    VX_CUDA_OK(launch_dependent(kernel, grid, block, 0, st, rp));
+    const int e = d64 ? (plan.blocks == 2 ? launch_rows<64, 2>(rp, items, st) : launch_rows<64, 1>(rp, items, st))
+                      : (plan.blocks == 2 ? launch_rows<128, 2>(rp, items, st) : launch_rows<128, 1>(rp, items, st));
+    if (e) return e;
   }
   JoinParams jp{p, {plan.prefix, plan.own}};
   const dim3 grid(static_cast<unsigned>(p.rows.rows), static_cast<unsigned>((p.q_heads * cache->head_dim + 1023) / 1024));
