@@ -1,11 +1,11 @@
 // Attention over shared prefixes and own tokens: how the work is cut, for the kernels that do the parts of it (vx_prefix_attn.cu,
 // vx_prefix_tiles.cu).
 //
-// A SPAN is one kind of keys: those of the groups' prefixes, or the sequences' own tokens.  Its owners (groups, sequences) have runs of
-// rows; row rho of an owner and a key head stands for token rho / per_kv of its run and query head rho % per_kv, so that all query
-// heads that share a key head read its keys together.  Rows are cut into tiles of TM, keys into chunks.  An item is one tile, one
-// chunk and one key head; it leaves (m, l, O) of its rows -- maximum, sum of 2^(x - m), sum of 2^(x - m) v, with x = scale log2(e) q.k --
-// as part `part0 + chunk` in scratch, from which a last kernel joins the parts of a row:
+// A SPAN is one kind of keys: those of the groups' prefixes, the sequences' own tokens, or both in a row (joint).  Its owners (groups,
+// sequences, sequences) have runs of rows; row rho of an owner and a key head stands for token rho / per_kv of its run and query head
+// rho % per_kv, so that all query heads that share a key head read its keys together.  Rows are cut into tiles, keys into chunks.  An
+// item is one tile, one chunk and one key head; it leaves (m, l, O) of its rows -- maximum, sum of 2^(x - m), sum of 2^(x - m) v, with
+// x = scale log2(e) q.k -- as part `part0 + chunk` in scratch, from which a last kernel joins the parts of a row:
 //   out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c,  m = max_c m_c.
 // The number of chunks is fixed on the host from the width of the tables; how many of them hold keys is known on the device only, and
 // both sides derive it from the same lengths, so empty parts are neither written nor read.
@@ -34,31 +34,29 @@ struct PrefixParams {
   int* status;
 };
 
+enum SpanKind : int32_t { kSpanPrefix = 0, kSpanOwn = 1, kSpanJoint = 2 };
+constexpr int kSpanAlign = 128;  // own keys of a joint span begin at the next multiple of this behind the prefix
+
 // One span as a kernel walks it.
 struct Span {
-  int32_t own;        // 1: own tokens, 0: prefixes
+  int32_t kind;
   int32_t slots;      // row tiles there can be; a slot without rows is skipped
   int32_t equal;      // tiles per owner where all have as many rows; 0: found from the offsets
   int32_t chunk;      // keys per chunk
   int32_t chunks;     // 0: the span is not walked
-  int32_t part0;      // first part in scratch
+  int32_t part0;      // first part in scratch; -1: the only part there is, its rows go to `out`
 };
+constexpr Span kNoSpan{0, 1, 1, 1, 0, 0};
 
-// Rows [first, first + n) of an owner, in tokens.
-struct OwnerRows {
-  int first, n;
-};
 __device__ __forceinline__ int sequence_row0(const PrefixParams& p, int s) {
   return p.rows.row_offsets ? min(max(p.rows.row_offsets[s], 0), p.rows.rows) : s;
 }
 __device__ __forceinline__ int group_sequence0(const PrefixParams& p, int g) {
   return p.group_offsets ? min(max(p.group_offsets[g], 0), p.rows.sequences) : g * p.group_size;
 }
-// first row of owner o (0 ... owners: the end of the last)
-__device__ __forceinline__ int owner_row0(const PrefixParams& p, bool own, int o) {
-  int s = own ? o : group_sequence0(p, o);
-  if (!p.rows.row_offsets) return s;
-  return sequence_row0(p, s);
+// first row of owner o (o = number of owners: the end of the last)
+__device__ __forceinline__ int owner_row0(const PrefixParams& p, bool sequences, int o) {
+  return sequence_row0(p, sequences ? o : group_sequence0(p, o));
 }
 
 // group of a sequence, -1: none
@@ -72,34 +70,34 @@ __device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
 // Keys of the prefix of group g, and own keys that a token of index i of its sequence sees: as far as the tables reach.
 __device__ __forceinline__ int prefix_keys(const PrefixParams& p, int g) {
   const int cap = p.prefix.pages * static_cast<int>(p.cache.page_size.d);
-  return min(max(p.prefix_lengths[g], 0), cap);
+  return g < 0 ? 0 : min(max(p.prefix_lengths[g], 0), cap);
 }
 __device__ __forceinline__ int own_keys(const PrefixParams& p, int length, int i) {
   const int cap = p.rows.table.pages * static_cast<int>(p.cache.page_size.d);
   return length < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(length) + i + 1, static_cast<int64_t>(cap)));
 }
+__device__ __forceinline__ int align_keys(int n) { return (n + kSpanAlign - 1) / kSpanAlign * kSpanAlign; }
 
-// What one item works on.
-struct Item {
+// Rows of an item.
+struct ItemRows {
   int owner;
   int row0, rows;   // first token of the owner's run, rows (token, head of the key head's group) of the run
   int rho0;         // first row of the tile
-  int key0, keys;   // keys [key0, keys) of the owner (keys: what the tile's last row sees)
-  int length;       // own span: tokens before the run
 };
 
 // Owner and tile of a slot.  With offsets, owner o has the slots [base(o), base(o + 1)), base(o) = floor(row0(o) per_kv / TM) + o: enough for
 // its tiles, and found by a search without a pass over all owners.
 template <int TM>
-__device__ __forceinline__ bool find_item(const PrefixParams& p, const Span& sp, int slot, int chunk, Item& it) {
+__device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp, int slot, ItemRows& it) {
   const int per = static_cast<int>(p.per_kv.d);
-  const int owners = sp.own ? p.rows.sequences : p.groups;
+  const bool sequences = sp.kind != kSpanPrefix;
+  const int owners = sequences ? p.rows.sequences : p.groups;
   int tile;
   if (sp.equal) {
     it.owner = slot / sp.equal;
     tile = slot - it.owner * sp.equal;
   } else {
-    auto base = [&](int o) { return static_cast<int>(static_cast<int64_t>(owner_row0(p, sp.own, o)) * per / TM) + o; };
+    auto base = [&](int o) { return static_cast<int>(static_cast<int64_t>(owner_row0(p, sequences, o)) * per / TM) + o; };
     int lo = 0, hi = owners;  // largest o with base(o) <= slot
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -110,29 +108,15 @@ __device__ __forceinline__ bool find_item(const PrefixParams& p, const Span& sp,
     tile = slot - base(lo);
   }
   if (it.owner >= owners || tile < 0) return false;
-  it.row0 = owner_row0(p, sp.own, it.owner);
-  const int n = owner_row0(p, sp.own, it.owner + 1) - it.row0;
+  it.row0 = owner_row0(p, sequences, it.owner);
+  const int n = owner_row0(p, sequences, it.owner + 1) - it.row0;
   it.rows = n * per;
   it.rho0 = tile * TM;
-  if (n <= 0 || it.rho0 >= it.rows) return false;
-  if (sp.own) {
-    it.length = p.rows.lengths[it.owner];
-    const int last = min(it.rho0 + TM, it.rows) - 1;
-    it.keys = own_keys(p, it.length, static_cast<int>(p.per_kv.div(last)));
-  } else {
-    it.length = 0;
-    it.keys = prefix_keys(p, it.owner);
-  }
-  const int64_t k0 = static_cast<int64_t>(chunk) * sp.chunk;
-  if (k0 >= it.keys) return false;
-  it.key0 = static_cast<int>(k0);
-  it.keys = static_cast<int>(min(static_cast<int64_t>(it.keys), k0 + sp.chunk));
-  return true;
+  return n > 0 && it.rho0 < it.rows;
 }
 
-constexpr int kTileRows = 256;  // rows that a CTA of prefix_tiles_kernel takes
-
 // Launches prefix_tiles_kernel on the spans that have chunks.
-int launch_prefix_tiles(const PrefixParams& p, int head_dim, const Span& prefix, const Span& own, void* stream);
+constexpr int kSlotRows = 128;  // rows of a slot of prefix_tiles_kernel
+int launch_prefix_tiles(const PrefixParams& p, int head_dim, bool paired, const Span& first, const Span& second, void* stream);
 
 }  // namespace vx

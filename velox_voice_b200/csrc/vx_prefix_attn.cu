@@ -105,9 +105,16 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
   const int head = n % p.kv_heads;  // heads of a token lie next to each other
   n /= p.kv_heads;
   const int chunk = n / sp.slots;
-  Item it;
-  if (!find_item<TM>(p, sp, n - chunk * sp.slots, chunk, it)) return;
-  const PagedTable& table = sp.own ? p.rows.table : p.prefix;
+  const bool own = sp.kind == kSpanOwn;
+  ItemRows it;
+  if (!find_rows<TM>(p, sp, n - chunk * sp.slots, it)) return;
+  const int length = own ? p.rows.lengths[it.owner] : 0;
+  // keys [key0, keys): those of the chunk that the tile's last row sees
+  int keys = own ? own_keys(p, length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(min(it.rho0 + TM, it.rows) - 1)))) : prefix_keys(p, it.owner);
+  if (static_cast<int64_t>(chunk) * sp.chunk >= keys) return;
+  const int key0 = chunk * sp.chunk;
+  keys = static_cast<int>(min(static_cast<int64_t>(keys), static_cast<int64_t>(key0) + sp.chunk));
+  const PagedTable& table = own ? p.rows.table : p.prefix;
   const __nv_bfloat16* const kb = p.cache.k.p + head * p.cache.k.head;
   const __nv_bfloat16* const vb = p.cache.v.p + head * p.cache.v.head;
   const int blocks = it.rows - it.rho0 > 8 ? RB : 1;  // that have rows
@@ -117,12 +124,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
   constexpr int LANES = D / 8, KEYS = 32 / LANES;  // lanes per key, keys per copy instruction
   const int piece = lane % LANES, sub = lane / LANES;
   const uint32_t ring = smem_u32(smem) + warp * Shape::kRing;
-  int j_load = it.key0 + warp * 16, s_load = 0;
+  int j_load = key0 + warp * 16, s_load = 0;
   uint32_t there_ring[NS];  // of each stage: bit k: key k is there
   auto fetch = [&](uint32_t& there) {  // the next 16 keys of this warp into stage s_load
     int64_t k_off = -1, v_off = -1;
     const int j = j_load + lane;
-    if (lane < 16 && j < it.keys) {
+    if (lane < 16 && j < keys) {
       uint32_t index, slot;
       p.cache.page_size.divmod(static_cast<uint32_t>(j), index, slot);
       const int page = page_of(table, it.owner, index, p.cache.pages);
@@ -152,7 +159,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
   for (int i = 0; i < NS; ++i) {
     there_ring[i] = 0;
     if (i < NS - 1) {
-      if (j_load < it.keys) fetch(there_ring[i]);
+      if (j_load < keys) fetch(there_ring[i]);
       cp_async_commit();
     }
   }
@@ -173,13 +180,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
     }
   }
   // keys that row 8 r + 2 c + e sees; the first row of the tile sees fewest
-  int limit[RB][2], min_limit = it.keys;
+  int limit[RB][2], min_limit = keys;
 #pragma unroll
   for (int r = 0; r < RB; ++r)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      limit[r][e] = sp.own ? own_keys(p, it.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0 + 8 * r + 2 * c + e)))) : it.keys;
-  if (sp.own) min_limit = own_keys(p, it.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0))));
+      limit[r][e] = own ? own_keys(p, length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0 + 8 * r + 2 * c + e)))) : keys;
+  if (own) min_limit = own_keys(p, length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0))));
 
   const float NEG_INF = __int_as_float(0xff800000);
   float m_ref[RB][2], l[RB][2], o[RB][VB][4][4];  // of rows 8 r + 2 c + e
@@ -278,16 +285,16 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
       }
     }
   };
-  int j0 = it.key0 + warp * 16;
+  int j0 = key0 + warp * 16;
   for (;;) {
     bool done = false;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      if (j0 >= it.keys) { done = true; break; }
+      if (j0 >= keys) { done = true; break; }
       cp_async_wait<NS - 2>();
       __syncwarp();
       // the stage behind (that of the step before, which every lane has read) is filled again
-      if (j_load < it.keys) fetch(there_ring[(i + NS - 1) % NS]);
+      if (j_load < keys) fetch(there_ring[(i + NS - 1) % NS]);
       cp_async_commit();
       step(there_ring[i], ring + i * 2 * Shape::kHalf, j0);
       j0 += STEP;
@@ -358,7 +365,7 @@ int launch_rows(const RowsParams& rp, int64_t items, cudaStream_t st) {
 // The parts of every row joined, and zeros for the rows that have none.  One block per row and 1,024 values of it.
 struct JoinParams {
   PrefixParams p;
-  Span span[2];  // prefix, own
+  Span span[2];
 };
 template <int D>
 __global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant__ JoinParams jp) {
@@ -371,9 +378,14 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant_
   const int h = col / D, d = col % D;
   int parts[2] = {0, 0}, s, i;
   if (row_sequence(p.rows, row, s, i)) {
-    const int g = group_of(p, s);
-    if (g >= 0 && jp.span[0].chunks) parts[0] = (prefix_keys(p, g) + jp.span[0].chunk - 1) / jp.span[0].chunk;
-    if (jp.span[1].chunks) parts[1] = (own_keys(p, p.rows.lengths[s], i) + jp.span[1].chunk - 1) / jp.span[1].chunk;
+    if (jp.span[0].part0 < 0) return;  // its row is there already
+    const int prefix = prefix_keys(p, group_of(p, s)), own = own_keys(p, p.rows.lengths[s], i);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const Span& sp = jp.span[e];
+      const int64_t keys = sp.kind == kSpanPrefix ? prefix : (sp.kind == kSpanOwn ? own : static_cast<int64_t>(align_keys(prefix)) + own);
+      if (sp.chunks) parts[e] = static_cast<int>((keys + sp.chunk - 1) / sp.chunk);
+    }
   }
   const int64_t at = static_cast<int64_t>(row) * p.q_heads + h, step = static_cast<int64_t>(p.rows.rows) * p.q_heads;
   const float NEG_INF = __int_as_float(0xff800000);
@@ -401,9 +413,9 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const __grid_constant_
 }
 
 struct Plan {
-  Span prefix, own;
-  bool prefix_tiles, own_tiles;  // which kernel walks the span
-  int blocks;                    // of eight rows, of the kernel for few rows
+  Span span[2];
+  enum Kernel { kRows, kTiles, kPairs } kernel[2];  // that walks the span
+  int blocks;                                       // of eight rows, of the kernel for few rows
   int parts;
   int64_t ml_bytes, bytes;
 };
@@ -456,31 +468,41 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
 
   plan = Plan{};
   const int64_t R = rows->rows, S = rows->sequences, G = d->groups;
-  if (R == 0 || S == 0) return 0;
+  plan.span[0] = plan.span[1] = kNoSpan;
+  if (R == 0 || S == 0 || cache->pages == 0) return 0;  // no key anywhere
   const int64_t cap_p = G > 0 ? d->prefix_pages * cache->page_size : 0, cap_o = rows->table_pages * cache->page_size;
   // The kernel of a span goes by its rows per owner and key head, on the average (which kernel takes a row changes no result beyond rounding).
   const bool single = !rows->row_offsets;
   const int64_t rows_p = cap_p > 0 ? R * per / G : 0, rows_o = cap_o > 0 ? R * per / S : 0;
-  plan.prefix_tiles = rows_p > kRowsKernel;
-  plan.own_tiles = rows_o > kRowsKernel;
-  plan.blocks = (!plan.prefix_tiles && rows_p > 8) || (!plan.own_tiles && rows_o > 8) ? 2 : 1;
-  auto cut = [&](Span& sp, int own, bool tiles, int64_t owners, int64_t cap, int64_t equal_rows) {
+  auto cut = [&](Span& sp, SpanKind kind, Plan::Kernel kernel, int64_t owners, int64_t cap, int64_t equal_rows) {
     if (cap <= 0 || owners <= 0) return;
-    const int tm = tiles ? kTileRows : 8 * plan.blocks;
-    sp.own = own;
+    const int tm = kernel == Plan::kPairs ? 2 * kSlotRows : (kernel == Plan::kTiles ? kSlotRows : 8 * plan.blocks);
+    sp.kind = kind;
     sp.equal = equal_rows > 0 ? static_cast<int32_t>((equal_rows + tm - 1) / tm) : 0;
     sp.slots = static_cast<int32_t>(sp.equal ? owners * sp.equal : R * per / tm + owners);
-    const int64_t items = static_cast<int64_t>(sp.slots) * p.kv_heads;
-    if (tiles) sp.chunk = chunk_keys(cap, items, sm_count(), 256, 1024, 4);
-    else sp.chunk = chunk_keys(cap, items, 2 * static_cast<int64_t>(sm_count()), 16 * PR_WARPS, cache->head_dim == 64 ? 512 : 256, 8);
+    const int64_t items = static_cast<int64_t>(sp.slots) * p.kv_heads, sms = sm_count();
+    if (kernel == Plan::kPairs) sp.chunk = chunk_keys(cap, items, sms, 256, 1024, 4);
+    else if (kernel == Plan::kTiles) sp.chunk = chunk_keys(cap, items, 2 * sms, 128, 512, owners == 1 ? 1 : 2);
+    else sp.chunk = chunk_keys(cap, items, 2 * sms, 16 * PR_WARPS, cache->head_dim == 64 ? 512 : 256, 8);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
-  cut(plan.prefix, 0, plan.prefix_tiles, G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
-  cut(plan.own, 1, plan.own_tiles, S, cap_o, single ? per : 0);
-  plan.own.part0 = plan.prefix.chunks;
-  plan.parts = plan.prefix.chunks + plan.own.chunks;
+  plan.span[0] = plan.span[1] = kNoSpan;
+  if (rows_o > kSlotRows) {
+    // whole prompts or long chunks: prefix and own tokens in a row, no joining of the two
+    plan.kernel[0] = plan.kernel[1] = Plan::kPairs;
+    cut(plan.span[0], kSpanJoint, Plan::kPairs, S, round_up(cap_p, kSpanAlign) + cap_o, single ? per : 0);
+    if (plan.span[0].chunks == 1) plan.span[0].part0 = -1;
+  } else {
+    plan.kernel[0] = rows_p > 2 * kSlotRows ? Plan::kPairs : (rows_p <= kRowsKernel ? Plan::kRows : Plan::kTiles);
+    plan.kernel[1] = rows_o <= kRowsKernel ? Plan::kRows : Plan::kTiles;
+    plan.blocks = (plan.kernel[0] == Plan::kRows && rows_p > 8) || (plan.kernel[1] == Plan::kRows && rows_o > 8) ? 2 : 1;
+    cut(plan.span[0], kSpanPrefix, plan.kernel[0], G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
+    cut(plan.span[1], kSpanOwn, plan.kernel[1], S, cap_o, single ? per : 0);
+    plan.span[1].part0 = plan.span[0].chunks;
+  }
+  plan.parts = plan.span[0].part0 < 0 ? 0 : plan.span[0].chunks + plan.span[1].chunks;
   const int64_t cells = R * d->q_heads;
-  plan.ml_bytes = (plan.parts * cells * 8 + 15) / 16 * 16;
+  plan.ml_bytes = round_up(plan.parts * cells * 8, 32);
   plan.bytes = plan.ml_bytes + plan.parts * cells * cache->head_dim * 4;
   return 0;
 }
@@ -505,22 +527,24 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
   if (p.rows.rows == 0) return 0;
   if (!d->q || !d->out) return fail(-1, "q and out must not be NULL");
   if (!pieces_ok(d->q, d->q_row, d->q_head, 2) || !pieces_ok(d->out, d->o_row, d->o_head, 2)) return fail(-1, "rows and heads of q and out must be 16-byte aligned");
-  if (plan.bytes > 0 && (!d->scratch || !aligned16(d->scratch) || d->scratch_bytes < plan.bytes))
-    return fail(-1, "scratch must be %lld bytes, 16-byte aligned", (long long)plan.bytes);
+  if (plan.bytes > 0 && (!d->scratch || (reinterpret_cast<uintptr_t>(d->scratch) & 31) != 0 || d->scratch_bytes < plan.bytes))
+    return fail(-1, "scratch must be %lld bytes, 32-byte aligned", (long long)plan.bytes);
   p.q = static_cast<const __nv_bfloat16*>(d->q); p.q_row = d->q_row; p.q_head = d->q_head;
   p.out = static_cast<__nv_bfloat16*>(d->out); p.o_row = d->o_row; p.o_head = d->o_head;
   p.part_ml = static_cast<float2*>(d->scratch);
   p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d->scratch) + plan.ml_bytes);
   const auto st = static_cast<cudaStream_t>(stream);
   const bool d64 = cache->head_dim == 64;
-  const Span none{0, 1, 1, 1, 0, 0};
   p.status = device_status_ptr();
-  if (plan.prefix_tiles || plan.own_tiles) {
-    const int e = launch_prefix_tiles(p, cache->head_dim, plan.prefix_tiles ? plan.prefix : none, plan.own_tiles ? plan.own : none, stream);
-    if (e) return e;
-  }
-  if ((!plan.prefix_tiles && plan.prefix.chunks > 0) || (!plan.own_tiles && plan.own.chunks > 0)) {
-    RowsParams rp{p, {plan.prefix_tiles ? none : plan.prefix, plan.own_tiles ? none : plan.own}, 0};
+  auto part = [&](Plan::Kernel k, int i) { return plan.kernel[i] == k ? plan.span[i] : kNoSpan; };  // the span, where kernel k walks it
+  auto walks = [&](Plan::Kernel k) { return part(k, 0).chunks > 0 || part(k, 1).chunks > 0; };
+  for (const Plan::Kernel k : {Plan::kPairs, Plan::kTiles})
+    if (walks(k)) {
+      const int e = launch_prefix_tiles(p, cache->head_dim, k == Plan::kPairs, part(k, 0), part(k, 1), stream);
+      if (e) return e;
+    }
+  if (walks(Plan::kRows)) {
+    RowsParams rp{p, {part(Plan::kRows, 0), part(Plan::kRows, 1)}, 0};
     const int64_t first = static_cast<int64_t>(rp.span[0].slots) * rp.span[0].chunks * p.kv_heads;
     const int64_t items = first + static_cast<int64_t>(rp.span[1].slots) * rp.span[1].chunks * p.kv_heads;
     if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
@@ -529,7 +553,7 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
                       : (plan.blocks == 2 ? launch_rows<128, 2>(rp, items, st) : launch_rows<128, 1>(rp, items, st));
     if (e) return e;
   }
-  JoinParams jp{p, {plan.prefix, plan.own}};
+  JoinParams jp{p, {plan.span[0], plan.span[1]}};
   const dim3 grid(static_cast<unsigned>(p.rows.rows), static_cast<unsigned>((p.q_heads * cache->head_dim + 1023) / 1024));
   const int threads = p.q_heads * cache->head_dim >= 1024 ? 256 : (p.q_heads * cache->head_dim / 4 + 31) / 32 * 32;
   auto join = d64 ? prefix_join_kernel<64> : prefix_join_kernel<128>;

@@ -1,16 +1,29 @@
-// Attention over shared prefixes and own tokens for many rows per owner and key head, on the 5th-generation tensor cores (the cut of the
-// work: vx_prefix.cuh; few rows: vx_prefix_attn.cu).
+// Attention over shared prefixes and own tokens on the 5th-generation tensor cores (the cut of the work: vx_prefix.cuh; few rows and keys:
+// vx_prefix_attn.cu).
 //
-// A CTA takes up to 256 rows of one owner and key head against one chunk of keys, in tiles of 128 keys, as two SLOTS of 128 rows with
-// tensor memory of their own: S = Q K^T (128 x 128, fp32), P (bf16, over S) and O (128 x head_dim).  While the softmax of one slot works, the
-// tensor cores have the products of the other.  With 128 rows or fewer both slots hold the same rows and take the key tiles in turn; their
-// two results are joined through shared memory at the end.
+// One CTA per SM goes through its items.  It has two SLOTS of 128 rows with tensor memory of their own; while the softmax of one slot works,
+// the tensor cores have the products of the other.
+//   PAIRED     both slots take one item of 256 rows, 128 keys a tile: every K and V tile is loaded once for both.  For many rows per owner,
+//              where the products are the bound.  Tensor memory of a slot: S (128 columns, P in bf16 over it) | O (head_dim).
+//   otherwise  each slot has a stream of items of its own, 64 keys a tile, and the tiles of the two take turns.  For few rows, where the keys'
+//              bytes are the bound: smaller tiles hold less of the shared memory while their softmax runs, so more of it is for copies in
+//              flight (with tiles of 128 keys a third of the time was lost), and S is double-buffered, so that the softmax of a slot
+//              finds its next S.  Tensor memory of a slot: S0 | S1 (64 columns each, P over them) | O.
+// Roles:
 //   warps 0..3, 4..7  softmax of slot 0, 1: a query row per thread straight out of tensor memory
-//   warps 8..11       loaders: 32 keys of every tile each, page by page (cp.async, 16 bytes; keys that are not there are filled with zeros
-//                     and marked in a word per 32 keys)
-//   warp 12           MMA issuer
+//   warps 8..11       loaders: a quarter of every tile's keys each, page by page (cp.async, 16 bytes; keys that are not there are filled with
+//                     zeros and marked in a bit mask), K and V into rings of their own in the order K0, K1, V0, K2, V1, ...
+//   warps 12, 15      MMA issuers.  A thread that issues is held while its products run, so the slots of two streams have one each: what it
+//                     has to wait for and to look up between two tiles passes under the other's products (one issuer for both spent 60 % of its
+//                     time between products).  PAIRED has one for both slots, whose products must not mix: two issuers without turns
+//                     took 27 % longer, with turns 8 %.
+//   warps 13, 14      one per stream of items: looks 32 items up at a time, a lane each, hands them to the other roles through a ring
+//                     and loads their queries
+// All roles run on into the next item as far as their rings and buffers let them, so that what an item costs to begin (its place in the tables,
+// its queries, its first keys) passes under the one before it.
 // Q, K and V lie in shared memory in rows of 128 bytes with the 128-byte swizzle, 64 columns a panel; V is read as an MN-major operand.
-// P is the A operand in tensor memory, so that shared memory is read for K, Q and V only.
+// P is the A operand in tensor memory, so that shared memory is read for K, Q and V only.  S of a tile is issued behind the P V product that
+// reads P from the same columns, by the same thread: the tensor cores take its products in order.
 // The reference maximum of a row moves only when a tile's maximum exceeds it by more than 8 in units of log2 (probabilities stay below
 // 2^8); then the row's sum and its O are scaled before P is handed over.
 // Every wait on a barrier is bounded.
@@ -29,32 +42,49 @@
 namespace vx {
 namespace {
 
-constexpr int PT_BN = 128;                 // keys per tile
-constexpr int PT_PANEL = 128 * 128;        // 128 rows of 64 bf16
-constexpr int PT_THREADS = 16 * 32;         // (warps 13..15 only fill the fourth warpgroup)
-constexpr int PT_MASKS = 8;                // tiles whose masks are kept
+constexpr int PT_THREADS = 16 * 32;
+constexpr int PT_MASKS = 16;               // tiles of a stream whose masks are kept: more than a ring of keys holds and a slot has begun
+constexpr int PT_ITEMS = 4;                // items of a stream that are known ahead
+constexpr int PT_Q_PANEL = kSlotRows * 128;  // 64 bf16 of every row
 constexpr uint32_t PT_TM_SLOT = 256, PT_TM_O = 128, PT_TM_COLS = 512;
 
-template <int D>
+template <int D, bool PAIRED>
 struct TileShape {
-  static constexpr int kPanels = D / 64;
-  static constexpr int kTile = kPanels * PT_PANEL;   // bytes of a K or V tile and of a slot's Q
-  static constexpr int kStages = D == 128 ? 5 : 10;
-  static constexpr int kSmem = (2 + kStages) * kTile + 1024;
+  static constexpr int kKeys = PAIRED ? 128 : 64;
+  static constexpr int kBuffers = PAIRED ? 1 : 2;             // of S
+  static constexpr int kPanel = kKeys * 128;                  // 64 bf16 of every key
+  static constexpr int kTile = D / 64 * kPanel;               // bytes of a K or V tile
+  static constexpr int kQ = D / 64 * PT_Q_PANEL;              // of a slot's queries
+  static constexpr int kStagesK = PAIRED ? (D == 128 ? 3 : 5) : 5 * (128 / D), kStagesV = PAIRED ? (D == 128 ? 2 : 5) : 5 * (128 / D);
+  static_assert(PAIRED || kStagesK == kStagesV);
+  static constexpr int kSmem = 2 * kQ + (kStagesK + kStagesV) * kTile + 1024;
 };
 
 struct TilesParams {
   PrefixParams p;
   Span span[2];
-  int32_t first_items;
+  int32_t first_items, items;
 };
 
-template <int NS>
+// What the roles know of an item.  Its keys are those from v0 on of the row prefix keys (padded to p128) | own keys.
+struct TileItem {
+  int tiles;              // 0: the stream ends
+  int n[2];               // tiles that the slots of a pair take
+  int head, row0, rows, rho0;
+  int v0, p128, p_keys, o_keys;
+  int group, sequence, length;
+  int part;
+};
+
+template <class Shape>
 struct TileBarriers {
-  uint64_t q_full, full[NS], empty[NS], s_full[2], p_full[2], o_full[2], mask_full[PT_MASKS];
-  uint32_t mask[PT_MASKS][4];
+  uint64_t k_full[Shape::kStagesK], k_empty[Shape::kStagesK], v_full[Shape::kStagesV], v_empty[Shape::kStagesV];
+  uint64_t s_full[2][Shape::kBuffers], p_full[2][Shape::kBuffers], pv_done[2][Shape::kBuffers], q_full[2], q_empty[2];
+  uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
+  alignas(8) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
+  int32_t place[2][PT_MASKS];  // of the tile among all of the CTA: its stage in both rings
+  TileItem item[2][PT_ITEMS];
   uint32_t tmem_base;
-  float2 ml[128];  // slot 1's, joined by slot 0
 };
 
 // bf16 x bf16 -> fp32, A K-major; B K-major or MN-major (b_mn)
@@ -90,59 +120,102 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// A whole 32-byte sector from one lane: lanes write rows of their own.
+__device__ __forceinline__ void store32(float* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 // bits [0, n) of a word
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1); }
 
-template <int D>
-__global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __grid_constant__ TilesParams tp) {
-  using Shape = TileShape<D>;
-  constexpr int NS = Shape::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* const q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* const ring = q_s + 2 * Shape::kTile;
-  __shared__ TileBarriers<NS> bar;
+// Item n of the launch; false: there is nothing to do for it.
+template <bool PAIRED, int KEYS>
+__device__ bool find_tile_item(const TilesParams& tp, int n, TileItem& t) {
+  constexpr int TM = PAIRED ? 2 * kSlotRows : kSlotRows;
   const PrefixParams& p = tp.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  pdl_wait();
-  pdl_launch_dependents();
-  int n = static_cast<int>(blockIdx.x);
   const bool second = n >= tp.first_items;
   if (second) n -= tp.first_items;
   const Span& sp = tp.span[second];
-  const int head = n % p.kv_heads;
+  t.head = n % p.kv_heads;
   n /= p.kv_heads;
   const int chunk = n / sp.slots;
-  Item it;
-  if (!find_item<kTileRows>(p, sp, n - chunk * sp.slots, chunk, it)) return;
-  const bool dual = it.rows - it.rho0 > 128;
-  // key tiles: of the CTA and of its slots
-  const int tiles = (it.keys - it.key0 + PT_BN - 1) / PT_BN;
-  int n_slot[2];
-  if (dual) {
-    n_slot[1] = tiles;
-    n_slot[0] = tiles;
-    if (sp.own) {  // what the last row of slot 0 sees
-      const int k0 = min(own_keys(p, it.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(it.rho0 + 127)))), it.keys) - it.key0;
-      n_slot[0] = k0 <= 0 ? 0 : (k0 + PT_BN - 1) / PT_BN;
-    }
+  ItemRows r;
+  if (!find_rows<TM>(p, sp, n - chunk * sp.slots, r)) return false;
+  t.row0 = r.row0; t.rows = r.rows; t.rho0 = r.rho0;
+  t.group = t.sequence = t.length = 0;
+  t.p_keys = t.o_keys = 0;
+  if (sp.kind == kSpanPrefix) {
+    t.group = r.owner;
+    t.p_keys = prefix_keys(p, r.owner);
   } else {
-    n_slot[0] = (tiles + 1) >> 1;
-    n_slot[1] = tiles >> 1;
+    t.sequence = r.owner;
+    t.length = p.rows.lengths[r.owner];
+    if (t.length < 0) return false;
+    if (sp.kind == kSpanJoint) {
+      t.group = group_of(p, r.owner);
+      t.p_keys = prefix_keys(p, t.group);
+    }
+    t.o_keys = own_keys(p, t.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(min(r.rho0 + TM, r.rows) - 1))));
   }
+  t.p128 = align_keys(t.p_keys);
+  const int64_t v0 = static_cast<int64_t>(chunk) * sp.chunk, end = sp.kind == kSpanPrefix ? t.p_keys : static_cast<int64_t>(t.p128) + t.o_keys;
+  if (v0 >= end) return false;
+  t.v0 = static_cast<int>(v0);
+  auto tiles_to = [&](int64_t e) {  // of the chunk, for rows that see keys up to e
+    if (e > v0 + sp.chunk) e = v0 + sp.chunk;
+    return e <= v0 ? 0 : static_cast<int>((e - v0 + KEYS - 1) / KEYS);
+  };
+  t.tiles = tiles_to(end);
+  if (PAIRED) {
+    const bool other = r.rows - r.rho0 > kSlotRows;
+    t.n[0] = t.n[1] = t.tiles;
+    if (!other) t.n[1] = 0;
+    else if (sp.kind != kSpanPrefix)
+      t.n[0] = tiles_to(static_cast<int64_t>(t.p128) + own_keys(p, t.length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(r.rho0 + kSlotRows - 1)))));
+  } else {
+    t.n[0] = t.n[1] = t.tiles;
+  }
+  t.part = sp.part0 < 0 ? -1 : sp.part0 + chunk;
+  return true;
+}
+
+template <int D, bool PAIRED>
+__global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __grid_constant__ TilesParams tp) {
+  using Shape = TileShape<D, PAIRED>;
+  constexpr int BN = Shape::kKeys, NB = Shape::kBuffers, NK = Shape::kStagesK, NV = Shape::kStagesV;
+  constexpr int STREAMS = PAIRED ? 1 : 2;
+  constexpr unsigned ALL = 0xffffffffu;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* const k_ring = q_s + 2 * Shape::kQ;
+  uint8_t* const v_ring = k_ring + NK * Shape::kTile;
+  __shared__ TileBarriers<Shape> bar;
+  const PrefixParams& p = tp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bar.q_full, dual ? 8 : 4);
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(&bar.full[s], 128);  // the loaders' threads
-      mbar_init(&bar.empty[s], 1);
+    for (int s = 0; s < NK; ++s) {
+      mbar_init(&bar.k_full[s], 128);  // the loaders' threads
+      mbar_init(&bar.k_empty[s], 1);
+    }
+    for (int s = 0; s < NV; ++s) {
+      mbar_init(&bar.v_full[s], 128);
+      mbar_init(&bar.v_empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bar.s_full[s], 1);
-      mbar_init(&bar.p_full[s], 4);
-      mbar_init(&bar.o_full[s], 1);
+      for (int i = 0; i < NB; ++i) {
+        mbar_init(&bar.s_full[s][i], 1);
+        mbar_init(&bar.p_full[s][i], 4);
+        mbar_init(&bar.pv_done[s][i], 1);
+      }
+      mbar_init(&bar.q_full[s], 32);
+      mbar_init(&bar.q_empty[s], 1);
+      for (int i = 0; i < PT_MASKS; ++i) mbar_init(&bar.mask_full[s][i], 4);
+      for (int i = 0; i < PT_ITEMS; ++i) {
+        mbar_init(&bar.item_full[s][i], 1);
+        mbar_init(&bar.item_empty[s][i], 4 + 1 + 8 / STREAMS);  // warps that read an item: loaders, MMA issuer, softmax
+      }
     }
-    for (int s = 0; s < PT_MASKS; ++s) mbar_init(&bar.mask_full[s], 4);
     mbar_fence_init();
   }
   if (warp == 12) {
@@ -153,281 +226,446 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bar.tmem_base;
+  pdl_wait();
+  pdl_launch_dependents();
   // Registers: 128 a thread at launch, 512 for a thread of each of the four warpgroups.  The softmax, which holds a row of S, takes 192 in
   // two of them, the other two leave 64 each (2 x 192 + 2 x 64 = 512); every warp of a warpgroup passes the same setmaxnreg.
+
+  // The items of a stream, one after another: waits for the next, copies it, hands its place back.
+  struct Items {
+    int at = 0;
+    uint32_t phase = 0;
+  };
+  auto next_item = [&](int stream, Items& c, TileItem& t) {
+    if (!__all_sync(ALL, mbar_wait_spin(&bar.item_full[stream][c.at], c.phase, p.status, 48))) return false;
+    t = bar.item[stream][c.at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar.item_empty[stream][c.at]);
+    if (++c.at == PT_ITEMS) { c.at = 0; c.phase ^= 1; }
+    return true;
+  };
 
   if (warp >= 8 && warp < 12) {
     // =========================== loaders ===========================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    // Order: K0, K1, V0, K2, V1, ..., V(tiles - 1), each into the next stage of the ring.
     const int w = warp - 8;
-    const PagedTable& table = sp.own ? p.rows.table : p.prefix;
-    const __nv_bfloat16* const kb = p.cache.k.p + head * p.cache.k.head;
-    const __nv_bfloat16* const vb = p.cache.v.p + head * p.cache.v.head;
+    constexpr int MINE = BN / 4;           // keys of a tile per warp
     constexpr int LANES = D / 8;           // lanes that share a key
     constexpr int KEYS = 32 / LANES;       // keys per instruction
     const int piece = lane % LANES, sub = lane / LANES;
-    const uint32_t ring_u = smem_u32(ring) + (piece >> 3) * PT_PANEL;
-    int stage = 0;
-    uint32_t phase = 0;
+    const uint32_t at = (piece >> 3) * Shape::kPanel;
     bool ok = true;
-    auto load = [&](const __nv_bfloat16* base, int64_t off) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&bar.empty[stage], phase ^ 1, p.status, 40));
-      if (!ok) return;
-      const uint32_t dst = ring_u + stage * Shape::kTile;
-#pragma unroll
-      for (int i = 0; i < 32 / KEYS; ++i) {
-        const int key = i * KEYS + sub;
-        const int64_t o = __shfl_sync(0xffffffffu, off, key);
-        cp_async16(dst + (w * 32 + key) * 128 + (((piece & 7) ^ (key & 7)) << 4), base + (o < 0 ? 0 : o) + piece * 8, o >= 0);
-      }
-      cp_async_arrive(&bar.full[stage]);
-      if (++stage == NS) { stage = 0; phase ^= 1; }
+    struct Ring {
+      int stage = 0;
+      uint32_t phase = 0;
     };
-    int64_t v_prev = -1;  // the tile before
-    for (int t = 0; t <= tiles && ok; ++t) {
-      int64_t k_off = -1, v_off = -1;
-      if (t < tiles) {
-        const int j = it.key0 + t * PT_BN + w * 32 + lane;
-        if (j < it.keys) {
-          uint32_t index, slot;
-          p.cache.page_size.divmod(static_cast<uint32_t>(j), index, slot);
-          const int page = page_of(table, it.owner, index, p.cache.pages);
-          if (page >= 0) {
-            k_off = page * p.cache.k.page + slot * p.cache.k.token;
-            v_off = page * p.cache.v.page + slot * p.cache.v.token;
-          }
-        }
-        const uint32_t there = __ballot_sync(0xffffffffu, k_off >= 0);
-        load(kb, k_off);
-        if (!ok) break;
-        // (the softmax is done with the tile PT_MASKS before this one: its P was there before the stage just filled was free)
-        if (lane == 0) {
-          bar.mask[t % PT_MASKS][w] = there;
-          mbar_arrive(&bar.mask_full[t % PT_MASKS]);
-        }
+    auto load = [&](Ring& r, int stages, uint64_t* full, uint64_t* empty, uint32_t ring, const __nv_bfloat16* base, int64_t off) {
+      ok = __all_sync(ALL, mbar_wait(&empty[r.stage], r.phase ^ 1, p.status, 40));
+      if (!ok) return;
+      const uint32_t dst = ring + at + r.stage * Shape::kTile;
+#pragma unroll
+      for (int i = 0; i < MINE / KEYS; ++i) {
+        const int key = i * KEYS + sub;
+        const int64_t o = __shfl_sync(ALL, off, key);
+        cp_async16(dst + (w * MINE + key) * 128 + (((piece & 7) ^ (key & 7)) << 4), base + (o < 0 ? 0 : o) + piece * 8, o >= 0);
       }
-      if (t > 0) load(vb, v_prev);
+      cp_async_arrive(&full[r.stage]);
+      if (++r.stage == stages) { r.stage = 0; r.phase ^= 1; }
+    };
+    Ring kr, vr;
+    auto load_k = [&](int head, int64_t off) { load(kr, NK, bar.k_full, bar.k_empty, smem_u32(k_ring), p.cache.k.p + head * p.cache.k.head, off); };
+    auto load_v = [&](int head, int64_t off) { load(vr, NV, bar.v_full, bar.v_empty, smem_u32(v_ring), p.cache.v.p + head * p.cache.v.head, off); };
+    // A stream's place: what of its present item the keys' places depend on.  The page of this lane's key of the next tile is looked up a
+    // tile ahead.
+    struct Place {
+      Items items;
+      int left = 0, masks = 0;  // tiles left of the item, tiles of the stream so far
+      int v = 0, p128 = 0, p_keys = 0, o_keys = 0, group = 0, sequence = 0, head = 0;
+      int page = -1;
+      uint32_t slot = 0;
+      bool over = false;
+    };
+    auto look_up = [&](Place& c) {
+      const bool own = c.v >= c.p128;
+      const int j = c.v - (own ? c.p128 : 0) + w * MINE + lane;
+      c.page = -1;
+      if (lane < MINE && j < (own ? c.o_keys : c.p_keys)) {
+        const PagedTable& table = own ? p.rows.table : p.prefix;
+        uint32_t index;
+        p.cache.page_size.divmod(static_cast<uint32_t>(j), index, c.slot);
+        c.page = table.table[static_cast<int64_t>(own ? c.sequence : c.group) * table.ld + index];  // (keys end where the table does)
+      }
+    };
+    int64_t v_prev = -1;  // of the tile before
+    int head_prev = -1;
+    int x = 0;            // tiles so far
+    // one tile of a stream, if it has one left
+    auto tile = [&](Place& c, int stream) {
+      if (c.over) return;
+      if (c.left == 0) {
+        TileItem t;
+        ok = ok && next_item(stream, c.items, t);
+        if (!ok || t.tiles == 0) {
+          c.over = true;
+          return;
+        }
+        c.left = t.tiles; c.v = t.v0; c.p128 = t.p128; c.p_keys = t.p_keys; c.o_keys = t.o_keys;
+        c.group = t.group; c.sequence = t.sequence; c.head = t.head;
+        look_up(c);
+      }
+      const bool in = c.page >= 0 && c.page < p.cache.pages;
+      const int64_t k_off = in ? c.page * p.cache.k.page + c.slot * p.cache.k.token : -1;
+      const int64_t v_off = in ? c.page * p.cache.v.page + c.slot * p.cache.v.token : -1;
+      const uint32_t there = __ballot_sync(ALL, in);
+      --c.left;
+      c.v += BN;
+      if (c.left > 0) look_up(c);
+      load_k(c.head, k_off);
+      if (!ok) return;
+      // (the softmax has read the mask PT_MASKS tiles of the stream before this one: PT_MASKS is more than NK + the tiles of a slot whose S is
+      // issued and whose P is not read)
+      if (lane == 0) {
+        uint16_t* const m = bar.mask[stream][c.masks % PT_MASKS];
+        if (MINE == 32) reinterpret_cast<uint32_t*>(m)[w] = there;
+        else m[w] = static_cast<uint16_t>(there);
+        if (w == 0) bar.place[stream][c.masks % PT_MASKS] = x;
+        mbar_arrive(&bar.mask_full[stream][c.masks % PT_MASKS]);
+      }
+      ++c.masks;
+      ++x;
+      if (head_prev >= 0) load_v(head_prev, v_prev);
       v_prev = v_off;
+      head_prev = c.head;
+    };
+    Place a, b;
+    b.over = STREAMS == 1;
+    while (ok && !(a.over && b.over)) {  // the streams take turns
+      tile(a, 0);
+      if (STREAMS == 2 && ok) tile(b, 1);
     }
+    if (ok && head_prev >= 0) load_v(head_prev, v_prev);
     cp_async_wait_all();
   } else if (warp >= 12) {
-    // =========================== MMA issuer ===========================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 12) {
-    const bool leader = elect_one();
-    const uint32_t idesc_s = idesc_bf16(128, PT_BN, false), idesc_o = idesc_bf16(128, 64, true);
-    const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    auto desc = [&](uint32_t lo) { return (static_cast<uint64_t>(desc_hi) << 32) | lo; };
-    const uint32_t q_lo = smem_u32(q_s) >> 4, ring_lo = smem_u32(ring) >> 4;
-    bool ok = mbar_wait_spin(&bar.q_full, 0, p.status, 41);
-    tc_fence_after();
-    auto k_stage = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
-    auto v_stage = [&](int j) { return j < tiles - 1 ? 2 * j + 2 : 2 * j + 1; };
-    // (the copies are writes of the generic proxy: the fence orders them before the products that read them)
-    auto landed = [&](int i) {
-      const bool there = mbar_wait_spin(&bar.full[i % NS], (i / NS) & 1, p.status, 42);
-      fence_proxy_async_smem();
-      return there;
-    };
-    auto issue_s = [&](int slot, int j) {
-      const uint32_t qa = q_lo + (dual ? slot : 0) * (Shape::kTile >> 4), kt = ring_lo + (k_stage(j) % NS) * (Shape::kTile >> 4);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t off = (i >> 2) * (PT_PANEL >> 4) + (i & 3) * 2;
-        if (leader) mma_bf16_ss(tmem_base + slot * PT_TM_SLOT, desc(qa + off), desc(kt + off), idesc_s, i != 0);
-      }
-      if (leader) tc_commit(&bar.s_full[slot]);
-    };
-    auto issue_o = [&](int slot, int j, bool first) {
-      const uint32_t vt = ring_lo + (v_stage(j) % NS) * (Shape::kTile >> 4), tm = tmem_base + slot * PT_TM_SLOT;
-#pragma unroll
-      for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-        for (int i = 0; i < PT_BN / 16; ++i)
-          if (leader) mma_bf16_ts(tm + PT_TM_O + h * 64, tm + i * 8, desc(vt + h * (PT_PANEL >> 4) + i * ((16 * 128) >> 4)), idesc_o, !(first && i == 0));
-    };
-    auto release = [&](int i) {
-      if (leader) tc_commit(&bar.empty[i % NS]);
-    };
-    if (dual) {
-      ok = ok && landed(0);
-      if (ok) {
+    if (warp == 12 || (warp == 15 && !PAIRED)) {
+      // =========================== MMA issuers ===========================
+      const bool leader = elect_one();
+      const int slot = warp == 12 ? 0 : 1;
+      // Descriptors: the low word is the shared address >> 4 and, for V (MN-major), the distance of its panels of 64 columns above bit 16; the
+      // high word has the distance of 8-row groups, version and swizzle.  Low words come out of a shuffle, so that the compiler knows
+      // them to be the same in all lanes and forms the descriptors in uniform registers.
+      const uint32_t idesc_s = idesc_bf16(128, BN, false), idesc_o = idesc_bf16(128, D, true);
+      const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      auto desc = [&](uint32_t lo) { return (static_cast<uint64_t>(desc_hi) << 32) | lo; };
+      const uint32_t q_lo = smem_u32(q_s) >> 4, k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
+      bool ok = true;
+      // (the copies are writes of the generic proxy: the fence orders them before the products that read them)
+      auto landed = [&](uint64_t* full, int stage, int phase) {
+        const bool there = __all_sync(ALL, mbar_wait_spin(&full[stage], phase & 1, p.status, 42));
+        if (leader) fence_proxy_async_smem();
+        return there;
+      };
+      auto issue_s = [&](int slot, int buffer, int stage) {
+        const uint32_t qa = __shfl_sync(ALL, q_lo + slot * (Shape::kQ >> 4), 0);
+        const uint32_t kt = __shfl_sync(ALL, k_lo + stage * (Shape::kTile >> 4), 0), ts = __shfl_sync(ALL, tmem_base + slot * PT_TM_SLOT + buffer * BN, 0);
         tc_fence_after();
-        if (n_slot[0] > 0) issue_s(0, 0);
-        issue_s(1, 0);
-        release(0);
-      }
-      for (int j = 0; j < tiles && ok; ++j) {
-        ok = landed(v_stage(j));
-        for (int slot = 0; slot < 2 && ok; ++slot) {
-          if (j >= n_slot[slot]) continue;
-          ok = mbar_wait_spin(&bar.p_full[slot], j & 1, p.status, 43);
-          if (!ok) break;
-          tc_fence_after();
-          issue_o(slot, j, j == 0);
-          if (j + 1 < n_slot[slot]) {
-            ok = landed(k_stage(j + 1));
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(slot, j + 1);
-          } else if (leader) {
-            tc_commit(&bar.o_full[slot]);
+        if (leader) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            mma_bf16_ss(ts, desc(qa + (i >> 2) * (PT_Q_PANEL >> 4) + (i & 3) * 2), desc(kt + (i >> 2) * (Shape::kPanel >> 4) + (i & 3) * 2), idesc_s, i != 0);
+          tc_commit(&bar.s_full[slot][buffer]);
+        }
+      };
+      auto issue_o = [&](int slot, int buffer, int stage, bool first) {  // P is there
+        const uint32_t vt = __shfl_sync(ALL, v_lo + stage * (Shape::kTile >> 4), 0) | (static_cast<uint32_t>(Shape::kPanel >> 4) << 16);
+        const uint32_t tm = __shfl_sync(ALL, tmem_base + slot * PT_TM_SLOT, 0), ps = __shfl_sync(ALL, tm + buffer * BN, 0);
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int i = 0; i < BN / 16; ++i)  // 16 keys are two groups of eight rows
+            mma_bf16_ts(tm + PT_TM_O, ps + i * 8, desc(vt + i * ((16 * 128) >> 4)), idesc_o, !(first && i == 0));
+        }
+      };
+      Items items;
+      TileItem t;
+      uint32_t q_phase = 0;
+      auto wait_q = [&](int i) {
+        const bool there = __all_sync(ALL, mbar_wait_spin(&bar.q_full[i], q_phase, p.status, 41));
+        q_phase ^= 1;
+        if (leader) fence_proxy_async_smem();
+        return there;
+      };
+      if (PAIRED) {
+        // Step x: P V of tile x and S of tile x + 1, slot by slot.
+        int x = -1, ks = 0, vs = 0;
+        uint32_t k_phase = 0, v_phase = 0, p_phase = 0;  // p_phase: a bit per slot
+        bool has[2] = {false, false}, fresh = false, last[2] = {false, false};  // of tile x: which slots take it, first and last of the item
+        auto wait_p = [&](int s) {
+          const bool there = __all_sync(ALL, mbar_wait_spin(&bar.p_full[s][0], (p_phase >> s) & 1, p.status, 43));
+          p_phase ^= 1u << s;
+          return there;
+        };
+        auto step = [&](bool more, bool has0, bool has1, bool first, bool last0, bool last1, bool end) {  // tile x + 1: whether there is one, ...
+          if (x >= 0) ok = landed(bar.v_full, vs, v_phase);
+          if (ok && has[0]) {
+            ok = wait_p(0);
+            if (ok) issue_o(0, 0, vs, fresh);
+            if (ok && last[0] && leader) tc_commit(&bar.pv_done[0][0]);
           }
+          if (ok && first) ok = wait_q(0);
+          if (ok && more) ok = landed(bar.k_full, ks, k_phase);
+          if (ok && has0) issue_s(0, 0, ks);
+          if (ok && has[1]) {
+            ok = wait_p(1);
+            if (ok) issue_o(1, 0, vs, fresh);
+            if (ok && last[1] && leader) tc_commit(&bar.pv_done[1][0]);
+          }
+          if (!ok) return;
+          if (has1) issue_s(1, 0, ks);
+          if (leader) {
+            if (x >= 0) tc_commit(&bar.v_empty[vs]);
+            if (more) tc_commit(&bar.k_empty[ks]);
+            if (end) tc_commit(&bar.q_empty[0]);
+          }
+          if (x >= 0 && ++vs == NV) { vs = 0; v_phase ^= 1; }
+          if (++ks == NK) { ks = 0; k_phase ^= 1; }
+          ++x;
+          has[0] = has0; has[1] = has1; fresh = first; last[0] = last0; last[1] = last1;
+        };
+        while (ok) {
+          ok = next_item(0, items, t);
+          if (!ok || t.tiles == 0) break;
+          for (int j = 0; ok && j < t.tiles; ++j) step(true, j < t.n[0], j < t.n[1], j == 0, j + 1 == t.n[0], j + 1 == t.n[1], j + 1 == t.tiles);
         }
-        release(v_stage(j));
-        if (j + 1 < tiles) release(k_stage(j + 1));
-      }
-    } else {
-      for (int j = 0; j < 2 && j < tiles && ok; ++j) {
-        ok = landed(k_stage(j));
-        if (!ok) break;
-        tc_fence_after();
-        issue_s(j, j);
-        release(k_stage(j));
-      }
-      for (int j = 0; j < tiles && ok; ++j) {
-        const int slot = j & 1;
-        ok = landed(v_stage(j)) && mbar_wait_spin(&bar.p_full[slot], (j >> 1) & 1, p.status, 43);
-        if (!ok) break;
-        tc_fence_after();
-        issue_o(slot, j, j < 2);
-        release(v_stage(j));
-        if (j + 2 < tiles) {
-          ok = landed(k_stage(j + 2));
+        if (ok && x >= 0) step(false, false, false, false, false, false, false);
+      } else {
+        // Up to two S ahead of P V.
+        int left = 0, m = 0;           // tiles of the item whose S is to come; tiles of the stream so far
+        bool first = false;
+        int x0 = 0, x1 = 0, open = 0;  // tiles whose P V is to come
+        bool f0 = false, f1 = false;   // first of their item
+        uint32_t s_buffer = 0, o_buffer = 0, p_phase = 0;
+        while (ok) {
+          if (left == 0 && open == 0) {
+            ok = next_item(slot, items, t);
+            if (!ok || t.tiles == 0) break;
+            left = t.tiles;
+            first = true;
+          }
+          if (left > 0 && open < NB) {
+            ok = (!first || wait_q(slot)) && __all_sync(ALL, mbar_wait_spin(&bar.mask_full[slot][m % PT_MASKS], (m / PT_MASKS) & 1, p.status, 51));
+            if (!ok) break;
+            const int x = bar.place[slot][m % PT_MASKS];
+            ++m;
+            ok = landed(bar.k_full, x % NK, x / NK);
+            if (!ok) break;
+            issue_s(slot, s_buffer, x % NK);
+            s_buffer ^= 1;
+            --left;
+            if (leader) {
+              tc_commit(&bar.k_empty[x % NK]);
+              if (left == 0) tc_commit(&bar.q_empty[slot]);
+            }
+            if (open == 0) { x0 = x; f0 = first; }
+            else { x1 = x; f1 = first; }
+            ++open;
+            first = false;
+            continue;
+          }
+          ok = landed(bar.v_full, x0 % NV, x0 / NV) && __all_sync(ALL, mbar_wait_spin(&bar.p_full[slot][o_buffer], (p_phase >> o_buffer) & 1, p.status, 43));
           if (!ok) break;
-          tc_fence_after();
-          issue_s(slot, j + 2);
-          release(k_stage(j + 2));
-        } else if (leader) {
-          tc_commit(&bar.o_full[slot]);
+          p_phase ^= 1u << o_buffer;
+          issue_o(slot, o_buffer, x0 % NV, f0);
+          if (leader) {
+            tc_commit(&bar.pv_done[slot][o_buffer]);
+            tc_commit(&bar.v_empty[x0 % NV]);
+          }
+          o_buffer ^= 1;
+          x0 = x1;
+          f0 = f1;
+          --open;
         }
       }
-    }
+    } else if (warp - 13 < STREAMS) {
+      // =========================== items and their queries ===========================
+      const int stream = warp - 13;
+      const int n_streams = static_cast<int>(gridDim.x) * STREAMS, first = static_cast<int>(blockIdx.x) * STREAMS + stream;
+      constexpr int LANES = D / 8, ROWS = 32 / LANES;
+      const int piece = lane % LANES, sub = lane / LANES;
+      int at = 0;
+      uint32_t phase = 0, q_phase = 0;
+      bool ok = true;
+      auto hand_out = [&](const TileItem& t, bool writer) {
+        ok = __all_sync(ALL, mbar_wait(&bar.item_empty[stream][at], phase ^ 1, p.status, 49));
+        if (!ok) return;
+        if (writer) bar.item[stream][at] = t;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.item_full[stream][at]);
+        if (++at == PT_ITEMS) { at = 0; phase ^= 1; }
+      };
+      for (int64_t n0 = first; n0 < tp.items && ok; n0 += 32ll * n_streams) {
+        TileItem t;
+        const int64_t n = n0 + static_cast<int64_t>(lane) * n_streams;
+        const bool valid = n < tp.items && find_tile_item<PAIRED, BN>(tp, static_cast<int>(n), t);
+        for (unsigned left = __ballot_sync(ALL, valid); left != 0 && ok; left &= left - 1) {
+          const int src = __ffs(left) - 1;
+          hand_out(t, lane == src);
+          if (!ok) break;
+          const int row0 = __shfl_sync(ALL, t.row0, src), rows = __shfl_sync(ALL, t.rows, src), rho0 = __shfl_sync(ALL, t.rho0, src);
+          const int64_t head0 = __shfl_sync(ALL, t.head, src) * static_cast<int64_t>(p.per_kv.d);
+          ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
+          if (!ok) break;
+          q_phase ^= 1;
+          // whole warps' worth of rows: those that do not exist are zeros
+          const int n_rows = min((rows - rho0 + 31) / 32 * 32, PAIRED ? 2 * kSlotRows : kSlotRows);
+          for (int r = sub; r < n_rows; r += ROWS) {
+            const bool there = rho0 + r < rows;
+            uint32_t tok, hq;
+            p.per_kv.divmod(static_cast<uint32_t>(there ? rho0 + r : 0), tok, hq);
+            const __nv_bfloat16* src_row = p.q + static_cast<int64_t>(row0 + static_cast<int>(tok)) * p.q_row + (head0 + hq) * p.q_head;
+            const int slot = PAIRED ? r >> 7 : stream, local = r & 127;
+            cp_async16(smem_u32(q_s) + slot * Shape::kQ + (piece >> 3) * PT_Q_PANEL + local * 128 + (((piece & 7) ^ (local & 7)) << 4), src_row + piece * 8, there);
+          }
+          cp_async_arrive(&bar.q_full[stream]);
+        }
+      }
+      TileItem end;
+      end.tiles = 0;
+      if (ok) hand_out(end, lane == 0);
+      cp_async_wait_all();
     }
   } else {
     // =========================== softmax: a row per thread ===========================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    const int slot = warp >> 2, quad = warp & 3, local = quad * 32 + lane;
+    constexpr int W = BN / 32;              // words of a row's mask, pieces of 32 keys
+    const int slot = warp >> 2, quad = warp & 3, stream = PAIRED ? 0 : slot;
     const uint32_t tm = tmem_base + slot * PT_TM_SLOT + (static_cast<uint32_t>(quad * 32) << 16);
-    const int rho = it.rho0 + (dual ? slot * 128 : 0) + local;
-    uint32_t tok, hq;
-    p.per_kv.divmod(static_cast<uint32_t>(rho), tok, hq);
-    const bool there = rho < it.rows;
-    const int64_t row = it.row0 + static_cast<int>(tok), qh = head * static_cast<int64_t>(p.per_kv.d) + hq;
-    if (dual || slot == 0) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (there ? row * p.q_row + qh * p.q_head : 0));
-      uint8_t* const dst = q_s + slot * Shape::kTile + local * 128;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (there) u = src[i];
-        *reinterpret_cast<uint4*>(dst + (i >> 3) * PT_PANEL + (((i & 7) ^ (local & 7)) << 4)) = u;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.q_full);
-    }
-    const int limit = there && sp.own ? own_keys(p, it.length, static_cast<int>(tok)) : it.keys;
-    const bool idle = rho - lane >= it.rows;  // a warp without rows: whatever its P holds stays in its own rows of O
     const float NEG_INF = __int_as_float(0xff800000);
-    float m_ref = NEG_INF, l = 0.0f;
+    Items items;
+    TileItem t;
+    int masks = 0;                          // tiles of the stream up to this item
+    uint32_t units = 0, mine_done = 0;      // tiles of the slot so far: unit n has buffer n % NB, phase n / NB; its items so far
     bool ok = true;
-    const int mine = n_slot[slot];
-    for (int u = 0; u < mine; ++u) {
-      const int t = dual ? u : 2 * u + slot;
-      if (idle) {
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.s_full[slot], u & 1, p.status, 47));
-        if (!ok) break;
-        if (lane == 0) mbar_arrive(&bar.p_full[slot]);
-        continue;
-      }
-      // which keys of the tile this row sees
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.mask_full[t % PT_MASKS], (t / PT_MASKS) & 1, p.status, 44));
-      if (!ok) break;
-      uint32_t seen[4];
-      bool all = true;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        seen[i] = bar.mask[t % PT_MASKS][i] & low_bits(limit - it.key0 - t * PT_BN - 32 * i);
-        all = all && seen[i] == 0xffffffffu;
-      }
-      const bool masked = __any_sync(0xffffffffu, !all);
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.s_full[slot], u & 1, p.status, 45));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t sc[4][32];
-      tc_ld_32x32b_x32(tm, sc[0]);
-      tc_ld_32x32b_x32(tm + 32, sc[1]);
-      tc_wait_ld();
-      tc_ld_32x32b_x32(tm + 64, sc[2]);
-      tc_ld_32x32b_x32(tm + 96, sc[3]);
-      float m4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-      auto largest = [&](int i) {
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((seen[i] >> e) & 1)) sc[i][e] = 0xff800000u;
+    while (true) {
+      ok = next_item(stream, items, t);
+      if (!ok || t.tiles == 0) break;
+      const int rho = t.rho0 + (PAIRED ? slot * kSlotRows : 0) + quad * 32 + lane;
+      uint32_t tok, hq;
+      p.per_kv.divmod(static_cast<uint32_t>(rho), tok, hq);
+      const bool there = rho < t.rows;
+      const bool idle = rho - lane >= t.rows;  // a warp without rows: whatever its P holds stays in its own rows of O
+      const int limit = there ? own_keys(p, t.length, static_cast<int>(tok)) : t.o_keys;
+      float m_ref = NEG_INF, l = 0.0f;
+      const int mine = PAIRED ? (slot ? t.n[1] : t.n[0]) : t.tiles;
+      for (int u = 0; u < mine; ++u, ++units) {
+        const uint32_t buffer = units % NB, parity = (units / NB) & 1;
+        const uint32_t tb = tm + buffer * BN;
+        if (idle) {
+          ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 47));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
+          continue;
         }
+        // which keys of the tile this row sees
+        const int mk = masks + u;
+        ok = __all_sync(ALL, mbar_wait(&bar.mask_full[stream][mk % PT_MASKS], (mk / PT_MASKS) & 1, p.status, 44));
+        if (!ok) break;
+        const int v = t.v0 + u * BN;
+        const int left = v >= t.p128 ? limit - (v - t.p128) : BN;  // (of the prefix, what the mask says)
+        uint32_t seen[W];
+        bool all = true;
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) m4[(e >> 1) & 3] = max3(m4[(e >> 1) & 3], __uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1]));
-      };
-      largest(0);
-      largest(1);
-      tc_wait_ld();
-      largest(2);
-      largest(3);
-      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-      const float m_tile = mx * p.scale2;
-      const bool moves = m_tile > m_ref + 8.0f;
-      if (__any_sync(0xffffffffu, moves)) {
-        const float alpha = moves ? ex2(m_ref - m_tile) : 1.0f;  // 0 for m_ref = -inf
-        if (moves) m_ref = m_tile;
-        l *= alpha;
-        if (u > 0) {  // (S of this tile was issued behind P V of the one before: O is complete)
+        for (int i = 0; i < W; ++i) {
+          seen[i] = reinterpret_cast<const uint32_t*>(bar.mask[stream][mk % PT_MASKS])[i] & low_bits(left - 32 * i);
+          all = all && seen[i] == 0xffffffffu;
+        }
+        const bool masked = __any_sync(ALL, !all);
+        ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 45));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sc[W][32];
+        float m4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+        auto largest = [&](int i) {
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t o[32];
-            tc_ld_32x32b_x32(tm + PT_TM_O + 32 * i, o);
-            tc_wait_ld();
+            for (int e = 0; e < 32; ++e)
+              if (!((seen[i] >> e) & 1)) sc[i][e] = 0xff800000u;
+          }
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tc_st_x16(tm + PT_TM_O + 32 * i, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
-            tc_st_x16(tm + PT_TM_O + 32 * i + 16, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
+          for (int e = 0; e < 32; e += 2) m4[(e >> 1) & 3] = max3(m4[(e >> 1) & 3], __uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1]));
+        };
+        tc_ld_32x32b_x32(tb, sc[0]);
+        if (W == 4) tc_ld_32x32b_x32(tb + 32, sc[1]);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = W / 2; i < W; ++i) tc_ld_32x32b_x32(tb + 32 * i, sc[i]);
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) largest(i);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = W / 2; i < W; ++i) largest(i);
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float m_tile = mx * p.scale2;
+        const bool moves = m_tile > m_ref + 8.0f;
+        if (__any_sync(ALL, moves)) {
+          const float alpha = moves ? ex2(m_ref - m_tile) : 1.0f;  // 0 for m_ref = -inf
+          if (moves) m_ref = m_tile;
+          l *= alpha;
+          if (u > 0) {
+            if (NB > 1) {  // P V of the tile before has to be complete (with one buffer this tile's S was issued behind it)
+              ok = __all_sync(ALL, mbar_wait(&bar.pv_done[slot][(units - 1) % NB], ((units - 1) / NB) & 1, p.status, 46));
+              if (!ok) break;
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t o[16];
+              tc_ld_x16(tm + PT_TM_O + 16 * i, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tc_st_x16(tm + PT_TM_O + 16 * i, o);
+            }
           }
         }
-      }
-      const float ref = m_ref == NEG_INF ? 0.0f : m_ref;
-      const uint64_t k2 = pack_f32x2(p.scale2, p.scale2), n2 = pack_f32x2(-ref, -ref);
-      uint64_t sum[2] = {0ull, 0ull};
+        const float ref = m_ref == NEG_INF ? 0.0f : m_ref;
+        const uint64_t k2 = pack_f32x2(p.scale2, p.scale2), n2 = pack_f32x2(-ref, -ref);
+        uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t pk[16];
+        for (int i = 0; i < W; ++i) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float x0, x1;
-          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1])), k2, n2), x0, x1);
-          x0 = ex2(x0);
-          x1 = ex2(x1);
-          sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], pack_f32x2(x0, x1));
-          pk[e >> 1] = pack_bf16(x0, x1);
+          for (int e = 0; e < 32; e += 2) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1])), k2, n2), x0, x1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], pack_f32x2(x0, x1));
+            pk[e >> 1] = pack_bf16(x0, x1);
+          }
+          tc_st_x16(tb + 16 * i, pk);  // over S, which is in registers
         }
-        tc_st_x16(tm + 16 * i, pk);  // over S, which is in registers
+        float a0, a1, b0, b1;
+        unpack_f32x2(sum[0], a0, a1);
+        unpack_f32x2(sum[1], b0, b1);
+        l += (a0 + a1) + (b0 + b1);
+        tc_wait_st_all();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
       }
-      float a0, a1, b0, b1;
-      unpack_f32x2(sum[0], a0, a1);
-      unpack_f32x2(sum[1], b0, b1);
-      l += (a0 + a1) + (b0 + b1);
-      tc_wait_st_all();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.p_full[slot]);
-    }
-    if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(&bar.o_full[slot], 0, p.status, 46));
-    tc_fence_after();
-    const int64_t at = (static_cast<int64_t>(sp.part0 + chunk) * p.rows.rows + row) * p.q_heads + qh;
-    if (dual) {
-      if (ok && mine > 0) {
+      masks += t.tiles;
+      if (!ok) break;
+      if (mine == 0) continue;
+      // P V of the last tile (PAIRED: said of that one only)
+      ok = __all_sync(ALL, mbar_wait(&bar.pv_done[slot][(units - 1) % NB], (PAIRED ? mine_done : (units - 1) / NB) & 1, p.status, 46));
+      if (!ok) break;
+      ++mine_done;
+      if (idle) continue;
+      tc_fence_after();
+      const int64_t row = t.row0 + static_cast<int>(tok), qh = t.head * static_cast<int64_t>(p.per_kv.d) + hq;
+      if (t.part >= 0) {
+        const int64_t at = (static_cast<int64_t>(t.part) * p.rows.rows + row) * p.q_heads + qh;
         if (there) p.part_ml[at] = make_float2(m_ref, l);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -436,33 +674,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           tc_wait_ld();
           if (there) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              reinterpret_cast<uint4*>(p.part_o + at * D + 32 * i)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e) store32(p.part_o + at * D + 32 * i + 8 * e, &o[8 * e]);
           }
         }
-      }
-    } else {
-      // Slot 1's sums to slot 0 through the shared memory of Q, which every S has been formed of by now (the last of them was issued ahead
-      // of slot 1's last P V).  16-byte pieces of a row in an order that depends on the row, so that lanes hit different banks.
-      if (slot == 1 && ok && mine > 0) {
-        bar.ml[local] = make_float2(m_ref, l);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          uint32_t o[32];
-          tc_ld_32x32b_x32(tm + PT_TM_O + 32 * i, o);
-          tc_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(q_s + local * (D * 4) + (((8 * i + e) ^ (local & 7)) << 4)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
-      }
-      named_bar_sync(1, 256);
-      if (slot == 0 && ok) {
-        const bool other = n_slot[1] > 0;
-        const float2 ml = other ? bar.ml[local] : make_float2(NEG_INF, 0.0f);
-        const float m = fmaxf(m_ref, ml.x), ref = m == NEG_INF ? 0.0f : m;
-        const float wa = ex2(m_ref - ref), wb = ex2(ml.x - ref);
-        if (there) p.part_ml[at] = make_float2(m, wa * l + (other ? wb * ml.y : 0.0f));
+      } else {
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        __nv_bfloat16* const dst = p.out + row * p.o_row + qh * p.o_head;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
@@ -470,19 +687,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           tc_wait_ld();
           if (there) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float4 x = make_float4(0, 0, 0, 0);
-              if (other) x = *reinterpret_cast<const float4*>(q_s + local * (D * 4) + (((8 * i + e) ^ (local & 7)) << 4));
-              float4 y;
-              y.x = wa * __uint_as_float(o[4 * e]) + wb * x.x;
-              y.y = wa * __uint_as_float(o[4 * e + 1]) + wb * x.y;
-              y.z = wa * __uint_as_float(o[4 * e + 2]) + wb * x.z;
-              y.w = wa * __uint_as_float(o[4 * e + 3]) + wb * x.w;
-              reinterpret_cast<float4*>(p.part_o + at * D + 32 * i)[e] = y;
+            for (int e = 0; e < 4; ++e) {  // (rows of `out` are 16-byte aligned)
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = pack_bf16(__uint_as_float(o[8 * e + 2 * k]) * inv, __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
+              reinterpret_cast<uint4*>(dst + 32 * i)[e] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         }
       }
+      tc_fence_before();
     }
   }
   tc_fence_before();
@@ -493,30 +707,34 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   }
 }
 
-template <int D>
-int launch(const TilesParams& tp, int64_t items, cudaStream_t st) {
+template <int D, bool PAIRED>
+int launch(const TilesParams& tp, cudaStream_t st) {
   int dev = 0;
   VX_CUDA_OK(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_done{0};
   const bool cached = dev >= 0 && dev < 64;
   if (!cached || !(attr_done.load(std::memory_order_acquire) & (1ull << dev))) {
-    VX_CUDA_OK(cudaFuncSetAttribute(prefix_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<D>::kSmem));
+    VX_CUDA_OK(cudaFuncSetAttribute(prefix_tiles_kernel<D, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<D, PAIRED>::kSmem));
     if (cached) attr_done.fetch_or(1ull << dev, std::memory_order_release);
   }
-  VX_CUDA_OK(launch_dependent(prefix_tiles_kernel<D>, dim3(static_cast<unsigned>(items)), dim3(PT_THREADS), TileShape<D>::kSmem, st, tp));
+  const int ctas = PAIRED ? tp.items : (tp.items + 1) / 2;
+  VX_CUDA_OK(launch_dependent(prefix_tiles_kernel<D, PAIRED>, dim3(static_cast<unsigned>(ctas < sm_count() ? ctas : sm_count())), dim3(PT_THREADS),
+                              TileShape<D, PAIRED>::kSmem, st, tp));
   return 0;
 }
 
 }  // namespace
 
-int launch_prefix_tiles(const PrefixParams& p, int head_dim, const Span& prefix, const Span& own, void* stream) {
-  TilesParams tp{p, {prefix, own}, 0};
-  const int64_t first = static_cast<int64_t>(prefix.slots) * prefix.chunks * p.kv_heads;
-  const int64_t items = first + static_cast<int64_t>(own.slots) * own.chunks * p.kv_heads;
+int launch_prefix_tiles(const PrefixParams& p, int head_dim, bool paired, const Span& a, const Span& b, void* stream) {
+  TilesParams tp{p, {a, b}, 0, 0};
+  const int64_t first = static_cast<int64_t>(a.slots) * a.chunks * p.kv_heads;
+  const int64_t items = first + static_cast<int64_t>(b.slots) * b.chunks * p.kv_heads;
   if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
   tp.first_items = static_cast<int32_t>(first);
+  tp.items = static_cast<int32_t>(items);
   const auto st = static_cast<cudaStream_t>(stream);
-  return head_dim == 64 ? launch<64>(tp, items, st) : launch<128>(tp, items, st);
+  if (head_dim == 64) return paired ? launch<64, true>(tp, st) : launch<64, false>(tp, st);
+  return paired ? launch<128, true>(tp, st) : launch<128, false>(tp, st);
 }
 
 }  // namespace vx
