@@ -36,10 +36,15 @@ namespace {
 constexpr int PR_WARPS = 4;
 constexpr int kRowsKernel = 16;  // rows per owner and key head up to which prefix_rows_kernel takes a span
 
+// CTAs of prefix_rows_kernel per SM, by its registers
+constexpr int rows_ctas(int blocks, int head_dim) { return blocks == 2 && head_dim == 128 ? 2 : 3; }
+
 struct RowsParams {
   PrefixParams p;
   Span span[2];
-  int32_t first_items;  // items of span[0]; those of span[1] follow
+  int32_t warps[2];      // of a CTA per item of the span: 1, 2 or 4
+  int32_t first_blocks;  // CTAs of span[0]; those of span[1] follow
+  int32_t beside;        // the launch in front is the tile kernel of this call, see below
 };
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -79,14 +84,14 @@ __device__ __forceinline__ void ld_shared16(uint32_t addr, uint32_t (&r)[4]) {
 template <int D>
 struct RowsShape {
   static constexpr int kHalf = 16 * D * 2;                       // bytes of the keys of a stage
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kStages = D == 128 ? 2 : 4;
   static constexpr int kRing = kStages * 2 * kHalf;              // of a warp
   static constexpr int kSmem = PR_WARPS * kRing;
 };
 
 // RB blocks of eight rows.
 template <int D, int RB>
-__global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __grid_constant__ RowsParams rp) {
+__global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_kernel(const __grid_constant__ RowsParams rp) {
   pdl_launch_dependents();
   using Shape = RowsShape<D>;
   constexpr int NS = Shape::kStages;
@@ -95,16 +100,28 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
   constexpr int TM = 8 * RB;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 ml_s[PR_WARPS][TM];
+  __shared__ uint32_t there_s[PR_WARPS][NS];  // bit k: key k of a stage is there
   const PrefixParams& p = rp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  pdl_wait();
+  // Beside the tile kernel of the same call: that one lets this launch start only behind its own wait, so everything in front of both is
+  // complete, and neither reads what the other writes.  The wait comes at the end then: whoever waits for this kernel waits for both.
+  struct Behind {
+    const bool last;
+    __device__ ~Behind() {
+      if (last) pdl_wait();
+    }
+  } behind{rp.beside != 0};
+  if (!rp.beside) pdl_wait();
   int n = static_cast<int>(blockIdx.x);
-  const bool second = n >= rp.first_items;
-  if (second) n -= rp.first_items;
+  const bool second = n >= rp.first_blocks;
+  if (second) n -= rp.first_blocks;
   const Span& sp = rp.span[second];
+  const int warps = rp.warps[second], team = warp / warps, rank = warp - team * warps;  // the warps of an item
+  n = n * (PR_WARPS / warps) + team;
   const int head = n % p.kv_heads;  // heads of a token lie next to each other
   n /= p.kv_heads;
   const int chunk = n / sp.slots;
+  if (chunk >= sp.chunks) return;
   const bool own = sp.kind == kSpanOwn;
   ItemRows it;
   if (!find_rows<TM>(p, sp, n - chunk * sp.slots, it)) return;
@@ -120,48 +137,60 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
   const int blocks = it.rows - it.rho0 > 8 ? RB : 1;  // that have rows
 
   // The ring: the copies of a step are one group, a warp waits for its own.
-  constexpr int STEP = 16 * PR_WARPS;
+  const int STEP = 16 * warps;
   constexpr int LANES = D / 8, KEYS = 32 / LANES;  // lanes per key, keys per copy instruction
   const int piece = lane % LANES, sub = lane / LANES;
   const uint32_t ring = smem_u32(smem) + warp * Shape::kRing;
-  int j_load = key0 + warp * 16, s_load = 0;
-  uint32_t there_ring[NS];  // of each stage: bit k: key k is there
-  auto fetch = [&](uint32_t& there) {  // the next 16 keys of this warp into stage s_load
+  const bool whole_pages = p.cache.page_size.d % 16 == 0;  // the 16 keys of a step lie on one page
+  int j_load = key0 + rank * 16;
+  auto fetch = [&](int stage) {  // the next 16 keys of this warp
+    const uint32_t dst = ring + stage * 2 * Shape::kHalf;
+    // Where they are: the first of them when they lie on one page (the others follow it), else key j_load + lane, handed around below.
     int64_t k_off = -1, v_off = -1;
-    const int j = j_load + lane;
-    if (lane < 16 && j < keys) {
-      uint32_t index, slot;
-      p.cache.page_size.divmod(static_cast<uint32_t>(j), index, slot);
-      const int page = page_of(table, it.owner, index, p.cache.pages);
-      if (page >= 0) {
-        k_off = page * p.cache.k.page + slot * p.cache.k.token;
-        v_off = page * p.cache.v.page + slot * p.cache.v.token;
+    {
+      const int j = j_load + (whole_pages ? 0 : lane & 15);
+      if (j < keys) {
+        uint32_t index, slot;
+        p.cache.page_size.divmod(static_cast<uint32_t>(j), index, slot);
+        const int page = page_of(table, it.owner, index, p.cache.pages);
+        if (page >= 0) {
+          k_off = page * p.cache.k.page + slot * p.cache.k.token;
+          v_off = page * p.cache.v.page + slot * p.cache.v.token;
+        }
       }
     }
-    there = __ballot_sync(0xffffffffu, k_off >= 0);
-    const uint32_t dst = ring + s_load * 2 * Shape::kHalf;
+    uint32_t there;
+    if (whole_pages) {
+      const int n = k_off >= 0 ? keys - j_load : 0;
+      there = n >= 16 ? 0xffffu : (1u << n) - 1;
+      const __nv_bfloat16* ka = kb + (n > 0 ? k_off + sub * p.cache.k.token : 0) + piece * 8;
+      const __nv_bfloat16* va = vb + (n > 0 ? v_off + sub * p.cache.v.token : 0) + piece * 8;
 #pragma unroll
-    for (int i = 0; i < 16 / KEYS; ++i) {
-      const int key = i * KEYS + sub;
-      const int64_t o = __shfl_sync(0xffffffffu, k_off, key);
-      cp_async16(dst + key * (D * 2) + ((piece ^ ((key & 1) << 2)) << 4), kb + (o < 0 ? 0 : o) + piece * 8, o >= 0);
+      for (int i = 0; i < 16 / KEYS; ++i) {
+        const int key = i * KEYS + sub;
+        const bool in = key < n;
+        cp_async16(dst + key * (D * 2) + ((piece ^ ((key & 1) << 2)) << 4), in ? ka : kb, in);
+        cp_async16(dst + Shape::kHalf + key * (D * 2) + ((piece ^ (((key >> 1) & 3) << 1)) << 4), in ? va : vb, in);
+        ka += KEYS * p.cache.k.token;
+        va += KEYS * p.cache.v.token;
+      }
+    } else {
+      there = __ballot_sync(0xffffffffu, k_off >= 0) & 0xffffu;
+#pragma unroll 1
+      for (int i = 0; i < 16 / KEYS; ++i) {
+        const int key = i * KEYS + sub;
+        const int64_t ko = __shfl_sync(0xffffffffu, k_off, key), vo = __shfl_sync(0xffffffffu, v_off, key);
+        cp_async16(dst + key * (D * 2) + ((piece ^ ((key & 1) << 2)) << 4), kb + (ko < 0 ? 0 : ko) + piece * 8, ko >= 0);
+        cp_async16(dst + Shape::kHalf + key * (D * 2) + ((piece ^ (((key >> 1) & 3) << 1)) << 4), vb + (vo < 0 ? 0 : vo) + piece * 8, vo >= 0);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 16 / KEYS; ++i) {
-      const int key = i * KEYS + sub;
-      const int64_t o = __shfl_sync(0xffffffffu, v_off, key);
-      cp_async16(dst + Shape::kHalf + key * (D * 2) + ((piece ^ (((key >> 1) & 3) << 1)) << 4), vb + (o < 0 ? 0 : o) + piece * 8, o >= 0);
-    }
+    if (lane == 0) there_s[warp][stage] = there;
     j_load += STEP;
-    if (++s_load == NS) s_load = 0;
   };
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    there_ring[i] = 0;
-    if (i < NS - 1) {
-      if (j_load < keys) fetch(there_ring[i]);
-      cp_async_commit();
-    }
+#pragma unroll 1
+  for (int i = 0; i < NS - 1; ++i) {
+    if (j_load < keys) fetch(i);
+    cp_async_commit();
   }
 
   // queries: row 8 r + g, the pieces of this lane
@@ -220,22 +249,24 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
         }
     }
     // scores in units of log2; keys that are not there or that the row does not see count as -inf
-    const bool edge = j0 + 16 > min_limit;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[r][e] *= p.scale2;
+    if (j0 + 16 > min_limit || there != 0xffffu) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((there >> (8 * (e >> 1) + g)) & 1) || j0 + 8 * (e >> 1) + g >= limit[r][e & 1]) s[r][e] = NEG_INF;
+    }
     bool moves = false;
     float mx[RB][2];
 #pragma unroll
     for (int r = 0; r < RB; ++r)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        mx[r][e] = NEG_INF;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          bool seen = (there >> (8 * b + g)) & 1;
-          if (edge) seen = seen && j0 + 8 * b + g < limit[r][e];
-          const float x = seen ? s[r][2 * b + e] * p.scale2 : NEG_INF;
-          s[r][2 * b + e] = x;
-          mx[r][e] = fmaxf(mx[r][e], x);
-        }
+        mx[r][e] = fmaxf(s[r][e], s[r][2 + e]);
         moves = moves || mx[r][e] > m_ref[r][e] + 8.0f;
       }
     if (__any_sync(0xffffffffu, moves)) {
@@ -285,28 +316,24 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
       }
     }
   };
-  int j0 = key0 + warp * 16;
-  for (;;) {
-    bool done = false;
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      if (j0 >= keys) { done = true; break; }
-      cp_async_wait<NS - 2>();
-      __syncwarp();
-      // the stage behind (that of the step before, which every lane has read) is filled again
-      if (j_load < keys) fetch(there_ring[(i + NS - 1) % NS]);
-      cp_async_commit();
-      step(there_ring[i], ring + i * 2 * Shape::kHalf, j0);
-      j0 += STEP;
-    }
-    if (done) break;
+  int stage = 0;
+#pragma unroll 1
+  for (int j0 = key0 + rank * 16; j0 < keys; j0 += STEP) {
+    cp_async_wait<NS - 2>();
+    __syncwarp();
+    // the stage behind (that of the step before, which every lane has read) is filled again
+    if (j_load < keys) fetch(stage == 0 ? NS - 1 : stage - 1);
+    cp_async_commit();
+    step(there_s[warp][stage], ring + stage * 2 * Shape::kHalf, j0);
+    if (++stage == NS) stage = 0;
   }
-  __syncthreads();  // every warp is done with its ring: the sums go there
+  named_bar_sync(1 + team, 32 * warps);  // every warp of the item is done with its ring: the sums go there
 
-  // the four warps' parts of a row
+  // the warps' parts of a row
   constexpr int PITCH = D + 4;
-  static_assert(PR_WARPS * TM * PITCH * 4 <= Shape::kSmem, "the sums fit in the rings");
+  static_assert(TM * PITCH * 4 <= Shape::kRing, "the sums of a warp fit in its ring");
   float* const o_s = reinterpret_cast<float*>(smem);
+  constexpr int OWN = Shape::kRing / 4;
 #pragma unroll
   for (int r = 0; r < RB; ++r)
 #pragma unroll
@@ -317,25 +344,23 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
       if (g == 0) ml_s[warp][lr] = make_float2(m_ref[r][e], l[r][e]);
 #pragma unroll
       for (int b = 0; b < VB; ++b) {  // columns 64 b + 8 g + 2 j + {0, 1}
-        float* dst = o_s + (warp * TM + lr) * PITCH + 64 * b + 8 * g;
+        float* dst = o_s + warp * OWN + lr * PITCH + 64 * b + 8 * g;
         reinterpret_cast<float4*>(dst)[0] = make_float4(o[r][b][0][e], o[r][b][0][2 + e], o[r][b][1][e], o[r][b][1][2 + e]);
         reinterpret_cast<float4*>(dst)[1] = make_float4(o[r][b][2][e], o[r][b][2][2 + e], o[r][b][3][e], o[r][b][3][2 + e]);
       }
     }
-  __syncthreads();
+  named_bar_sync(1 + team, 32 * warps);
   constexpr int PIECES = D / 4;
-  for (int i = threadIdx.x; i < TM * PIECES; i += PR_WARPS * 32) {
+  for (int i = rank * 32 + lane; i < TM * PIECES; i += 32 * warps) {
     const int lr = i / PIECES, col = (i % PIECES) * 4, rho = it.rho0 + lr;
     if (rho >= it.rows) break;
     float m = NEG_INF, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < PR_WARPS; ++w) m = fmaxf(m, ml_s[w][lr].x);
+    for (int w = team * warps; w < (team + 1) * warps; ++w) m = fmaxf(m, ml_s[w][lr].x);
     const float ref = m == NEG_INF ? 0.0f : m;
     float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-    for (int w = 0; w < PR_WARPS; ++w) {
+    for (int w = team * warps; w < (team + 1) * warps; ++w) {
       const float a = ex2(ml_s[w][lr].x - ref);
-      const float4 x = *reinterpret_cast<const float4*>(o_s + (w * TM + lr) * PITCH + col);
+      const float4 x = *reinterpret_cast<const float4*>(o_s + w * OWN + lr * PITCH + col);
       sum += a * ml_s[w][lr].y;
       acc.x += a * x.x; acc.y += a * x.y; acc.z += a * x.z; acc.w += a * x.w;
     }
@@ -349,7 +374,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) prefix_rows_kernel(const __g
 }
 
 template <int D, int RB>
-int launch_rows(const RowsParams& rp, int64_t items, cudaStream_t st) {
+int launch_rows(const RowsParams& rp, int64_t blocks, cudaStream_t st) {
   int dev = 0;
   VX_CUDA_OK(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_done{0};
@@ -358,7 +383,7 @@ int launch_rows(const RowsParams& rp, int64_t items, cudaStream_t st) {
     VX_CUDA_OK(cudaFuncSetAttribute(prefix_rows_kernel<D, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsShape<D>::kSmem));
     if (cached) attr_done.fetch_or(1ull << dev, std::memory_order_release);
   }
-  VX_CUDA_OK(launch_dependent(prefix_rows_kernel<D, RB>, dim3(static_cast<unsigned>(items)), dim3(PR_WARPS * 32), RowsShape<D>::kSmem, st, rp));
+  VX_CUDA_OK(launch_dependent(prefix_rows_kernel<D, RB>, dim3(static_cast<unsigned>(blocks)), dim3(PR_WARPS * 32), RowsShape<D>::kSmem, st, rp));
   return 0;
 }
 
@@ -437,6 +462,8 @@ int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int64_t unit, 
   return static_cast<int>(c < all ? c : all);
 }
 
+int64_t rows_resident(int blocks, int head_dim) { return static_cast<int64_t>(rows_ctas(blocks, head_dim)) * sm_count(); }
+
 int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, PrefixParams& p, Plan& plan) {
   const int rc = check_paged(cache, rows, p.cache, p.rows);
   if (rc) return rc;
@@ -483,7 +510,7 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     const int64_t items = static_cast<int64_t>(sp.slots) * p.kv_heads, sms = sm_count();
     if (kernel == Plan::kPairs) sp.chunk = chunk_keys(cap, items, sms, 256, 1024, 4);
     else if (kernel == Plan::kTiles) sp.chunk = chunk_keys(cap, items, 2 * sms, 128, 512, owners == 1 ? 1 : 2);
-    else sp.chunk = chunk_keys(cap, items, 2 * sms, 16 * PR_WARPS, cache->head_dim == 64 ? 512 : 256, 8);
+    else sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim), 16 * PR_WARPS, cache->head_dim == 64 ? 512 : 256, 8);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
   plan.span[0] = plan.span[1] = kNoSpan;
@@ -544,13 +571,19 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
       if (e) return e;
     }
   if (walks(Plan::kRows)) {
-    RowsParams rp{p, {part(Plan::kRows, 0), part(Plan::kRows, 1)}, 0};
-    const int64_t first = static_cast<int64_t>(rp.span[0].slots) * rp.span[0].chunks * p.kv_heads;
-    const int64_t items = first + static_cast<int64_t>(rp.span[1].slots) * rp.span[1].chunks * p.kv_heads;
-    if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
-    rp.first_items = static_cast<int32_t>(first);
-    const int e = d64 ? (plan.blocks == 2 ? launch_rows<64, 2>(rp, items, st) : launch_rows<64, 1>(rp, items, st))
-                      : (plan.blocks == 2 ? launch_rows<128, 2>(rp, items, st) : launch_rows<128, 1>(rp, items, st));
+    RowsParams rp{p, {part(Plan::kRows, 0), part(Plan::kRows, 1)}, {1, 1}, 0, walks(Plan::kPairs) || walks(Plan::kTiles) ? 1 : 0};
+    int64_t blocks = 0;
+    for (int i = 0; i < 2; ++i) {
+      const Span& sp = rp.span[i];
+      const int64_t items = static_cast<int64_t>(sp.slots) * sp.chunks * p.kv_heads;
+      // All four warps of a CTA on an item while one round of CTAs takes them all, else so many that each has about 128 keys.
+      rp.warps[i] = items <= rows_resident(plan.blocks, cache->head_dim) || sp.chunk > 256 ? 4 : (sp.chunk > 128 ? 2 : 1);
+      blocks += (items * rp.warps[i] + PR_WARPS - 1) / PR_WARPS;
+      if (i == 0) rp.first_blocks = static_cast<int32_t>(blocks);
+    }
+    if (blocks >= (1ll << 31)) return fail(-1, "too much work for one call (%lld blocks)", (long long)blocks);
+    const int e = d64 ? (plan.blocks == 2 ? launch_rows<64, 2>(rp, blocks, st) : launch_rows<64, 1>(rp, blocks, st))
+                      : (plan.blocks == 2 ? launch_rows<128, 2>(rp, blocks, st) : launch_rows<128, 1>(rp, blocks, st));
     if (e) return e;
   }
   JoinParams jp{p, {plan.span[0], plan.span[1]}};

@@ -193,28 +193,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   const PrefixParams& p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < NK; ++s) {
-      mbar_init(&bar.k_full[s], 128);  // the loaders' threads
-      mbar_init(&bar.k_empty[s], 1);
+  if (warp < 2) {  // each lane some barriers
+    const int s = warp;  // slot, stream
+    for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], 4);
+    if (lane < PT_ITEMS) {
+      mbar_init(&bar.item_full[s][lane], 1);
+      mbar_init(&bar.item_empty[s][lane], 4 + 1 + 8 / STREAMS);  // warps that read an item: loaders, MMA issuer, softmax
     }
-    for (int s = 0; s < NV; ++s) {
-      mbar_init(&bar.v_full[s], 128);
-      mbar_init(&bar.v_empty[s], 1);
+    if (lane < NB) {
+      mbar_init(&bar.s_full[s][lane], 1);
+      mbar_init(&bar.p_full[s][lane], 4);
+      mbar_init(&bar.pv_done[s][lane], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      for (int i = 0; i < NB; ++i) {
-        mbar_init(&bar.s_full[s][i], 1);
-        mbar_init(&bar.p_full[s][i], 4);
-        mbar_init(&bar.pv_done[s][i], 1);
-      }
+    if (lane == 0) {
       mbar_init(&bar.q_full[s], 32);
       mbar_init(&bar.q_empty[s], 1);
-      for (int i = 0; i < PT_MASKS; ++i) mbar_init(&bar.mask_full[s][i], 4);
-      for (int i = 0; i < PT_ITEMS; ++i) {
-        mbar_init(&bar.item_full[s][i], 1);
-        mbar_init(&bar.item_empty[s][i], 4 + 1 + 8 / STREAMS);  // warps that read an item: loaders, MMA issuer, softmax
-      }
+    }
+    const int n = s == 0 ? NK : NV;
+    if (lane < n) {
+      mbar_init(s == 0 ? &bar.k_full[lane] : &bar.v_full[lane], 128);  // the loaders' threads
+      mbar_init(s == 0 ? &bar.k_empty[lane] : &bar.v_empty[lane], 1);
     }
     mbar_fence_init();
   }
