@@ -108,6 +108,7 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 // The barrier is arrived at once for this thread when its copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
@@ -257,45 +258,72 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       int stage = 0;
       uint32_t phase = 0;
     };
-    auto load = [&](Ring& r, int stages, uint64_t* full, uint64_t* empty, uint32_t ring, const __nv_bfloat16* base, int64_t off) {
+    // Where the warp's keys of a tile are: off, n of the first and the number there when they lie on one page (the others follow the first),
+    // else off of key `lane`, -1 where it is not there.
+    const bool whole_pages = p.cache.page_size.d % MINE == 0;
+    auto load = [&](Ring& r, int stages, uint64_t* full, uint64_t* empty, uint32_t ring, const __nv_bfloat16* base, int64_t token, int64_t off, int n) {
       ok = __all_sync(ALL, mbar_wait(&empty[r.stage], r.phase ^ 1, p.status, 40));
       if (!ok) return;
-      const uint32_t dst = ring + at + r.stage * Shape::kTile;
+      const uint32_t dst = ring + at + r.stage * Shape::kTile + (w * MINE + sub) * 128;
+      const uint32_t swz = ((piece & 7) ^ sub) << 4;  // (key & 7 = sub + a multiple of KEYS)
+      if (whole_pages) {
+        const __nv_bfloat16* src = base + off + sub * token + piece * 8;
+        const int64_t step = KEYS * token;
+        if (n == MINE) {
 #pragma unroll
-      for (int i = 0; i < MINE / KEYS; ++i) {
-        const int key = i * KEYS + sub;
-        const int64_t o = __shfl_sync(ALL, off, key);
-        cp_async16(dst + (w * MINE + key) * 128 + (((piece & 7) ^ (key & 7)) << 4), base + (o < 0 ? 0 : o) + piece * 8, o >= 0);
+          for (int i = 0; i < MINE / KEYS; ++i) {
+            cp_async16(dst + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), src);
+            src += step;
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < MINE / KEYS; ++i) {
+            const bool in = i * KEYS + sub < n;
+            cp_async16(dst + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), in ? src : base, in);
+            src += step;
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < MINE / KEYS; ++i) {
+          const int64_t o = __shfl_sync(ALL, off, i * KEYS + sub);
+          cp_async16(dst + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), base + (o < 0 ? 0 : o) + piece * 8, o >= 0);
+        }
       }
       cp_async_arrive(&full[r.stage]);
       if (++r.stage == stages) { r.stage = 0; r.phase ^= 1; }
     };
     Ring kr, vr;
-    auto load_k = [&](int head, int64_t off) { load(kr, NK, bar.k_full, bar.k_empty, smem_u32(k_ring), p.cache.k.p + head * p.cache.k.head, off); };
-    auto load_v = [&](int head, int64_t off) { load(vr, NV, bar.v_full, bar.v_empty, smem_u32(v_ring), p.cache.v.p + head * p.cache.v.head, off); };
-    // A stream's place: what of its present item the keys' places depend on.  The page of this lane's key of the next tile is looked up a
-    // tile ahead.
+    auto load_k = [&](int head, int64_t off, int n) {
+      load(kr, NK, bar.k_full, bar.k_empty, smem_u32(k_ring), p.cache.k.p + head * p.cache.k.head, p.cache.k.token, off, n);
+    };
+    auto load_v = [&](int head, int64_t off, int n) {
+      load(vr, NV, bar.v_full, bar.v_empty, smem_u32(v_ring), p.cache.v.p + head * p.cache.v.head, p.cache.v.token, off, n);
+    };
+    // A stream's place: what of its present item the keys' places depend on.  The page of the next tile's keys is looked up a tile ahead.
     struct Place {
       Items items;
       int left = 0, masks = 0;  // tiles left of the item, tiles of the stream so far
       int v = 0, p128 = 0, p_keys = 0, o_keys = 0, group = 0, sequence = 0, head = 0;
-      int page = -1;
+      int page = -1, n = 0;     // n: keys of this warp that the item has
       uint32_t slot = 0;
       bool over = false;
     };
     auto look_up = [&](Place& c) {
       const bool own = c.v >= c.p128;
-      const int j = c.v - (own ? c.p128 : 0) + w * MINE + lane;
+      const int first = c.v - (own ? c.p128 : 0) + w * MINE;
+      c.n = min((own ? c.o_keys : c.p_keys) - first, MINE);
+      const int i = whole_pages ? 0 : lane, j = first + i;
       c.page = -1;
-      if (lane < MINE && j < (own ? c.o_keys : c.p_keys)) {
+      if (i < c.n) {
         const PagedTable& table = own ? p.rows.table : p.prefix;
         uint32_t index;
         p.cache.page_size.divmod(static_cast<uint32_t>(j), index, c.slot);
         c.page = table.table[static_cast<int64_t>(own ? c.sequence : c.group) * table.ld + index];  // (keys end where the table does)
       }
     };
-    int64_t v_prev = -1;  // of the tile before
-    int head_prev = -1;
+    int64_t v_prev = 0;  // of the tile before
+    int head_prev = -1, n_prev = 0;
     int x = 0;            // tiles so far
     // one tile of a stream, if it has one left
     auto tile = [&](Place& c, int stream) {
@@ -312,13 +340,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         look_up(c);
       }
       const bool in = c.page >= 0 && c.page < p.cache.pages;
-      const int64_t k_off = in ? c.page * p.cache.k.page + c.slot * p.cache.k.token : -1;
-      const int64_t v_off = in ? c.page * p.cache.v.page + c.slot * p.cache.v.token : -1;
-      const uint32_t there = __ballot_sync(ALL, in);
+      const int64_t none = whole_pages ? 0 : -1;
+      const int64_t k_off = in ? c.page * p.cache.k.page + c.slot * p.cache.k.token : none;
+      const int64_t v_off = in ? c.page * p.cache.v.page + c.slot * p.cache.v.token : none;
+      const int n = in ? c.n : 0;  // (whole pages)
+      const uint32_t there = whole_pages ? low_bits(n) : __ballot_sync(ALL, in);
       --c.left;
       c.v += BN;
       if (c.left > 0) look_up(c);
-      load_k(c.head, k_off);
+      load_k(c.head, k_off, n);
       if (!ok) return;
       // (the softmax has read the mask PT_MASKS tiles of the stream before this one: PT_MASKS is more than NK + the tiles of a slot whose S is
       // issued and whose P is not read)
@@ -331,8 +361,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       }
       ++c.masks;
       ++x;
-      if (head_prev >= 0) load_v(head_prev, v_prev);
+      if (head_prev >= 0) load_v(head_prev, v_prev, n_prev);
       v_prev = v_off;
+      n_prev = n;
       head_prev = c.head;
     };
     Place a, b;
@@ -341,7 +372,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       tile(a, 0);
       if (STREAMS == 2 && ok) tile(b, 1);
     }
-    if (ok && head_prev >= 0) load_v(head_prev, v_prev);
+    if (ok && head_prev >= 0) load_v(head_prev, v_prev, n_prev);
     cp_async_wait_all();
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
