@@ -66,13 +66,31 @@ __device__ __forceinline__ int find_owner(const int32_t* offsets, int n, int x) 
   return lo;
 }
 
+// Largest o in [0, n) with first(o) <= x (first ascending), and 0 if there is none, by a whole warp: 32 places a turn instead of one, each
+// turn one round trip to memory (120 sequences: 2 instead of 7, 3 us of a CTA that lives for 8).
+template <class First>
+__device__ __forceinline__ int find_by_warp(int n, int x, First first) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, lane == 0 || (at < hi && first(at) <= x));
+    lo += (31 - __clz(below)) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
 // Sequence of a row and the row's index among the call's rows of that sequence; false: no sequence, or one that takes no part.
+// WARP: all lanes of the warp ask for the same row.
+template <bool WARP = false>
 __device__ __forceinline__ bool row_sequence(const KvRows& kr, int row, int& s, int& i) {
   s = row;
   i = 0;
   if (kr.sequences == 0) return false;
   if (kr.row_offsets) {
-    s = find_owner(kr.row_offsets, kr.sequences, row);
+    if (WARP) s = find_by_warp(kr.sequences, row, [&](int o) { return kr.row_offsets[o]; });
+    else s = find_owner(kr.row_offsets, kr.sequences, row);
     i = row - kr.row_offsets[s];
     if (i < 0 || row >= kr.row_offsets[s + 1]) return false;
   }

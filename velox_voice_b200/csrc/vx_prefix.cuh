@@ -59,11 +59,12 @@ __device__ __forceinline__ int owner_row0(const PrefixParams& p, bool sequences,
   return sequence_row0(p, sequences ? o : group_sequence0(p, o));
 }
 
-// group of a sequence, -1: none
+// group of a sequence, -1: none (WARP: all lanes of the warp ask for the same one)
+template <bool WARP = false>
 __device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
   if (p.groups == 0) return -1;
   if (!p.group_offsets) return s / p.group_size;
-  const int g = find_owner(p.group_offsets, p.groups, s);
+  const int g = WARP ? find_by_warp(p.groups, s, [&](int o) { return p.group_offsets[o]; }) : find_owner(p.group_offsets, p.groups, s);
   return s >= p.group_offsets[g] && s < p.group_offsets[g + 1] ? g : -1;
 }
 
@@ -86,8 +87,8 @@ struct ItemRows {
 };
 
 // Owner and tile of a slot.  With offsets, owner o has the slots [base(o), base(o + 1)), base(o) = floor(row0(o) per_kv / TM) + o: enough for
-// its tiles, and found by a search without a pass over all owners.
-template <int TM>
+// its tiles, and found by a search without a pass over all owners.  WARP: all lanes of the warp ask for the same slot.
+template <int TM, bool WARP = false>
 __device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp, int slot, ItemRows& it) {
   const int per = static_cast<int>(p.per_kv.d);
   const bool sequences = sp.kind != kSpanPrefix;
@@ -99,7 +100,8 @@ __device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp,
   } else {
     auto base = [&](int o) { return static_cast<int>(static_cast<int64_t>(owner_row0(p, sequences, o)) * per / TM) + o; };
     int lo = 0, hi = owners;  // largest o with base(o) <= slot
-    while (hi - lo > 1) {
+    if (WARP) lo = find_by_warp(owners, slot, base);
+    while (!WARP && hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (base(mid) <= slot) lo = mid;
       else hi = mid;

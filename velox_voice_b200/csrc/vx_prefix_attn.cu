@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_k
   if (chunk >= sp.chunks) return;
   const bool own = sp.kind == kSpanOwn;
   ItemRows it;
-  if (!find_rows<TM>(p, sp, n - chunk * sp.slots, it)) return;
+  if (!find_rows<TM, true>(p, sp, n - chunk * sp.slots, it)) return;
   const int length = own ? p.rows.lengths[it.owner] : 0;
   // keys [key0, keys): those of the chunk that the tile's last row sees
   int keys = own ? own_keys(p, length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(min(it.rho0 + TM, it.rows) - 1)))) : prefix_keys(p, it.owner);
@@ -409,9 +409,9 @@ __global__ void __launch_bounds__(JN_WARPS * 32) prefix_join_kernel(const __grid
   pdl_wait();
   const bool in = h < p.q_heads;
   int parts[2] = {0, 0}, s, i;
-  if (row_sequence(p.rows, row, s, i)) {
+  if (row_sequence<true>(p.rows, row, s, i)) {
     if (jp.span[0].part0 < 0) return;  // its row is there already
-    const int prefix = prefix_keys(p, group_of(p, s)), own = own_keys(p, p.rows.lengths[s], i);
+    const int prefix = prefix_keys(p, group_of<true>(p, s)), own = own_keys(p, p.rows.lengths[s], i);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const Span& sp = jp.span[e];
