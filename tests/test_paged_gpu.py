@@ -330,6 +330,77 @@ def test_attention_long_own_context(ops, heads, kv, d):
     check_attention(ops, lengths=[3000, 17], rows_of=[35, 70], heads=heads, kv=kv, d=d, ps=64)
 
 
+def dense_reference(q, k_pages, v_pages, table, length, ptable, prefix, groups, scale=None):
+    """fp64 on the device, for sequences of one length and groups of one size: q [n, tokens, heads, d], `length` own tokens before them.
+    Returns (out, spread) like the oracle."""
+    n, tokens, heads, d = q.shape
+    ps, kv = k_pages.shape[1], k_pages.shape[2]
+    own = length + tokens
+    out, spread = torch.empty(n, tokens, heads, d, dtype=torch.float64, device="cuda"), torch.empty(n, tokens, heads, d, dtype=torch.float64, device="cuda")
+    j = torch.arange(own, device="cuda")
+    late = j > length + torch.arange(tokens, device="cuda")[:, None]
+    jp = torch.arange(prefix, device="cuda")
+    for s in range(n):
+        parts = []
+        for cache in (k_pages, v_pages):
+            x = cache[table[s].long()[j // ps], j % ps]
+            if prefix:
+                x = torch.cat([cache[ptable[s // (n // groups)].long()[jp // ps], jp % ps], x])
+            parts.append(x.double().permute(1, 0, 2))  # [kv, keys, d]
+        x = torch.einsum("htd,hjd->htj", q[s].double().transpose(0, 1), parts[0].repeat_interleave(heads // kv, 0)) * (d ** -0.5 if scale is None else scale)
+        x[:, :, prefix:].masked_fill_(late, float("-inf"))
+        w = torch.softmax(x, -1)
+        v = parts[1].repeat_interleave(heads // kv, 0)
+        out[s], spread[s] = (w @ v).transpose(0, 1), (w @ v.abs()).transpose(0, 1)
+    return out, spread
+
+
+@pytest.mark.parametrize("n,tokens,groups,heads,kv,d,length,prefix", [
+    (1250, 3, 50, 64, 8, 128, 150, 300),   # more items for every stream of the tile kernel than are looked up at a time, pairs for the prefixes
+    (50, 600, 5, 32, 32, 64, 3, 100),      # the same for pairs that take prefix and own tokens in a row
+    (600, 1, 3, 16, 4, 64, 300, 5000),     # many rows of a group, few of a sequence
+    (3000, 1, 1, 8, 8, 64, 20, 0),         # short own runs, a warp each
+    (2, 1, 2, 32, 8, 128, 40000, 30000),   # few rows over many keys: many parts of a row
+    (7, 700, 1, 12, 4, 128, 900, 3000),
+])
+def test_attention_large_calls(ops, n, tokens, groups, heads, kv, d, length, prefix):
+    ps = 16
+    width, pw = -(-(length + tokens) // ps), -(-prefix // ps)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    order = torch.randperm(n * width + groups * pw, generator=g, device="cuda").to(torch.int32)
+    table, ptable = order[:n * width].view(n, width), order[n * width:].view(groups, pw)
+    k_pages, v_pages = make_cache(order.numel(), ps, kv, d, seed=n)
+    q = torch.randn(n, tokens, heads, d, generator=g, device="cuda").bfloat16()
+    kw = dict(prefix_table=ptable, prefix_lengths=ints([prefix] * groups)) if prefix else {}
+    off = None if tokens == 1 else ints([tokens * i for i in range(n + 1)])
+    out = ops.prefix_attention(q.view(-1, heads, d), k_pages, v_pages, table, ints([length] * n), row_offsets=off, **kw).view(q.shape)
+    want, spread = dense_reference(q, k_pages, v_pages, table, length, ptable, prefix, groups)
+    err = (out.double() - want).abs() - (2.0 ** -8 * (want.abs() + spread) + 2.0 ** -13 * spread)
+    assert (err <= 0).all(), err.max().item()
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_attention_random_calls(ops, seed):
+    rng = np.random.default_rng(seed)
+    heads, kv, d = [(2, 2, 64), (8, 2, 64), (6, 1, 128), (4, 4, 128), (10, 2, 128), (16, 1, 64)][rng.integers(6)]
+    groups = int(rng.integers(0, 5))
+    sizes = [int(rng.integers(0, 9)) for _ in range(groups)] if groups else [int(rng.integers(1, 12))]
+    n = max(sum(sizes) + int(rng.integers(0, 2)), 1)  # perhaps a sequence of no group
+    tokens = [int(rng.integers(0, [2, 9, 40, 130][rng.integers(4)])) for _ in range(n)] if rng.random() < 0.7 else None
+    top = [3, 60, 300][rng.integers(3)]
+    lengths = [int(rng.integers(-1, top)) for _ in range(n)]
+    prefix = [int(rng.integers(0, [5, 200, 900][rng.integers(3)])) for _ in range(groups)]
+
+    def edit(t):
+        if rng.random() < 0.5:
+            t[rng.random(t.shape) < 0.2] = [-1, 10 ** 7][rng.integers(2)]
+
+    check_attention(ops, lengths=lengths, rows_of=tokens, prefix=prefix, sizes=sizes if groups else None, heads=heads, kv=kv, d=d,
+                    ps=[1, 5, 16, 24, 32, 64][rng.integers(6)], layout=["tokens", "heads", "wide"][rng.integers(3)], spread=[0.5, 1.0, 4.0][rng.integers(3)],
+                    seed=seed, edit=edit, edit_prefix=edit, first_row=int(rng.integers(0, 3)) if tokens else 0, last_rows=int(rng.integers(0, 3)) if tokens else 0,
+                    extra_width=[0, 0, 3, 400][rng.integers(4)])
+
+
 def test_attention_offsets_beyond_32_bits(ops):
     """Pages more than 2^31 elements into the cache."""
     ps, kv, d = 64, 8, 128
