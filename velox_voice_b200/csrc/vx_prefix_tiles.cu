@@ -11,8 +11,10 @@
 //              finds its next S.  Tensor memory of a slot: S0 | S1 (64 columns each, P over them) | O.
 // Roles:
 //   warps 0..3, 4..7  softmax of slot 0, 1: a query row per thread straight out of tensor memory
-//   warps 8..11       loaders: a quarter of every tile's keys each, page by page (cp.async, 16 bytes; keys that are not there are filled with
-//                     zeros and marked in a bit mask), K and V into rings of their own in the order K0, K1, V0, K2, V1, ...
+//   warps 8..11       loaders, K and V into rings of the stream, page by page (cp.async, 16 bytes; keys that are not there are filled with zeros
+//                     and marked in a bit mask).  PAIRED each takes a quarter of every tile (with whole tiles in turn a tile was 2 us late); else
+//                     two warps per stream take its tiles in turn (with quarters 1,500 of 1,950 cycles went into what a tile costs whatever its
+//                     size, and the loaders were the bound).
 //   warps 12, 15      MMA issuers.  A thread that issues is held while its products run, so the slots of two streams have one each: what it
 //                     has to wait for and to look up between two tiles passes under the other's products (one issuer for both spent 60 % of its
 //                     time between products).  PAIRED has one for both slots, whose products must not mix: two issuers without turns
@@ -55,9 +57,10 @@ struct TileShape {
   static constexpr int kPanel = kKeys * 128;                  // 64 bf16 of every key
   static constexpr int kTile = D / 64 * kPanel;               // bytes of a K or V tile
   static constexpr int kQ = D / 64 * PT_Q_PANEL;              // of a slot's queries
-  static constexpr int kStagesK = PAIRED ? (D == 128 ? 3 : 5) : 5 * (128 / D), kStagesV = PAIRED ? (D == 128 ? 2 : 5) : 5 * (128 / D);
-  static_assert(PAIRED || kStagesK == kStagesV);
-  static constexpr int kSmem = 2 * kQ + (kStagesK + kStagesV) * kTile + 1024;
+  static constexpr int kStreams = PAIRED ? 1 : 2;
+  static constexpr int kParts = PAIRED ? 4 : 1;               // loaders that share a tile
+  static constexpr int kStagesK = D == 128 ? 3 : 5, kStagesV = D == 128 ? 2 : 5;  // of a stream
+  static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + 1024;
 };
 
 struct TilesParams {
@@ -78,11 +81,11 @@ struct TileItem {
 
 template <class Shape>
 struct TileBarriers {
-  uint64_t k_full[Shape::kStagesK], k_empty[Shape::kStagesK], v_full[Shape::kStagesV], v_empty[Shape::kStagesV];
+  uint64_t k_full[Shape::kStreams][Shape::kStagesK], k_empty[Shape::kStreams][Shape::kStagesK];
+  uint64_t v_full[Shape::kStreams][Shape::kStagesV], v_empty[Shape::kStreams][Shape::kStagesV];
   uint64_t s_full[2][Shape::kBuffers], p_full[2][Shape::kBuffers], pv_done[2][Shape::kBuffers], q_full[2], q_empty[2];
   uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
-  alignas(8) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
-  int32_t place[2][PT_MASKS];  // of the tile among all of the CTA: its stage in both rings
+  alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
   TileItem item[2][PT_ITEMS];
   uint32_t tmem_base;
 };
@@ -189,17 +192,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* const k_ring = q_s + 2 * Shape::kQ;
-  uint8_t* const v_ring = k_ring + NK * Shape::kTile;
+  uint8_t* const v_ring = k_ring + STREAMS * NK * Shape::kTile;
   __shared__ TileBarriers<Shape> bar;
   const PrefixParams& p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp < 2) {  // each lane some barriers
     const int s = warp;  // slot, stream
-    for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], 4);
+    for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], Shape::kParts);
     if (lane < PT_ITEMS) {
       mbar_init(&bar.item_full[s][lane], 1);
-      mbar_init(&bar.item_empty[s][lane], 4 + 1 + 8 / STREAMS);  // warps that read an item: loaders, MMA issuer, softmax
+      mbar_init(&bar.item_empty[s][lane], 4 / STREAMS + 1 + 8 / STREAMS);  // warps that read an item: loaders, MMA issuer, softmax
     }
     if (lane < NB) {
       mbar_init(&bar.s_full[s][lane], 1);
@@ -210,10 +213,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       mbar_init(&bar.q_full[s], 32);
       mbar_init(&bar.q_empty[s], 1);
     }
-    const int n = s == 0 ? NK : NV;
-    if (lane < n) {
-      mbar_init(s == 0 ? &bar.k_full[lane] : &bar.v_full[lane], 128);  // the loaders' threads
-      mbar_init(s == 0 ? &bar.k_empty[lane] : &bar.v_empty[lane], 1);
+    if (s < STREAMS && lane < NK) {
+      mbar_init(&bar.k_full[s][lane], 32 * Shape::kParts);  // threads of the loaders that share a tile
+      mbar_init(&bar.k_empty[s][lane], 1);
+    }
+    if (s < STREAMS && lane < NV) {
+      mbar_init(&bar.v_full[s][lane], 32 * Shape::kParts);
+      mbar_init(&bar.v_empty[s][lane], 1);
     }
     mbar_fence_init();
   }
@@ -227,8 +233,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   const uint32_t tmem_base = bar.tmem_base;
   pdl_wait();
   pdl_launch_dependents();
-  // Registers: 128 a thread at launch, 512 for a thread of each of the four warpgroups.  The softmax, which holds a row of S, takes 192 in
-  // two of them, the other two leave 64 each (2 x 192 + 2 x 64 = 512); every warp of a warpgroup passes the same setmaxnreg.
+  // Registers: 128 a thread at launch, 512 for a thread of each of the four warpgroups.  The softmax, which holds a row of S, takes more in
+  // two of them, the other two leave as many (2 n + 2 (256 - n) = 512); every warp of a warpgroup passes the same setmaxnreg.
+  constexpr int SOFTMAX_REGS = PAIRED ? 192 : 168;
 
   // The items of a stream, one after another: waits for the next, copies it, hands its place back.
   struct Items {
@@ -246,136 +253,139 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 
   if (warp >= 8 && warp < 12) {
     // =========================== loaders ===========================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    const int w = warp - 8;
-    constexpr int MINE = BN / 4;           // keys of a tile per warp
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - SOFTMAX_REGS));
+    constexpr int PARTS = Shape::kParts, TEAM = 4 / STREAMS / PARTS;  // loaders that share a tile, that take tiles in turn
+    constexpr int MINE = BN / PARTS, GROUPS = MINE / 16, PER_LANE = MINE / 32;
+    const int stream = (warp - 8) / (4 / STREAMS), part = (warp - 8) % PARTS, rank = (warp - 8) / PARTS % TEAM;
     constexpr int LANES = D / 8;           // lanes that share a key
     constexpr int KEYS = 32 / LANES;       // keys per instruction
     const int piece = lane % LANES, sub = lane / LANES;
-    const uint32_t at = (piece >> 3) * Shape::kPanel;
+    const uint32_t at = (piece >> 3) * Shape::kPanel + (part * MINE + sub) * 128, swz = ((piece & 7) ^ sub) << 4;  // (key & 7 = sub + a multiple of KEYS)
+    const bool whole_pages = p.cache.page_size.d % 16 == 0;  // 16 keys from a multiple of 16 on lie on one page
     bool ok = true;
-    struct Ring {
-      int stage = 0;
-      uint32_t phase = 0;
-    };
-    // Where the warp's keys of a tile are: off, n of the first and the number there when they lie on one page (the others follow the first),
-    // else off of key `lane`, -1 where it is not there.
-    const bool whole_pages = p.cache.page_size.d % MINE == 0;
-    auto load = [&](Ring& r, int stages, uint64_t* full, uint64_t* empty, uint32_t ring, const __nv_bfloat16* base, int64_t token, int64_t off, int n) {
-      ok = __all_sync(ALL, mbar_wait(&empty[r.stage], r.phase ^ 1, p.status, 40));
-      if (!ok) return;
-      const uint32_t dst = ring + at + r.stage * Shape::kTile + (w * MINE + sub) * 128;
-      const uint32_t swz = ((piece & 7) ^ sub) << 4;  // (key & 7 = sub + a multiple of KEYS)
-      if (whole_pages) {
-        const __nv_bfloat16* src = base + off + sub * token + piece * 8;
-        const int64_t step = KEYS * token;
-        if (n == MINE) {
+    // Where this warp's keys of a tile are, a table entry looked up per lane: with whole pages lane i has the first of keys [16 i, 16 i + 16) and
+    // how many of them there are, otherwise keys lane and lane + 32.
+    int page[PER_LANE], n = 0;
+    uint32_t place[PER_LANE];
+    TileItem t;
+    t.tiles = 0;
+    auto look_up = [&](int tile) {
+      const int v = t.v0 + tile * BN;
+      const bool own = v >= t.p128;
+      const int first = v - (own ? t.p128 : 0) + part * MINE, end = own ? t.o_keys : t.p_keys;
+      const PagedTable& table = own ? p.rows.table : p.prefix;
+      const int32_t* const row = table.table + static_cast<int64_t>(own ? t.sequence : t.group) * table.ld;
 #pragma unroll
-          for (int i = 0; i < MINE / KEYS; ++i) {
-            cp_async16(dst + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), src);
-            src += step;
-          }
-        } else {
+      for (int e = 0; e < PER_LANE; ++e) {
+        const int j = first + (whole_pages ? 16 * lane : lane + 32 * e);
+        if (e == 0) n = whole_pages && lane < GROUPS ? min(max(end - j, 0), 16) : 0;
+        page[e] = -1;
+        if (whole_pages ? e == 0 && n > 0 : j < end) {
+          uint32_t index;
+          p.cache.page_size.divmod(static_cast<uint32_t>(j), index, place[e]);
+          page[e] = row[index];  // (keys end where the table does)
+        }
+      }
+    };
+    struct Where {
+      int64_t off[PER_LANE];  // -1: not there (whole pages: see n)
+      int n, head;
+    };
+    auto where = [&](const PagedTensor& c) {
+      Where w;
+#pragma unroll
+      for (int e = 0; e < PER_LANE; ++e) w.off[e] = page[e] >= 0 ? page[e] * c.page + place[e] * c.token : (whole_pages ? 0 : -1);
+      w.n = n;
+      w.head = t.head;
+      return w;
+    };
+    auto copy = [&](uint64_t* full, uint32_t dst, const PagedTensor& c, const Where& w) {
+      const __nv_bfloat16* const base = c.p + w.head * c.head + piece * 8;
+      if (whole_pages) {
+        const int64_t step = KEYS * c.token;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int in = __shfl_sync(ALL, w.n, g);
+          const __nv_bfloat16* src = base + __shfl_sync(ALL, w.off[0], g) + sub * c.token;
+          if (in == 16) {
+#pragma unroll
+            for (int i = 0; i < 16 / KEYS; ++i) {
+              cp_async16(dst + g * 2048 + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), src);
+              src += step;
+            }
+          } else {
 #pragma unroll 1
-          for (int i = 0; i < MINE / KEYS; ++i) {
-            const bool in = i * KEYS + sub < n;
-            cp_async16(dst + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), in ? src : base, in);
-            src += step;
+            for (int i = 0; i < 16 / KEYS; ++i) {
+              const bool there = i * KEYS + sub < in;
+              cp_async16(dst + g * 2048 + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), there ? src : base, there);
+              src += step;
+            }
           }
         }
       } else {
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) {
 #pragma unroll 1
-        for (int i = 0; i < MINE / KEYS; ++i) {
-          const int64_t o = __shfl_sync(ALL, off, i * KEYS + sub);
-          cp_async16(dst + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), base + (o < 0 ? 0 : o) + piece * 8, o >= 0);
+          for (int i = 0; i < 32 / KEYS; ++i) {
+            const int64_t o = __shfl_sync(ALL, w.off[e], i * KEYS + sub);
+            cp_async16(dst + e * 4096 + i * (KEYS * 128) + (swz ^ (((i * KEYS) & 7) << 4)), base + (o < 0 ? 0 : o), o >= 0);
+          }
         }
       }
-      cp_async_arrive(&full[r.stage]);
-      if (++r.stage == stages) { r.stage = 0; r.phase ^= 1; }
+      cp_async_arrive(full);
     };
-    Ring kr, vr;
-    auto load_k = [&](int head, int64_t off, int n) {
-      load(kr, NK, bar.k_full, bar.k_empty, smem_u32(k_ring), p.cache.k.p + head * p.cache.k.head, p.cache.k.token, off, n);
+    const uint32_t k_at = smem_u32(k_ring) + stream * NK * Shape::kTile + at, v_at = smem_u32(v_ring) + stream * NV * Shape::kTile + at;
+    // K of tile m, then V of the tile before (PAIRED: its stage is free later than that of the next K) or of the same
+    auto load_v = [&](int m, const Where& w) {
+      const int vs = m % NV;
+      ok = __all_sync(ALL, mbar_wait(&bar.v_empty[stream][vs], (m / NV + 1) & 1, p.status, 53));
+      if (ok) copy(&bar.v_full[stream][vs], v_at + vs * Shape::kTile, p.cache.v, w);
     };
-    auto load_v = [&](int head, int64_t off, int n) {
-      load(vr, NV, bar.v_full, bar.v_empty, smem_u32(v_ring), p.cache.v.p + head * p.cache.v.head, p.cache.v.token, off, n);
-    };
-    // A stream's place: what of its present item the keys' places depend on.  The page of the next tile's keys is looked up a tile ahead.
-    struct Place {
-      Items items;
-      int left = 0, masks = 0;  // tiles left of the item, tiles of the stream so far
-      int v = 0, p128 = 0, p_keys = 0, o_keys = 0, group = 0, sequence = 0, head = 0;
-      int page = -1, n = 0;     // n: keys of this warp that the item has
-      uint32_t slot = 0;
-      bool over = false;
-    };
-    auto look_up = [&](Place& c) {
-      const bool own = c.v >= c.p128;
-      const int first = c.v - (own ? c.p128 : 0) + w * MINE;
-      c.n = min((own ? c.o_keys : c.p_keys) - first, MINE);
-      const int i = whole_pages ? 0 : lane, j = first + i;
-      c.page = -1;
-      if (i < c.n) {
-        const PagedTable& table = own ? p.rows.table : p.prefix;
-        uint32_t index;
-        p.cache.page_size.divmod(static_cast<uint32_t>(j), index, c.slot);
-        c.page = table.table[static_cast<int64_t>(own ? c.sequence : c.group) * table.ld + index];  // (keys end where the table does)
-      }
-    };
-    int64_t v_prev = 0;  // of the tile before
-    int head_prev = -1, n_prev = 0;
-    int x = 0;            // tiles so far
-    // one tile of a stream, if it has one left
-    auto tile = [&](Place& c, int stream) {
-      if (c.over) return;
-      if (c.left == 0) {
-        TileItem t;
-        ok = ok && next_item(stream, c.items, t);
-        if (!ok || t.tiles == 0) {
-          c.over = true;
-          return;
+    Items items;
+    Where v_due;
+    int first = 0;   // tile of the stream that the item begins with
+    while (ok) {
+      ok = next_item(stream, items, t);
+      if (!ok || t.tiles == 0) break;
+      int tile = (rank - first % TEAM + TEAM) % TEAM;  // this warp's are tiles rank, rank + TEAM, ... of the stream
+      if (tile < t.tiles) look_up(tile);
+      for (; ok && tile < t.tiles; tile += TEAM) {
+        const int m = first + tile, ks = m % NK;
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e)
+          if (page[e] >= p.cache.pages) page[e] = -1;
+        if (page[0] < 0) n = 0;
+        const Where k_where = where(p.cache.k), v_where = where(p.cache.v);
+        // which keys are there, in a word per lane (whole pages: 16 keys, else 32)
+        uint32_t there[PER_LANE];
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) there[e] = whole_pages ? low_bits(n) : __ballot_sync(ALL, page[e] >= 0);
+        if (tile + TEAM < t.tiles) look_up(tile + TEAM);
+        // (the m-th tile is the m / stages-th use of its stage)
+        ok = __all_sync(ALL, mbar_wait(&bar.k_empty[stream][ks], (m / NK + 1) & 1, p.status, 40));
+        if (!ok) break;
+        copy(&bar.k_full[stream][ks], k_at + ks * Shape::kTile, p.cache.k, k_where);
+        // (the softmax has read the mask PT_MASKS tiles of the stream before this one: PT_MASKS is more than NK + the tiles of a slot whose S is
+        // issued and whose P is not read)
+        uint16_t* const mask = bar.mask[stream][m % PT_MASKS] + part * (MINE / 16);
+        if (whole_pages) {
+          if (lane < GROUPS) mask[lane] = static_cast<uint16_t>(there[0]);
+        } else if (lane == 0) {
+#pragma unroll
+          for (int e = 0; e < PER_LANE; ++e) reinterpret_cast<uint32_t*>(mask)[e] = there[e];
         }
-        c.left = t.tiles; c.v = t.v0; c.p128 = t.p128; c.p_keys = t.p_keys; c.o_keys = t.o_keys;
-        c.group = t.group; c.sequence = t.sequence; c.head = t.head;
-        look_up(c);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.mask_full[stream][m % PT_MASKS]);
+        if (!PAIRED) load_v(m, v_where);
+        else if (m > 0) load_v(m - 1, v_due);
+        v_due = v_where;
       }
-      const bool in = c.page >= 0 && c.page < p.cache.pages;
-      const int64_t none = whole_pages ? 0 : -1;
-      const int64_t k_off = in ? c.page * p.cache.k.page + c.slot * p.cache.k.token : none;
-      const int64_t v_off = in ? c.page * p.cache.v.page + c.slot * p.cache.v.token : none;
-      const int n = in ? c.n : 0;  // (whole pages)
-      const uint32_t there = whole_pages ? low_bits(n) : __ballot_sync(ALL, in);
-      --c.left;
-      c.v += BN;
-      if (c.left > 0) look_up(c);
-      load_k(c.head, k_off, n);
-      if (!ok) return;
-      // (the softmax has read the mask PT_MASKS tiles of the stream before this one: PT_MASKS is more than NK + the tiles of a slot whose S is
-      // issued and whose P is not read)
-      if (lane == 0) {
-        uint16_t* const m = bar.mask[stream][c.masks % PT_MASKS];
-        if (MINE == 32) reinterpret_cast<uint32_t*>(m)[w] = there;
-        else m[w] = static_cast<uint16_t>(there);
-        if (w == 0) bar.place[stream][c.masks % PT_MASKS] = x;
-        mbar_arrive(&bar.mask_full[stream][c.masks % PT_MASKS]);
-      }
-      ++c.masks;
-      ++x;
-      if (head_prev >= 0) load_v(head_prev, v_prev, n_prev);
-      v_prev = v_off;
-      n_prev = n;
-      head_prev = c.head;
-    };
-    Place a, b;
-    b.over = STREAMS == 1;
-    while (ok && !(a.over && b.over)) {  // the streams take turns
-      tile(a, 0);
-      if (STREAMS == 2 && ok) tile(b, 1);
+      first += t.tiles;
     }
-    if (ok && head_prev >= 0) load_v(head_prev, v_prev, n_prev);
+    if (PAIRED && ok && first > 0) load_v(first - 1, v_due);
     cp_async_wait_all();
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - SOFTMAX_REGS));
     if (warp == 12 || (warp == 15 && !PAIRED)) {
       // =========================== MMA issuers ===========================
       const bool leader = elect_one();
@@ -435,14 +445,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           return there;
         };
         auto step = [&](bool more, bool has0, bool has1, bool first, bool last0, bool last1, bool end) {  // tile x + 1: whether there is one, ...
-          if (x >= 0) ok = landed(bar.v_full, vs, v_phase);
+          if (x >= 0) ok = landed(bar.v_full[0], vs, v_phase);
           if (ok && has[0]) {
             ok = wait_p(0);
             if (ok) issue_o(0, 0, vs, fresh);
             if (ok && last[0] && leader) tc_commit(&bar.pv_done[0][0]);
           }
           if (ok && first) ok = wait_q(0);
-          if (ok && more) ok = landed(bar.k_full, ks, k_phase);
+          if (ok && more) ok = landed(bar.k_full[0], ks, k_phase);
           if (ok && has0) issue_s(0, 0, ks);
           if (ok && has[1]) {
             ok = wait_p(1);
@@ -452,8 +462,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           if (!ok) return;
           if (has1) issue_s(1, 0, ks);
           if (leader) {
-            if (x >= 0) tc_commit(&bar.v_empty[vs]);
-            if (more) tc_commit(&bar.k_empty[ks]);
+            if (x >= 0) tc_commit(&bar.v_empty[0][vs]);
+            if (more) tc_commit(&bar.k_empty[0][ks]);
             if (end) tc_commit(&bar.q_empty[0]);
           }
           if (x >= 0 && ++vs == NV) { vs = 0; v_phase ^= 1; }
@@ -469,11 +479,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         if (ok && x >= 0) step(false, false, false, false, false, false, false);
       } else {
         // Up to two S ahead of P V.
-        int left = 0, m = 0;           // tiles of the item whose S is to come; tiles of the stream so far
+        int left = 0, open = 0;        // tiles of the item whose S is to come; tiles whose P V is to come
+        int ks = 0, vs = 0;
+        uint32_t k_phase = 0, v_phase = 0, s_buffer = 0, o_buffer = 0, p_phase = 0, firsts = 0;  // firsts: a bit per open tile: first of its item
         bool first = false;
-        int x0 = 0, x1 = 0, open = 0;  // tiles whose P V is to come
-        bool f0 = false, f1 = false;   // first of their item
-        uint32_t s_buffer = 0, o_buffer = 0, p_phase = 0;
         while (ok) {
           if (left == 0 && open == 0) {
             ok = next_item(slot, items, t);
@@ -482,36 +491,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             first = true;
           }
           if (left > 0 && open < NB) {
-            ok = (!first || wait_q(slot)) && __all_sync(ALL, mbar_wait_spin(&bar.mask_full[slot][m % PT_MASKS], (m / PT_MASKS) & 1, p.status, 51));
+            ok = (!first || wait_q(slot)) && landed(bar.k_full[slot], ks, k_phase);
             if (!ok) break;
-            const int x = bar.place[slot][m % PT_MASKS];
-            ++m;
-            ok = landed(bar.k_full, x % NK, x / NK);
-            if (!ok) break;
-            issue_s(slot, s_buffer, x % NK);
+            issue_s(slot, s_buffer, slot * NK + ks);
             s_buffer ^= 1;
             --left;
             if (leader) {
-              tc_commit(&bar.k_empty[x % NK]);
+              tc_commit(&bar.k_empty[slot][ks]);
               if (left == 0) tc_commit(&bar.q_empty[slot]);
             }
-            if (open == 0) { x0 = x; f0 = first; }
-            else { x1 = x; f1 = first; }
+            if (++ks == NK) { ks = 0; k_phase ^= 1; }
+            firsts |= (first ? 1u : 0u) << open;
             ++open;
             first = false;
             continue;
           }
-          ok = landed(bar.v_full, x0 % NV, x0 / NV) && __all_sync(ALL, mbar_wait_spin(&bar.p_full[slot][o_buffer], (p_phase >> o_buffer) & 1, p.status, 43));
+          ok = landed(bar.v_full[slot], vs, v_phase) && __all_sync(ALL, mbar_wait_spin(&bar.p_full[slot][o_buffer], (p_phase >> o_buffer) & 1, p.status, 43));
           if (!ok) break;
           p_phase ^= 1u << o_buffer;
-          issue_o(slot, o_buffer, x0 % NV, f0);
+          issue_o(slot, o_buffer, slot * NV + vs, (firsts & 1) != 0);
           if (leader) {
             tc_commit(&bar.pv_done[slot][o_buffer]);
-            tc_commit(&bar.v_empty[x0 % NV]);
+            tc_commit(&bar.v_empty[slot][vs]);
           }
+          if (++vs == NV) { vs = 0; v_phase ^= 1; }
           o_buffer ^= 1;
-          x0 = x1;
-          f0 = f1;
+          firsts >>= 1;
           --open;
         }
       }
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     }
   } else {
     // =========================== softmax: a row per thread ===========================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     constexpr int W = BN / 32;              // words of a row's mask, pieces of 32 keys
     const int slot = warp >> 2, quad = warp & 3, stream = PAIRED ? 0 : slot;
     const uint32_t tm = tmem_base + slot * PT_TM_SLOT + (static_cast<uint32_t>(quad * 32) << 16);
@@ -584,6 +589,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const bool there = rho < t.rows;
       const bool idle = rho - lane >= t.rows;  // a warp without rows: whatever its P holds stays in its own rows of O
       const int limit = there ? own_keys(p, t.length, static_cast<int>(tok)) : t.o_keys;
+      const int warp_limit = __shfl_sync(ALL, limit, 0);  // limits ascend with the rows
       float m_ref = NEG_INF, l = 0.0f;
       const int mine = PAIRED ? (slot ? t.n[1] : t.n[0]) : t.tiles;
       for (int u = 0; u < mine; ++u, ++units) {
@@ -595,21 +601,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           if (lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
           continue;
         }
-        // which keys of the tile this row sees
+        // which keys of the tile this row sees: as a rule all of them
         const int mk = masks + u;
-        ok = __all_sync(ALL, mbar_wait(&bar.mask_full[stream][mk % PT_MASKS], (mk / PT_MASKS) & 1, p.status, 44));
-        if (!ok) break;
+        const bool marked = mbar_wait(&bar.mask_full[stream][mk % PT_MASKS], (mk / PT_MASKS) & 1, p.status, 44);
+        const uint32_t* const words = reinterpret_cast<const uint32_t*>(bar.mask[stream][mk % PT_MASKS]);
         const int v = t.v0 + u * BN;
-        const int left = v >= t.p128 ? limit - (v - t.p128) : BN;  // (of the prefix, what the mask says)
-        uint32_t seen[W];
-        bool all = true;
+        uint32_t seen[W], both = 0xffffffffu;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          seen[i] = reinterpret_cast<const uint32_t*>(bar.mask[stream][mk % PT_MASKS])[i] & low_bits(left - 32 * i);
-          all = all && seen[i] == 0xffffffffu;
+          seen[i] = words[i];
+          both &= seen[i];
         }
-        const bool masked = __any_sync(ALL, !all);
-        ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 45));
+        bool masked = both != 0xffffffffu;
+        if (v >= t.p128 && v - t.p128 + BN > warp_limit) {  // own tokens that the first row of the warp does not see
+          masked = true;
+#pragma unroll
+          for (int i = 0; i < W; ++i) seen[i] &= low_bits(limit - (v - t.p128) - 32 * i);
+        }
+        const bool formed = mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 45);
+        ok = __all_sync(ALL, marked && formed);
         if (!ok) break;
         tc_fence_after();
         uint32_t sc[W][32];
