@@ -193,6 +193,30 @@ def test_attention_argument_errors():
         r.rows, r.row_offsets = 2 ** 29, 4096
 
     _refused(go(many), b"2^31")
+
+    def wide(c, r):
+        r.table_pages = r.ld_table = 2 ** 26
+
+    def wider(c, r):
+        r.table_pages = r.ld_table = 2 ** 60
+
+    _refused(go(wide, **{**prefix, "prefix_pages": 2 ** 27 - 2 ** 26, "ld_prefix": 2 ** 27}), b"together")
+    _refused(go(wider), b"2^31")
+    _refused(go(**{**prefix, "prefix_pages": 2 ** 60, "ld_prefix": 2 ** 60}), b"2^31")
+    _refused(go(**{**prefix, "groups": 2 ** 31 - 1, "group_offsets": 4096}), b"2^31")
+    for bad in (0.0, -1.0, float("nan"), float("inf")):
+        _refused(go(scale=bad), b"scale")
+    need = go(scratch=True)
+    assert need > 0 and need % 32 == 0
+
+    def at(address, size):  # of the scratch
+        c, r, _, p = _descs()
+        p.scratch, p.scratch_bytes = address, size
+        return lib.vx_prefix_attention(C.byref(c), C.byref(r), C.byref(p), None)
+
+    _refused(at(None, need), b"scratch")
+    _refused(at(4096 + 16, need), b"scratch")
+    _refused(at(4096, need - 1), b"scratch")
     assert go(scratch=True, q_heads=3) == -1
 
     def empty(c, r):

@@ -445,6 +445,38 @@ def test_attention_nan_and_infinities_in_seen_places_stay_with_their_rows(ops):
     assert torch.equal(got[2, 1][keep], want[2, 1][keep])
 
 
+@pytest.mark.parametrize("heads,kv,d,tokens,length,prefix", [
+    (4, 4, 64, 3, 37, 90), (4, 2, 64, 7, 0, 0), (8, 8, 128, 5, 61, 0), (8, 2, 128, 4, 14, 200),     # few rows
+    (4, 4, 64, 40, 250, 90), (8, 2, 128, 30, 170, 0), (8, 1, 128, 12, 300, 20),                       # more
+    (4, 4, 64, 300, 70, 200), (8, 2, 128, 300, 0, 0), (2, 1, 128, 130, 5, 130)])                      # prompts
+def test_attention_values_that_are_not_finite_stay_out_of_earlier_rows(ops, heads, kv, d, tokens, length, prefix):
+    """Infinities and NaN among the new tokens: the rows in front of them do not see them."""
+    ps, n = 16, 3
+    own, pre = -(-(length + tokens) // ps), -(-prefix // ps)
+    table = np.arange(n * own).reshape(n, own)
+    ptable = n * own + np.arange(pre)[None]
+    k_pages, v_pages = make_cache(n * own + pre + 1, ps, kv, d)
+    at = lambda s, i: (int(table[s, (length + i) // ps]), (length + i) % ps)  # noqa: E731
+    for i in {tokens // 2, tokens - 1}:
+        v_pages[at(0, i)][0, 5] = float("inf")
+        v_pages[at(0, i)][kv - 1, d - 1] = float("nan")
+    for i in range(tokens - tokens // 3, tokens):  # many of them, in tiles that follow one another
+        v_pages[at(1, i)][:, i % d] = float("-inf") if i % 2 else float("nan")
+    k_pages[at(1, tokens - 1)][kv - 1, 3] = float("nan")
+    q = torch.randn(n * tokens, heads, d, device="cuda").bfloat16()
+    off = np.arange(n + 1) * tokens
+    kw = dict(prefix_table=ints(ptable), prefix_lengths=ints([prefix])) if prefix else {}
+    got = f64(ops.prefix_attention(q, k_pages, v_pages, ints(table), ints([length] * n), row_offsets=ints(off), **kw))
+    torch.cuda.synchronize()
+    with np.errstate(invalid="ignore"):
+        want, width = P.prefix_attention_ref(f64(q), f64(k_pages), f64(v_pages), table, np.array([length] * n), ptable if prefix else None, [prefix], off)
+    ok = np.isfinite(want)
+    assert ok[0].all() and ok[tokens // 2 - 1].all() and not ok[tokens - 1].all() and ok[2 * tokens:].all()
+    assert (np.isfinite(got) == ok).all(), f"{(np.isfinite(got) != ok).sum()} values"
+    assert (np.isnan(got) == np.isnan(want)).all() and (got[np.isinf(want)] == want[np.isinf(want)]).all()
+    assert (np.abs(got - want)[ok] <= (2.0 ** -8 * (np.abs(want) + width) + 2.0 ** -13 * width)[ok]).all()
+
+
 def test_attention_nothing(ops):
     k_pages, v_pages = make_cache(2, 16, 2, 64)
     e = torch.empty(0, 2, 64, device="cuda", dtype=torch.bfloat16)

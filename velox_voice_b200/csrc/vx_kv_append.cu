@@ -35,7 +35,7 @@ int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c,
   if (rows->rows < 0 || rows->rows > kMax || rows->sequences < 0 || rows->sequences > kMax) return fail(-1, "vx_kv_rows: bad shape");
   if (!rows->row_offsets && rows->rows != rows->sequences)
     return fail(-1, "vx_kv_rows: without row_offsets every sequence has one row (rows %lld, sequences %lld)", (long long)rows->rows, (long long)rows->sequences);
-  if (rows->table_pages < 0 || rows->table_pages * cache->page_size > kMax) return fail(-1, "vx_kv_rows: a sequence may have up to 2^31 - 1 tokens");
+  if (rows->table_pages < 0 || rows->table_pages > kMax / cache->page_size) return fail(-1, "vx_kv_rows: a sequence may have up to 2^31 - 1 tokens");
   if (rows->rows > 0 && rows->sequences > 0) {
     if (!rows->lengths) return fail(-1, "vx_kv_rows: lengths must not be NULL");
     if (rows->table_pages > 0 && (!rows->page_table || rows->ld_table < rows->table_pages)) return fail(-1, "vx_kv_rows: page_table NULL or its rows too short");

@@ -9,6 +9,10 @@
 //   out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c,  m = max_c m_c.
 // The number of chunks is fixed on the host from the width of the tables; how many of them hold keys is known on the device only, and
 // both sides derive it from the same lengths, so empty parts are neither written nor read.
+//
+// Places that no row of a tile sees are filled with zeros.  New tokens of a sequence lie in one tile with rows that see them and rows that do
+// not, and a probability of 0 times a value that is not finite would reach the latter: where such a tile holds one, its product with the
+// values is formed another way.
 #pragma once
 
 #include "vx_paged.cuh"
@@ -116,6 +120,10 @@ __device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp,
   it.rho0 = tile * TM;
   return n > 0 && it.rho0 < it.rows;
 }
+
+// Not 0 if one of the two bf16 values of a word is an infinity or NaN, gathered in `sum` (0 x is 0 or NaN).
+__device__ __forceinline__ void note_not_finite(uint32_t& sum, uint32_t two) { asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(two), "r"(0u)); }
+__device__ __forceinline__ bool any_not_finite(uint32_t sum) { return (sum & 0x7fff7fffu) != 0; }
 
 // Launches prefix_tiles_kernel on the spans that have chunks.
 constexpr int kSlotRows = 128;  // rows of a slot of prefix_tiles_kernel

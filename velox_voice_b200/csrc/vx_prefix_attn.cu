@@ -249,6 +249,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_k
           mma_bf16_16816(s[r], k0[2], k1[2], k0[3], k1[3], q[r][i][2], q[r][i][3]);
         }
     }
+    const bool late = j0 + 16 > min_limit && min_limit < keys;  // keys that rows of the tile do not see
     // scores in units of log2; keys that are not there or that the row does not see count as -inf
 #pragma unroll
     for (int r = 0; r < RB; ++r)
@@ -307,6 +308,41 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_k
       uint32_t v[4][4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) ld_shared16(at + v_at + b * 128 + ((e & 1) + 8 * (e >> 1)) * (D * 2), v[e]);
+      if (late) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) note_not_finite(sum, v[e][j]);
+        if (__any_sync(0xffffffffu, any_not_finite(sum))) {
+          // Row by row, with zeros for the values of the keys that the row does not see.
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+#pragma unroll 1
+            for (int n = 0; n < 8; ++n) {
+              const int lim0 = __shfl_sync(0xffffffffu, limit[r][0], n >> 1), lim1 = __shfl_sync(0xffffffffu, limit[r][1], n >> 1);
+              const int sees = (n & 1 ? lim1 : lim0) - j0 - 2 * c;  // of the keys from 2 c on
+              const uint32_t in0 = (sees > 0 ? 0xffffu : 0u) | (sees > 1 ? 0xffff0000u : 0u), in1 = (sees > 8 ? 0xffffu : 0u) | (sees > 9 ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_bf16_16816(t, __byte_perm(v[0][j], v[1][j], 0x5410) & in0, __byte_perm(v[0][j], v[1][j], 0x7632) & in0,
+                               __byte_perm(v[2][j], v[3][j], 0x5410) & in1, __byte_perm(v[2][j], v[3][j], 0x7632) & in1, pt[r][0], pt[r][1]);
+                if (c == n >> 1) {
+                  if (n & 1) {
+                    o[r][b][j][1] += t[1];
+                    o[r][b][j][3] += t[3];
+                  } else {
+                    o[r][b][j][0] += t[0];
+                    o[r][b][j][2] += t[2];
+                  }
+                }
+              }
+            }
+          }
+          continue;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5410), a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
@@ -530,12 +566,12 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
   if (cache->head_dim != 64 && cache->head_dim != 128) return fail(-1, "head_dim must be 64 or 128 (got %d)", cache->head_dim);
   if (d->q_heads < 1 || d->q_heads > 65535 || d->q_heads % cache->kv_heads != 0)
     return fail(-1, "q_heads (%d) must be a multiple of kv_heads (%d)", d->q_heads, cache->kv_heads);
-  if (rows->rows * d->q_heads >= (1ll << 31)) return fail(-1, "rows * q_heads must stay below 2^31");
   if (d->groups < 0 || d->groups > (1ll << 31) - 1) return fail(-1, "bad number of groups %lld", (long long)d->groups);
+  if (rows->rows * d->q_heads + (rows->sequences + d->groups) * cache->kv_heads >= (1ll << 31)) return fail(-1, "rows * q_heads and (sequences + groups) * kv_heads must stay below 2^31 together");
   if (d->groups > 0) {
     if (!d->group_offsets && rows->sequences % d->groups != 0)
       return fail(-1, "without group_offsets the groups are of one size (sequences %lld, groups %lld)", (long long)rows->sequences, (long long)d->groups);
-    if (d->prefix_pages < 0 || d->prefix_pages * cache->page_size > (1ll << 31) - 1) return fail(-1, "a prefix may have up to 2^31 - 1 tokens");
+    if (d->prefix_pages < 0 || d->prefix_pages > ((1ll << 31) - 1) / cache->page_size) return fail(-1, "a prefix may have up to 2^31 - 1 tokens");
     if (!d->prefix_lengths || (d->prefix_pages > 0 && (!d->prefix_table || d->ld_prefix < d->prefix_pages)))
       return fail(-1, "prefix_lengths or prefix_table is NULL, or its rows are too short");
   }
@@ -556,6 +592,7 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
   plan.span[0] = plan.span[1] = kNoSpan;
   if (R == 0 || S == 0 || cache->pages == 0) return 0;  // no key anywhere
   const int64_t cap_p = G > 0 ? d->prefix_pages * cache->page_size : 0, cap_o = rows->table_pages * cache->page_size;
+  if (cap_p + cap_o > (1ll << 31) - 1024) return fail(-1, "prefix and own tokens of a sequence may be 2^31 - 1024 together");  // (indexes of keys are 32 bits)
   // The kernel of a span goes by its rows per owner and key head, on the average (which kernel takes a row changes no result beyond rounding).
   const bool single = !rows->row_offsets;
   const int64_t rows_p = cap_p > 0 ? R * per / G : 0, rows_o = cap_o > 0 ? R * per / S : 0;

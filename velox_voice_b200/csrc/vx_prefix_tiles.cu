@@ -35,6 +35,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "vx_common.cuh"
 #include "vx_prefix.cuh"
@@ -181,6 +182,76 @@ __device__ bool find_tile_item(const TilesParams& tp, int n, TileItem& t) {
   }
   t.part = sp.part0 < 0 ? -1 : sp.part0 + chunk;
   return true;
+}
+
+// Whether one of the keys [from, to) of a tile has a value that is not finite.  All lanes of the warp.
+template <int D, int PANEL>
+__device__ __forceinline__ bool values_not_finite(const uint8_t* tile, int from, int to) {
+  const int lane = threadIdx.x & 31;
+  uint32_t sum = 0;
+#pragma unroll 4
+  for (int key = from + (lane >> 3); key < to; key += 4)
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const uint4 w = *reinterpret_cast<const uint4*>(tile + i * PANEL + key * 128 + (lane & 7) * 16);
+      note_not_finite(sum, w.x);
+      note_not_finite(sum, w.y);
+      note_not_finite(sum, w.z);
+      note_not_finite(sum, w.w);
+    }
+  return __any_sync(0xffffffffu, any_not_finite(sum));
+}
+
+// O of this lane's row behind a tile, into `o`: P of the tile (tensor memory, bf16) times the values of the keys that the row sees (those of
+// the mask `there` below `sees`), added to what tensor memory holds (`first`: nothing).  For tiles that values_not_finite is true of; all
+// lanes of the warp.
+template <int D, int KEYS>
+__device__ __noinline__ void add_tile_apart(float* o, uint32_t o_tmem, uint32_t p_tmem, bool first, const uint32_t* there, int sees, const uint8_t* tile) {
+#pragma unroll 1
+  for (int i = 0; i < D / 16; ++i) {
+    uint32_t x[16];
+    tc_ld_x16(o_tmem + 16 * i, x);
+    tc_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[16 * i + e] = first ? 0.0f : __uint_as_float(x[e]);
+  }
+#pragma unroll 1
+  for (int i = 0; i < KEYS / 32; ++i) {
+    uint32_t x[16];
+    tc_ld_x16(p_tmem + 16 * i, x);
+    tc_wait_ld();
+#pragma unroll 1
+    for (int e = 0; e < 32; ++e) {
+      uint32_t two = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) two = k == e >> 1 ? x[k] : two;
+      const float w = __uint_as_float(e & 1 ? two & 0xffff0000u : two << 16);
+      const int key = 32 * i + e;
+      if (!((there[i] >> e) & 1) || key >= sees) continue;
+#pragma unroll 1
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 u = *reinterpret_cast<const uint4*>(tile + (c >> 3) * (KEYS * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+        const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[8 * c + 2 * k] += w * __uint_as_float(v[k] << 16);
+          o[8 * c + 2 * k + 1] += w * __uint_as_float(v[k] & 0xffff0000u);
+        }
+      }
+    }
+    __syncwarp();
+  }
+}
+template <int D>
+__device__ __noinline__ void put_back(const float* o, uint32_t o_tmem) {
+#pragma unroll 1
+  for (int i = 0; i < D / 16; ++i) {
+    uint32_t x[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[16 * i + e]);
+    tc_st_x16(o_tmem + 16 * i, x);
+  }
+  tc_wait_st_all();
 }
 
 template <int D, bool PAIRED>
@@ -591,15 +662,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const int limit = there ? own_keys(p, t.length, static_cast<int>(tok)) : t.o_keys;
       const int warp_limit = __shfl_sync(ALL, limit, 0);  // limits ascend with the rows
       float m_ref = NEG_INF, l = 0.0f;
+      float o_apart[D];    // O behind the tile before, where that was formed apart (in local memory)
+      bool apart = false;
       const int mine = PAIRED ? (slot ? t.n[1] : t.n[0]) : t.tiles;
-      for (int u = 0; u < mine; ++u, ++units) {
+      // One tile.  LATE: it has own tokens that rows of the warp see and others do not.
+      auto do_tile = [&](auto late, int u) {
+        constexpr bool LATE = decltype(late)::value;
         const uint32_t buffer = units % NB, parity = (units / NB) & 1;
         const uint32_t tb = tm + buffer * BN;
         if (idle) {
           ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 47));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
-          continue;
+          if (ok && lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
+          return;
         }
         // which keys of the tile this row sees: as a rule all of them
         const int mk = masks + u;
@@ -613,14 +687,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           both &= seen[i];
         }
         bool masked = both != 0xffffffffu;
-        if (v >= t.p128 && v - t.p128 + BN > warp_limit) {  // own tokens that the first row of the warp does not see
+        if (LATE) {
           masked = true;
 #pragma unroll
           for (int i = 0; i < W; ++i) seen[i] &= low_bits(limit - (v - t.p128) - 32 * i);
         }
         const bool formed = mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 45);
         ok = __all_sync(ALL, marked && formed);
-        if (!ok) break;
+        if (!ok) return;
         tc_fence_after();
         uint32_t sc[W][32];
         float m4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
@@ -646,16 +720,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         const float m_tile = mx * p.scale2;
         const bool moves = m_tile > m_ref + 8.0f;
-        if (__any_sync(ALL, moves)) {
+        // P V of the tile before has to be complete before O is touched (with one buffer this tile's S was issued behind it)
+        auto o_is_there = [&] {
+          if (NB > 1) ok = __all_sync(ALL, mbar_wait(&bar.pv_done[slot][(units - 1) % NB], ((units - 1) / NB) & 1, p.status, 46));
+          tc_fence_after();
+          return ok;
+        };
+        if (__any_sync(ALL, moves || (LATE && apart))) {
           const float alpha = moves ? ex2(m_ref - m_tile) : 1.0f;  // 0 for m_ref = -inf
           if (moves) m_ref = m_tile;
           l *= alpha;
           if (u > 0) {
-            if (NB > 1) {  // P V of the tile before has to be complete (with one buffer this tile's S was issued behind it)
-              ok = __all_sync(ALL, mbar_wait(&bar.pv_done[slot][(units - 1) % NB], ((units - 1) / NB) & 1, p.status, 46));
-              if (!ok) break;
-              tc_fence_after();
-            }
+            if (!o_is_there()) return;
+            if (LATE && apart) put_back<D>(o_apart, tm + PT_TM_O);
+            if (LATE) apart = false;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
               uint32_t o[16];
@@ -689,10 +767,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         unpack_f32x2(sum[1], b0, b1);
         l += (a0 + a1) + (b0 + b1);
         tc_wait_st_all();
+        if (LATE) {
+          ok = __all_sync(ALL, mbar_wait(&bar.v_full[stream][mk % NV], (mk / NV) & 1, p.status, 54));
+          if (!ok) return;
+          const uint8_t* const values = v_ring + (stream * NV + mk % NV) * Shape::kTile;
+          if (values_not_finite<D, Shape::kPanel>(values, max(warp_limit - (v - t.p128), 0), min(t.o_keys - (v - t.p128), BN))) {
+            if (u > 0 && !o_is_there()) return;
+            add_tile_apart<D, BN>(o_apart, tm + PT_TM_O, tb, u == 0, words, limit - (v - t.p128), values);
+            apart = true;
+          }
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
-      }
+      };
+      // the late tiles begin with the one that has the first own token that the first row does not see
+      const int first_late = warp_limit >= t.o_keys ? mine : min(max(t.p128 + warp_limit - t.v0, 0) / BN, mine);
+      int u = 0;
+      for (; ok && u < first_late; ++u, ++units) do_tile(std::false_type{}, u);
+      for (; ok && u < mine; ++u, ++units) do_tile(std::true_type{}, u);
       masks += t.tiles;
       if (!ok) break;
       if (mine == 0) continue;
@@ -702,6 +795,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       ++mine_done;
       if (idle) continue;
       tc_fence_after();
+      if (apart) put_back<D>(o_apart, tm + PT_TM_O);
       const int64_t row = t.row0 + static_cast<int>(tok), qh = t.head * static_cast<int64_t>(p.per_kv.d) + hq;
       if (t.part >= 0) {
         const int64_t at = (static_cast<int64_t>(t.part) * p.rows.rows + row) * p.q_heads + qh;
