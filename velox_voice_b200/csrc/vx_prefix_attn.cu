@@ -34,7 +34,6 @@ namespace vx {
 namespace {
 
 constexpr int PR_WARPS = 4;
-constexpr int kRowsKernel = 16;  // rows per owner and key head up to which prefix_rows_kernel takes a span
 
 // CTAs of prefix_rows_kernel per SM, as many as its registers allow: what a CTA needs before and behind its keys passes under the others'
 // keys.  (16 groups of ten hypotheses over 3,750 frames, head_dim 64: 47 us with 2, 37 with 3, 31 with 4.)
@@ -593,7 +592,8 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
   if (R == 0 || S == 0 || cache->pages == 0) return 0;  // no key anywhere
   const int64_t cap_p = G > 0 ? d->prefix_pages * cache->page_size : 0, cap_o = rows->table_pages * cache->page_size;
   if (cap_p + cap_o > (1ll << 31) - 1024) return fail(-1, "prefix and own tokens of a sequence may be 2^31 - 1024 together");  // (indexes of keys are 32 bits)
-  // The kernel of a span goes by its rows per owner and key head, on the average (which kernel takes a row changes no result beyond rounding).
+  // The kernel of a span goes by its rows per owner and key head, on the average, and its keys, as many as the tables have place for (which
+  // kernel takes a row changes no result beyond rounding).
   const bool single = !rows->row_offsets;
   const int64_t rows_p = cap_p > 0 ? R * per / G : 0, rows_o = cap_o > 0 ? R * per / S : 0;
   auto cut = [&](Span& sp, SpanKind kind, Plan::Kernel kernel, int64_t owners, int64_t cap, int64_t equal_rows) {
@@ -614,8 +614,24 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     cut(plan.span[0], kSpanJoint, Plan::kPairs, S, round_up(cap_p, kSpanAlign) + cap_o, single ? per : 0);
     if (plan.span[0].chunks == 1) plan.span[0].part0 = -1;
   } else {
-    plan.kernel[0] = rows_p > (cache->head_dim == 64 ? 4 : 2) * kSlotRows ? Plan::kPairs : (rows_p <= kRowsKernel ? Plan::kRows : Plan::kTiles);
-    plan.kernel[1] = rows_o <= kRowsKernel || (rows_o <= 64 && cap_o <= 128) ? Plan::kRows : Plan::kTiles;
+    // prefix_rows_kernel walks the keys once per 16 rows, without much to set up; the tile kernel starts slower and walks them once per 128.
+    // One group, 8 key heads, single tokens, rows kernel against tiles, in us:
+    //   head_dim 64    16 rows  4,000 keys 21 : 24   40,000 keys 34 : 42     32 rows  4,000 keys 23 : 25   16,000 keys 30 : 32   40,000 keys 52 : 44
+    //   head_dim 128    8 rows  4,000 keys 24 : 28   40,000 keys 60 : 58     16 rows  4,000 keys 26 : 28   16,000 keys 38 : 39   40,000 keys 73 : 60
+    //                  32 rows  4,000 keys 24 : 31    8,000 keys 34 : 34     48 rows  4,000 keys 30 : 32    8,000 keys 48 : 34
+    // A rule that meets these: what the walks read together.
+    const double bytes = 4.0 * static_cast<double>(G * cap_p) * cache->kv_heads * cache->head_dim;  // of the keys and values
+    const bool few = rows_p <= (cache->head_dim == 64 ? 16 : 8) || (rows_p <= 64 && static_cast<double>((rows_p + 15) / 16) * bytes <= 64.0 * 1048576.0);
+    // Pairs of slots share their keys; with an odd number of slots one of a pair idles.  One group of 30,000 keys, 8 key heads, slots by
+    // themselves against pairs, in us: head_dim 64  300 rows 85 : 99  400 rows 124 : 110   head_dim 128  360 rows 99 : 132  512 rows 143 : 155
+    // 560 rows 171 : 167  800 rows 218 : 202.
+    plan.kernel[0] = few ? Plan::kRows : (rows_p > (cache->head_dim == 64 ? 3 : 4) * kSlotRows ? Plan::kPairs : Plan::kTiles);
+    // Own tokens of many sequences are many short walks, whose start counts for more.  160 sequences without a prefix, new tokens behind a
+    // history, 8 key heads, rows kernel against tiles, in us:
+    //   head_dim 64   12 rows  0 + 12 keys 18 : 33  500 + 12 51 : 70    24 rows  0 + 24 27 : 39  2,000 + 24 159 : 188    48 rows  100 + 48 57 : 61  500 + 48 104 : 102
+    //   head_dim 128  16 rows  0 + 4 keys 29 : 39   500 + 4 85 : 84     32 rows  0 + 8 41 : 47   100 + 8 53 : 55  500 + 8 125 : 92    64 rows  0 + 16 68 : 64
+    const int64_t width = rows_o * cache->head_dim;
+    plan.kernel[1] = width <= 32 * 64 || (width <= 64 * 64 && cap_o <= 256) ? Plan::kRows : Plan::kTiles;
     plan.blocks = (plan.kernel[0] == Plan::kRows && rows_p > 8) || (plan.kernel[1] == Plan::kRows && rows_o > 8) ? 2 : 1;
     cut(plan.span[0], kSpanPrefix, plan.kernel[0], G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
     cut(plan.span[1], kSpanOwn, plan.kernel[1], S, cap_o, single ? per : 0);
