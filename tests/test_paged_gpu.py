@@ -379,6 +379,23 @@ def test_attention_large_calls(ops, n, tokens, groups, heads, kv, d, length, pre
     assert (err <= 0).all(), err.max().item()
 
 
+@pytest.mark.parametrize("length", [1600, 3600])
+def test_attention_many_prompts_with_odd_ends(ops, length):
+    """Runs whose last rows leave the second tile of a pair without any, several of them per SM, over more keys than there are masks kept; rows
+    that a single key rules."""
+    n, tokens, heads, d, ps, prefix = 80, 300, 4, 64, 16, 137
+    width, pw = -(-(length + tokens) // ps), -(-prefix // ps)
+    order = torch.randperm(n * width + pw, generator=torch.Generator().manual_seed(1)).to("cuda", torch.int32)
+    table, ptable = order[:n * width].view(n, width), order[n * width:].view(1, pw)
+    k_pages, v_pages = make_cache(order.numel(), ps, heads, d)
+    q = (torch.randn(n, tokens, heads, d, generator=torch.Generator().manual_seed(2)) * 6).to("cuda", torch.bfloat16)
+    out = ops.prefix_attention(q.view(-1, heads, d), k_pages, v_pages, table, ints([length] * n), ptable, ints([prefix]),
+                               row_offsets=ints([tokens * i for i in range(n + 1)])).view(q.shape)
+    want, spread = dense_reference(q, k_pages, v_pages, table, length, ptable, prefix, 1)
+    err = (out.double() - want).abs() - (2.0 ** -8 * (want.abs() + spread) + 2.0 ** -13 * spread)
+    assert (err <= 0).all(), err.max().item()
+
+
 @pytest.mark.parametrize("seed", range(40))
 def test_attention_random_calls(ops, seed):
     rng = np.random.default_rng(seed)

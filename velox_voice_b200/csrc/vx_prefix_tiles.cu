@@ -783,6 +783,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       };
       // the late tiles begin with the one that has the first own token that the first row does not see
       const int first_late = warp_limit >= t.o_keys ? mine : min(max(t.p128 + warp_limit - t.v0, 0) / BN, mine);
+      // A slot that took none of the last tiles may be far ahead of the loaders, where the phase of a mask says nothing yet: its first S tells
+      // that they have come here.
+      if (PAIRED && mine > 0 && !idle) ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][units % NB], (units / NB) & 1, p.status, 55));
       int u = 0;
       for (; ok && u < first_late; ++u, ++units) do_tile(std::false_type{}, u);
       for (; ok && u < mine; ++u, ++units) do_tile(std::true_type{}, u);
