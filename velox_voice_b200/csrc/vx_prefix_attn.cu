@@ -6,19 +6,23 @@
 // How the work is cut: vx_prefix.cuh.  This file has the kernel for few rows per owner and key head, the kernel that joins the parts, and
 // the entry points.
 //
-// prefix_rows_kernel: up to 16 rows against one chunk of keys per CTA of four warps, which take 16 (head_dim 128) or 32 (64) keys in turn.
-// Every key and value is read once, by one lane, straight into the registers that the tensor cores take it from; shared memory holds only
-// what the four warps join at the end.  Keys and values are the m16 side of m16n8k16 products, so that eight rows fill one and
-// nothing is computed for rows that do not exist.  With lane = 4 g + c:
+// prefix_rows_kernel: up to 16 rows against one chunk of keys, by one, two or four of a CTA's four warps; each takes 16 keys in turn through a
+// ring of its own in shared memory (cp.async, two or three stages of 16 keys and their values), so that no warp waits for another before the
+// end, where their sums are joined.  Keys and values are the m16 side of m16n8k16 products: eight rows fill one, and nothing is computed for
+// rows that do not exist.  With lane = 4 g + c:
 //   S^T = K Q^T: the order of the terms of a sum over head_dim is free.  A lane reads 16 bytes = 8 values of keys g and g + 8 at 8 (c + 4 i);
 //     the registers are the A fragments of two products whose 16 "k" are the values 8 (c + 4 i) + {0, 1, 2, 3} (then {4, ..., 7}) of the
 //     four c; Q is read in the same order.
 //   O^T += V^T P^T: the accumulators hold P^T by keys; transposed in 8 x 8 blocks (movmatrix) they are the B fragment.  A lane reads 8 values
 //     of each of the keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 at 64 b + 8 g and pairs two keys' values with byte permutes; product j of block b has
 //     columns 64 b + 8 g + 2 j (rows g of its A) and 64 b + 8 g + 2 j + 1 (rows g + 8).
+// (ldmatrix gives the same fragments from rows of 16 bytes; with the reads above the pieces of a key lie in shared memory as they lie in the
+// cache.  mma.sync and not tcgen05: its M is 128 rows, of which these calls have 1 to 16.)
 // The reference maximum of a row moves only when a score exceeds it by more than 8 (probabilities stay below 2^8), so most steps
-// need a vote and no shuffles; sums are kept per lane until the end.  K of the next step is requested when S is formed, V when O is.
-// What bounds it: HBM, each chunk read once; a step's products cost a tenth of the time that its bytes take.
+// need a vote and no shuffles; sums are kept per lane until the end.
+// What bounds it: HBM where there is enough to read -- eight prompts of 4,096 to 32,768 tokens, their rows' own tokens and the join behind them
+// in 105 us, 5.4 TB/s; 64 KB in flight per SM reach 6.7 TB/s on such reads -- and else the latency of a CTA: tables, first keys and joining
+// the warps are 8 of the 31 us that 16 groups of ten hypotheses over 3,750 frames take (head_dim 64, 113 MB, 3.6 TB/s).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -92,7 +96,6 @@ struct RowsShape {
 // RB blocks of eight rows.
 template <int D, int RB>
 __global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_kernel(const __grid_constant__ RowsParams rp) {
-  pdl_launch_dependents();
   using Shape = RowsShape<D>;
   constexpr int NS = Shape::kStages;
   constexpr int KC = D / 32;               // 16-byte pieces of a key per lane
@@ -112,6 +115,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_k
     }
   } behind{rp.beside != 0};
   if (!rp.beside) pdl_wait();
+  pdl_launch_dependents();  // (behind the wait: see the kernel that joins the parts)
   int n = static_cast<int>(blockIdx.x);
   const bool second = n >= rp.first_blocks;
   if (second) n -= rp.first_blocks;
@@ -423,30 +427,32 @@ int launch_rows(const RowsParams& rp, int64_t blocks, cudaStream_t st) {
   return 0;
 }
 
-// The parts of every row joined, and zeros for the rows that have none.  WARPS warps of a block of eight share a row and query head: a lane
-// weighs one part of up to 32 (maximum, then 2^(m_c - m) and the sum over l), then the warp adds the parts up, head_dim / 4 lanes on
-// one; with several warps each takes every WARPS-th block of parts and shared memory joins them.  (A thread that walked through all parts by
-// itself took 45 us for the 157 parts of a prefix of 40,000 keys.)
+// The parts of every row joined, and zeros for the rows that have none.  WARPS warps of a block of eight share a row and query head, a slice of
+// the parts each; a warp requests the sums of PARTS parts (at head_dim 64 half a warp has one) together with their maxima, weighs them (maximum,
+// then 2^(m_c - m)) and adds them up; shared memory joins the warps.  Many rows of up to four parts, four at a time: fewer
+// registers, more rows on an SM (16 utterances with ten hypotheses of 60 tokens: a call of 93 us against 103; 32 rows of two parts: 10 against 8).  What a row is, is looked up ahead of the wait: the kernels in front let
+// this one start behind a wait of their own, so all that was there before this call is complete.
+// What bounds it: one round trip to the parts in L2, or their bytes where rows are many.
 struct JoinParams {
   PrefixParams p;
   Span span[2];
+  int32_t first;  // no kernel of this call is in front
 };
 constexpr int JN_WARPS = 8;
-template <int D, int WARPS>
-__global__ void __launch_bounds__(JN_WARPS * 32) prefix_join_kernel(const __grid_constant__ JoinParams jp) {
+template <int D, int WARPS, int PARTS>
+__global__ void __launch_bounds__(JN_WARPS * 32, PARTS > 4 ? 4 : (D == 64 ? 8 : 5)) prefix_join_kernel(const __grid_constant__ JoinParams jp) {
   pdl_launch_dependents();
   constexpr unsigned ALL = 0xffffffffu;
-  constexpr int LANES = D / 4, SUB = 32 / LANES;  // lanes per part, parts at a time
+  constexpr int LANES = D / 4, SUB = 32 / LANES, LOADS = PARTS / SUB;  // lanes per part, parts per load; PARTS at a time
   __shared__ float4 o_s[WARPS > 1 ? JN_WARPS : 1][32];
   __shared__ float2 ml_s[WARPS > 1 ? JN_WARPS : 1];
   const PrefixParams& p = jp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / WARPS, rank = warp % WARPS;
   const int row = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y) * (JN_WARPS / WARPS) + team;
-  pdl_wait();
+  if (jp.first) pdl_wait();
   const bool in = h < p.q_heads;
   int parts[2] = {0, 0}, s, i;
   if (row_sequence<true>(p.rows, row, s, i)) {
-    if (jp.span[0].part0 < 0) return;  // its row is there already
     const int prefix = prefix_keys(p, group_of<true>(p, s)), own = own_keys(p, p.rows.lengths[s], i);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -455,38 +461,36 @@ __global__ void __launch_bounds__(JN_WARPS * 32) prefix_join_kernel(const __grid
       if (sp.chunks) parts[e] = static_cast<int>((keys + sp.chunk - 1) / sp.chunk);
     }
   }
+  if (!jp.first) pdl_wait();
   // part n of the row: those of span 0, then those of span 1
-  const int n_parts = in ? parts[0] + parts[1] : 0;
+  const int n_parts = in ? parts[0] + parts[1] : 0, slice = (n_parts + WARPS - 1) / WARPS;
   const int64_t at = static_cast<int64_t>(row) * p.q_heads + h, step = static_cast<int64_t>(p.rows.rows) * p.q_heads;
   auto place = [&](int n) { return at + (n < parts[0] ? jp.span[0].part0 + n : jp.span[1].part0 + n - parts[0]) * step; };
   const float NEG_INF = __int_as_float(0xff800000);
   float m = NEG_INF, sum = 0.0f;
   float4 acc = make_float4(0, 0, 0, 0);
-  const int sub = lane / LANES, col = (lane % LANES) * 4;
-  for (int n0 = rank * 32; n0 < n_parts; n0 += WARPS * 32) {
+  const int sub = lane / LANES, col = (lane % LANES) * 4, end = min(n_parts, (rank + 1) * slice);
+  for (int n0 = rank * slice; n0 < end; n0 += PARTS) {
     float2 ml = make_float2(NEG_INF, 0.0f);
-    int64_t my = 0;
-    if (n0 + lane < n_parts) {
-      my = place(n0 + lane);
-      ml = p.part_ml[my];
+    if (lane < PARTS && n0 + lane < end) ml = p.part_ml[place(n0 + lane)];
+    float4 x[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int n = n0 + k * SUB + sub;
+      x[k] = make_float4(0, 0, 0, 0);
+      if (n < end) x[k] = *reinterpret_cast<const float4*>(p.part_o + place(n) * D + col);
     }
     float mx = ml.x;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(ALL, mx, x));
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(ALL, mx, o));
     const float m_new = fmaxf(m, mx), ref = m_new == NEG_INF ? 0.0f : m_new, alpha = ex2(m - ref), w = ex2(ml.x - ref);
     m = m_new;
     sum = sum * alpha + w * ml.y;
     acc.x *= alpha; acc.y *= alpha; acc.z *= alpha; acc.w *= alpha;
-    const int n = min(32, n_parts - n0);
-#pragma unroll 8
-    for (int k = 0; k < n; k += SUB) {
-      const int c = k + sub;  // (SUB = 2 and n odd: the last c is n, whose weight is 0)
-      const int64_t a = __shfl_sync(ALL, my, c & 31);
-      const float wc = __shfl_sync(ALL, w, c & 31);
-      if (c < n) {
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + a * D + col);
-        acc.x += wc * x.x; acc.y += wc * x.y; acc.z += wc * x.z; acc.w += wc * x.w;
-      }
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const float wc = __shfl_sync(ALL, w, k * SUB + sub);  // (0 behind the end)
+      acc.x += wc * x[k].x; acc.y += wc * x[k].y; acc.z += wc * x[k].z; acc.w += wc * x[k].w;
     }
   }
 #pragma unroll
@@ -519,13 +523,31 @@ __global__ void __launch_bounds__(JN_WARPS * 32) prefix_join_kernel(const __grid
     *reinterpret_cast<uint2*>(p.out + row * p.o_row + h * p.o_head + col) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
+// Where the tile kernel wrote the rows itself: zeros for those of no sequence, a warp per row.
+template <int D>
+__global__ void __launch_bounds__(JN_WARPS * 32) prefix_rest_kernel(const __grid_constant__ JoinParams jp) {
+  pdl_launch_dependents();
+  const PrefixParams& p = jp.p;
+  const int row = static_cast<int>(blockIdx.x) * JN_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  int s, i;
+  const bool rest = row < p.rows.rows && !row_sequence<true>(p.rows, row, s, i);
+  pdl_wait();
+  if (!rest) return;
+  for (int n = lane; n < p.q_heads * (D / 8); n += 32) *reinterpret_cast<uint4*>(p.out + row * p.o_row + n / (D / 8) * p.o_head + n % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+}
+
 template <int D>
 cudaError_t launch_join(const JoinParams& jp, int parts, cudaStream_t st) {
-  // warps per row and head: one for up to 32 parts, more only while there are few rows to fill the SMs with
+  if (jp.span[0].part0 < 0)
+    return launch_dependent(prefix_rest_kernel<D>, dim3(static_cast<unsigned>((jp.p.rows.rows + JN_WARPS - 1) / JN_WARPS)), dim3(JN_WARPS * 32), 0, st, jp);
+  // warps per row and head: so many that each has its parts in one turn, while the SMs have room for them
+  constexpr int AT_ONCE = D == 64 ? 16 : 8;
   const int64_t cells = static_cast<int64_t>(jp.p.rows.rows) * jp.p.q_heads;
-  int warps = parts > 128 ? 8 : (parts > 64 ? 4 : (parts > 32 ? 2 : 1));
-  while (warps > 1 && cells * warps > 64 * static_cast<int64_t>(sm_count())) warps >>= 1;
-  auto kernel = warps == 8 ? prefix_join_kernel<D, 8> : (warps == 4 ? prefix_join_kernel<D, 4> : (warps == 2 ? prefix_join_kernel<D, 2> : prefix_join_kernel<D, 1>));
+  int warps = 1;
+  while (warps < 8 && parts > warps * AT_ONCE && 2 * warps * cells <= 32 * static_cast<int64_t>(sm_count())) warps <<= 1;
+  auto kernel = parts <= 4 && cells > 64 * static_cast<int64_t>(sm_count()) ? prefix_join_kernel<D, 1, 4>
+                           : (warps == 8 ? prefix_join_kernel<D, 8, AT_ONCE>
+                                         : (warps == 4 ? prefix_join_kernel<D, 4, AT_ONCE> : (warps == 2 ? prefix_join_kernel<D, 2, AT_ONCE> : prefix_join_kernel<D, 1, AT_ONCE>)));
   const int per_block = JN_WARPS / warps;
   return launch_dependent(kernel, dim3(static_cast<unsigned>(jp.p.rows.rows), static_cast<unsigned>((jp.p.q_heads + per_block - 1) / per_block)), dim3(JN_WARPS * 32), 0, st, jp);
 }
@@ -696,7 +718,7 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
                       : (plan.blocks == 2 ? launch_rows<128, 2>(rp, blocks, st) : launch_rows<128, 1>(rp, blocks, st));
     if (e) return e;
   }
-  JoinParams jp{p, {plan.span[0], plan.span[1]}};
+  JoinParams jp{p, {plan.span[0], plan.span[1]}, plan.parts == 0 && plan.span[0].part0 >= 0 ? 1 : 0};
   VX_CUDA_OK(d64 ? launch_join<64>(jp, plan.parts, st) : launch_join<128>(jp, plan.parts, st));
   return 0;
 }

@@ -28,6 +28,11 @@
 // reads P from the same columns, by the same thread: the tensor cores take its products in order.
 // The reference maximum of a row moves only when a tile's maximum exceeds it by more than 8 in units of log2 (probabilities stay below
 // 2^8); then the row's sum and its O are scaled before P is handed over.
+// What bounds it.  PAIRED: the round trip of a slot -- 2,000 cycles of softmax (1,024 of them exponentials: 128 x 128 at 16 a cycle for each of
+// two slots), then P V and the next S, 1,024 cycles of the tensor cores, with hand-over and the other slot's products in between: 3,870 cycles
+// a tile of 256 rows by 128 keys, 1.1 PFLOP/s over chunks of 2,048 tokens behind 16,384 (32 query heads on 8 key heads of 128).  Otherwise:
+// bytes from L2 and HBM where there are many keys (32 rows over 90,000 keys, 104 us, 3.8 TB/s), the softmax of a tile (some 1,950 cycles) where
+// keys are shared by many rows, and what a CTA costs to begin and end, 12 us, where an SM has a few tiles only.
 // Every wait on a barrier is bounded.
 
 #include <cuda_bf16.h>
