@@ -20,7 +20,7 @@
 //                     time between products).  PAIRED has one for both slots, whose products must not mix: two issuers without turns
 //                     took 27 % longer, with turns 8 %.
 //   warps 13, 14      one per stream of items: looks 32 items up at a time, a lane each, hands them to the other roles through a ring
-//                     and loads their queries
+//                     and loads their queries (PAIRED the second warp loads those of the second slot)
 // All roles run on into the next item as far as their rings and buffers let them, so that what an item costs to begin (its place in the tables,
 // its queries, its first keys) passes under the one before it.
 // Q, K and V lie in shared memory in rows of 128 bytes with the 128-byte swizzle, 64 columns a panel; V is read as an MN-major operand.
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], Shape::kParts);
     if (lane < PT_ITEMS) {
       mbar_init(&bar.item_full[s][lane], 1);
-      mbar_init(&bar.item_empty[s][lane], 4 / STREAMS + 1 + 8 / STREAMS);  // warps that read an item: loaders, MMA issuer, softmax
+      mbar_init(&bar.item_empty[s][lane], 4 / STREAMS + 1 + 8 / STREAMS + (PAIRED ? 1 : 0));  // warps that read an item: loaders, MMA issuer, softmax, the second slot's queries
     }
     if (lane < NB) {
       mbar_init(&bar.s_full[s][lane], 1);
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       mbar_init(&bar.pv_done[s][lane], 1);
     }
     if (lane == 0) {
-      mbar_init(&bar.q_full[s], 32);
+      mbar_init(&bar.q_full[s], 64 / STREAMS);  // threads that load queries
       mbar_init(&bar.q_empty[s], 1);
     }
     if (s < STREAMS && lane < NK) {
@@ -596,53 +596,67 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           --open;
         }
       }
-    } else if (warp - 13 < STREAMS) {
-      // =========================== items and their queries ===========================
-      const int stream = warp - 13;
-      const int n_streams = static_cast<int>(gridDim.x) * STREAMS, first = static_cast<int>(blockIdx.x) * STREAMS + stream;
+    } else if (warp < 15) {
+      // =========================== items and queries ===========================
+      const int slot = warp - 13, stream = PAIRED ? 0 : slot;
       constexpr int LANES = D / 8, ROWS = 32 / LANES;
       const int piece = lane % LANES, sub = lane / LANES;
-      int at = 0;
-      uint32_t phase = 0, q_phase = 0;
+      uint32_t q_phase = 0;
       bool ok = true;
-      auto hand_out = [&](const TileItem& t, bool writer) {
-        ok = __all_sync(ALL, mbar_wait(&bar.item_empty[stream][at], phase ^ 1, p.status, 49));
+      // The queries of the slot's rows [rho0, rho0 + 128) of `rows`, by whole warps of them: rows that do not exist are zeros.
+      auto load_q = [&](int row0, int rows, int rho0, int head) {
+        ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
         if (!ok) return;
-        if (writer) bar.item[stream][at] = t;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.item_full[stream][at]);
-        if (++at == PT_ITEMS) { at = 0; phase ^= 1; }
-      };
-      for (int64_t n0 = first; n0 < tp.items && ok; n0 += 32ll * n_streams) {
-        TileItem t;
-        const int64_t n = n0 + static_cast<int64_t>(lane) * n_streams;
-        const bool valid = n < tp.items && find_tile_item<PAIRED, BN>(tp, static_cast<int>(n), t);
-        for (unsigned left = __ballot_sync(ALL, valid); left != 0 && ok; left &= left - 1) {
-          const int src = __ffs(left) - 1;
-          hand_out(t, lane == src);
-          if (!ok) break;
-          const int row0 = __shfl_sync(ALL, t.row0, src), rows = __shfl_sync(ALL, t.rows, src), rho0 = __shfl_sync(ALL, t.rho0, src);
-          const int64_t head0 = __shfl_sync(ALL, t.head, src) * static_cast<int64_t>(p.per_kv.d);
-          ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
-          if (!ok) break;
-          q_phase ^= 1;
-          // whole warps' worth of rows: those that do not exist are zeros
-          const int n_rows = min((rows - rho0 + 31) / 32 * 32, PAIRED ? 2 * kSlotRows : kSlotRows);
-          for (int r = sub; r < n_rows; r += ROWS) {
-            const bool there = rho0 + r < rows;
-            uint32_t tok, hq;
-            p.per_kv.divmod(static_cast<uint32_t>(there ? rho0 + r : 0), tok, hq);
-            const __nv_bfloat16* src_row = p.q + static_cast<int64_t>(row0 + static_cast<int>(tok)) * p.q_row + (head0 + hq) * p.q_head;
-            const int slot = PAIRED ? r >> 7 : stream, local = r & 127;
-            cp_async16(smem_u32(q_s) + slot * Shape::kQ + (piece >> 3) * PT_Q_PANEL + local * 128 + (((piece & 7) ^ (local & 7)) << 4), src_row + piece * 8, there);
-          }
-          cp_async_arrive(&bar.q_full[stream]);
+        q_phase ^= 1;
+        const int n_rows = min((rows - rho0 + 31) / 32 * 32, kSlotRows);
+        const uint32_t dst = smem_u32(q_s) + slot * Shape::kQ + (piece >> 3) * PT_Q_PANEL;
+        const __nv_bfloat16* const src = p.q + row0 * p.q_row + head * static_cast<int64_t>(p.per_kv.d) * p.q_head + piece * 8;
+#pragma unroll 4
+        for (int r = sub; r < n_rows; r += ROWS) {
+          const bool there = rho0 + r < rows;
+          uint32_t tok, hq;
+          p.per_kv.divmod(static_cast<uint32_t>(there ? rho0 + r : 0), tok, hq);
+          cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4), src + tok * p.q_row + hq * p.q_head, there);
         }
+        cp_async_arrive(&bar.q_full[stream]);
+      };
+      if (PAIRED && slot == 1) {  // the second slot's
+        Items items;
+        TileItem t;
+        while (ok) {
+          ok = next_item(stream, items, t);
+          if (!ok || t.tiles == 0) break;
+          load_q(t.row0, t.rows, t.rho0 + kSlotRows, t.head);
+        }
+        cp_async_wait_all();
+      } else {
+        const int n_streams = static_cast<int>(gridDim.x) * STREAMS, first = static_cast<int>(blockIdx.x) * STREAMS + stream;
+        int at = 0;
+        uint32_t phase = 0;
+        auto hand_out = [&](const TileItem& t, bool writer) {
+          ok = __all_sync(ALL, mbar_wait(&bar.item_empty[stream][at], phase ^ 1, p.status, 49));
+          if (!ok) return;
+          if (writer) bar.item[stream][at] = t;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.item_full[stream][at]);
+          if (++at == PT_ITEMS) { at = 0; phase ^= 1; }
+        };
+        for (int64_t n0 = first; n0 < tp.items && ok; n0 += 32ll * n_streams) {
+          TileItem t;
+          const int64_t n = n0 + static_cast<int64_t>(lane) * n_streams;
+          const bool valid = n < tp.items && find_tile_item<PAIRED, BN>(tp, static_cast<int>(n), t);
+          for (unsigned left = __ballot_sync(ALL, valid); left != 0 && ok; left &= left - 1) {
+            const int src = __ffs(left) - 1;
+            hand_out(t, lane == src);
+            if (!ok) break;
+            load_q(__shfl_sync(ALL, t.row0, src), __shfl_sync(ALL, t.rows, src), __shfl_sync(ALL, t.rho0, src), __shfl_sync(ALL, t.head, src));
+          }
+        }
+        TileItem end;
+        end.tiles = 0;
+        if (ok) hand_out(end, lane == 0);
+        cp_async_wait_all();
       }
-      TileItem end;
-      end.tiles = 0;
-      if (ok) hand_out(end, lane == 0);
-      cp_async_wait_all();
     }
   } else {
     // =========================== softmax: a row per thread ===========================
