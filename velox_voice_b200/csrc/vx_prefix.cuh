@@ -63,12 +63,11 @@ __device__ __forceinline__ int owner_row0(const PrefixParams& p, bool sequences,
   return sequence_row0(p, sequences ? o : group_sequence0(p, o));
 }
 
-// group of a sequence, -1: none (WARP: all lanes of the warp ask for the same one)
-template <bool WARP = false>
+// group of a sequence, -1: none; all lanes of the warp ask for the same one
 __device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
   if (p.groups == 0) return -1;
   if (!p.group_offsets) return s / p.group_size;
-  const int g = WARP ? find_by_warp(p.groups, s, [&](int o) { return p.group_offsets[o]; }) : find_owner(p.group_offsets, p.groups, s);
+  const int g = find_by_warp(p.groups, s, [&](int o) { return p.group_offsets[o]; });
   return s >= p.group_offsets[g] && s < p.group_offsets[g + 1] ? g : -1;
 }
 
@@ -91,8 +90,8 @@ struct ItemRows {
 };
 
 // Owner and tile of a slot.  With offsets, owner o has the slots [base(o), base(o + 1)), base(o) = floor(row0(o) per_kv / TM) + o: enough for
-// its tiles, and found by a search without a pass over all owners.  WARP: all lanes of the warp ask for the same slot.
-template <int TM, bool WARP = false>
+// its tiles, and found by a search without a pass over all owners.  All lanes of the warp ask for the same slot.
+template <int TM>
 __device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp, int slot, ItemRows& it) {
   const int per = static_cast<int>(p.per_kv.d);
   const bool sequences = sp.kind != kSpanPrefix;
@@ -103,15 +102,8 @@ __device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp,
     tile = slot - it.owner * sp.equal;
   } else {
     auto base = [&](int o) { return static_cast<int>(static_cast<int64_t>(owner_row0(p, sequences, o)) * per / TM) + o; };
-    int lo = 0, hi = owners;  // largest o with base(o) <= slot
-    if (WARP) lo = find_by_warp(owners, slot, base);
-    while (!WARP && hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (base(mid) <= slot) lo = mid;
-      else hi = mid;
-    }
-    it.owner = lo;
-    tile = slot - base(lo);
+    it.owner = find_by_warp(owners, slot, base);  // the largest with base(o) <= slot
+    tile = slot - base(it.owner);
   }
   if (it.owner >= owners || tile < 0) return false;
   it.row0 = owner_row0(p, sequences, it.owner);
@@ -119,6 +111,91 @@ __device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp,
   it.rows = n * per;
   it.rho0 = tile * TM;
   return n > 0 && it.rho0 < it.rows;
+}
+
+// The tiles of a span counted by a warp, without the slots that have no rows: a kernel whose CTAs take items in turn shares them out evenly.
+struct SpanTiles {
+  int block;   // owners per lane
+  int before;  // tiles of the owners in front of this lane's
+  int tiles;   // all of them
+  int row0, rows;  // with one owner per lane: its run
+};
+__device__ __forceinline__ int scan_by_warp(int n) {  // the sum up to this lane, its own included
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, n, x);
+    if (lane >= x) n += y;
+  }
+  return n;
+}
+template <int TM>
+__device__ __forceinline__ int owner_tiles(const PrefixParams& p, bool sequences, int o, int& row0, int& rows) {
+  row0 = owner_row0(p, sequences, o);
+  rows = (owner_row0(p, sequences, o + 1) - row0) * static_cast<int>(p.per_kv.d);
+  return rows > 0 ? (rows - 1) / TM + 1 : 0;
+}
+template <int TM>
+__device__ __forceinline__ SpanTiles count_tiles(const PrefixParams& p, const Span& sp) {
+  const bool sequences = sp.kind != kSpanPrefix;
+  const int owners = sequences ? p.rows.sequences : p.groups, lane = threadIdx.x & 31;
+  SpanTiles st{};
+  if (sp.chunks == 0) return st;
+  if (sp.equal) {
+    st.tiles = owners * sp.equal;
+    return st;
+  }
+  st.block = (owners + 31) / 32;
+  int n = 0;
+#pragma unroll 4
+  for (int i = 0; i < st.block; ++i)
+    if (lane * st.block + i < owners) n += owner_tiles<TM>(p, sequences, lane * st.block + i, st.row0, st.rows);
+  const int sum = scan_by_warp(n);
+  st.before = sum - n;
+  st.tiles = min(max(__shfl_sync(0xffffffffu, sum, 31), 0), sp.slots);  // (offsets that do not ascend)
+  return st;
+}
+// Rows of tile t; all lanes of the warp ask for the same one.
+template <int TM>
+__device__ __forceinline__ bool find_tile(const PrefixParams& p, const Span& sp, const SpanTiles& st, int t, ItemRows& it) {
+  const bool sequences = sp.kind != kSpanPrefix;
+  const int owners = sequences ? p.rows.sequences : p.groups, lane = threadIdx.x & 31;
+  int tile = 0;
+  if (sp.equal) {
+    it.owner = t / sp.equal;
+    tile = t - it.owner * sp.equal;
+  } else {
+    const int src = 31 - __clz(__ballot_sync(0xffffffffu, lane == 0 || st.before <= t));  // the lane that counted it
+    const int before = __shfl_sync(0xffffffffu, st.before, src);
+    it.row0 = __shfl_sync(0xffffffffu, st.row0, src);
+    it.rows = __shfl_sync(0xffffffffu, st.rows, src);
+    it.owner = src;
+    tile = t - before;
+    if (st.block > 1) {  // 32 of its owners at a time
+      it.owner = -1;
+      int first = before;
+      for (int o = src * st.block, end = min(o + st.block, owners); o < end; o += 32) {
+        int row0, rows;
+        const int n = o + lane < end ? owner_tiles<TM>(p, sequences, o + lane, row0, rows) : 0, sum = scan_by_warp(n), all = __shfl_sync(0xffffffffu, sum, 31);
+        if (t < first + all) {
+          const int k = __ffs(__ballot_sync(0xffffffffu, t < first + sum)) - 1;
+          it.owner = o + k;
+          it.row0 = __shfl_sync(0xffffffffu, row0, k);
+          it.rows = __shfl_sync(0xffffffffu, rows, k);
+          tile = t - first - __shfl_sync(0xffffffffu, sum - n, k);
+          break;
+        }
+        first += all;
+      }
+      if (it.owner < 0) return false;
+    }
+  }
+  if (sp.equal) {
+    it.row0 = owner_row0(p, sequences, it.owner);
+    it.rows = (owner_row0(p, sequences, it.owner + 1) - it.row0) * static_cast<int>(p.per_kv.d);
+  }
+  it.rho0 = tile * TM;
+  return tile >= 0 && it.rho0 < it.rows;
 }
 
 // Not 0 if one of the two bf16 values of a word is an infinity or NaN, gathered in `sum` (0 x is 0 or NaN).

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_k
   if (chunk >= sp.chunks) return;
   const bool own = sp.kind == kSpanOwn;
   ItemRows it;
-  if (!find_rows<TM, true>(p, sp, n - chunk * sp.slots, it)) return;
+  if (!find_rows<TM>(p, sp, n - chunk * sp.slots, it)) return;
   const int length = own ? p.rows.lengths[it.owner] : 0;
   // keys [key0, keys): those of the chunk that the tile's last row sees
   int keys = own ? own_keys(p, length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(min(it.rho0 + TM, it.rows) - 1)))) : prefix_keys(p, it.owner);
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(JN_WARPS * 32, PARTS > 4 ? 4 : (D == 64 ? 8 : 
   const bool in = h < p.q_heads;
   int parts[2] = {0, 0}, s, i;
   if (row_sequence<true>(p.rows, row, s, i)) {
-    const int prefix = prefix_keys(p, group_of<true>(p, s)), own = own_keys(p, p.rows.lengths[s], i);
+    const int prefix = prefix_keys(p, group_of(p, s)), own = own_keys(p, p.rows.lengths[s], i);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const Span& sp = jp.span[e];
@@ -577,6 +577,26 @@ int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int64_t unit, 
   return static_cast<int>(c < all ? c : all);
 }
 
+// The same for pairs of slots, whose items are long: the number of cuts that an estimate finds fastest.  A CTA takes its items one after
+// another, a tile of 128 keys in 2.0 (head_dim 128) or 1.4 us, with 4 us for what an item costs besides; `cells` rows and heads leave sums per
+// part, written and read at 4.5 TB/s, where there is more than one part (`joint`: or none).
+int pair_chunk_keys(int64_t capacity, int64_t items, int head_dim, int64_t cells, bool joint) {
+  constexpr int64_t unit = 256;
+  int64_t best = round_up(capacity, unit);
+  double best_us = 1e30;
+  for (int64_t cuts = 1; cuts <= 64; ++cuts) {
+    const int64_t chunk = round_up((capacity + cuts - 1) / cuts, unit), n = (capacity + chunk - 1) / chunk;
+    const double turns = static_cast<double>((items * n + sm_count() - 1) / sm_count());
+    const double us = turns * (static_cast<double>(chunk) / 128 * (head_dim == 128 ? 2.0 : 1.4) + 4.0) + (joint && n == 1 ? 0.0 : static_cast<double>(n * cells * head_dim) * 8.0 / 4.5e6);
+    if (us < best_us) {
+      best_us = us;
+      best = chunk;
+    }
+    if (chunk == unit) break;
+  }
+  return static_cast<int>(best);
+}
+
 int64_t rows_resident(int blocks, int head_dim) { return static_cast<int64_t>(rows_ctas(blocks, head_dim)) * sm_count(); }
 
 int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, PrefixParams& p, Plan& plan) {
@@ -625,7 +645,10 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     sp.equal = equal_rows > 0 ? static_cast<int32_t>((equal_rows + tm - 1) / tm) : 0;
     sp.slots = static_cast<int32_t>(sp.equal ? owners * sp.equal : R * per / tm + owners);
     const int64_t items = static_cast<int64_t>(sp.slots) * p.kv_heads, sms = sm_count();
-    if (kernel == Plan::kPairs) sp.chunk = chunk_keys(cap, items, sms, 256, 1024, 4);
+    if (kernel == Plan::kPairs) {  // (slots are places for tiles; of tiles there are as many as owners of average size have)
+      const int64_t tiles = owners * ((R * per / owners + tm - 1) / tm);
+      sp.chunk = pair_chunk_keys(cap, (tiles < sp.slots ? tiles : sp.slots) * p.kv_heads, cache->head_dim, R * d->q_heads, kind == kSpanJoint);
+    }
     else if (kernel == Plan::kTiles) sp.chunk = chunk_keys(cap, items, 2 * sms, 128, 256, owners == 1 ? 1 : 3);
     else sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim), 16 * PR_WARPS, cache->head_dim == 64 ? 1024 : 256, 3);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);

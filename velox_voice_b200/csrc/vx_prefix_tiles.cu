@@ -19,8 +19,7 @@
 //                     has to wait for and to look up between two tiles passes under the other's products (one issuer for both spent 60 % of its
 //                     time between products).  PAIRED has one for both slots, whose products must not mix: two issuers without turns
 //                     took 27 % longer, with turns 8 %.
-//   warps 13, 14      one per stream of items: looks 32 items up at a time, a lane each, hands them to the other roles through a ring
-//                     and loads their queries (PAIRED the second warp loads those of the second slot)
+//   warps 13, 14      one per stream of items: looks them up, hands them to the other roles through a ring and loads their queries (PAIRED the second warp loads those of the second slot)
 // All roles run on into the next item as far as their rings and buffers let them, so that what an item costs to begin (its place in the tables,
 // its queries, its first keys) passes under the one before it.
 // Q, K and V lie in shared memory in rows of 128 bytes with the 128-byte swizzle, 64 columns a panel; V is read as an MN-major operand.
@@ -72,7 +71,6 @@ struct TileShape {
 struct TilesParams {
   PrefixParams p;
   Span span[2];
-  int32_t first_items, items;
 };
 
 // What the roles know of an item.  Its keys are those from v0 on of the row prefix keys (padded to p128) | own keys.
@@ -138,19 +136,15 @@ __device__ __forceinline__ void store32(float* dst, const uint32_t* v) {
 // bits [0, n) of a word
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1); }
 
-// Item n of the launch; false: there is nothing to do for it.
+// Item n of a span, heads next to each other, then tiles, then chunks; false: there is nothing to do for it.  All lanes of the warp.
 template <bool PAIRED, int KEYS>
-__device__ bool find_tile_item(const TilesParams& tp, int n, TileItem& t) {
+__device__ bool find_tile_item(const PrefixParams& p, const Span& sp, const SpanTiles& st, uint32_t n, TileItem& t) {
   constexpr int TM = PAIRED ? 2 * kSlotRows : kSlotRows;
-  const PrefixParams& p = tp.p;
-  const bool second = n >= tp.first_items;
-  if (second) n -= tp.first_items;
-  const Span& sp = tp.span[second];
-  t.head = n % p.kv_heads;
-  n /= p.kv_heads;
-  const int chunk = n / sp.slots;
+  const uint32_t kv = static_cast<uint32_t>(p.kv_heads), tile = n / kv, tiles = static_cast<uint32_t>(st.tiles);
+  t.head = static_cast<int>(n - tile * kv);
+  const int chunk = static_cast<int>(tile / tiles);
   ItemRows r;
-  if (!find_rows<TM>(p, sp, n - chunk * sp.slots, r)) return false;
+  if (!find_tile<TM>(p, sp, st, static_cast<int>(tile - static_cast<uint32_t>(chunk) * tiles), r)) return false;
   t.row0 = r.row0; t.rows = r.rows; t.rho0 = r.rho0;
   t.group = t.sequence = t.length = 0;
   t.p_keys = t.o_keys = 0;
@@ -630,7 +624,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         }
         cp_async_wait_all();
       } else {
-        const int n_streams = static_cast<int>(gridDim.x) * STREAMS, first = static_cast<int>(blockIdx.x) * STREAMS + stream;
+        const uint32_t n_streams = gridDim.x * STREAMS, first = blockIdx.x * STREAMS + static_cast<uint32_t>(stream);
         int at = 0;
         uint32_t phase = 0;
         auto hand_out = [&](const TileItem& t, bool writer) {
@@ -641,16 +635,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           if (lane == 0) mbar_arrive(&bar.item_full[stream][at]);
           if (++at == PT_ITEMS) { at = 0; phase ^= 1; }
         };
-        for (int64_t n0 = first; n0 < tp.items && ok; n0 += 32ll * n_streams) {
+        // A stream has an item of every round, in turn from both ends of it: with causal rows the later tiles have more keys.  (The host saw to
+        // it that items are below 2^31.)
+        constexpr int TM = PAIRED ? 2 * kSlotRows : kSlotRows;
+        SpanTiles st0{}, st1{};
+        uint32_t items0 = 0, items = 0;  // of the first span, of both
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e) {  // (one copy of the code: what is fetched for the first time counts here)
+          st0 = st1;
+          items0 = items;
+          st1 = count_tiles<TM>(p, tp.span[e]);
+          items += static_cast<uint32_t>(st1.tiles * tp.span[e].chunks * p.kv_heads);
+        }
+#pragma unroll 1
+        for (uint32_t n0 = 0, odd = 0; n0 < items && ok; n0 += n_streams, odd ^= 1) {
+          const uint32_t n = n0 + (odd ? n_streams - 1 - first : first);
+          if (n >= items) continue;
+          const bool second = n >= items0;
           TileItem t;
-          const int64_t n = n0 + static_cast<int64_t>(lane) * n_streams;
-          const bool valid = n < tp.items && find_tile_item<PAIRED, BN>(tp, static_cast<int>(n), t);
-          for (unsigned left = __ballot_sync(ALL, valid); left != 0 && ok; left &= left - 1) {
-            const int src = __ffs(left) - 1;
-            hand_out(t, lane == src);
-            if (!ok) break;
-            load_q(__shfl_sync(ALL, t.row0, src), __shfl_sync(ALL, t.rows, src), __shfl_sync(ALL, t.rho0, src), __shfl_sync(ALL, t.head, src));
-          }
+          if (!find_tile_item<PAIRED, BN>(p, tp.span[second], second ? st1 : st0, second ? n - items0 : n, t)) continue;
+          hand_out(t, lane == 0);
+          if (ok) load_q(t.row0, t.rows, t.rho0, t.head);
         }
         TileItem end;
         end.tiles = 0;
@@ -863,7 +868,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 }
 
 template <int D, bool PAIRED>
-int launch(const TilesParams& tp, cudaStream_t st) {
+int launch(const TilesParams& tp, int64_t items, cudaStream_t st) {  // `items`: at most
   int dev = 0;
   VX_CUDA_OK(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_done{0};
@@ -872,7 +877,7 @@ int launch(const TilesParams& tp, cudaStream_t st) {
     VX_CUDA_OK(cudaFuncSetAttribute(prefix_tiles_kernel<D, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<D, PAIRED>::kSmem));
     if (cached) attr_done.fetch_or(1ull << dev, std::memory_order_release);
   }
-  const int ctas = PAIRED ? tp.items : (tp.items + 1) / 2;
+  const int64_t ctas = PAIRED ? items : (items + 1) / 2;
   VX_CUDA_OK(launch_dependent(prefix_tiles_kernel<D, PAIRED>, dim3(static_cast<unsigned>(ctas < sm_count() ? ctas : sm_count())), dim3(PT_THREADS),
                               TileShape<D, PAIRED>::kSmem, st, tp));
   return 0;
@@ -881,15 +886,13 @@ int launch(const TilesParams& tp, cudaStream_t st) {
 }  // namespace
 
 int launch_prefix_tiles(const PrefixParams& p, int head_dim, bool paired, const Span& a, const Span& b, void* stream) {
-  TilesParams tp{p, {a, b}, 0, 0};
+  const TilesParams tp{p, {a, b}};
   const int64_t first = static_cast<int64_t>(a.slots) * a.chunks * p.kv_heads;
   const int64_t items = first + static_cast<int64_t>(b.slots) * b.chunks * p.kv_heads;
   if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
-  tp.first_items = static_cast<int32_t>(first);
-  tp.items = static_cast<int32_t>(items);
   const auto st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 64) return paired ? launch<64, true>(tp, st) : launch<64, false>(tp, st);
-  return paired ? launch<128, true>(tp, st) : launch<128, false>(tp, st);
+  if (head_dim == 64) return paired ? launch<64, true>(tp, items, st) : launch<64, false>(tp, items, st);
+  return paired ? launch<128, true>(tp, items, st) : launch<128, false>(tp, items, st);
 }
 
 }  // namespace vx
