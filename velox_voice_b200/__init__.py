@@ -2,12 +2,13 @@
 
 A thin PyTorch host layer over ``libvelox_b200.so`` (C ABI, ``include/velox_b200.h``):
 activation quantize/pack fused behind LayerNorm, tcgen05 block-scaled FP4 / FP8 GEMMs with
-fused bias / Swish / GLU / residual epilogues, and frame-sharded multi-GPU execution.
+fused bias / Swish / GLU / residual epilogues, and frame-sharded multi-GPU execution; a paged cache of keys
+and values with the attention of hypotheses that share a prefix.
 """
 
 import importlib
 
-__all__ = ["ops", "linear", "stack", "install", "build"]
+__all__ = ["ops", "linear", "stack", "decoder", "install", "build"]
 
 
 def __getattr__(name):

@@ -8,7 +8,7 @@
 // interleaved: 16 consecutive values), so cosines and sines are 64 consecutive bytes of the table and no value is read twice.  Where a
 // row goes -- sequence, page, place -- is looked up once per row and block, not per thread.
 // What bounds it: HBM (each input byte read once, each output byte written once; the table's rows come from L1 for all heads but the first):
-// 90,000 tokens, 32 query and 8 key heads of 128, 2.2 GB in 385 us, 5.7 TB/s.  Small calls: the launch (4.5 us for 64 tokens).
+// 24 sequences of 5,000 tokens, 32 query and 8 key heads of 128, 2.2 GB in 388 us, 5.7 TB/s.  Small calls: the launch (4.5 us for 64 tokens).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
