@@ -66,6 +66,10 @@ struct TileShape {
   static constexpr int kQ = D / 64 * PT_Q_PANEL;              // of a slot's queries
   static constexpr int kStreams = PAIRED ? 1 : 2;
   static constexpr int kParts = PAIRED ? 4 : 1;               // loaders that share a tile
+  // P of a tile handed over in halves, so that the products of the first run under the exponentials of the second.  Gains where the products are
+  // short (16 utterances, prompts of 200 tokens behind 6,000, head_dim 64: 363 -> 339 us) and loses where an issuer that waits for the second
+  // half keeps the other slot's products waiting (four chunks of 2,048 behind 16,384, head_dim 128: 1,710 -> 1,755).
+  static constexpr bool kHalves = PAIRED && D == 64;
   static constexpr int kStagesK = D == 128 ? 3 : 5, kStagesV = D == 128 ? 2 : 5;  // of a stream
   static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + 1024;
 };
@@ -89,6 +93,7 @@ template <class Shape>
 struct TileBarriers {
   uint64_t k_full[Shape::kStreams][Shape::kStagesK], k_empty[Shape::kStreams][Shape::kStagesK];
   uint64_t v_full[Shape::kStreams][Shape::kStagesV], v_empty[Shape::kStreams][Shape::kStagesV];
+  uint64_t p_half[2];  // kHalves: the first half of a tile's P
   uint64_t s_full[2][Shape::kBuffers], p_full[2][Shape::kBuffers], pv_done[2][Shape::kBuffers], q_full[2], q_empty[2];
   uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
   alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
@@ -284,6 +289,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     if (lane == 0) {
       mbar_init(&bar.q_full[s], 64 / STREAMS);  // threads that load queries
       mbar_init(&bar.q_empty[s], 1);
+      mbar_init(&bar.p_half[s], 4);
     }
     if (s < STREAMS && lane < NK) {
       mbar_init(&bar.k_full[s][lane], 32 * Shape::kParts);  // threads of the loaders that share a tile
@@ -487,13 +493,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           tc_commit(&bar.s_full[slot][buffer]);
         }
       };
-      auto issue_o = [&](int slot, int buffer, int stage, bool first) {  // P is there
+      auto issue_o = [&](int slot, int buffer, int stage, bool first, int from, int to) {  // P of these 16s of keys is there
         const uint32_t vt = __shfl_sync(ALL, v_lo + stage * (Shape::kTile >> 4), 0) | (static_cast<uint32_t>(Shape::kPanel >> 4) << 16);
         const uint32_t tm = __shfl_sync(ALL, tmem_base + slot * PT_TM_SLOT, 0), ps = __shfl_sync(ALL, tm + buffer * BN, 0);
         tc_fence_after();
         if (leader) {
 #pragma unroll
-          for (int i = 0; i < BN / 16; ++i)  // 16 keys are two groups of eight rows
+          for (int i = from; i < to; ++i)  // 16 keys are two groups of eight rows
             mma_bf16_ts(tm + PT_TM_O, ps + i * 8, desc(vt + i * ((16 * 128) >> 4)), idesc_o, !(first && i == 0));
         }
       };
@@ -511,24 +517,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         int x = -1, ks = 0, vs = 0;
         uint32_t k_phase = 0, v_phase = 0, p_phase = 0;  // p_phase: a bit per slot
         bool has[2] = {false, false}, fresh = false, last[2] = {false, false};  // of tile x: which slots take it, first and last of the item
-        auto wait_p = [&](int s) {
-          const bool there = __all_sync(ALL, mbar_wait_spin(&bar.p_full[s][0], (p_phase >> s) & 1, p.status, 43));
+        auto take_p = [&](int s, int stage, bool first) {
+          const uint32_t phase = (p_phase >> s) & 1;
           p_phase ^= 1u << s;
+          constexpr int FIRST = Shape::kHalves ? BN / 32 : 0;
+          bool there = true;
+          if (Shape::kHalves) {
+            there = __all_sync(ALL, mbar_wait_spin(&bar.p_half[s], phase, p.status, 56));
+            if (there) issue_o(s, 0, stage, first, 0, FIRST);
+          }
+          there = there && __all_sync(ALL, mbar_wait_spin(&bar.p_full[s][0], phase, p.status, 43));
+          if (there) issue_o(s, 0, stage, first, FIRST, BN / 16);
           return there;
         };
         auto step = [&](bool more, bool has0, bool has1, bool first, bool last0, bool last1, bool end) {  // tile x + 1: whether there is one, ...
           if (x >= 0) ok = landed(bar.v_full[0], vs, v_phase);
           if (ok && has[0]) {
-            ok = wait_p(0);
-            if (ok) issue_o(0, 0, vs, fresh);
+            ok = take_p(0, vs, fresh);
             if (ok && last[0] && leader) tc_commit(&bar.pv_done[0][0]);
           }
           if (ok && first) ok = wait_q(0);
           if (ok && more) ok = landed(bar.k_full[0], ks, k_phase);
           if (ok && has0) issue_s(0, 0, ks);
           if (ok && has[1]) {
-            ok = wait_p(1);
-            if (ok) issue_o(1, 0, vs, fresh);
+            ok = take_p(1, vs, fresh);
             if (ok && last[1] && leader) tc_commit(&bar.pv_done[1][0]);
           }
           if (!ok) return;
@@ -581,7 +593,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           ok = landed(bar.v_full[slot], vs, v_phase) && __all_sync(ALL, mbar_wait_spin(&bar.p_full[slot][o_buffer], (p_phase >> o_buffer) & 1, p.status, 43));
           if (!ok) break;
           p_phase ^= 1u << o_buffer;
-          issue_o(slot, o_buffer, slot * NV + vs, (firsts & 1) != 0);
+          issue_o(slot, o_buffer, slot * NV + vs, (firsts & 1) != 0, 0, BN / 16);
           if (leader) {
             tc_commit(&bar.pv_done[slot][o_buffer]);
             tc_commit(&bar.v_empty[slot][vs]);
@@ -698,7 +710,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         const uint32_t tb = tm + buffer * BN;
         if (idle) {
           ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 47));
-          if (ok && lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
+          if (ok && lane == 0) {
+            if (Shape::kHalves) mbar_arrive(&bar.p_half[slot]);
+            mbar_arrive(&bar.p_full[slot][buffer]);
+          }
           return;
         }
         // which keys of the tile this row sees: as a rule all of them
@@ -787,6 +802,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             pk[e >> 1] = pack_bf16(x0, x1);
           }
           tc_st_x16(tb + 16 * i, pk);  // over S, which is in registers
+          if (Shape::kHalves && !LATE && i == W / 2 - 1) {
+            tc_wait_st_all();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.p_half[slot]);
+          }
         }
         float a0, a1, b0, b1;
         unpack_f32x2(sum[0], a0, a1);
@@ -805,7 +826,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.p_full[slot][buffer]);
+        if (lane == 0) {
+          if (Shape::kHalves && LATE) mbar_arrive(&bar.p_half[slot]);
+          mbar_arrive(&bar.p_full[slot][buffer]);
+        }
       };
       // the late tiles begin with the one that has the first own token that the first row does not see
       const int first_late = warp_limit >= t.o_keys ? mine : min(max(t.p128 + warp_limit - t.v0, 0) / BN, mine);
