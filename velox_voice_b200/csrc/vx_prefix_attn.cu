@@ -668,10 +668,14 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     // A rule that meets these: what the walks read together.
     const double bytes = 4.0 * static_cast<double>(G * cap_p) * cache->kv_heads * cache->head_dim;  // of the keys and values
     const bool few = rows_p <= (cache->head_dim == 64 ? 16 : 8) || (rows_p <= 64 && static_cast<double>((rows_p + 15) / 16) * bytes <= 64.0 * 1048576.0);
-    // Pairs of slots share their keys; with an odd number of slots one of a pair idles.  One group of 30,000 keys, 8 key heads, slots by
-    // themselves against pairs, in us: head_dim 64  300 rows 85 : 99  400 rows 124 : 110   head_dim 128  360 rows 99 : 132  512 rows 143 : 155
-    // 560 rows 171 : 167  800 rows 218 : 202.
-    plan.kernel[0] = few ? Plan::kRows : (rows_p > (cache->head_dim == 64 ? 3 : 4) * kSlotRows ? Plan::kPairs : Plan::kTiles);
+    // Pairs of slots share their keys, which counts where there are many; with an odd number of slots one of a pair idles, and a pair starts
+    // slower.  8 key heads, slots by themselves against pairs, in us:
+    //   head_dim 64, 6 MB of keys and values   256 rows 28 : 30   500 33 : 38      49 MB (8 groups)  256 rows 83 : 77   384 112 : 112   500 146 : 125
+    //                61 MB (1 group)           256 rows 54 : 56   384 85 : 81   500 126 : 84
+    //   head_dim 128, 12 MB  256 rows 28 : 32   512 36 : 40   600 42 : 40          34 MB  256 rows 58 : 63
+    //                98 MB (8 groups)  200 rows 76 : 65   360 108 : 97   512 147 : 108   123 MB (1 group)  200 rows 67 : 62   256 65 : 65   360 97 : 87   512 146 : 93
+    const bool pairs = rows_p > 4 * kSlotRows || (rows_p > 3 * kSlotRows && bytes > 32.0 * 1048576.0) || (rows_p > kSlotRows && bytes > 64.0 * 1048576.0);
+    plan.kernel[0] = few ? Plan::kRows : (pairs ? Plan::kPairs : Plan::kTiles);
     // Own tokens of many sequences are many short walks, whose start counts for more.  160 sequences without a prefix, new tokens behind a
     // history, 8 key heads, rows kernel against tiles, in us:
     //   head_dim 64   12 rows  0 + 12 keys 18 : 33  500 + 12 51 : 70    24 rows  0 + 24 27 : 39  2,000 + 24 159 : 188    48 rows  100 + 48 57 : 61  500 + 48 104 : 102
