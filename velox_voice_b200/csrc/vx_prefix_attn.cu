@@ -578,22 +578,21 @@ int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int64_t unit, 
   return static_cast<int>(c < all ? c : all);
 }
 
-// The same for pairs of slots, whose items are long: the number of cuts that an estimate finds fastest.  A CTA takes its items one after
-// another, a tile of 128 keys in 2.0 (head_dim 128) or 1.4 us, with 4 us for what an item costs besides; `cells` rows and heads leave sums per
-// part, written and read at 4.5 TB/s, where there is more than one part (`joint`: or none).
-int pair_chunk_keys(int64_t capacity, int64_t items, int head_dim, int64_t cells, bool joint) {
-  constexpr int64_t unit = 256;
+// The same for the tile kernel, whose items are long: the number of cuts that an estimate finds fastest.  `streams` take items one after another, 128
+// keys in `us`, with 4 us for what an item costs besides; `cells` rows and heads leave sums per part, written and read at 4.5 TB/s, where
+// there is more than one part (`joint`: or none).
+int tile_chunk_keys(int64_t capacity, int64_t items, int64_t streams, int64_t unit, double us, int head_dim, int64_t cells, bool joint) {
   int64_t best = round_up(capacity, unit);
   double best_us = 1e30;
-  for (int64_t cuts = 1; cuts <= 64; ++cuts) {
+  for (int64_t cuts = 1; cuts <= 512; ++cuts) {
     const int64_t chunk = round_up((capacity + cuts - 1) / cuts, unit), n = (capacity + chunk - 1) / chunk;
-    const double turns = static_cast<double>((items * n + sm_count() - 1) / sm_count());
-    const double us = turns * (static_cast<double>(chunk) / 128 * (head_dim == 128 ? 2.0 : 1.4) + 4.0) + (joint && n == 1 ? 0.0 : static_cast<double>(n * cells * head_dim) * 8.0 / 4.5e6);
-    if (us < best_us) {
-      best_us = us;
+    const double turns = static_cast<double>((items * n + streams - 1) / streams);
+    const double all = turns * (static_cast<double>(chunk) / 128 * us + 4.0) + (joint && n == 1 ? 0.0 : static_cast<double>(n * cells * head_dim) * 8.0 / 4.5e6);
+    if (all < best_us) {
+      best_us = all;
       best = chunk;
     }
-    if (chunk == unit) break;
+    if (chunk == unit || turns > 64) break;
   }
   return static_cast<int>(best);
 }
@@ -646,11 +645,11 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     sp.equal = equal_rows > 0 ? static_cast<int32_t>((equal_rows + tm - 1) / tm) : 0;
     sp.slots = static_cast<int32_t>(sp.equal ? owners * sp.equal : R * per / tm + owners);
     const int64_t items = static_cast<int64_t>(sp.slots) * p.kv_heads, sms = sm_count();
-    if (kernel == Plan::kPairs) {  // (slots are places for tiles; of tiles there are as many as owners of average size have)
-      const int64_t tiles = owners * ((R * per / owners + tm - 1) / tm);
-      sp.chunk = pair_chunk_keys(cap, (tiles < sp.slots ? tiles : sp.slots) * p.kv_heads, cache->head_dim, R * d->q_heads, kind == kSpanJoint);
+    if (kernel != Plan::kRows) {  // (slots are places for tiles; of tiles there are as many as owners of average size have)
+      const int64_t tiles = owners * ((R * per / owners + tm - 1) / tm), n = (tiles < sp.slots ? tiles : sp.slots) * p.kv_heads;
+      const bool paired = kernel == Plan::kPairs;
+      sp.chunk = tile_chunk_keys(cap, n, paired ? sms : 2 * sms, paired ? 256 : 128, paired && cache->head_dim == 64 ? 1.4 : 2.0, cache->head_dim, R * d->q_heads, kind == kSpanJoint);
     }
-    else if (kernel == Plan::kTiles) sp.chunk = chunk_keys(cap, items, 2 * sms, 128, 256, owners == 1 ? 1 : 3);
     else sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim), 16 * PR_WARPS, cache->head_dim == 64 ? 1024 : 256, 3);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
