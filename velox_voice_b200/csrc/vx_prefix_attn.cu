@@ -26,6 +26,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <atomic>
@@ -578,21 +579,30 @@ int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int64_t unit, 
   return static_cast<int>(c < all ? c : all);
 }
 
-// The same for the tile kernel, whose items are long: the number of cuts that an estimate finds fastest.  `streams` take items one after another, 128
-// keys in `us`, with 4 us for what an item costs besides; `cells` rows and heads leave sums per part, written and read at 4.5 TB/s, where
-// there is more than one part (`joint`: or none).
+// The same for the tile kernel, whose items are long: the cut that an estimate finds fastest.  `streams` take items one after another, 128 keys
+// in `us`, with 4 us for what an item costs besides; `cells` rows and heads leave sums per part, written and read at 4.5 TB/s, where there is
+// more than one part (`joint`: or none).  Tried: for each number of turns that the streams take, as many cuts as fill them, and where the keys
+// and the parts of a turn cost the same.
 int tile_chunk_keys(int64_t capacity, int64_t items, int64_t streams, int64_t unit, double us, int head_dim, int64_t cells, bool joint) {
+  const double part_us = static_cast<double>(cells * head_dim) * 8.0 / 4.5e6, walk_us = static_cast<double>(capacity) / 128 * us;
+  const int64_t most = (capacity + unit - 1) / unit, turns0 = (items + streams - 1) / streams;
   int64_t best = round_up(capacity, unit);
-  double best_us = 1e30;
-  for (int64_t cuts = 1; cuts <= 512; ++cuts) {
-    const int64_t chunk = round_up((capacity + cuts - 1) / cuts, unit), n = (capacity + chunk - 1) / chunk;
+  double best_us = 1e300;
+  auto look_at = [&](int64_t cuts) {
+    const int64_t c = cuts < 1 ? 1 : (cuts > most ? most : cuts), chunk = round_up((capacity + c - 1) / c, unit), n = (capacity + chunk - 1) / chunk;
     const double turns = static_cast<double>((items * n + streams - 1) / streams);
-    const double all = turns * (static_cast<double>(chunk) / 128 * us + 4.0) + (joint && n == 1 ? 0.0 : static_cast<double>(n * cells * head_dim) * 8.0 / 4.5e6);
+    const double all = turns * (static_cast<double>(chunk) / 128 * us + 4.0) + (joint && n == 1 ? 0.0 : static_cast<double>(n) * part_us);
     if (all < best_us) {
       best_us = all;
       best = chunk;
     }
-    if (chunk == unit || turns > 64) break;
+  };
+  look_at(1);
+  for (int64_t turns = turns0; turns < turns0 + 8; ++turns) {
+    const int64_t full = turns * streams / items, even = static_cast<int64_t>(sqrt(static_cast<double>(turns) * walk_us / part_us) + 0.5);
+    look_at(full);
+    if (even < full) look_at(even);
+    if (full >= most) break;
   }
   return static_cast<int>(best);
 }
