@@ -362,6 +362,8 @@ def dense_reference(q, k_pages, v_pages, table, length, ptable, prefix, groups, 
     (3000, 1, 1, 8, 8, 64, 20, 0),         # short own runs, a warp each
     (2, 1, 2, 32, 8, 128, 40000, 30000),   # few rows over many keys: many parts of a row
     (7, 700, 1, 12, 4, 128, 900, 3000),
+    (1500, 40, 1, 2, 2, 64, 290, 50),      # more owners than a warp counts at a time, with own tiles
+    (1100, 140, 11, 2, 1, 64, 0, 40),      # the same for pairs
 ])
 def test_attention_large_calls(ops, n, tokens, groups, heads, kv, d, length, prefix):
     ps = 16
