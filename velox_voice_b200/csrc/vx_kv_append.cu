@@ -8,7 +8,7 @@
 // interleaved: 16 consecutive values), so cosines and sines are 64 consecutive bytes of the table and no value is read twice.  Where a
 // row goes -- sequence, page, place -- is looked up once per row and block, not per thread.
 // What bounds it: HBM (each input byte read once, each output byte written once; the table's rows come from L1 for all heads but the first):
-// 24 sequences of 5,000 tokens, 32 query and 8 key heads of 128, 2.2 GB in 388 us, 5.7 TB/s.  Small calls: the launch (4.5 us for 64 tokens).
+// 24 sequences of 5,000 tokens, 32 query and 8 key heads of 128, 2.2 GB in 353 us, 6.3 TB/s.  Small calls: the launch (2.8 us for 10 tokens).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -55,6 +55,8 @@ int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c,
 namespace {
 
 constexpr int AP_THREADS = 256;
+constexpr int AP_BLOCKS = 6;     // per SM, at 40 registers a thread: five of 46 take 375 us at the size above, seven or eight, which spill, 507
+constexpr int AP_UNITS = 16;     // of a thread in large calls, since a block looks its rows up before it moves any: 4 take 422 us there, 8 391, 16 375 (of five blocks)
 constexpr int AP_MAX_ROWS = 32;  // rows of a block at most
 
 struct AppendParams {
@@ -109,7 +111,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(AP_THREADS, AP_BLOCKS) kv_append_kernel(const AppendParams p) {
   pdl_launch_dependents();
   __shared__ RowPlace place[AP_MAX_ROWS];
   const int row0 = static_cast<int>(blockIdx.x) * p.rows_per_block;
@@ -247,8 +249,8 @@ extern "C" int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, co
   p.units_per_head = FastDiv(static_cast<uint32_t>(D / 16));
   const int64_t upr = static_cast<int64_t>(p.q_heads + 2 * p.kv_heads) * (D / 16);
   p.units_per_row = FastDiv(static_cast<uint32_t>(upr));
-  // Rows per block: four units per thread keep enough loads in flight; fewer rows while that leaves SMs without a block.
-  int64_t rpb = (4 * AP_THREADS + upr - 1) / upr;
+  // Rows per block; fewer while that leaves SMs without a block.
+  int64_t rpb = (AP_UNITS * AP_THREADS + upr - 1) / upr;
   const int64_t fill = p.rows.rows / (4 * sm_count());
   if (rpb > fill) rpb = fill;
   if (rpb > AP_MAX_ROWS) rpb = AP_MAX_ROWS;
