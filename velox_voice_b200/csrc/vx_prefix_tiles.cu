@@ -21,7 +21,8 @@
 //                     has to wait for and to look up between two tiles passes under the other's products (one issuer for both spent 60 % of its
 //                     time between products).  PAIRED has one for both slots, whose products must not mix: two issuers without turns
 //                     took 27 % longer, with turns 8 %.
-//   warps 13, 14      one per stream of items: looks them up, hands them to the other roles through a ring and loads their queries (PAIRED the second warp loads those of the second slot)
+//   warps 13, 14      one per stream of items: looks them up, hands them to the other roles through a ring and loads their queries
+//                     (PAIRED the second warp loads those of the second slot)
 // All roles run on into the next item as far as their rings and buffers let them, so that what an item costs to begin (its place in the tables,
 // its queries, its first keys) passes under the one before it.
 // Q, K and V lie in shared memory in rows of 128 bytes with the 128-byte swizzle, 64 columns a panel; V is read as an MN-major operand.
@@ -30,9 +31,9 @@
 // The reference maximum of a row moves only when a tile's maximum exceeds it by more than 8 in units of log2 (probabilities stay below
 // 2^8); then the row's sum and its O are scaled before P is handed over.
 // What bounds it.  PAIRED: the round trip of a slot -- 2,000 cycles of softmax (1,024 of them exponentials: 128 x 128 at 16 a cycle for each of
-// two slots), then P V and the next S, 1,024 cycles of the tensor cores, with hand-over and the other slot's products in between: 3,870 cycles
-// a tile of 256 rows by 128 keys, 1.1 PFLOP/s over chunks of 2,048 tokens behind 16,384 (32 query heads on 8 key heads of 128).  Otherwise:
-// bytes from L2 and HBM where there are many keys (32 rows over 90,000 keys, 104 us, 3.8 TB/s), the softmax of a tile (some 1,950 cycles) where
+// two slots), then P V and the next S, 1,024 cycles of the tensor cores, with hand-over and the other slot's products in between: 3,900 cycles
+// a tile of 256 rows by 128 keys, 1.16 PFLOP/s over chunks of 2,048 tokens behind 16,384 (32 query heads on 8 key heads of 128).  Otherwise:
+// bytes from L2 and HBM where there are many keys (32 rows over 90,000 keys, 102 us, 3.9 TB/s), the softmax of a tile (some 1,950 cycles) where
 // keys are shared by many rows, and what a CTA costs to begin and end where an SM has a few tiles only (one tile each: 10 us at head_dim 64).
 // Every wait on a barrier is bounded.
 
