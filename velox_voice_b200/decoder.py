@@ -70,11 +70,12 @@ def make_weights(cfg: DecoderConfig, seed: int = 0) -> Dict[str, torch.Tensor]:
 
 @dataclass
 class Utterances:
-    """Frames that have been read: their pages (int32 [utterances, pages]) and numbers (int32 [utterances])."""
+    """Frames that have been read: their pages (int32 [utterances, pages]) and numbers (int32 [utterances]; `counts` on the host)."""
 
     table: torch.Tensor
     lengths: torch.Tensor
     pages: List[int]
+    counts: List[int]
 
 
 @dataclass
@@ -150,16 +151,20 @@ class HypothesisDecoder:
         """Encoder frames bf16 [sum(counts), d_model], one utterance after another, into the cache."""
         if frames.dim() != 2 or frames.shape != (sum(counts), self.cfg.d_model) or min(counts) < 1:
             raise ValueError(f"frames must be [{sum(counts)}, {self.cfg.d_model}] with at least one frame per utterance, got {tuple(frames.shape)}")
+        if max(counts) > self.cfg.positions:  # (rows at positions that the table does not have are not stored)
+            raise ValueError(f"{max(counts)} frames, but the decoder has {self.cfg.positions} positions")
         dev = self.k_pages.device
         table, ids = self._take(counts)
         n = torch.tensor(counts, dtype=torch.int32).to(dev)
         offsets = torch.zeros(len(counts) + 1, dtype=torch.int32, device=dev)
         offsets[1:] = n.cumsum(0)
         self._blocks(frames, table, torch.zeros_like(n), row_offsets=offsets)
-        return Utterances(table, n, ids)
+        return Utterances(table, n, ids, list(counts))
 
     def begin(self, utterances: Utterances, beams: int, max_tokens: int) -> Hypotheses:
-        """Room for `beams` hypotheses of every utterance."""
+        """Room for `beams` hypotheses of every utterance, `max_tokens` each."""
+        if max(utterances.counts) + max_tokens > self.cfg.positions:
+            raise ValueError(f"{max(utterances.counts)} frames and {max_tokens} tokens, but the decoder has {self.cfg.positions} positions")
         total = beams * utterances.lengths.shape[0]
         table, ids = self._take([max_tokens] * total)
         starts = utterances.lengths.repeat_interleave(beams)
