@@ -6,15 +6,26 @@ import torch
 from velox_voice_b200 import decoder as D
 
 
+class Head:
+    """Stands for the output layer."""
+
+    def __call__(self, x):
+        return x
+
+    argmax = __call__
+
+
 @pytest.fixture
-def dec():
+def dec(monkeypatch):
     """A decoder of 64 positions and 40 pages of four tokens, whose blocks only say how many rows they were given."""
+    monkeypatch.setattr(D.ops, "ln_quantize", lambda x, *a: x)
     d = object.__new__(D.HypothesisDecoder)
     d.cfg = D.DecoderConfig(blocks=1, d_model=64, heads=1, kv_heads=1, page_size=4, positions=64)
     d.k_pages = torch.zeros(1, 40, 4, 1, 64)
     d._free = list(range(40))
     d.rows = []
     d.embed = torch.zeros(10, 64)
+    d.after, d.head = (None, None), Head()
     d._blocks = lambda x, *a, **k: (d.rows.append(x.shape[0]), x)[1]
     return d
 
@@ -39,3 +50,35 @@ def test_begin_refuses_tokens_beyond_the_positions(dec):
     with pytest.raises(ValueError, match="positions"):
         dec.begin(utt, 1, 5)
     assert len(dec._free) == 40 - 3 - 15 - 2
+
+
+def test_step_refuses_tokens_beyond_the_room(dec):
+    """A token without a page is not stored; the hypothesis would go on without it."""
+    hyp = dec.begin(dec.read(frames(10), [4, 6]), 2, 3)
+    ids = torch.zeros(4, dtype=torch.long)
+    for _ in range(3):
+        dec.step(hyp, ids)
+    with pytest.raises(RuntimeError, match="room"):
+        dec.step(hyp, ids)
+    assert hyp.lengths.tolist() == [3] * 4 and dec.rows == [10, 4, 4, 4]
+
+
+def test_score_refuses_tokens_beyond_the_room(dec):
+    hyp = dec.begin(dec.read(frames(6), [6]), 3, 5)
+    dec.step(hyp, torch.zeros(3, dtype=torch.long))
+    dec.score(hyp, torch.zeros(6, dtype=torch.long), [4, 2, 0])
+    assert hyp.lengths.tolist() == [5, 3, 1]
+    with pytest.raises(RuntimeError, match="room"):
+        dec.score(hyp, torch.zeros(4, dtype=torch.long), [0, 3, 1])
+    dec.score(hyp, torch.zeros(3, dtype=torch.long), [0, 2, 1])
+    with pytest.raises(RuntimeError, match="room"):
+        dec.step(hyp, torch.zeros(3, dtype=torch.long))
+    assert hyp.lengths.tolist() == [5, 5, 2]
+
+
+def test_score_refuses_counts_that_do_not_fit_the_ids(dec):
+    hyp = dec.begin(dec.read(frames(6), [6]), 3, 5)
+    for ids, counts in ((6, [4, 2]), (6, [2, 2, 1]), (5, [2, 2, 2]), (4, [5, -1, 0])):
+        with pytest.raises(ValueError, match="counts"):
+            dec.score(hyp, torch.zeros(ids, dtype=torch.long), counts)
+    assert hyp.lengths.tolist() == [0, 0, 0] and dec.rows == [6]

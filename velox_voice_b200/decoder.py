@@ -80,7 +80,8 @@ class Utterances:
 
 @dataclass
 class Hypotheses:
-    """`beams` hypotheses of every utterance, in the utterances' order."""
+    """`beams` hypotheses of every utterance, in the utterances' order.  `tokens`: how many each has been given, finished or not, counted on the
+    host against `max_tokens` (a program that moves `lengths` back moves `tokens` too)."""
 
     utterances: Utterances
     beams: int
@@ -88,6 +89,8 @@ class Hypotheses:
     lengths: torch.Tensor  # int32: tokens in the cache; negative: finished
     starts: torch.Tensor   # int32: position of the first token
     pages: List[int]
+    max_tokens: int
+    tokens: List[int]
 
 
 class HypothesisDecoder:
@@ -168,7 +171,15 @@ class HypothesisDecoder:
         total = beams * utterances.lengths.shape[0]
         table, ids = self._take([max_tokens] * total)
         starts = utterances.lengths.repeat_interleave(beams)
-        return Hypotheses(utterances, beams, table, torch.zeros_like(starts), starts, ids)
+        return Hypotheses(utterances, beams, table, torch.zeros_like(starts), starts, ids, max_tokens, [0] * total)
+
+    @staticmethod
+    def _grown(hyp: Hypotheses, counts: Sequence[int]) -> List[int]:
+        """Tokens of every hypothesis with so many more: a token without a place in a page would not be stored."""
+        tokens = [t + c for t, c in zip(hyp.tokens, counts)]
+        if max(tokens) > hyp.max_tokens:
+            raise RuntimeError(f"no room: hypotheses of {hyp.max_tokens} tokens at most, {max(tokens)} wanted")
+        return tokens
 
     def _hidden(self, hyp: Hypotheses, ids: torch.Tensor, row_offsets=None) -> torch.Tensor:
         u = hyp.utterances
@@ -177,17 +188,28 @@ class HypothesisDecoder:
 
     def step(self, hyp: Hypotheses, ids: torch.Tensor) -> torch.Tensor:
         """One token per hypothesis (ids [utterances * beams]) -> the likeliest next ones, int32."""
+        tokens = self._grown(hyp, [1] * len(hyp.tokens))
+        out = self._step(hyp, ids)
+        hyp.tokens = tokens
+        return out
+
+    def _step(self, hyp: Hypotheses, ids: torch.Tensor) -> torch.Tensor:
         x = self._hidden(hyp, ids)
         hyp.lengths.add_((hyp.lengths >= 0).to(torch.int32))
         return self.head.argmax(ops.ln_quantize(x, *self.after, self.cfg.eps, self.cfg.fmt))
 
     def score(self, hyp: Hypotheses, ids: torch.Tensor, counts: Sequence[int]) -> torch.Tensor:
         """Whole continuations at once: ids [sum(counts)], hypothesis after hypothesis -> bf16 logits [sum(counts), vocab]."""
-        n = torch.tensor(list(counts), dtype=torch.int32).to(hyp.table.device)
+        counts = list(counts)
+        if len(counts) != len(hyp.tokens) or min(counts) < 0 or sum(counts) != ids.numel():
+            raise ValueError(f"counts must be those of {len(hyp.tokens)} hypotheses and sum to {ids.numel()} ids, got {counts}")
+        tokens = self._grown(hyp, counts)
+        n = torch.tensor(counts, dtype=torch.int32).to(hyp.table.device)
         offsets = torch.zeros(n.numel() + 1, dtype=torch.int32, device=n.device)
         offsets[1:] = n.cumsum(0)
         x = self._hidden(hyp, ids, offsets)
         hyp.lengths.add_(torch.where(hyp.lengths >= 0, n, 0))
+        hyp.tokens = tokens
         return self.head(ops.ln_quantize(x, *self.after, self.cfg.eps, self.cfg.fmt))
 
     def compile_step(self, hyp: Hypotheses):
@@ -197,16 +219,18 @@ class HypothesisDecoder:
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            self.step(hyp, ids)
+            self._step(hyp, ids)
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            out = self.step(hyp, ids)
+            out = self._step(hyp, ids)
         hyp.lengths.copy_(kept)
 
         def run(new_ids: torch.Tensor) -> torch.Tensor:
+            tokens = self._grown(hyp, [1] * len(hyp.tokens))
             ids.copy_(new_ids)
             graph.replay()
+            hyp.tokens = tokens
             return out
 
         return run
