@@ -82,3 +82,22 @@ def test_score_refuses_counts_that_do_not_fit_the_ids(dec):
         with pytest.raises(ValueError, match="counts"):
             dec.score(hyp, torch.zeros(ids, dtype=torch.long), counts)
     assert hyp.lengths.tolist() == [0, 0, 0] and dec.rows == [6]
+
+
+def test_pages_that_were_handed_back_are_not_used(dec):
+    """They may be another owner's by then."""
+    utt = dec.read(frames(6), [6])
+    hyp, other = dec.begin(utt, 2, 5), dec.begin(utt, 1, 5)
+    ids = torch.zeros(2, dtype=torch.long)
+    dec.step(hyp, ids)
+    dec.release(hyp)
+    for call in (lambda: dec.step(hyp, ids), lambda: dec.score(hyp, ids, [1, 1]), lambda: dec.compile_step(hyp)):
+        with pytest.raises(RuntimeError, match="handed back"):
+            call()
+    dec.release(utt)
+    for call in (lambda: dec.step(other, ids[:1]), lambda: dec.score(other, ids[:1], [1]), lambda: dec.begin(utt, 1, 1)):
+        with pytest.raises(RuntimeError, match="handed back"):
+            call()
+    dec.release(other)
+    dec.release(other)
+    assert sorted(dec._free) == list(range(40)) and dec.rows == [6, 2]

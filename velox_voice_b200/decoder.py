@@ -76,6 +76,7 @@ class Utterances:
     lengths: torch.Tensor
     pages: List[int]
     counts: List[int]
+    released: bool = False
 
 
 @dataclass
@@ -91,6 +92,7 @@ class Hypotheses:
     pages: List[int]
     max_tokens: int
     tokens: List[int]
+    released: bool = False
 
 
 class HypothesisDecoder:
@@ -132,7 +134,7 @@ class HypothesisDecoder:
     def release(self, owner) -> None:
         """Hands the pages of utterances or hypotheses back."""
         self._free += owner.pages
-        owner.pages = []
+        owner.pages, owner.released = [], True
 
     # ---- the blocks
     def _blocks(self, x: torch.Tensor, table, lengths, *, starts=None, row_offsets=None, prefix_table=None, prefix_lengths=None) -> torch.Tensor:
@@ -166,6 +168,7 @@ class HypothesisDecoder:
 
     def begin(self, utterances: Utterances, beams: int, max_tokens: int) -> Hypotheses:
         """Room for `beams` hypotheses of every utterance, `max_tokens` each."""
+        self._held(utterances)
         if max(utterances.counts) + max_tokens > self.cfg.positions:
             raise ValueError(f"{max(utterances.counts)} frames and {max_tokens} tokens, but the decoder has {self.cfg.positions} positions")
         total = beams * utterances.lengths.shape[0]
@@ -174,8 +177,13 @@ class HypothesisDecoder:
         return Hypotheses(utterances, beams, table, torch.zeros_like(starts), starts, ids, max_tokens, [0] * total)
 
     @staticmethod
-    def _grown(hyp: Hypotheses, counts: Sequence[int]) -> List[int]:
+    def _held(*owners) -> None:
+        if any(o.released for o in owners):
+            raise RuntimeError("the pages have been handed back: they may be another owner's")
+
+    def _grown(self, hyp: Hypotheses, counts: Sequence[int]) -> List[int]:
         """Tokens of every hypothesis with so many more: a token without a place in a page would not be stored."""
+        self._held(hyp, hyp.utterances)
         tokens = [t + c for t, c in zip(hyp.tokens, counts)]
         if max(tokens) > hyp.max_tokens:
             raise RuntimeError(f"no room: hypotheses of {hyp.max_tokens} tokens at most, {max(tokens)} wanted")
@@ -214,6 +222,7 @@ class HypothesisDecoder:
 
     def compile_step(self, hyp: Hypotheses):
         """``step`` as a CUDA graph: a function of ids (copied in) that returns the graph's own output."""
+        self._held(hyp, hyp.utterances)
         ids = torch.zeros(hyp.lengths.shape[0], dtype=torch.int64, device=hyp.table.device)
         kept = hyp.lengths.clone()
         side = torch.cuda.Stream()
