@@ -101,3 +101,11 @@ def test_pages_that_were_handed_back_are_not_used(dec):
     dec.release(other)
     dec.release(other)
     assert sorted(dec._free) == list(range(40)) and dec.rows == [6, 2]
+
+
+def test_begin_refuses_no_beams_and_negative_room(dec):
+    utt = dec.read(frames(6), [6])
+    for beams, tokens in ((0, 5), (-1, 5), (2, -1)):
+        with pytest.raises(ValueError, match="beams"):
+            dec.begin(utt, beams, tokens)
+    assert len(dec._free) == 38

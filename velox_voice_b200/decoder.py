@@ -168,6 +168,8 @@ class HypothesisDecoder:
 
     def begin(self, utterances: Utterances, beams: int, max_tokens: int) -> Hypotheses:
         """Room for `beams` hypotheses of every utterance, `max_tokens` each."""
+        if beams < 1 or max_tokens < 0:
+            raise ValueError(f"beams must be 1 or more and max_tokens 0 or more, got {beams} and {max_tokens}")
         self._held(utterances)
         if max(utterances.counts) + max_tokens > self.cfg.positions:
             raise ValueError(f"{max(utterances.counts)} frames and {max_tokens} tokens, but the decoder has {self.cfg.positions} positions")
