@@ -109,3 +109,13 @@ def test_begin_refuses_no_beams_and_negative_room(dec):
         with pytest.raises(ValueError, match="beams"):
             dec.begin(utt, beams, tokens)
     assert len(dec._free) == 38
+
+
+def test_a_read_that_fails_keeps_no_pages(dec):
+    def fails(*a, **k):
+        raise TypeError("frames of another type")
+
+    dec._blocks = fails
+    with pytest.raises(TypeError):
+        dec.read(frames(30), [10, 20])
+    assert sorted(dec._free) == list(range(40))

@@ -160,10 +160,14 @@ class HypothesisDecoder:
             raise ValueError(f"{max(counts)} frames, but the decoder has {self.cfg.positions} positions")
         dev = self.k_pages.device
         table, ids = self._take(counts)
-        n = torch.tensor(counts, dtype=torch.int32).to(dev)
-        offsets = torch.zeros(len(counts) + 1, dtype=torch.int32, device=dev)
-        offsets[1:] = n.cumsum(0)
-        self._blocks(frames, table, torch.zeros_like(n), row_offsets=offsets)
+        try:
+            n = torch.tensor(counts, dtype=torch.int32).to(dev)
+            offsets = torch.zeros(len(counts) + 1, dtype=torch.int32, device=dev)
+            offsets[1:] = n.cumsum(0)
+            self._blocks(frames, table, torch.zeros_like(n), row_offsets=offsets)
+        except BaseException:
+            self._free += ids
+            raise
         return Utterances(table, n, ids, list(counts))
 
     def begin(self, utterances: Utterances, beams: int, max_tokens: int) -> Hypotheses:
