@@ -404,7 +404,7 @@ typedef struct {
   int64_t k_row, k_head, v_row, v_head, q_row, q_head;
   void* q_out;         /* bf16 [rows, q_heads, head_dim], must be given with q; may be q where q is bf16 */
   int64_t qo_row, qo_head;
-  const float* rotary; /* NULL: no rotation */
+  const float* rotary; /* NULL: no rotation.  (With 0 positions any other aligned address: it is not read, all rows are left out) */
   int64_t positions, ld_rotary;
   const int32_t* starts; /* i32 [sequences]: position of a sequence's first own token; NULL: 0 */
   int32_t q_heads, rot_dim; /* rot_dim: a multiple of 16, at most head_dim */

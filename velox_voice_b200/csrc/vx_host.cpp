@@ -1258,7 +1258,7 @@ PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
     if (!is_cuda_tensor(p[7])) Py_RETURN_NONE;
     const at::Tensor& r = THPVariable_Unpack(p[7]);
     if (r.scalar_type() != at::kFloat || r.dim() != 2 || r.device() != dev || r.size(1) % 16 != 0 || r.size(1) < 16 || r.size(1) > cache.head_dim || !in_pieces(r)) Py_RETURN_NONE;
-    d.rotary = static_cast<const float*>(r.data_ptr());
+    d.rotary = r.size(0) > 0 ? static_cast<const float*>(r.data_ptr()) : reinterpret_cast<const float*>(16);  // (NULL is no table at all)
     d.positions = r.size(0); d.rot_dim = static_cast<int>(r.size(1)); d.ld_rotary = r.size(0) > 1 ? r.stride(0) : r.size(1);
     d.interleaved = as_bool(p[8]);
   }

@@ -856,7 +856,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
             raise ValueError(f"rot_dim must be a multiple of 16 up to head_dim {k.shape[2]}, got {rotary.shape[1]}")
         if not _in_pieces(rotary):
             rotary = rotary.clone(memory_format=torch.contiguous_format)
-        d.rotary, d.positions, d.rot_dim = rotary.data_ptr(), rotary.shape[0], rotary.shape[1]
+        d.rotary, d.positions, d.rot_dim = rotary.data_ptr() or 16, rotary.shape[0], rotary.shape[1]  # (NULL is no table at all)
         d.ld_rotary = rotary.stride(0) if rotary.shape[0] > 1 else rotary.shape[1]
         d.interleaved = int(interleaved)
     r, keep = _kv_rows(rows, page_table, lengths, row_offsets, dev)
