@@ -373,7 +373,8 @@ typedef struct {
  *   lengths      i32 [sequences]: own tokens of a sequence that the cache holds BEFORE the rows of this call (the same numbers for
  *                vx_kv_append and the vx_prefix_attention behind it); negative: the sequence takes no part
  *   row_offsets  i32 [sequences + 1], ascending: rows [o_s, o_{s+1}) are the next tokens of sequence s; NULL: one row each.  Rows
- *                outside [o_0, o_sequences) belong to no sequence
+ *                outside [o_0, o_sequences) belong to no sequence.  Offsets may lie in front of row 0 or behind the last row: those
+ *                tokens are not the call's, and the ones in front count
  *   page_table   i32 [sequences][table_pages], row stride ld_table: entry j is the page of the sequence's own tokens
  *                [j page_size, (j + 1) page_size).  An entry outside [0, pages) is a page that is not there.
  * All of it is device memory that is checked where it is read: no value of an entry makes a kernel leave the cache. */

@@ -3,10 +3,12 @@ large numbers, tables whose rows are one row.
 
 Tolerances are those of test_paged_gpu.py; where nothing is rounded the results are compared bit by bit."""
 
+import numpy as np
 import pytest
 import torch
 
-from test_paged_gpu import ints, make_cache, ops  # noqa: F401
+from oracle import paged as P
+from test_paged_gpu import check_append, check_attention, f64, ints, make_cache, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +26,55 @@ def test_append_with_an_empty_rotary_table_leaves_everything_out(ops, interleave
     out2 = ops.kv_append(k, k, k_pages, v_pages, ints([[0], [1], [2]]), ints([0, 3, 15]), q=q, rotary=ops.rotary_table(9, 32)[:0])
     torch.cuda.synchronize()
     assert not out.any() and not out2.any() and torch.equal(k_pages, old[0]) and torch.equal(v_pages, old[1])
+
+
+# ------------------------------------------------------------------------------------------------ offsets
+
+
+def test_append_rows_between_sound_offsets_arrive(ops):  # noqa: F811
+    """Sequence 1 has rows 0 to 3 as its tokens 5 to 8 (its offset is 5 rows in front of the call), sequence 2 the rest; the offsets around them
+    make no sense."""
+    k_pages, v_pages = make_cache(8, 16, 2, 64)
+    want = k_pages.clone(), v_pages.clone()
+    k, v, q = (torch.randn(12, 2, 64, device="cuda").bfloat16() for _ in range(3))
+    for cache, x in zip(want, (k, v)):
+        cache[1, 5:9], cache[2, 0:8] = x[:4], x[4:]
+    q_out = torch.full_like(q, float("nan"))
+    ops.kv_append(k, v, k_pages, v_pages, ints([[0], [1], [2]]), ints([0, 0, 0]), q=q, row_offsets=ints([2 ** 31 - 1, -5, 4, 2 ** 31 - 1]), q_out=q_out)
+    torch.cuda.synchronize()
+    assert torch.equal(q_out, q) and torch.equal(k_pages, want[0]) and torch.equal(v_pages, want[1])
+
+
+@pytest.mark.parametrize("rows_of,first", [([4, 3, 6], -3), ([4, 3, 6], -6), ([40, 0, 9], -17)])
+def test_append_offsets_in_front_of_the_rows(ops, rows_of, first):  # noqa: F811
+    check_append(ops, rows_of=rows_of, lengths=[2, 15, 0], first_row=first, last_rows=2, starts=[3, 0, 9])
+
+
+@pytest.mark.parametrize("heads,kv,d,rows_of,lengths,first", [
+    (8, 8, 64, [4, 3, 6], [5, 9, 0], -3), (8, 2, 128, [4, 3, 6], [5, 70, 0], -6),          # few rows
+    (16, 1, 64, [7, 5, 6], [30, 0, 90], -4), (16, 1, 128, [7, 5, 6], [30, 200, 9], -9),    # more
+    (2, 2, 64, [200, 150], [0, 40], -30), (8, 2, 128, [90, 60, 70], [300, 0, 11], -110)])  # prompts
+@pytest.mark.parametrize("prefix", [(), (150,)])
+def test_attention_offsets_in_front_of_the_rows(ops, heads, kv, d, rows_of, lengths, first, prefix):  # noqa: F811
+    """The first rows of a run that the call does not have count as tokens in front of those that it has."""
+    torch.empty(2 ** 26, dtype=torch.float32, device="cuda").fill_(float("nan"))  # (what scratch may be given)
+    check_attention(ops, lengths=lengths, rows_of=rows_of, prefix=prefix, heads=heads, kv=kv, d=d, first_row=first, last_rows=2)
+
+
+def test_offsets_as_far_in_front_as_there_are_numbers(ops):  # noqa: F811
+    """Tokens behind 2^31 others: beyond the table, at positions that `starts` brings back."""
+    k_pages, v_pages = make_cache(4, 16, 2, 64)
+    old = k_pages.clone()
+    q, k = torch.randn(2, 4, 64, device="cuda").bfloat16(), torch.randn(2, 2, 64, device="cuda").bfloat16()
+    off, t, n = [-2 ** 31, 2], ints([[2, 1]]), ints([0])
+    rot = ops.rotary_table(9, 64)
+    plain = ops.kv_append(k, k, k_pages, v_pages, t, n, q=q, row_offsets=ints(off))
+    turned = ops.kv_append(k, k, k_pages, v_pages, t, n, q=q, row_offsets=ints(off), rotary=rot, starts=ints([-2 ** 31 + 5]))
+    got = ops.prefix_attention(q, k_pages, v_pages, t, n, row_offsets=ints(off))
+    torch.cuda.synchronize()
+    assert torch.equal(k_pages, old) and torch.equal(plain, q)
+    # rows 0 and 1 are tokens 2^31 and 2^31 + 1 at positions 5 and 6
+    want = np.stack([P.rotate(x, f64(rot)[5 + i], False) for i, x in enumerate(f64(q))])
+    assert (np.abs(f64(turned) - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -22 * 12).all()
+    want, width = P.prefix_attention_ref(f64(q), f64(k_pages), f64(v_pages), np.array([[2, 1]]), np.array([0]), row_offsets=np.array(off))
+    assert (np.abs(f64(got) - want) <= 2.0 ** -8 * (np.abs(want) + width) + 2.0 ** -13 * width).all()

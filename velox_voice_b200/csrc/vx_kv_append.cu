@@ -119,9 +119,10 @@ __global__ void __launch_bounds__(AP_THREADS, AP_BLOCKS) kv_append_kernel(const 
   pdl_wait();
   if (static_cast<int>(threadIdx.x) < n_rows) {
     RowPlace pl{-1, -1, -1};
-    int s, i;
+    int s;
+    int64_t i;
     if (row_sequence(p.rows, row0 + threadIdx.x, s, i)) {
-      const int64_t t = static_cast<int64_t>(p.rows.lengths[s]) + i;
+      const int64_t t = p.rows.lengths[s] + i;
       const int64_t pos = t + (p.starts ? p.starts[s] : 0);
       if (!p.rotary) pl.position = 0;
       else if (pos >= 0 && pos < p.positions) pl.position = static_cast<int32_t>(pos);

@@ -81,17 +81,18 @@ __device__ __forceinline__ int find_by_warp(int n, int x, First first) {
   return lo;
 }
 
-// Sequence of a row and the row's index among the call's rows of that sequence; false: no sequence, or one that takes no part.
+// Sequence of a row and the row's index among the new tokens of that sequence, from its offset, which may lie in front of the call's rows; false:
+// no sequence, or one that takes no part.
 // WARP: all lanes of the warp ask for the same row.
 template <bool WARP = false>
-__device__ __forceinline__ bool row_sequence(const KvRows& kr, int row, int& s, int& i) {
+__device__ __forceinline__ bool row_sequence(const KvRows& kr, int row, int& s, int64_t& i) {
   s = row;
   i = 0;
   if (kr.sequences == 0) return false;
   if (kr.row_offsets) {
     if (WARP) s = find_by_warp(kr.sequences, row, [&](int o) { return kr.row_offsets[o]; });
     else s = find_owner(kr.row_offsets, kr.sequences, row);
-    i = row - kr.row_offsets[s];
+    i = static_cast<int64_t>(row) - kr.row_offsets[s];
     if (i < 0 || row >= kr.row_offsets[s + 1]) return false;
   }
   return kr.lengths[s] >= 0;

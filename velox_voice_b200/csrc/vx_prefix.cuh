@@ -71,14 +71,22 @@ __device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
   return s >= p.group_offsets[g] && s < p.group_offsets[g + 1] ? g : -1;
 }
 
-// Keys of the prefix of group g, and own keys that a token of index i of its sequence sees: as far as the tables reach.
+// Keys of the prefix of group g, and own keys that the i-th token behind `length` others of its sequence sees: as far as the tables reach.
 __device__ __forceinline__ int prefix_keys(const PrefixParams& p, int g) {
   const int cap = p.prefix.pages * static_cast<int>(p.cache.page_size.d);
   return g < 0 ? 0 : min(max(p.prefix_lengths[g], 0), cap);
 }
-__device__ __forceinline__ int own_keys(const PrefixParams& p, int length, int i) {
+__device__ __forceinline__ int own_keys(const PrefixParams& p, int length, int64_t i) {
   const int cap = p.rows.table.pages * static_cast<int>(p.cache.page_size.d);
-  return length < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(length) + i + 1, static_cast<int64_t>(cap)));
+  return length < 0 ? 0 : static_cast<int>(min(length + i + 1, static_cast<int64_t>(cap)));
+}
+// Tokens of sequence s in front of its first row that the call has, as far as the table reaches: those of the cache and, where its offset lies
+// in front of the call's rows, those between; negative: it takes no part.
+__device__ __forceinline__ int tokens_before(const PrefixParams& p, int s) {
+  const int length = p.rows.lengths[s];
+  if (length < 0 || !p.rows.row_offsets) return length;
+  const int64_t cap = static_cast<int64_t>(p.rows.table.pages) * static_cast<int>(p.cache.page_size.d);
+  return static_cast<int>(min(length + max(-static_cast<int64_t>(p.rows.row_offsets[s]), static_cast<int64_t>(0)), cap));
 }
 __device__ __forceinline__ int align_keys(int n) { return (n + kSpanAlign - 1) / kSpanAlign * kSpanAlign; }
 

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows_ctas(RB, D)) prefix_rows_k
   const bool own = sp.kind == kSpanOwn;
   ItemRows it;
   if (!find_rows<TM>(p, sp, n - chunk * sp.slots, it)) return;
-  const int length = own ? p.rows.lengths[it.owner] : 0;
+  const int length = own ? tokens_before(p, it.owner) : 0;
   // keys [key0, keys): those of the chunk that the tile's last row sees
   int keys = own ? own_keys(p, length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(min(it.rho0 + TM, it.rows) - 1)))) : prefix_keys(p, it.owner);
   if (static_cast<int64_t>(chunk) * sp.chunk >= keys) return;
@@ -453,7 +453,8 @@ __global__ void __launch_bounds__(JN_WARPS * 32, PARTS > 4 ? 4 : (D == 64 ? 8 : 
   const int row = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y) * (JN_WARPS / WARPS) + team;
   if (jp.first) pdl_wait();
   const bool in = h < p.q_heads;
-  int parts[2] = {0, 0}, s, i;
+  int parts[2] = {0, 0}, s;
+  int64_t i;
   if (row_sequence<true>(p.rows, row, s, i)) {
     const int prefix = prefix_keys(p, group_of(p, s)), own = own_keys(p, p.rows.lengths[s], i);
 #pragma unroll
@@ -531,7 +532,8 @@ __global__ void __launch_bounds__(JN_WARPS * 32) prefix_rest_kernel(const __grid
   pdl_launch_dependents();
   const PrefixParams& p = jp.p;
   const int row = static_cast<int>(blockIdx.x) * JN_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  int s, i;
+  int s;
+  int64_t i;
   const bool rest = row < p.rows.rows && !row_sequence<true>(p.rows, row, s, i);
   pdl_wait();
   if (!rest) return;

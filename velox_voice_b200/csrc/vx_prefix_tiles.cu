@@ -161,7 +161,7 @@ __device__ bool find_tile_item(const PrefixParams& p, const Span& sp, const Span
     t.p_keys = prefix_keys(p, r.owner);
   } else {
     t.sequence = r.owner;
-    t.length = p.rows.lengths[r.owner];
+    t.length = tokens_before(p, r.owner);
     if (t.length < 0) return false;
     if (sp.kind == kSpanJoint) {
       t.group = group_of(p, r.owner);
