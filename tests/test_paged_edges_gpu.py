@@ -78,3 +78,44 @@ def test_offsets_as_far_in_front_as_there_are_numbers(ops):  # noqa: F811
     assert (np.abs(f64(turned) - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -22 * 12).all()
     want, width = P.prefix_attention_ref(f64(q), f64(k_pages), f64(v_pages), np.array([[2, 1]]), np.array([0]), row_offsets=np.array(off))
     assert (np.abs(f64(got) - want) <= 2.0 ** -8 * (np.abs(want) + width) + 2.0 ** -13 * width).all()
+
+
+# ------------------------------------------------------------------------------------------------ scores
+
+
+@pytest.mark.parametrize("heads,kv,d,n,tokens,length,prefix", [
+    (4, 4, 64, 2, 3, 37, 90), (8, 8, 128, 2, 1, 61, 120),      # few rows
+    (16, 1, 64, 2, 5, 70, 130), (16, 1, 128, 2, 5, 70, 130),   # more, two streams of items
+    (16, 1, 64, 5, 7, 10, 200),                                # pairs over the prefix
+    (2, 2, 64, 2, 140, 20, 100), (8, 2, 128, 2, 40, 60, 300)])  # pairs, prefix and own tokens in a row
+@pytest.mark.parametrize("sign,low", [(1.0, 32), (-1.0, 32), (1.0, 26), (-1.0, 26), (1.0, 14)])
+def test_attention_scores_that_are_large_numbers(ops, heads, kv, d, n, tokens, length, prefix, sign, low):  # noqa: F811
+    """Scores of 2^low to 2^(low + 6), exact in fp32 and so far apart that the largest takes all of the weight: the result is its value, bit by
+    bit where the scores are as large as that."""
+    ps, own = 16, length + tokens
+    width, pw = -(-own // ps), -(-prefix // ps)
+    table, ptable = np.arange(n * width).reshape(n, width), n * width + np.arange(pw)[None]
+    k_pages, v_pages = make_cache(n * width + pw, ps, kv, d)
+    keys = prefix + n * own
+    rank = np.stack([np.random.default_rng(c).permutation(keys) for c in range(d)])            # [d, keys]
+    value = (128 + rank % 128) * 2.0 ** (rank // 128 + low - 24)                                    # ascending with the rank, eight bits
+    ids = np.concatenate([ptable[0][np.arange(prefix) // ps] * ps + np.arange(prefix) % ps] +
+                         [table[s][np.arange(own) // ps] * ps + np.arange(own) % ps for s in range(n)])
+    flat = k_pages.view(-1, kv, d)
+    flat[torch.from_numpy(ids).cuda()] = torch.from_numpy(np.ascontiguousarray(value.T))[:, None].expand(keys, kv, d).to("cuda", torch.bfloat16)
+    rows = n * tokens
+    column = np.arange(rows * heads).reshape(rows, heads) % d
+    q = torch.zeros(rows, heads, d)
+    q.scatter_(2, torch.from_numpy(column)[..., None], sign * 2.0 ** 20)
+    off = np.arange(n + 1) * tokens
+    got = ops.prefix_attention(q.cuda().bfloat16(), k_pages, v_pages, ints(table), ints([length] * n), ints(ptable), ints([prefix]), row_offsets=ints(off), scale=0.125)
+    values = f64(v_pages).reshape(-1, kv, d)[ids]
+    want = np.empty((rows, heads, d))
+    for r in range(rows):
+        s, i = divmod(r, tokens)
+        seen = np.concatenate([np.arange(prefix), prefix + s * own + np.arange(length + i + 1)])
+        for h in range(heads):
+            best = seen[(sign * rank[column[r, h]][seen]).argmax()]
+            want[r, h] = values[best, h // (heads // kv)]
+    got = f64(got)
+    assert (np.abs(got - want) <= (0.0 if low == 32 else 2.0 ** -7 + 2.0 ** -13) * np.abs(want)).all(), f"{(got != want).any(-1).sum()} of {rows * heads} rows differ, {np.isnan(got).any(-1).sum()} NaN"

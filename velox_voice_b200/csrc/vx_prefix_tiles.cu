@@ -141,6 +141,16 @@ __device__ __forceinline__ void store32(float* dst, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
+// The factor of a row's scores and its reference maximum.  2^(scale2 s - m) has the product unrounded and m rounded: it is off by 2^(half a unit of m),
+// the same for all keys of the row and in its sum, which leaves the range where m is 2^31 or more.  From 2^30 on scale2 without its mantissa
+// stands in, and products are exact: two different scores are 64 or more in log2 apart there, 32 with the smaller factor, so that the
+// largest takes all of the weight either way.
+constexpr float PT_LARGE = 1073741824.0f;
+__device__ __forceinline__ float without_mantissa(float x) { return __uint_as_float(__float_as_uint(x) & 0x7f800000u); }
+// such a reference maximum in units of log2, for the parts of a row and where it moves
+__device__ __forceinline__ float in_log2(float m, float factor, float scale2) {
+  return factor == scale2 ? m : m * __uint_as_float((__float_as_uint(scale2) & 0x007fffffu) | 0x3f800000u);
+}
 // bits [0, n) of a word
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1); }
 
@@ -700,7 +710,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const bool idle = rho - lane >= t.rows;  // a warp without rows: whatever its P holds stays in its own rows of O
       const int limit = there ? own_keys(p, t.length, static_cast<int>(tok)) : t.o_keys;
       const int warp_limit = __shfl_sync(ALL, limit, 0);  // limits ascend with the rows
-      float m_ref = NEG_INF, l = 0.0f;
+      float factor = p.scale2, m_ref = NEG_INF, l = 0.0f;
       float o_apart[D];    // O behind the tile before, where that was formed apart (in local memory)
       bool apart = false;
       const int mine = PAIRED ? (slot ? t.n[1] : t.n[0]) : t.tiles;
@@ -760,7 +770,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 #pragma unroll
         for (int i = W / 2; i < W; ++i) largest(i);
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        const float m_tile = mx * p.scale2;
+        const float m_tile = mx * factor;
         const bool moves = m_tile > m_ref + 8.0f;
         // P V of the tile before has to be complete before O is touched (with one buffer this tile's S was issued behind it)
         auto o_is_there = [&] {
@@ -769,8 +779,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           return ok;
         };
         if (__any_sync(ALL, moves || (LATE && apart))) {
-          const float alpha = moves ? ex2(m_ref - m_tile) : 1.0f;  // 0 for m_ref = -inf
-          if (moves) m_ref = m_tile;
+          float alpha = 1.0f;
+          if (moves) {
+            const float before = in_log2(m_ref, factor, p.scale2);
+            factor = p.scale2;
+            m_ref = mx * factor;
+            alpha = ex2(before - m_ref);  // 0 for -inf
+            if (fabsf(m_ref) >= PT_LARGE) {
+              factor = without_mantissa(factor);
+              m_ref = mx * factor;
+            }
+          }
           l *= alpha;
           if (u > 0) {
             if (!o_is_there()) return;
@@ -788,7 +807,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           }
         }
         const float ref = m_ref == NEG_INF ? 0.0f : m_ref;
-        const uint64_t k2 = pack_f32x2(p.scale2, p.scale2), n2 = pack_f32x2(-ref, -ref);
+        const uint64_t k2 = pack_f32x2(factor, factor), n2 = pack_f32x2(-ref, -ref);
         uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < W; ++i) {
@@ -853,7 +872,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const int64_t row = t.row0 + static_cast<int>(tok), qh = t.head * static_cast<int64_t>(p.per_kv.d) + hq;
       if (t.part >= 0) {
         const int64_t at = (static_cast<int64_t>(t.part) * p.rows.rows + row) * p.q_heads + qh;
-        if (there) p.part_ml[at] = make_float2(m_ref, l);
+        if (there) p.part_ml[at] = make_float2(in_log2(m_ref, factor, p.scale2), l);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
