@@ -422,7 +422,7 @@ int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_kv_a
  *   groups         sequences [group_offsets[g], group_offsets[g + 1]) belong to group g (i32 [groups + 1], ascending); NULL: groups of
  *                  sequences / groups each.  0 groups: no prefix
  *   out            bf16 [rows, q_heads, head_dim]
- *   scale          positive and finite
+ *   scale          positive; scale log2(e) finite
  *   scratch        vx_prefix_attention_scratch(cache, rows, desc) bytes, 32-byte aligned
  * bf16 operands, fp32 scores, softmax statistics and sums; probabilities are rounded to bf16 for the second product.  What lies in unread places
  * of the cache (NaN included) does not reach a result.  head_dim 64 or 128. */

@@ -628,7 +628,8 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     if (!d->prefix_lengths || (d->prefix_pages > 0 && (!d->prefix_table || d->ld_prefix < d->prefix_pages)))
       return fail(-1, "prefix_lengths or prefix_table is NULL, or its rows are too short");
   }
-  if (!(d->scale > 0.0f) || d->scale > 3.0e38f) return fail(-1, "scale must be positive and finite");
+  p.scale2 = d->scale * 1.4426950408889634f;
+  if (!(d->scale > 0.0f) || !(p.scale2 < INFINITY)) return fail(-1, "scale must be positive and finite, scale log2(e) too");
   const int per = d->q_heads / cache->kv_heads;
   p.q_heads = d->q_heads;
   p.kv_heads = cache->kv_heads;
@@ -638,7 +639,6 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
   p.group_size = p.groups > 0 && !p.group_offsets ? static_cast<int32_t>(rows->sequences / d->groups) : 0;
   p.prefix = {d->prefix_table, d->ld_prefix, static_cast<int32_t>(d->prefix_pages)};
   p.prefix_lengths = d->prefix_lengths;
-  p.scale2 = d->scale * 1.4426950408889634f;
 
   plan = Plan{};
   const int64_t R = rows->rows, S = rows->sequences, G = d->groups;
