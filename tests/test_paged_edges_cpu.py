@@ -1,9 +1,12 @@
 """Edges of the paged cache's arguments that the C entry points decide without a device (descriptors whose pointers are never dereferenced)."""
 
 import ctypes as C
+import re
+import subprocess
 
 import pytest
 
+from test_device_sources_cpu import source
 from test_paged_cpu import _descs, _refused
 from velox_voice_b200 import _lib
 
@@ -24,3 +27,25 @@ def attend(edit=None, **kw):
 def test_scales_whose_product_with_log2e_overflows_are_refused(scale, ok):
     """(A scale that is taken comes as far as the check of the scratch.)"""
     _refused(attend(scale=scale), b"scratch" if ok else b"scale")
+
+
+# ------------------------------------------------------------------------------------------------ rows
+
+
+def test_rows_of_a_tile_stay_inside_the_run(tmp_path):
+    """Offsets that do not ascend can ask for any tile of a run: its first row must not wrap around.  (2^24 owners and more; the function is compiled
+    for the host.)"""
+    text = source("vx_prefix.cuh")
+    body = re.search(r"int first_row\([^{]*\{[^}]*\}", text).group(0)
+    src, lib = tmp_path / "first_row.cpp", tmp_path / "first_row.so"
+    src.write_text('extern "C" ' + body)
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", str(src), "-o", str(lib)], check=True)
+    f = C.CDLL(str(lib)).first_row
+    assert [f(t, 128, 300) for t in (-1, 0, 1, 2, 3)] == [-1, 0, 128, 256, -1]
+    assert [f(t, 8, 8) for t in (0, 1)] == [0, -1] and f(0, 16, 0) == -1 and f(0, 16, -5) == -1
+    for tile in (2 ** 24, 2 ** 28, 2 ** 31 - 1, -2 ** 31):
+        for tm in (8, 16, 128, 256):
+            assert f(tile, tm, 100) == -1 and f(tile, tm, 2 ** 31 - 1) in (-1, tile * tm)
+    assert f((2 ** 31 - 2) // 256, 256, 2 ** 31 - 1) == (2 ** 31 - 2) // 256 * 256
+    # and it is what both searches take
+    assert not re.search(r"rho0 = tile \* ", text) and len(re.findall(r"rho0 = first_row\(", text)) == 2

@@ -70,15 +70,15 @@ __device__ __forceinline__ int find_owner(const int32_t* offsets, int n, int x) 
 // turn one round trip to memory (120 sequences: 2 instead of 7, 3 us of a CTA that lives for 8).
 template <class First>
 __device__ __forceinline__ int find_by_warp(int n, int x, First first) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = n;
+  const unsigned lane = threadIdx.x & 31;
+  unsigned lo = 0, hi = n;  // (unsigned: lo + 31 step can pass 2^31)
   while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const unsigned below = __ballot_sync(0xffffffffu, lane == 0 || (at < hi && first(at) <= x));
+    const unsigned step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, lane == 0 || (at < hi && first(static_cast<int>(at)) <= x));
     lo += (31 - __clz(below)) * step;
     hi = min(hi, lo + step);
   }
-  return lo;
+  return static_cast<int>(lo);
 }
 
 // Sequence of a row and the row's index among the new tokens of that sequence, from its offset, which may lie in front of the call's rows; false:

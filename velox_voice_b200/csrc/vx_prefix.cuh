@@ -90,6 +90,9 @@ __device__ __forceinline__ int tokens_before(const PrefixParams& p, int s) {
 }
 __device__ __forceinline__ int align_keys(int n) { return (n + kSpanAlign - 1) / kSpanAlign * kSpanAlign; }
 
+// First row of a tile of a run of so many rows, -1: it has none.  (Compared before it is multiplied: offsets that do not ascend ask for any tile.)
+__device__ __forceinline__ constexpr int first_row(int tile, int tm, int rows) { return tile >= 0 && rows > 0 && tile <= (rows - 1) / tm ? tile * tm : -1; }
+
 // Rows of an item.
 struct ItemRows {
   int owner;
@@ -113,12 +116,12 @@ __device__ __forceinline__ bool find_rows(const PrefixParams& p, const Span& sp,
     it.owner = find_by_warp(owners, slot, base);  // the largest with base(o) <= slot
     tile = slot - base(it.owner);
   }
-  if (it.owner >= owners || tile < 0) return false;
+  if (it.owner >= owners) return false;
   it.row0 = owner_row0(p, sequences, it.owner);
   const int n = owner_row0(p, sequences, it.owner + 1) - it.row0;
   it.rows = n * per;
-  it.rho0 = tile * TM;
-  return n > 0 && it.rho0 < it.rows;
+  it.rho0 = first_row(tile, TM, it.rows);
+  return it.rho0 >= 0;
 }
 
 // The tiles of a span counted by a warp, without the slots that have no rows: a kernel whose CTAs take items in turn shares them out evenly.
@@ -202,8 +205,8 @@ __device__ __forceinline__ bool find_tile(const PrefixParams& p, const Span& sp,
     it.row0 = owner_row0(p, sequences, it.owner);
     it.rows = (owner_row0(p, sequences, it.owner + 1) - it.row0) * static_cast<int>(p.per_kv.d);
   }
-  it.rho0 = tile * TM;
-  return tile >= 0 && it.rho0 < it.rows;
+  it.rho0 = first_row(tile, TM, it.rows);
+  return it.rho0 >= 0;
 }
 
 // Not 0 if one of the two bf16 values of a word is an infinity or NaN, gathered in `sum` (0 x is 0 or NaN).
