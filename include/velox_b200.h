@@ -403,7 +403,7 @@ typedef struct {
   const void* v;
   const void* q;       /* [rows, q_heads, head_dim] or NULL */
   int64_t k_row, k_head, v_row, v_head, q_row, q_head;
-  void* q_out;         /* bf16 [rows, q_heads, head_dim], must be given with q; may be q where q is bf16 */
+  void* q_out;         /* bf16 [rows, q_heads, head_dim], no two rows or heads in one place; must be given with q; may be q where q is bf16 */
   int64_t qo_row, qo_head;
   const float* rotary; /* NULL: no rotation.  (With 0 positions any other aligned address: it is not read, all rows are left out) */
   int64_t positions, ld_rotary;
@@ -421,7 +421,7 @@ int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_kv_a
  * rows of its group.  A row without any key, of no sequence or of one that takes no part: zeros.
  *   groups         sequences [group_offsets[g], group_offsets[g + 1]) belong to group g (i32 [groups + 1], ascending); NULL: groups of
  *                  sequences / groups each.  0 groups: no prefix
- *   out            bf16 [rows, q_heads, head_dim]
+ *   out            bf16 [rows, q_heads, head_dim], no two rows or heads in one place
  *   scale          positive; scale log2(e) finite
  *   scratch        vx_prefix_attention_scratch(cache, rows, desc) bytes, 32-byte aligned
  * bf16 operands, fp32 scores, softmax statistics and sums; probabilities are rounded to bf16 for the second product.  What lies in unread places

@@ -49,3 +49,26 @@ def test_rows_of_a_tile_stay_inside_the_run(tmp_path):
     assert f((2 ** 31 - 2) // 256, 256, 2 ** 31 - 1) == (2 ** 31 - 2) // 256 * 256
     # and it is what both searches take
     assert not re.search(r"rho0 = tile \* ", text) and len(re.findall(r"rho0 = first_row\(", text)) == 2
+
+
+# ------------------------------------------------------------------------------------------------ results
+
+
+def test_results_that_share_places_are_refused():
+    def append(**kw):
+        c, r, a, _ = _descs()
+        for k, v in {**dict(q=4096, q_out=8192, q_heads=4, q_row=256, q_head=64, qo_row=256, qo_head=64), **kw}.items():
+            setattr(a, k, v)
+        return _lib.load().vx_kv_append(C.byref(c), C.byref(r), C.byref(a), None)
+
+    for kw in (dict(qo_row=0), dict(qo_head=0), dict(qo_row=56), dict(qo_head=-8)):
+        _refused(append(**kw), b"one place")
+    for kw in (dict(o_row=0), dict(o_head=0), dict(o_row=-32), dict(o_head=56)):
+        _refused(attend(**kw), b"one place")
+
+    def single(c, r):
+        r.rows = r.sequences = 1
+        c.kv_heads = 1
+
+    # the stride of a single row or head says nothing
+    _refused(attend(single, o_row=0, o_head=0, q_heads=1), b"scratch")

@@ -236,6 +236,7 @@ extern "C" int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, co
   if (!pieces_ok(d->k, d->k_row, d->k_head, es) || !pieces_ok(d->v, d->v_row, d->v_head, es) ||
       (has_q && (!pieces_ok(d->q, d->q_row, d->q_head, es) || !pieces_ok(d->q_out, d->qo_row, d->qo_head, 2))))
     return fail(-1, "rows and heads of q, k, v and q_out must be 16-byte aligned");
+  if (has_q && shares_places(p.rows.rows, d->qo_row, d->q_heads, d->qo_head, D)) return fail(-1, "two rows or heads of q_out in one place (stride below head_dim)");
   if (d->q == d->q_out && has_q && (d->dtype != VX_BF16 || d->q_row != d->qo_row || d->q_head != d->qo_head)) return fail(-1, "q_out may be q only as the same bf16 tensor");
   p.k = d->k; p.v = d->v; p.q = d->q;
   p.k_row = d->k_row; p.k_head = d->k_head; p.v_row = d->v_row; p.v_head = d->v_head; p.q_row = d->q_row; p.q_head = d->q_head;

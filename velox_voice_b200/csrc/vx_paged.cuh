@@ -109,5 +109,9 @@ __device__ __forceinline__ int page_of(const PagedTable& t, int owner, uint32_t 
 int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c, KvRows& r);
 // Element strides and address of a bf16 / fp32 operand whose 16-byte pieces are read whole.
 inline bool pieces_ok(const void* p, int64_t a, int64_t b, int elem) { return aligned16(p) && a * elem % 16 == 0 && b * elem % 16 == 0; }
+// A result [rows, heads, head_dim] whose rows or heads lie in one place.
+inline bool shares_places(int64_t rows, int64_t row, int64_t heads, int64_t head, int head_dim) {
+  return (rows > 1 && row < head_dim && row > -head_dim) || (heads > 1 && head < head_dim && head > -head_dim);
+}
 
 }  // namespace vx

@@ -725,6 +725,7 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
   if (p.rows.rows == 0) return 0;
   if (!d->q || !d->out) return fail(-1, "q and out must not be NULL");
   if (!pieces_ok(d->q, d->q_row, d->q_head, 2) || !pieces_ok(d->out, d->o_row, d->o_head, 2)) return fail(-1, "rows and heads of q and out must be 16-byte aligned");
+  if (shares_places(p.rows.rows, d->o_row, d->q_heads, d->o_head, cache->head_dim)) return fail(-1, "two rows or heads of out in one place (stride below head_dim)");
   if (plan.bytes > 0 && (!d->scratch || (reinterpret_cast<uintptr_t>(d->scratch) & 31) != 0 || d->scratch_bytes < plan.bytes))
     return fail(-1, "scratch must be %lld bytes, 32-byte aligned", (long long)plan.bytes);
   p.q = static_cast<const __nv_bfloat16*>(d->q); p.q_row = d->q_row; p.q_head = d->q_head;
