@@ -119,3 +119,25 @@ def test_attention_scores_that_are_large_numbers(ops, heads, kv, d, n, tokens, l
             want[r, h] = values[best, h // (heads // kv)]
     got = f64(got)
     assert (np.abs(got - want) <= (0.0 if low == 32 else 2.0 ** -7 + 2.0 ** -13) * np.abs(want)).all(), f"{(got != want).any(-1).sum()} of {rows * heads} rows differ, {np.isnan(got).any(-1).sum()} NaN"
+
+
+# ------------------------------------------------------------------------------------------------ tables
+
+
+def test_tables_whose_rows_are_one_row(ops):  # noqa: F811
+    """Expanded tables: every sequence on the same pages, every group with the same prefix, every position with the same angles."""
+    k_pages, v_pages = make_cache(6, 16, 2, 64)
+    q = torch.randn(3, 4, 64, device="cuda").bfloat16()
+    t, p, n, m = ints([[0, 1]]).expand(3, 2), ints([[2, 3]]).expand(3, 2), ints([3, 9, 20]), ints([25]).expand(3)
+    want = ops.prefix_attention(q, k_pages, v_pages, t.contiguous(), n, p.contiguous(), m.contiguous())
+    assert torch.equal(ops.prefix_attention(q, k_pages, v_pages, t, n, p, m), want)
+    one = ints([[4]]).expand(3, 1)
+    want = ops.prefix_attention(q, k_pages, v_pages, one.contiguous(), ints([3, 9, 2]))
+    assert torch.equal(ops.prefix_attention(q, k_pages, v_pages, one, ints([3, 9, 2])), want)
+    rot = ops.rotary_table(9, 64)[4:5].expand(30, 64)
+    k = torch.randn(3, 2, 64, device="cuda").bfloat16()
+    caches = [(k_pages.clone(), v_pages.clone()) for _ in range(2)]
+    a = ops.kv_append(k, k, *caches[0], t, n, q=q, rotary=rot)
+    b = ops.kv_append(k, k, *caches[1], t.contiguous(), n, q=q, rotary=rot.contiguous())
+    assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(*caches))
+    assert not torch.equal(caches[0][0], k_pages)

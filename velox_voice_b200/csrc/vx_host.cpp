@@ -1189,13 +1189,15 @@ bool in_pieces(const at::Tensor& t) {
     if (step(t, static_cast<int>(i)) * es % 16 != 0) return false;
   return true;
 }
-// int32 [n] or [n, m] (n, m < 0: any) on `dev`, rows contiguous
+// rows one behind the other (not those of an expanded tensor)
+bool rows_apart(const at::Tensor& t) { return t.size(0) <= 1 || t.stride(0) >= t.size(1); }
+// int32 [n] or [n, m] (n, m < 0: any) on `dev`, rows contiguous and apart
 bool int32_arg(PyObject* o, int64_t n, int64_t m, int dims, const at::Device& dev, const at::Tensor** t) {
   if (!is_cuda_tensor(o)) return false;
   const at::Tensor& x = THPVariable_Unpack(o);
   *t = &x;
   if (x.scalar_type() != at::kInt || x.dim() != dims || x.device() != dev || (n >= 0 && x.size(0) != n)) return false;
-  if (dims == 2 && m >= 0 && x.size(1) != m) return false;
+  if (dims == 2 && ((m >= 0 && x.size(1) != m) || !rows_apart(x))) return false;
   return x.size(dims - 1) <= 1 || x.stride(dims - 1) == 1;
 }
 const int32_t* int32_ptr(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
@@ -1257,7 +1259,7 @@ PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
   if (p[7] != Py_None) {
     if (!is_cuda_tensor(p[7])) Py_RETURN_NONE;
     const at::Tensor& r = THPVariable_Unpack(p[7]);
-    if (r.scalar_type() != at::kFloat || r.dim() != 2 || r.device() != dev || r.size(1) % 16 != 0 || r.size(1) < 16 || r.size(1) > cache.head_dim || !in_pieces(r)) Py_RETURN_NONE;
+    if (r.scalar_type() != at::kFloat || r.dim() != 2 || r.device() != dev || r.size(1) % 16 != 0 || r.size(1) < 16 || r.size(1) > cache.head_dim || !in_pieces(r) || !rows_apart(r)) Py_RETURN_NONE;
     d.rotary = r.size(0) > 0 ? static_cast<const float*>(r.data_ptr()) : reinterpret_cast<const float*>(16);  // (NULL is no table at all)
     d.positions = r.size(0); d.rot_dim = static_cast<int>(r.size(1)); d.ld_rotary = r.size(0) > 1 ? r.stride(0) : r.size(1);
     d.interleaved = as_bool(p[8]);

@@ -741,14 +741,15 @@ def rotary_table(positions: int, rot_dim: int, base: float = 10000.0, *, device=
 
 
 def _int32_on(t, name: str, shape, dev) -> torch.Tensor:
-    """int32 tensor of the given shape (None: any size) on the cache's device, rows contiguous."""
+    """int32 tensor of the given shape (None: any size) on the cache's device, rows contiguous and one behind the other (expanded ones are copied)."""
     _require_cuda(t, name)
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
     if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
         want = ", ".join("n" if n is None else str(n) for n in shape)
         raise ValueError(f"{name} must be int32 [{want}], got {t.dtype} {tuple(t.shape)}")
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    apart = t.dim() < 2 or t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
+    return t if apart and (t.stride(-1) == 1 or t.shape[-1] <= 1) else t.contiguous()
 
 
 def _step(t: torch.Tensor, dim: int) -> int:
@@ -854,7 +855,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
             raise ValueError("rotary must be float32 [positions, rot_dim] on the cache's device")
         if rotary.shape[1] % 16 != 0 or not 16 <= rotary.shape[1] <= k.shape[2]:
             raise ValueError(f"rot_dim must be a multiple of 16 up to head_dim {k.shape[2]}, got {rotary.shape[1]}")
-        if not _in_pieces(rotary):
+        if not _in_pieces(rotary) or (rotary.shape[0] > 1 and rotary.stride(0) < rotary.shape[1]):
             rotary = rotary.clone(memory_format=torch.contiguous_format)
         d.rotary, d.positions, d.rot_dim = rotary.data_ptr() or 16, rotary.shape[0], rotary.shape[1]  # (NULL is no table at all)
         d.ld_rotary = rotary.stride(0) if rotary.shape[0] > 1 else rotary.shape[1]
