@@ -444,6 +444,8 @@ typedef struct {
   int64_t scratch_bytes;
 } vx_prefix_attention_desc;
 int64_t vx_prefix_attention_scratch(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
+/* Kernels that the call launches. */
+int vx_prefix_attention_launches(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
 int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc, void* stream);
 
 /* Block-scaled FP4 GEMM for callers that cannot allocate device memory.  (No counterpart in

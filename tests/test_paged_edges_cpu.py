@@ -72,3 +72,32 @@ def test_results_that_share_places_are_refused():
 
     # the stride of a single row or head says nothing
     _refused(attend(single, o_row=0, o_head=0, q_heads=1), b"scratch")
+
+
+# ------------------------------------------------------------------------------------------------ launches
+
+
+@pytest.mark.parametrize("rows,sequences,heads,width,prefix,launches", [
+    (0, 0, 4, 4, 0, 0),            # nothing
+    (3, 0, 4, 4, 0, 1),            # rows of no sequence: zeros
+    (3, 3, 4, 0, 0, 1),            # no keys
+    (3, 3, 4, 4, 9, 2),            # few rows: both spans in one launch, then the join
+    (300, 3, 64, 4, 9, 2),         # prompts: prefix and own tokens in a row, then the rows of no sequence
+    (200, 200, 4, 4, 9, 3),        # tile kernel over the prefix, few rows over the own tokens
+    (1200, 1200, 4, 4, 900, 3),    # pairs over the prefix
+    (60, 3, 8, 16, 9, 2),          # tile kernel over both
+    (1600, 80, 8, 16, 900, 3),     # pairs, then slots by themselves
+])
+def test_launches_of_a_call(rows, sequences, heads, width, prefix, launches):
+    c, r, _, p = _descs()
+    r.rows, r.sequences, r.ld_table, r.table_pages, r.row_offsets = rows, sequences, max(width, 1), width, 4096
+    p.q_heads, p.q_row = heads, 64 * heads
+    if prefix:
+        p.groups, p.group_offsets, p.prefix_table, p.ld_prefix, p.prefix_pages, p.prefix_lengths = 1, 4096, 4096, prefix, prefix, 8192
+    assert _lib.load().vx_prefix_attention_launches(C.byref(c), C.byref(r), C.byref(p)) == launches
+
+
+def test_launches_of_a_call_that_is_refused():
+    c, r, _, p = _descs()
+    p.q_heads = 3
+    _refused(_lib.load().vx_prefix_attention_launches(C.byref(c), C.byref(r), C.byref(p)), b"multiple")

@@ -141,3 +141,43 @@ def test_tables_whose_rows_are_one_row(ops):  # noqa: F811
     b = ops.kv_append(k, k, *caches[1], t.contiguous(), n, q=q, rotary=rot.contiguous())
     assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(*caches))
     assert not torch.equal(caches[0][0], k_pages)
+
+
+# ------------------------------------------------------------------------------------------------ launches
+
+
+def kernels(call):
+    """Kernel nodes of a graph that the call is captured into."""
+    from cuda.bindings import runtime as rt
+
+    call()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    _, _, n = rt.cudaGraphGetNodes(rt.cudaGraph_t(graph.raw_cuda_graph()), 0)
+    _, nodes, n = rt.cudaGraphGetNodes(rt.cudaGraph_t(graph.raw_cuda_graph()), n)
+    kinds = [rt.cudaGraphNodeGetType(x)[1] for x in nodes[:n]]
+    return sum(k == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for k in kinds)
+
+
+@pytest.mark.parametrize("heads,kv,n,tokens,prefix", [(4, 4, 3, 1, 90), (4, 4, 3, 0, 90), (2, 2, 2, 140, 90), (16, 1, 40, 1, 300), (16, 1, 2, 5, 130), (16, 1, 5, 7, 200)])
+@pytest.mark.parametrize("native", [True, False])
+def test_launches_are_counted(ops, monkeypatch, heads, kv, n, tokens, prefix, native):  # noqa: F811
+    rows, pw = n * tokens, -(-prefix // 16)
+    k_pages, v_pages = make_cache(n * 10 + pw, 16, kv, 64)
+    t, p = ints(np.arange(n * 10).reshape(n, 10)), ints(n * 10 + np.arange(pw)[None])
+    q, k = torch.randn(rows, heads, 64, device="cuda").bfloat16(), torch.randn(rows, kv, 64, device="cuda").bfloat16()
+    lengths, off, m = ints([9] * n), ints(np.arange(n + 1) * tokens), ints([prefix])
+    ops.kv_append(k, k, k_pages, v_pages, t, lengths, row_offsets=off)  # (the native host path is there)
+    if not native:
+        class Declines:
+            kv_append = prefix_attention = staticmethod(lambda *a: None)
+            launches = staticmethod(lambda: 0)
+            reset_launches = staticmethod(lambda: None)
+
+        monkeypatch.setattr(ops, "_native", Declines)
+    for call in (lambda: ops.kv_append(k, k, k_pages, v_pages, t, lengths, row_offsets=off), lambda: ops.prefix_attention(q, k_pages, v_pages, t, lengths, p, m, row_offsets=off)):
+        before = ops.launch_count()
+        call()
+        counted = ops.launch_count() - before
+        assert counted == kernels(call)

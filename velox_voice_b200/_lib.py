@@ -77,6 +77,7 @@ EXPORTS = (
     "vx_kv_append",
     "vx_prefix_attention",
     "vx_prefix_attention_scratch",
+    "vx_prefix_attention_launches",
 )
 
 
@@ -313,6 +314,8 @@ def load(build_if_missing: bool = True) -> C.CDLL:
         lib.vx_kv_append.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(KvAppendDesc), vp]
         lib.vx_prefix_attention_scratch.restype = i64
         lib.vx_prefix_attention_scratch.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc)]
+        lib.vx_prefix_attention_launches.restype = i32
+        lib.vx_prefix_attention_launches.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc)]
         lib.vx_prefix_attention.restype = i32
         lib.vx_prefix_attention.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc), vp]
         lib.vx_ctc_topk_threshold.restype = i32

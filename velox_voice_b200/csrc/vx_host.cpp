@@ -31,7 +31,7 @@ namespace {
   X(vx_last_error) X(vx_quantize_pack) X(vx_ln_quantize_pack) X(vx_ln2_quantize_pack) X(vx_amax) X(vx_bsgemm)        \
   X(vx_bsgemm_natural_sf_supported) X(vx_bsgemm_residual_ln_supported) X(vx_bsgemm_residual_ln) X(vx_bsgemm_residual_ln2) X(vx_argmax_ids) X(vx_relpos_attention)   \
   X(vx_power_mel_log) X(vx_power_mel_log_supported) X(vx_sf_from_natural_pair) X(vx_rowscale_linear) X(vx_rowscale_linear_scratch) X(vx_ctc_topk_rows) X(vx_ctc_topk)        \
-  X(vx_conformer_pass_supported) X(vx_conformer_pass_scratch) X(vx_conformer_pass) X(vx_kv_append) X(vx_prefix_attention) X(vx_prefix_attention_scratch)
+  X(vx_conformer_pass_supported) X(vx_conformer_pass_scratch) X(vx_conformer_pass) X(vx_kv_append) X(vx_prefix_attention) X(vx_prefix_attention_scratch) X(vx_prefix_attention_launches)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   VX_FUNCS(X)
@@ -1273,7 +1273,7 @@ PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
     if (q && !out.defined()) out = empty(q->sizes(), at::kBFloat16, dev);
     if (q) { d.q_out = out.data_ptr(); d.qo_row = step(out, 0); d.qo_head = step(out, 1); }
     check(g.vx_kv_append(&cache, &rows, &d, stream()), "vx_kv_append");
-    count();
+    count(rows.rows > 0 ? 1 : 0);
   }
   if (!q) Py_RETURN_TRUE;
   return p[11] != Py_None ? Py_NewRef(p[11]) : wrap(out);
@@ -1325,7 +1325,7 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
       d.scratch = scratch.data_ptr(); d.scratch_bytes = size;
     }
     check(g.vx_prefix_attention(&cache, &rows, &d, stream()), "vx_prefix_attention");
-    count(2);
+    count(g.vx_prefix_attention_launches(&cache, &rows, &d));
   }
   return p[10] != Py_None ? Py_NewRef(p[10]) : wrap(out);
   VX_END

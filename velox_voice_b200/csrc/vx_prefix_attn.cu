@@ -562,6 +562,9 @@ struct Plan {
   int blocks;                                       // of eight rows, of the kernel for few rows
   int parts;
   int64_t ml_bytes, bytes;
+
+  Span part(Kernel k, int i) const { return kernel[i] == k ? span[i] : kNoSpan; }  // the span, where kernel k walks it
+  bool walks(Kernel k) const { return part(k, 0).chunks > 0 || part(k, 1).chunks > 0; }
 };
 
 int64_t round_up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
@@ -716,6 +719,17 @@ extern "C" int64_t vx_prefix_attention_scratch(const vx_kv_cache* cache, const v
   return rc ? rc : plan.bytes;
 }
 
+extern "C" int vx_prefix_attention_launches(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
+  using namespace vx;
+  PrefixParams p{};
+  Plan plan;
+  const int rc = check_prefix(cache, rows, d, p, plan);
+  if (rc) return rc;
+  int n = p.rows.rows > 0 ? 1 : 0;  // the join
+  for (const Plan::Kernel k : {Plan::kRows, Plan::kTiles, Plan::kPairs}) n += plan.walks(k) ? 1 : 0;
+  return n;
+}
+
 extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, void* stream) {
   using namespace vx;
   PrefixParams p{};
@@ -735,15 +749,13 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
   const auto st = static_cast<cudaStream_t>(stream);
   const bool d64 = cache->head_dim == 64;
   p.status = device_status_ptr();
-  auto part = [&](Plan::Kernel k, int i) { return plan.kernel[i] == k ? plan.span[i] : kNoSpan; };  // the span, where kernel k walks it
-  auto walks = [&](Plan::Kernel k) { return part(k, 0).chunks > 0 || part(k, 1).chunks > 0; };
   for (const Plan::Kernel k : {Plan::kPairs, Plan::kTiles})
-    if (walks(k)) {
-      const int e = launch_prefix_tiles(p, cache->head_dim, k == Plan::kPairs, part(k, 0), part(k, 1), stream);
+    if (plan.walks(k)) {
+      const int e = launch_prefix_tiles(p, cache->head_dim, k == Plan::kPairs, plan.part(k, 0), plan.part(k, 1), stream);
       if (e) return e;
     }
-  if (walks(Plan::kRows)) {
-    RowsParams rp{p, {part(Plan::kRows, 0), part(Plan::kRows, 1)}, {1, 1}, 0, walks(Plan::kPairs) || walks(Plan::kTiles) ? 1 : 0};
+  if (plan.walks(Plan::kRows)) {
+    RowsParams rp{p, {plan.part(Plan::kRows, 0), plan.part(Plan::kRows, 1)}, {1, 1}, 0, plan.walks(Plan::kPairs) || plan.walks(Plan::kTiles) ? 1 : 0};
     int64_t blocks = 0;
     for (int i = 0; i < 2; ++i) {
       const Span& sp = rp.span[i];

@@ -865,7 +865,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
         starts = _int32_on(starts, "starts", (r.sequences,), dev)
         d.starts = starts.data_ptr()
     _lib.check(_lib.load().vx_kv_append(C.byref(cache), C.byref(r), C.byref(d), _stream()), "vx_kv_append")
-    _count()
+    _count(1 if rows else 0)
     del keep
     return q_out
 
@@ -927,7 +927,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     d.scratch, d.scratch_bytes = _ptr(scratch), size
     _lib.check(lib.vx_prefix_attention(C.byref(cache), C.byref(r), C.byref(d), _stream()), "vx_prefix_attention")
-    _count(2)
+    _count(int(lib.vx_prefix_attention_launches(C.byref(cache), C.byref(r), C.byref(d))))
     del keep, prefix_table, prefix_lengths, group_offsets
     return out
 
