@@ -417,8 +417,9 @@ int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_kv_a
 /* Attention of new tokens over a prefix that the sequences of a group share and over their own tokens:
  *   out[r, h] = sum_j softmax_j(scale q[r, h] . k_j) v_j,  key head h / (q_heads / kv_heads),
  * j over the keys [0, prefix_lengths[g]) of the pages prefix_table[g] and over own tokens t <= lengths[s] + i of the sequence
- * (row r is its i-th new token, which vx_kv_append has stored), both without the pages that are not there.  The prefix is read once for all
- * rows of its group.  A row without any key, of no sequence or of one that takes no part: zeros.
+ * (row r is its i-th new token, which vx_kv_append has stored), both without the pages that are not there.  The rows of a group walk
+ * the prefix together, up to 16, 128 or 256 (row, head) pairs of a key head at a time; where sequences have more than 128 such pairs of their own
+ * on the average, those of each sequence do.  A row without any key, of no sequence or of one that takes no part: zeros.
  *   groups         sequences [group_offsets[g], group_offsets[g + 1]) belong to group g (i32 [groups + 1], ascending); NULL: groups of
  *                  sequences / groups each.  0 groups: no prefix
  *   out            bf16 [rows, q_heads, head_dim], no two rows or heads in one place

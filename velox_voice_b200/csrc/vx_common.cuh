@@ -57,6 +57,9 @@ bool pdl_enabled();
 // one operand's scales do not trigger, and the GEMMs read weights ahead only when the caller says that they are constants (VX_GEMM_CONST_B), not
 // for an operand that the previous launch may just have produced.  Biases, LayerNorm parameters and filterbanks may be an fp32 result of a GEMM
 // that triggered early: they are read behind the wait.
+// Where the launch in front is known to trigger behind a wait of its own, all that was there before that launch is complete when its dependents
+// start, and they may read it ahead of their wait: the later kernels of a vx_prefix_attention call (rows beside tiles, the join) read the
+// call's arguments so.  What the launch in front writes is read behind the wait, which every thread still executes.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                                     Args&&... args) {

@@ -8,7 +8,8 @@
 // interleaved: 16 consecutive values), so cosines and sines are 64 consecutive bytes of the table and no value is read twice.  Where a
 // row goes -- sequence, page, place -- is looked up once per row and block, not per thread.
 // What bounds it: HBM (each input byte read once, each output byte written once; the table's rows come from L1 for all heads but the first):
-// 24 sequences of 5,000 tokens, 32 query and 8 key heads of 128, 2.2 GB in 353 us, 6.3 TB/s.  Small calls: the launch (2.8 us for 10 tokens).
+// 89,978 tokens of 24 sequences, 32 query and 8 key heads of 128, half of each rotated, 2.2 GB in 354 us, 6.3 TB/s.  Small calls: the launch (2.8 us
+// for 10 tokens).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

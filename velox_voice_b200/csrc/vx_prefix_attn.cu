@@ -20,9 +20,9 @@
 // cache.  mma.sync and not tcgen05: its M is 128 rows, of which these calls have 1 to 16.)
 // The reference maximum of a row moves only when a score exceeds it by more than 8 (probabilities stay below 2^8), so most steps
 // need a vote and no shuffles; sums are kept per lane until the end.
-// What bounds it: HBM where there is enough to read -- with the tile kernel, which has the prefixes, and the join, 566 MB of a batch of 192
-// sequences over eight prompts take 102 us, 5.5 TB/s -- and else the latency of a CTA: 16 groups of ten hypotheses, head_dim 64, take 6.6 us
-// over 64 frames, 13.4 over 1,000 and 25.9 over 3,750 (123 MB, 4.7 TB/s).
+// What bounds it: HBM where there is enough to read -- with the tile kernel, which has the prefixes, and the join, 566 MB of a batch of 149
+// sequences over eight prompts take 100 us, 5.7 TB/s -- and else the latency of a CTA and its issue slots: 16 groups of ten hypotheses, 8
+// heads of 64, take 6.7 us over 64 frames, 16 over 1,000 and 34 over 3,750 (123 MB, 3.7 TB/s; issue slots 57 % busy).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -41,7 +41,7 @@ namespace {
 constexpr int PR_WARPS = 4;
 
 // CTAs of prefix_rows_kernel per SM, as many as its registers allow: what a CTA needs before and behind its keys passes under the others'
-// keys.  (16 groups of ten hypotheses over 3,750 frames, head_dim 64: 47 us with 2, 37 with 3, 31 with 4.)
+// keys.  (16 groups of ten hypotheses, head_dim 64: over 64 frames 8.5 us with 2 or 3, 6.7 with 4, over 1,000 16 with any, over 3,750 37.5, 37.5 and 33.6.)
 constexpr int rows_ctas(int blocks, int head_dim) { return head_dim == 64 ? 4 : (blocks == 2 ? 2 : 3); }
 
 struct RowsParams {
@@ -431,7 +431,7 @@ int launch_rows(const RowsParams& rp, int64_t blocks, cudaStream_t st) {
 // The parts of every row joined, and zeros for the rows that have none.  WARPS warps of a block of eight share a row and query head, a slice of
 // the parts each; a warp requests the sums of PARTS parts (at head_dim 64 half a warp has one) together with their maxima, weighs them (maximum,
 // then 2^(m_c - m)) and adds them up; shared memory joins the warps.  Many rows of up to four parts, four at a time: fewer
-// registers, more rows on an SM (16 utterances with ten hypotheses of 60 tokens: a call of 93 us against 103; 32 rows of two parts: 10 against 8).  What a row is, is looked up ahead of the wait: the kernels in front let
+// registers, more rows on an SM (16 utterances with 124 hypotheses of 30 to 60 tokens: a call of 93 us against 103; 32 rows of two parts: 10 against 8).  What a row is, is looked up ahead of the wait: the kernels in front let
 // this one start behind a wait of their own, so all that was there before this call is complete.
 // What bounds it: one round trip to the parts in L2, or their bytes where rows are many: 64 rows of 32 heads of 128 with 17 parts (18 MB) are done 7 us
 // after the kernel in front (a lane that requested one part after the other: 11), 32 rows with 2 parts 2 us.
@@ -569,9 +569,12 @@ struct Plan {
 
 int64_t round_up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 
-// Keys per chunk for a span of `items` tiles times key heads.  Short runs are cut so that one round of CTAs (`resident`) takes them all;
-// long ones into several rounds, since owners differ in length and the last round should cost little.  Each part costs its sums in
-// scratch, so no chunk is below `least` keys there.
+// Keys per chunk for a span of `items` tiles times key heads.  Short runs are cut into shares of one round of CTAs (`resident`), rounded up to
+// a unit, which can make a few more CTAs than the round has places (128 items over 3,584 keys: shares of 774, chunks of 832, 640 CTAs for 592 places); long
+// ones into several rounds, since owners differ in length and the last round should cost little.  Each part costs its sums in
+// scratch, so no chunk is below `least` keys there.  `capacity` is what the tables have place for, not what lengths (on the device) fill: wide
+// tables and a long owner among short ones get chunks that are too long (64 rows over 8,191 keys, 32 heads on 8 of 128: 39 us, with
+// a table for 131,072 144; 199 sequences of 100 tokens and one of 100,000: 1.5 ms, 120,000 tokens in equal runs 0.1).
 int chunk_keys(int64_t capacity, int64_t items, int64_t resident, int64_t unit, int64_t least, int64_t rounds) {
   const int64_t one_round = (capacity * items + resident - 1) / resident;
   int64_t c = one_round;
@@ -669,31 +672,40 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
   if (rows_o > kSlotRows) {
-    // whole prompts or long chunks: prefix and own tokens in a row, no joining of the two
+    // Whole prompts or long chunks: prefix and own tokens in a row, no joining of the two, but a walk of the prefix per sequence.  8 key heads,
+    // prompts without a history, the two apart (prefix by groups) against in a row, in us:
+    //   head_dim 64    130 rows  4 sequences, one prefix of 1,000 keys 42 : 26   of 8,000 62 : 54     64 sequences, 1,000 133 : 120   8,000 349 : 514
+    //                  256 rows                               49 : 32            77 : 60                            211 : 124         592 : 544
+    //                  512 rows                               58 : 40           112 : 93                            393 : 214       1,130 : 945
+    //   head_dim 128   132 rows                               46 : 30            69 : 59                            140 : 119         376 : 559
+    //                  256 rows                               52 : 35            85 : 67                            239 : 122         664 : 576
+    // (in a row loses where many sequences with few rows share a long prefix: their second slots are empty)
     plan.kernel[0] = plan.kernel[1] = Plan::kPairs;
     cut(plan.span[0], kSpanJoint, Plan::kPairs, S, round_up(cap_p, kSpanAlign) + cap_o, single ? per : 0);
     if (plan.span[0].chunks == 1) plan.span[0].part0 = -1;
   } else {
     // prefix_rows_kernel walks the keys once per 16 rows, without much to set up; the tile kernel starts slower and walks them once per 128.
     // One group, 8 key heads, single tokens, rows kernel against tiles, in us:
-    //   head_dim 64    16 rows  4,000 keys 21 : 24   40,000 keys 34 : 42     32 rows  4,000 keys 23 : 25   16,000 keys 30 : 32   40,000 keys 52 : 44
-    //   head_dim 128    8 rows  4,000 keys 24 : 28   40,000 keys 60 : 58     16 rows  4,000 keys 26 : 28   16,000 keys 38 : 39   40,000 keys 73 : 60
-    //                  32 rows  4,000 keys 24 : 31    8,000 keys 34 : 34     48 rows  4,000 keys 30 : 32    8,000 keys 48 : 34
-    // A rule that meets these: what the walks read together.
+    //   head_dim 64    16 rows  4,000 keys 17 : 21   16,000 keys 20 : 28   40,000 keys 30 : 40     32 rows  4,000 keys 20 : 22   16,000 keys 26 : 30   40,000 keys 48 : 41
+    //   head_dim 128    8 rows  4,000 keys 15 : 20   16,000 keys 28 : 32   40,000 keys 53 : 50     16 rows  4,000 keys 17 : 22   16,000 keys 30 : 32   40,000 keys 57 : 50
+    //                  32 rows  4,000 keys 20 : 24    8,000 keys 26 : 26   16,000 keys 44 : 32     48 rows  4,000 keys 24 : 24    8,000 keys 38 : 28
+    // A rule that meets these within 3 us: what the walks read together.
     const double bytes = 4.0 * static_cast<double>(G * cap_p) * cache->kv_heads * cache->head_dim;  // of the keys and values
     const bool few = rows_p <= (cache->head_dim == 64 ? 16 : 8) || (rows_p <= 64 && static_cast<double>((rows_p + 15) / 16) * bytes <= 64.0 * 1048576.0);
     // Pairs of slots share their keys, which counts where there are many; with an odd number of slots one of a pair idles, and a pair starts
     // slower.  8 key heads, slots by themselves against pairs, in us:
-    //   head_dim 64, 6 MB of keys and values   256 rows 28 : 30   500 33 : 38      49 MB (8 groups)  256 rows 83 : 77   384 112 : 112   500 146 : 125
-    //                61 MB (1 group)           256 rows 54 : 56   384 85 : 81   500 126 : 84
-    //   head_dim 128, 12 MB  256 rows 28 : 32   512 36 : 40   600 42 : 40          34 MB  256 rows 58 : 63
-    //                98 MB (8 groups)  200 rows 76 : 65   360 108 : 97   512 147 : 108   123 MB (1 group)  200 rows 67 : 62   256 65 : 65   360 97 : 87   512 146 : 93
+    //   head_dim 64, 6 MB of keys and values   256 rows 28 : 30   500 34 : 37      49 MB (8 groups)  256 rows 79 : 79   384 108 : 116   500 136 : 132
+    //                61 MB (1 group)           256 rows 58 : 56   384 75 : 83   500 91 : 86
+    //   head_dim 128, 12 MB  256 rows 28 : 32   512 36 : 38   600 36 : 38          34 MB  256 rows 39 : 42
+    //                98 MB (8 groups)  200 rows 67 : 65   360 101 : 101   512 124 : 116   123 MB (1 group)  200 rows 67 : 63   256 67 : 65   360 85 : 89   512 108 : 95
+    // (The rule below meets these within 4 us.)
     const bool pairs = rows_p > 4 * kSlotRows || (rows_p > 3 * kSlotRows && bytes > 32.0 * 1048576.0) || (rows_p > kSlotRows && bytes > 64.0 * 1048576.0);
     plan.kernel[0] = few ? Plan::kRows : (pairs ? Plan::kPairs : Plan::kTiles);
     // Own tokens of many sequences are many short walks, whose start counts for more.  160 sequences without a prefix, new tokens behind a
     // history, 8 key heads, rows kernel against tiles, in us:
-    //   head_dim 64   12 rows  0 + 12 keys 18 : 33  500 + 12 51 : 70    24 rows  0 + 24 27 : 39  2,000 + 24 159 : 188    48 rows  100 + 48 57 : 61  500 + 48 104 : 102
-    //   head_dim 128  16 rows  0 + 4 keys 29 : 39   500 + 4 85 : 84     32 rows  0 + 8 41 : 47   100 + 8 53 : 55  500 + 8 125 : 92    64 rows  0 + 16 68 : 64
+    //   head_dim 64   12 rows  0 + 12 keys 22 : 38  500 + 12 62 : 79    24 rows  0 + 24 34 : 46  2,000 + 24 224 : 225    48 rows  100 + 48 75 : 75  500 + 48 139 : 110
+    //   head_dim 128  16 rows  0 + 4 keys 36 : 44   500 + 4 106 : 99    32 rows  0 + 8 54 : 54   100 + 8 79 : 65  500 + 8 163 : 111    64 rows  0 + 16 91 : 79
+    // (The rule below misses at head_dim 128, 16 rows with 500 tokens before them and 32 with 100.)
     const int64_t width = rows_o * cache->head_dim;
     plan.kernel[1] = width <= 32 * 64 || (width <= 64 * 64 && cap_o <= 256) ? Plan::kRows : Plan::kTiles;
     plan.blocks = (plan.kernel[0] == Plan::kRows && rows_p > 8) || (plan.kernel[1] == Plan::kRows && rows_o > 8) ? 2 : 1;
@@ -761,7 +773,7 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
       const Span& sp = rp.span[i];
       const int64_t items = static_cast<int64_t>(sp.slots) * sp.chunks * p.kv_heads;
       // All four warps of a CTA on an item while one round of CTAs takes them all, else so many that each has about 128 keys: twice as many take
-      // 28 us for 27 (64 hypotheses, 2,000 frames and 200 tokens) and 37 for 32 (160 of 60 tokens), half as many 29 and 32.
+      // 28 us for 27 (64 hypotheses of 102 to 198 tokens, four utterances of 1,005 to 1,792 frames) and 37 for 32 (124 of 30 to 60 tokens), half as many 29 and 32.
       rp.warps[i] = items <= rows_resident(plan.blocks, cache->head_dim) || sp.chunk > 256 ? 4 : (sp.chunk > 128 ? 2 : 1);
       blocks += (items * rp.warps[i] + PR_WARPS - 1) / PR_WARPS;
       if (i == 0) rp.first_blocks = static_cast<int32_t>(blocks);

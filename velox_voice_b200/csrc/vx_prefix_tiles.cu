@@ -5,7 +5,7 @@
 // the tensor cores have the products of the other.
 //   PAIRED     both slots take one item of 256 rows, 128 keys a tile: every K and V tile is loaded once for both.  For many rows per owner,
 //              where the products are the bound.  Tensor memory of a slot: S (128 columns, P in bf16 over it) | O (head_dim).  (Tiles of 64 keys
-//              and two S here too, an MMA issuer per slot: 2,125 us against 1,815 for four chunks of 2,048 tokens behind 16,384; a product of
+//              and two S here too, an MMA issuer per slot: 2,125 us against 1,815 for 6,906 tokens of four prompts behind 16,384; a product of
 //              64 columns reads all of Q from shared memory for half the work.)
 //   otherwise  each slot has a stream of items of its own, 64 keys a tile, and the tiles of the two take turns.  For few rows, where the keys'
 //              bytes are the bound: smaller tiles hold less of the shared memory while their softmax runs, so more of it is for copies in
@@ -32,9 +32,10 @@
 // 2^8); then the row's sum and its O are scaled before P is handed over.
 // What bounds it.  PAIRED: the round trip of a slot -- 2,000 cycles of softmax (1,024 of them exponentials: 128 x 128 at 16 a cycle for each of
 // two slots), then P V and the next S, 1,024 cycles of the tensor cores, with hand-over and the other slot's products in between: 3,900 cycles
-// a tile of 256 rows by 128 keys, 1.16 PFLOP/s over chunks of 2,048 tokens behind 16,384 (32 query heads on 8 key heads of 128).  Otherwise:
-// bytes from L2 and HBM where there are many keys (32 rows over 90,000 keys, 102 us, 3.9 TB/s), the softmax of a tile (some 1,950 cycles) where
-// keys are shared by many rows, and what a CTA costs to begin and end where an SM has a few tiles only (one tile each: 10 us at head_dim 64).
+// a tile of 256 rows by 128 keys: 6,906 tokens of four prompts behind 16,384 (32 query heads on 8 key heads of 128) take 1,780 us with pauses
+// between the calls, 1.12 PFLOP/s, and 2,040, 0.98, in calls one after the other, where the power cap lowers the clock.  Otherwise: bytes from L2
+// and HBM where there are many keys (128 rows a head over 90,000 keys, 84 us, 4.4 TB/s), the softmax of a tile (some 1,950 cycles) where keys are shared by many
+// rows, and what a CTA costs to begin and end where an SM has a few tiles only (16 groups of 100 rows over 64 keys, one tile each: 11 us at head_dim 64).
 // Every wait on a barrier is bounded.
 
 #include <cuda_bf16.h>
@@ -68,8 +69,8 @@ struct TileShape {
   static constexpr int kStreams = PAIRED ? 1 : 2;
   static constexpr int kParts = PAIRED ? 4 : 1;               // loaders that share a tile
   // P of a tile handed over in halves, so that the products of the first run under the exponentials of the second.  Gains where the products are
-  // short (16 utterances, prompts of 200 tokens behind 6,000, head_dim 64: 363 -> 339 us) and loses where an issuer that waits for the second
-  // half keeps the other slot's products waiting (four chunks of 2,048 behind 16,384, head_dim 128: 1,710 -> 1,755).
+  // short (16 utterances of 3,116 to 5,510 frames, 9,894 tokens of 66 prompts, head_dim 64: 363 -> 339 us) and loses where an issuer that waits for the
+  // second half keeps the other slot's products waiting (6,906 tokens of four prompts behind 16,384, head_dim 128: 1,710 -> 1,755).
   static constexpr bool kHalves = PAIRED && D == 64;
   static constexpr int kStagesK = D == 128 ? 3 : 5, kStagesV = D == 128 ? 2 : 5;  // of a stream
   static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + 1024;

@@ -874,9 +874,9 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                      prefix_table: Optional[torch.Tensor] = None, prefix_lengths: Optional[torch.Tensor] = None, *,
                      row_offsets: Optional[torch.Tensor] = None, group_offsets: Optional[torch.Tensor] = None,
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Attention of new tokens over a prefix that the sequences of a group share, read once for all of them, and over their own
-    tokens (``vx_prefix_attention``).  q bf16 [rows, heads, head_dim] -> bf16 [rows, heads, head_dim]; heads a multiple of kv_heads,
-    head_dim 64 or 128.
+    """Attention of new tokens over a prefix that the sequences of a group share and read together (whole prompts: one by one), and
+    over their own tokens (``vx_prefix_attention``).  q bf16 [rows, heads, head_dim] -> bf16 [rows, heads, head_dim]; heads a
+    multiple of kv_heads, head_dim 64 or 128.
 
     Row r, the i-th new token of sequence s (``row_offsets``, ``lengths``, ``page_table`` as for :func:`kv_append`, called before
     with the same ``lengths``), attends to own tokens t <= lengths[s] + i and to the prefix of its group: keys
