@@ -414,6 +414,32 @@ typedef struct {
 /* head_dim: a multiple of 16, at most 256 */
 int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_kv_append_desc* desc, void* stream);
 
+/* The same cache in 4 bits.  k, v u8: a page is kv_heads * (page_size / 16) units of 9 * head_dim bytes, heads outermost; a unit holds 16
+ * tokens of a head,
+ *   codes   [16][head_dim / 2]   two E2M1 values a byte, the even one in the low half
+ *   scales  [16][head_dim / 16]  E4M3, one for 16 values of a token; the sign bit is not looked at, 0x7f stands for 480
+ * and stands for values  code * scale * k_scale (v_scale): 4.5 bits each.  Whatever its bytes are, they stand for finite values. */
+typedef struct {
+  int32_t struct_size; /* sizeof(vx_kv_cache_fp4) */
+  int32_t page_size;   /* tokens per page, a multiple of 16 */
+  int64_t pages;
+  int32_t kv_heads, head_dim; /* head_dim: a multiple of 16, at most 256 */
+  void* k;                    /* 16-byte aligned */
+  void* v;
+  int64_t k_page, v_page;     /* bytes from page to page, multiples of 16 */
+  float k_scale, v_scale;     /* powers of two from 2^-32 to 2^32 */
+} vx_kv_cache_fp4;
+
+/* vx_kv_append into a cache in 4 bits.  With x a rotated key, its products and sums rounded to fp32 one by one, or a value, and g the tensor's scale:
+ *   scale byte = E4M3(min(RN32(max |x| of the 16 / g / 6), 448)), to nearest, ties to even;  s its value
+ *   code       = E2M1(x / (g s)), to nearest, ties to the even code, up to 6;  0 where s is 0
+ * (The quantizers of the linear path end at 4.0, as the reference's do; here nothing has to be like them.)  What is not finite is stored as the largest
+ * finite value or, where it is NaN, as any. */
+int vx_kv_append_fp4(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_kv_append_desc* desc, void* stream);
+
+/* Values of the pages of one tensor of such a cache: out bf16 [pages, page_size, kv_heads, head_dim], exact. */
+int vx_kv_values_fp4(const void* pages, int64_t n_pages, int64_t page_bytes, int page_size, int kv_heads, int head_dim, float scale, void* out, void* stream);
+
 /* Attention of new tokens over a prefix that the sequences of a group share and over their own tokens:
  *   out[r, h] = sum_j softmax_j(scale q[r, h] . k_j) v_j,  key head h / (q_heads / kv_heads),
  * j over the keys [0, prefix_lengths[g]) of the pages prefix_table[g] and over own tokens t <= lengths[s] + i of the sequence
@@ -448,6 +474,12 @@ int64_t vx_prefix_attention_scratch(const vx_kv_cache* cache, const vx_kv_rows* 
 /* Kernels that the call launches. */
 int vx_prefix_attention_launches(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
 int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc, void* stream);
+
+/* The same over a cache in 4 bits.  Queries and probabilities as fp16 operands (a query by a power of two of its own, so that its largest value is in
+ * [1, 2): below 2^115), keys and values exactly; fp32 scores, statistics and sums. */
+int64_t vx_prefix_attention_fp4_scratch(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
+int vx_prefix_attention_fp4_launches(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
+int vx_prefix_attention_fp4(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc, void* stream);
 
 /* Block-scaled FP4 GEMM for callers that cannot allocate device memory.  (No counterpart in
  * the reference: its Python wrappers allocate through torch.)

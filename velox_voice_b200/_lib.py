@@ -78,6 +78,11 @@ EXPORTS = (
     "vx_prefix_attention",
     "vx_prefix_attention_scratch",
     "vx_prefix_attention_launches",
+    "vx_kv_append_fp4",
+    "vx_kv_values_fp4",
+    "vx_prefix_attention_fp4",
+    "vx_prefix_attention_fp4_scratch",
+    "vx_prefix_attention_fp4_launches",
 )
 
 
@@ -144,6 +149,24 @@ class KvCache(C.Structure):
         ("v_page", C.c_int64),
         ("v_token", C.c_int64),
         ("v_head", C.c_int64),
+    ]
+
+
+class KvCacheFp4(C.Structure):
+    """``vx_kv_cache_fp4``."""
+
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("page_size", C.c_int32),
+        ("pages", C.c_int64),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_page", C.c_int64),
+        ("v_page", C.c_int64),
+        ("k_scale", C.c_float),
+        ("v_scale", C.c_float),
     ]
 
 
@@ -318,6 +341,16 @@ def load(build_if_missing: bool = True) -> C.CDLL:
         lib.vx_prefix_attention_launches.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc)]
         lib.vx_prefix_attention.restype = i32
         lib.vx_prefix_attention.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc), vp]
+        lib.vx_kv_append_fp4.restype = i32
+        lib.vx_kv_append_fp4.argtypes = [C.POINTER(KvCacheFp4), C.POINTER(KvRows), C.POINTER(KvAppendDesc), vp]
+        lib.vx_kv_values_fp4.restype = i32
+        lib.vx_kv_values_fp4.argtypes = [vp, i64, i64, i32, i32, i32, f32, vp, vp]
+        lib.vx_prefix_attention_fp4_scratch.restype = i64
+        lib.vx_prefix_attention_fp4_scratch.argtypes = [C.POINTER(KvCacheFp4), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc)]
+        lib.vx_prefix_attention_fp4_launches.restype = i32
+        lib.vx_prefix_attention_fp4_launches.argtypes = [C.POINTER(KvCacheFp4), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc)]
+        lib.vx_prefix_attention_fp4.restype = i32
+        lib.vx_prefix_attention_fp4.argtypes = [C.POINTER(KvCacheFp4), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc), vp]
         lib.vx_ctc_topk_threshold.restype = i32
         lib.vx_ctc_topk_threshold.argtypes = [vp, i64, i64, i32, vp, vp]
         lib.vx_ctc_topk_finish.restype = i32

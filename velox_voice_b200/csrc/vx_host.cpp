@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -31,7 +32,8 @@ namespace {
   X(vx_last_error) X(vx_quantize_pack) X(vx_ln_quantize_pack) X(vx_ln2_quantize_pack) X(vx_amax) X(vx_bsgemm)        \
   X(vx_bsgemm_natural_sf_supported) X(vx_bsgemm_residual_ln_supported) X(vx_bsgemm_residual_ln) X(vx_bsgemm_residual_ln2) X(vx_argmax_ids) X(vx_relpos_attention)   \
   X(vx_power_mel_log) X(vx_power_mel_log_supported) X(vx_sf_from_natural_pair) X(vx_rowscale_linear) X(vx_rowscale_linear_scratch) X(vx_ctc_topk_rows) X(vx_ctc_topk)        \
-  X(vx_conformer_pass_supported) X(vx_conformer_pass_scratch) X(vx_conformer_pass) X(vx_kv_append) X(vx_prefix_attention) X(vx_prefix_attention_scratch) X(vx_prefix_attention_launches)
+  X(vx_conformer_pass_supported) X(vx_conformer_pass_scratch) X(vx_conformer_pass) X(vx_kv_append) X(vx_prefix_attention) X(vx_prefix_attention_scratch) X(vx_prefix_attention_launches)        \
+  X(vx_kv_append_fp4) X(vx_kv_values_fp4) X(vx_prefix_attention_fp4) X(vx_prefix_attention_fp4_scratch) X(vx_prefix_attention_fp4_launches)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   VX_FUNCS(X)
@@ -1213,6 +1215,49 @@ bool paged_cache(PyObject* ko, PyObject* vo, vx_kv_cache& c, at::Device& dev) {
        k.data_ptr(), v.data_ptr(), step(k, 0), step(k, 1), step(k, 2), step(v, 0), step(v, 1), step(v, 2)};
   return true;
 }
+// u8 [pages, kv_heads, page_size / 16, 9 head_dim], pages contiguous and apart
+bool fp4_pages(PyObject* o, const at::Tensor** t) {
+  if (!is_cuda_tensor(o)) return false;
+  const at::Tensor& x = THPVariable_Unpack(o);
+  *t = &x;
+  if (x.scalar_type() != at::kByte || x.dim() != 4 || x.size(1) < 1 || x.size(2) < 1 || x.size(1) > 65535 || x.size(2) > (1 << 27) - 1 || x.size(3) % 144 != 0 || x.size(3) < 144 ||
+      x.size(3) > 2304 || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) != 0)
+    return false;
+  const int64_t unit = x.size(3), head = x.size(2) * unit;
+  return x.stride(3) == 1 && (x.size(2) == 1 || x.stride(2) == unit) && (x.size(1) == 1 || x.stride(1) == head) && step(x, 0) % 16 == 0 &&
+         (x.size(0) <= 1 || x.stride(0) >= x.size(1) * head);
+}
+// Either cache: `fp4` says which.  What is wrong with its scales is for the general route.
+struct AnyCache {
+  bool fp4;
+  vx_kv_cache b16;
+  vx_kv_cache_fp4 b4;
+  int kv_heads, head_dim;
+};
+bool any_cache(PyObject* ko, PyObject* vo, PyObject* k_scale, PyObject* v_scale, AnyCache& c, at::Device& dev) {
+  if (!is_cuda_tensor(ko)) return false;
+  if (!PyFloat_CheckExact(k_scale) || !PyFloat_CheckExact(v_scale)) return false;
+  const double ks = PyFloat_AS_DOUBLE(k_scale), vs = PyFloat_AS_DOUBLE(v_scale);
+  c.fp4 = THPVariable_Unpack(ko).scalar_type() == at::kByte;
+  if (!c.fp4) {
+    if (ks != 1.0 || vs != 1.0 || !paged_cache(ko, vo, c.b16, dev)) return false;
+    c.kv_heads = c.b16.kv_heads;
+    c.head_dim = c.b16.head_dim;
+    return true;
+  }
+  const at::Tensor *k, *v;
+  if (!fp4_pages(ko, &k) || !fp4_pages(vo, &v) || k->sizes() != v->sizes() || k->device() != v->device()) return false;
+  for (const double x : {ks, vs}) {
+    int e;
+    if (!(x >= 0x1p-32 && x <= 0x1p32) || std::frexp(x, &e) != 0.5) return false;
+  }
+  dev = k->device();
+  c.kv_heads = static_cast<int>(k->size(1));
+  c.head_dim = static_cast<int>(k->size(3) / 9);
+  c.b4 = {static_cast<int32_t>(sizeof(vx_kv_cache_fp4)), static_cast<int32_t>(16 * k->size(2)), k->size(0), c.kv_heads, c.head_dim, k->data_ptr(), v->data_ptr(), step(*k, 0), step(*v, 0),
+          static_cast<float>(ks), static_cast<float>(vs)};
+  return true;
+}
 bool paged_rows(int64_t rows, PyObject* table, PyObject* lengths, PyObject* offsets, const at::Device& dev, vx_kv_rows& r) {
   const at::Tensor *t, *n, *o = nullptr;
   if (!int32_arg(table, -1, -1, 2, dev, &t) || !int32_arg(lengths, t->size(0), -1, 1, dev, &n)) return false;
@@ -1229,17 +1274,17 @@ bool heads3d(PyObject* o, int64_t rows, int64_t heads, int64_t dim, const at::De
   return x.dim() == 3 && x.device() == dev && x.size(2) == dim && (rows < 0 || x.size(0) == rows) && (heads < 0 || x.size(1) == heads) && in_pieces(x);
 }
 
-// kv_append(k, v, k_pages, v_pages, page_table, lengths, q | None, rotary | None, interleaved, row_offsets | None, starts | None, q_out | None)
+// kv_append(k, v, k_pages, v_pages, page_table, lengths, q | None, rotary | None, interleaved, row_offsets | None, starts | None, q_out | None, k_scale, v_scale)
 //   -> q_out | True (no queries) | None
 PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
   VX_BEGIN
-  VX_ARGS(12)
-  vx_kv_cache cache;
+  VX_ARGS(14)
+  AnyCache cache;
   vx_kv_rows rows;
   vx_kv_append_desc d{};
   at::Device dev(at::kCUDA);
   const at::Tensor *k, *v, *q = nullptr, *t;
-  if (!paged_cache(p[2], p[3], cache, dev) || !heads3d(p[0], -1, cache.kv_heads, cache.head_dim, dev, &k) ||
+  if (!any_cache(p[2], p[3], p[12], p[13], cache, dev) || !heads3d(p[0], -1, cache.kv_heads, cache.head_dim, dev, &k) ||
       !heads3d(p[1], k->size(0), cache.kv_heads, cache.head_dim, dev, &v) || !paged_rows(k->size(0), p[4], p[5], p[9], dev, rows))
     Py_RETURN_NONE;
   d.struct_size = sizeof(vx_kv_append_desc);
@@ -1272,7 +1317,8 @@ PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
     NoGil nogil;
     if (q && !out.defined()) out = empty(q->sizes(), at::kBFloat16, dev);
     if (q) { d.q_out = out.data_ptr(); d.qo_row = step(out, 0); d.qo_head = step(out, 1); }
-    check(g.vx_kv_append(&cache, &rows, &d, stream()), "vx_kv_append");
+    if (cache.fp4) check(g.vx_kv_append_fp4(&cache.b4, &rows, &d, stream()), "vx_kv_append_fp4");
+    else check(g.vx_kv_append(&cache.b16, &rows, &d, stream()), "vx_kv_append");
     count(rows.rows > 0 ? 1 : 0);
   }
   if (!q) Py_RETURN_TRUE;
@@ -1281,16 +1327,16 @@ PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
 }
 
 // prefix_attention(q, k_pages, v_pages, page_table, lengths, prefix_table | None, prefix_lengths | None, row_offsets | None, group_offsets | None,
-//   scale | None, out | None) -> out | None
+//   scale | None, out | None, k_scale, v_scale) -> out | None
 PyObject* py_prefix_attention(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
   VX_BEGIN
-  VX_ARGS(11)
-  vx_kv_cache cache;
+  VX_ARGS(13)
+  AnyCache cache;
   vx_kv_rows rows;
   vx_prefix_attention_desc d{};
   at::Device dev(at::kCUDA);
   const at::Tensor *q, *t, *n, *o;
-  if (!paged_cache(p[1], p[2], cache, dev) || !heads3d(p[0], -1, -1, cache.head_dim, dev, &q) || q->scalar_type() != at::kBFloat16 ||
+  if (!any_cache(p[1], p[2], p[11], p[12], cache, dev) || !heads3d(p[0], -1, -1, cache.head_dim, dev, &q) || q->scalar_type() != at::kBFloat16 ||
       (cache.head_dim != 64 && cache.head_dim != 128) || q->size(1) < 1 || q->size(1) % cache.kv_heads != 0 || !paged_rows(q->size(0), p[3], p[4], p[7], dev, rows))
     Py_RETURN_NONE;
   d.struct_size = sizeof(vx_prefix_attention_desc);
@@ -1318,16 +1364,40 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
     NoGil nogil;
     if (!out.defined()) out = empty(q->sizes(), at::kBFloat16, dev);
     d.out = out.data_ptr(); d.o_row = step(out, 0); d.o_head = step(out, 1);
-    const int64_t size = g.vx_prefix_attention_scratch(&cache, &rows, &d);
-    if (size < 0) check(static_cast<int>(size), "vx_prefix_attention");
+    const char* const what = cache.fp4 ? "vx_prefix_attention_fp4" : "vx_prefix_attention";
+    const int64_t size = cache.fp4 ? g.vx_prefix_attention_fp4_scratch(&cache.b4, &rows, &d) : g.vx_prefix_attention_scratch(&cache.b16, &rows, &d);
+    if (size < 0) check(static_cast<int>(size), what);
     if (size > 0) {
       scratch = empty({size}, at::kByte, dev);
       d.scratch = scratch.data_ptr(); d.scratch_bytes = size;
     }
-    check(g.vx_prefix_attention(&cache, &rows, &d, stream()), "vx_prefix_attention");
-    count(g.vx_prefix_attention_launches(&cache, &rows, &d));
+    check(cache.fp4 ? g.vx_prefix_attention_fp4(&cache.b4, &rows, &d, stream()) : g.vx_prefix_attention(&cache.b16, &rows, &d, stream()), what);
+    count(cache.fp4 ? g.vx_prefix_attention_fp4_launches(&cache.b4, &rows, &d) : g.vx_prefix_attention_launches(&cache.b16, &rows, &d));
   }
   return p[10] != Py_None ? Py_NewRef(p[10]) : wrap(out);
+  VX_END
+}
+
+// kv_values(pages, scale, out | None) -> out | None
+PyObject* py_kv_values(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
+  VX_BEGIN
+  VX_ARGS(3)
+  const at::Tensor* x;
+  if (p[2] != Py_None || !PyFloat_CheckExact(p[1]) || !fp4_pages(p[0], &x)) Py_RETURN_NONE;
+  const double s = PyFloat_AS_DOUBLE(p[1]);
+  int e;
+  if (!(s >= 0x1p-32 && s <= 0x1p32) || std::frexp(s, &e) != 0.5) Py_RETURN_NONE;
+  at::Tensor out;
+  {
+    NoGil nogil;
+    const int64_t D = x->size(3) / 9;
+    out = empty({x->size(0), 16 * x->size(2), x->size(1), D}, at::kBFloat16, x->device());
+    check(g.vx_kv_values_fp4(x->data_ptr(), x->size(0), step(*x, 0), static_cast<int>(16 * x->size(2)), static_cast<int>(x->size(1)), static_cast<int>(D), static_cast<float>(s), out.data_ptr(),
+                             stream()),
+          "vx_kv_values_fp4");
+    count(x->size(0) > 0 ? 1 : 0);
+  }
+  return wrap(out);
   VX_END
 }
 
@@ -1370,6 +1440,7 @@ PyMethodDef kMethods[] = {
     VX_METHOD("power_mel_log", py_power_mel_log),
     VX_METHOD("kv_append", py_kv_append),
     VX_METHOD("prefix_attention", py_prefix_attention),
+    VX_METHOD("kv_values", py_kv_values),
     VX_METHOD("stack_plan", py_stack_plan),
     VX_METHOD("stack_plan_current", py_stack_plan_current),
     VX_METHOD("stack_forward", py_stack_forward),

@@ -11,20 +11,50 @@
 // 89,978 tokens of 24 sequences, 32 query and 8 key heads of 128, half of each rotated, 2.2 GB in 354 us, 6.3 TB/s.  Small calls: the launch (2.8 us
 // for 10 tokens).
 
+//
+// Into a cache in 4 bits (FP4): a thread takes the 16 values of one scale of a key or value; for a rotated key it loads the partners of its values
+// too, so that no thread waits for another's maximum (a second load of the same bytes, from L1).
+
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "vx_common.cuh"
 #include "vx_paged.cuh"
 #include "vx_ptx.cuh"
+#include "vx_quant_math.cuh"
 
 namespace vx {
 
-int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c, KvRows& r) {
-  if (!cache || cache->struct_size != static_cast<int32_t>(sizeof(vx_kv_cache))) return fail(-1, "vx_kv_cache: struct_size");
+namespace {
+int check_rows(const vx_kv_rows* rows, int page_size, KvRows& r) {
   if (!rows || rows->struct_size != static_cast<int32_t>(sizeof(vx_kv_rows))) return fail(-1, "vx_kv_rows: struct_size");
   if (rows->reserved != 0) return fail(-1, "vx_kv_rows: reserved must be 0");
+  constexpr int64_t kMax = (1ll << 31) - 1;
+  if (rows->rows < 0 || rows->rows > kMax || rows->sequences < 0 || rows->sequences > kMax) return fail(-1, "vx_kv_rows: bad shape");
+  if (!rows->row_offsets && rows->rows != rows->sequences)
+    return fail(-1, "vx_kv_rows: without row_offsets every sequence has one row (rows %lld, sequences %lld)", (long long)rows->rows, (long long)rows->sequences);
+  if (rows->table_pages < 0 || rows->table_pages > kMax / page_size) return fail(-1, "vx_kv_rows: a sequence may have up to 2^31 - 1 tokens");
+  if (rows->rows > 0 && rows->sequences > 0) {
+    if (!rows->lengths) return fail(-1, "vx_kv_rows: lengths must not be NULL");
+    if (rows->table_pages > 0 && (!rows->page_table || rows->ld_table < rows->table_pages)) return fail(-1, "vx_kv_rows: page_table NULL or its rows too short");
+  }
+  r.rows = static_cast<int32_t>(rows->rows);
+  r.sequences = static_cast<int32_t>(rows->sequences);
+  r.lengths = rows->lengths;
+  r.row_offsets = rows->row_offsets;
+  r.table = {rows->page_table, rows->ld_table, static_cast<int32_t>(rows->table_pages)};
+  return 0;
+}
+bool power_of_two(float x) {
+  int e;
+  return x >= 0x1p-32f && x <= 0x1p32f && frexpf(x, &e) == 0.5f;
+}
+}  // namespace
+
+int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c, KvRows& r) {
+  if (!cache || cache->struct_size != static_cast<int32_t>(sizeof(vx_kv_cache))) return fail(-1, "vx_kv_cache: struct_size");
   constexpr int64_t kMax = (1ll << 31) - 1;
   if (cache->page_size < 1 || cache->pages < 0 || cache->pages > kMax || cache->kv_heads < 1 || cache->kv_heads > 65535)
     return fail(-1, "vx_kv_cache: bad shape (pages %lld, page_size %d, kv_heads %d)", (long long)cache->pages, cache->page_size, cache->kv_heads);
@@ -33,23 +63,31 @@ int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c,
   for (const int64_t s : strides)
     if (s < 0 || s % 8 != 0) return fail(-1, "vx_kv_cache: strides must be multiples of 8 elements");
   if (!aligned16(cache->k) || !aligned16(cache->v)) return fail(-1, "vx_kv_cache: k and v must be 16-byte aligned");
-  if (rows->rows < 0 || rows->rows > kMax || rows->sequences < 0 || rows->sequences > kMax) return fail(-1, "vx_kv_rows: bad shape");
-  if (!rows->row_offsets && rows->rows != rows->sequences)
-    return fail(-1, "vx_kv_rows: without row_offsets every sequence has one row (rows %lld, sequences %lld)", (long long)rows->rows, (long long)rows->sequences);
-  if (rows->table_pages < 0 || rows->table_pages > kMax / cache->page_size) return fail(-1, "vx_kv_rows: a sequence may have up to 2^31 - 1 tokens");
-  if (rows->rows > 0 && rows->sequences > 0) {
-    if (!rows->lengths) return fail(-1, "vx_kv_rows: lengths must not be NULL");
-    if (rows->table_pages > 0 && (!rows->page_table || rows->ld_table < rows->table_pages)) return fail(-1, "vx_kv_rows: page_table NULL or its rows too short");
-  }
+  if (const int rc = check_rows(rows, cache->page_size, r)) return rc;
   c.k = {static_cast<__nv_bfloat16*>(cache->k), cache->k_page, cache->k_token, cache->k_head};
   c.v = {static_cast<__nv_bfloat16*>(cache->v), cache->v_page, cache->v_token, cache->v_head};
   c.page_size = FastDiv(static_cast<uint32_t>(cache->page_size));
   c.pages = static_cast<int32_t>(cache->pages);
-  r.rows = static_cast<int32_t>(rows->rows);
-  r.sequences = static_cast<int32_t>(rows->sequences);
-  r.lengths = rows->lengths;
-  r.row_offsets = rows->row_offsets;
-  r.table = {rows->page_table, rows->ld_table, static_cast<int32_t>(rows->table_pages)};
+  return 0;
+}
+
+int check_paged(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, Fp4Cache& c, KvRows& r) {
+  if (!cache || cache->struct_size != static_cast<int32_t>(sizeof(vx_kv_cache_fp4))) return fail(-1, "vx_kv_cache_fp4: struct_size");
+  constexpr int64_t kMax = (1ll << 31) - 1;
+  if (cache->page_size < 16 || cache->page_size % 16 != 0) return fail(-1, "vx_kv_cache_fp4: page_size must be a multiple of 16 (got %d)", cache->page_size);
+  if (cache->pages < 0 || cache->pages > kMax || cache->kv_heads < 1 || cache->kv_heads > 65535)
+    return fail(-1, "vx_kv_cache_fp4: bad shape (pages %lld, kv_heads %d)", (long long)cache->pages, cache->kv_heads);
+  const int D = cache->head_dim;
+  if (D < 16 || D > 256 || D % 16 != 0) return fail(-1, "head_dim must be a multiple of 16 up to 256 (got %d)", D);
+  if (cache->pages > 0 && (!cache->k || !cache->v)) return fail(-1, "vx_kv_cache_fp4: k and v must not be NULL");
+  if (!aligned16(cache->k) || !aligned16(cache->v)) return fail(-1, "vx_kv_cache_fp4: k and v must be 16-byte aligned");
+  const int64_t page = static_cast<int64_t>(cache->kv_heads) * (cache->page_size / kFp4Tokens) * kFp4Unit * D;
+  for (const int64_t s : {cache->k_page, cache->v_page})
+    if (s % 16 != 0 || s < 0 || (cache->pages > 1 && s < page)) return fail(-1, "vx_kv_cache_fp4: pages must be a multiple of 16 bytes apart, %lld or more", (long long)page);
+  if (!power_of_two(cache->k_scale) || !power_of_two(cache->v_scale)) return fail(-1, "k_scale and v_scale must be powers of two from 2^-32 to 2^32");
+  if (const int rc = check_rows(rows, cache->page_size, r)) return rc;
+  c = {static_cast<uint8_t*>(cache->k), static_cast<uint8_t*>(cache->v), cache->k_page, cache->v_page, cache->k_scale, cache->v_scale,
+       FastDiv(static_cast<uint32_t>(cache->page_size / kFp4Tokens)), static_cast<int32_t>(cache->pages)};
   return 0;
 }
 
@@ -57,11 +95,13 @@ namespace {
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_BLOCKS = 6;     // per SM, at 40 registers a thread: five of 46 take 375 us at the size above, seven or eight, which spill, 507
+constexpr int AP_BLOCKS_FP4 = 4;
 constexpr int AP_UNITS = 16;     // of a thread in large calls, since a block looks its rows up before it moves any: 4 take 422 us there, 8 391, 16 375 (of five blocks)
 constexpr int AP_MAX_ROWS = 32;  // rows of a block at most
 
 struct AppendParams {
   PagedCache cache;
+  Fp4Cache fp4;
   KvRows rows;
   const void *k, *v, *q;
   int64_t k_row, k_head, v_row, v_head, q_row, q_head;
@@ -75,12 +115,14 @@ struct AppendParams {
   int32_t half;                          // rot_dim / 2; 0: interleaved (or no rotation)
   int32_t rows_per_block;
   FastDiv units_per_row, units_per_head;
+  int32_t head_dim;
 };
 
 // where the rows of a block go
 struct RowPlace {
-  int64_t k, v;      // offset of the token's place in the cache, -1: not stored
+  int64_t k, v;      // offset of the token's place in the cache, -1: not stored; FP4: of its unit of head 0, in bytes
   int32_t position;  // -1: left out
+  int32_t token;     // FP4: of the unit
 };
 
 template <typename T>
@@ -111,15 +153,71 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Pieces of eight: the rotated values from c0 on of a key, every product and sum rounded (the bytes of a cache in 4 bits are then a function of the inputs
+// and not of how a compiler contracts them).
 template <typename T>
-__global__ void __launch_bounds__(AP_THREADS, AP_BLOCKS) kv_append_kernel(const AppendParams p) {
+__device__ __forceinline__ void rotated8(const AppendParams& p, const T* src, const float* cs, int c0, float (&x)[8]) {
+  load8(src + c0, x);
+  const int rot = 16 * p.rot_units;
+  if (c0 >= rot) return;
+  if (p.half) {
+    const bool second = c0 >= p.half;
+    float y[8], c[8], s[8];
+    load8(src + (second ? c0 - p.half : c0 + p.half), y);
+    load8(cs + (second ? c0 - p.half : c0), c);
+    load8(cs + (second ? c0 : c0 + p.half), s);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = __fmul_rn(x[j], c[j]), b = __fmul_rn(y[j], s[j]);
+      x[j] = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
+    }
+  } else {
+    const float4 c = *reinterpret_cast<const float4*>(cs + c0 / 2), s = *reinterpret_cast<const float4*>(cs + rot / 2 + c0 / 2);
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float e = x[2 * j], o = x[2 * j + 1];
+      x[2 * j] = __fsub_rn(__fmul_rn(e, cc[j]), __fmul_rn(o, ss[j]));
+      x[2 * j + 1] = __fadd_rn(__fmul_rn(o, cc[j]), __fmul_rn(e, ss[j]));
+    }
+  }
+}
+
+// Sixteen values to codes and their scale.  Divided by 16 values' scale the quotient is rounded to fp32 first: a value whose significand has 24 bits at most,
+// over a scale whose significand has 4, is a border between two codes exactly or is off it by more than half a unit, so the code is that of the
+// exact quotient.  (A quotient in the range of fp32's subnormals is far below the first border.)
+__device__ __forceinline__ uint2 quantize16(const float (&a)[8], const float (&b)[8], float inv_g, uint32_t& byte) {
+  const float most = __fmul_rn(fmaxf(amax8(a), amax8(b)), inv_g);
+  byte = __nv_cvt_float_to_fp8(__fdiv_rn(most, 6.0f), __NV_SATFINITE, __NV_E4M3) & 0x7fu;
+  const float s = e4m3_to_float(byte);
+  if (byte == 0) return make_uint2(0, 0);
+  uint32_t w[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(__fmul_rn(e ? b[j] : a[j], inv_g), s);
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(w[e])
+        : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+template <typename T, bool FP4>
+__global__ void __launch_bounds__(AP_THREADS, FP4 ? AP_BLOCKS_FP4 : AP_BLOCKS) kv_append_kernel(const __grid_constant__ AppendParams p) {
   pdl_launch_dependents();
   __shared__ RowPlace place[AP_MAX_ROWS];
   const int row0 = static_cast<int>(blockIdx.x) * p.rows_per_block;
   const int n_rows = min(p.rows_per_block, p.rows.rows - row0);
   pdl_wait();
   if (static_cast<int>(threadIdx.x) < n_rows) {
-    RowPlace pl{-1, -1, -1};
+    RowPlace pl{-1, -1, -1, 0};
     int s;
     int64_t i;
     if (row_sequence(p.rows, row0 + threadIdx.x, s, i)) {
@@ -129,11 +227,13 @@ __global__ void __launch_bounds__(AP_THREADS, AP_BLOCKS) kv_append_kernel(const 
       else if (pos >= 0 && pos < p.positions) pl.position = static_cast<int32_t>(pos);
       if (pl.position >= 0 && t < (1ll << 31)) {
         uint32_t index, slot;
-        p.cache.page_size.divmod(static_cast<uint32_t>(t), index, slot);
-        const int page = page_of(p.rows.table, s, index, p.cache.pages);
+        if (FP4) p.fp4.page_units.divmod(static_cast<uint32_t>(t) / kFp4Tokens, index, slot);
+        else p.cache.page_size.divmod(static_cast<uint32_t>(t), index, slot);
+        const int page = page_of(p.rows.table, s, index, FP4 ? p.fp4.pages : p.cache.pages);
         if (page >= 0) {
-          pl.k = page * p.cache.k.page + slot * p.cache.k.token;
-          pl.v = page * p.cache.v.page + slot * p.cache.v.token;
+          pl.k = FP4 ? page * p.fp4.k_page + static_cast<int64_t>(slot) * (kFp4Unit * p.head_dim) : page * p.cache.k.page + slot * p.cache.k.token;
+          pl.v = FP4 ? page * p.fp4.v_page + static_cast<int64_t>(slot) * (kFp4Unit * p.head_dim) : page * p.cache.v.page + slot * p.cache.v.token;
+          pl.token = static_cast<int32_t>(t % kFp4Tokens);
         }
       }
     }
@@ -151,6 +251,29 @@ __global__ void __launch_bounds__(AP_THREADS, AP_BLOCKS) kv_append_kernel(const 
     const T* src;
     __nv_bfloat16* dst;
     bool rotates = static_cast<int>(u) < p.rot_units;
+    if (FP4 && static_cast<int>(head) >= p.q_heads) {  // 16 values of a scale
+      head -= p.q_heads;
+      const bool key = static_cast<int>(head) < p.kv_heads;
+      if (!key) head -= p.kv_heads;
+      if ((key ? pl.k : pl.v) < 0) continue;
+      const int c = 16 * static_cast<int>(u), D = p.head_dim;
+      uint8_t* const at = (key ? p.fp4.k + pl.k : p.fp4.v + pl.v) + static_cast<int64_t>(head) * p.fp4.page_units.d * (kFp4Unit * D);
+      float a[8], b[8];
+      if (key) {
+        const T* const x = static_cast<const T*>(p.k) + row * p.k_row + head * p.k_head;
+        const float* const cs = p.rotary + pl.position * p.ld_rotary;
+        rotated8(p, x, cs, c, a);
+        rotated8(p, x, cs, c + 8, b);
+      } else {
+        const T* const x = static_cast<const T*>(p.v) + row * p.v_row + head * p.v_head + c;
+        load8(x, a);
+        load8(x + 8, b);
+      }
+      uint32_t byte;
+      *reinterpret_cast<uint2*>(at + pl.token * (D / 2) + c / 2) = quantize16(a, b, key ? 1.0f / p.fp4.k_scale : 1.0f / p.fp4.v_scale, byte);
+      at[8 * D + pl.token * (D / 16) + u] = static_cast<uint8_t>(byte);
+      continue;
+    }
     if (static_cast<int>(head) < p.q_heads) {
       src = static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head;
       dst = p.q_out + row * p.qo_row + head * p.qo_head;
@@ -207,17 +330,11 @@ __global__ void __launch_bounds__(AP_THREADS, AP_BLOCKS) kv_append_kernel(const 
   }
 }
 
-}  // namespace
-}  // namespace vx
-
-extern "C" int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_kv_append_desc* d, void* stream) {
-  using namespace vx;
-  AppendParams p{};
-  const int rc = check_paged(cache, rows, p.cache, p.rows);
-  if (rc) return rc;
+// What the entry points share: the rest of the parameters, the launch.  `cache` has been checked; D, kv_heads: its own.
+template <bool FP4>
+int append(AppendParams& p, const vx_kv_append_desc* d, int D, int kv_heads, void* stream) {
   if (!d || d->struct_size != static_cast<int32_t>(sizeof(vx_kv_append_desc))) return fail(-1, "vx_kv_append_desc: struct_size");
   if (d->reserved != 0) return fail(-1, "vx_kv_append_desc: reserved must be 0");
-  const int D = cache->head_dim;
   if (D < 16 || D > 256 || D % 16 != 0) return fail(-1, "head_dim must be a multiple of 16 up to 256 (got %d)", D);
   if (d->dtype != VX_F32 && d->dtype != VX_BF16) return fail(-1, "dtype must be VX_F32 or VX_BF16");
   const bool has_q = d->q != nullptr;
@@ -229,10 +346,12 @@ extern "C" int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, co
   }
   if (p.rows.rows == 0) return 0;
   if (!d->k || !d->v) return fail(-1, "k and v must not be NULL");
-  const int64_t extent[3] = {cache->pages, cache->page_size, cache->kv_heads};
-  const int64_t k_step[3] = {cache->k_page, cache->k_token, cache->k_head}, v_step[3] = {cache->v_page, cache->v_token, cache->v_head};
-  for (int i = 0; i < 3; ++i)
-    if (extent[i] > 1 && (k_step[i] < D || v_step[i] < D)) return fail(-1, "two tokens or heads of the cache in one place (stride below head_dim)");
+  if (!FP4) {
+    const int64_t extent[3] = {p.cache.pages, static_cast<int64_t>(p.cache.page_size.d), kv_heads};
+    const int64_t k_step[3] = {p.cache.k.page, p.cache.k.token, p.cache.k.head}, v_step[3] = {p.cache.v.page, p.cache.v.token, p.cache.v.head};
+    for (int i = 0; i < 3; ++i)
+      if (extent[i] > 1 && (k_step[i] < D || v_step[i] < D)) return fail(-1, "two tokens or heads of the cache in one place (stride below head_dim)");
+  }
   const int es = d->dtype == VX_F32 ? 4 : 2;
   if (!pieces_ok(d->k, d->k_row, d->k_head, es) || !pieces_ok(d->v, d->v_row, d->v_head, es) ||
       (has_q && (!pieces_ok(d->q, d->q_row, d->q_head, es) || !pieces_ok(d->q_out, d->qo_row, d->qo_head, 2))))
@@ -246,7 +365,8 @@ extern "C" int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, co
   p.positions = static_cast<int32_t>(d->positions < (1ll << 31) - 1 ? d->positions : (1ll << 31) - 1);
   p.starts = d->starts;
   p.q_heads = has_q ? d->q_heads : 0;
-  p.kv_heads = cache->kv_heads;
+  p.kv_heads = kv_heads;
+  p.head_dim = D;
   p.rot_units = d->rotary ? d->rot_dim / 16 : 0;
   p.half = d->rotary && !d->interleaved ? d->rot_dim / 2 : 0;
   p.units_per_head = FastDiv(static_cast<uint32_t>(D / 16));
@@ -261,7 +381,94 @@ extern "C" int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, co
   p.rows_per_block = static_cast<int32_t>(rpb);
   const dim3 grid(static_cast<unsigned>((p.rows.rows + rpb - 1) / rpb));
   const auto st = static_cast<cudaStream_t>(stream);
-  if (d->dtype == VX_F32) VX_CUDA_OK(launch_dependent(kv_append_kernel<float>, grid, dim3(AP_THREADS), 0, st, p));
-  else VX_CUDA_OK(launch_dependent(kv_append_kernel<__nv_bfloat16>, grid, dim3(AP_THREADS), 0, st, p));
+  if (d->dtype == VX_F32) VX_CUDA_OK(launch_dependent(kv_append_kernel<float, FP4>, grid, dim3(AP_THREADS), 0, st, p));
+  else VX_CUDA_OK(launch_dependent(kv_append_kernel<__nv_bfloat16, FP4>, grid, dim3(AP_THREADS), 0, st, p));
+  return 0;
+}
+
+// Values of a cache in 4 bits: a thread takes the 16 values of a scale, 32 bytes of the result; neighbours follow each other in a head of a token.
+struct ValuesParams {
+  const uint8_t* pages;
+  int64_t page_bytes, total;  // total: scales
+  float scale;
+  int32_t head_dim;
+  FastDiv per_head, heads, tokens;
+  __nv_bfloat16* out;
+};
+__global__ void __launch_bounds__(256) kv_values_kernel(const ValuesParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int D = p.head_dim;
+  for (int64_t n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; n < p.total; n += static_cast<int64_t>(gridDim.x) * 256) {
+    // page, token, head, scale of the head
+    const uint32_t per_token = p.per_head.d * p.heads.d;
+    const int64_t place = n / per_token;
+    uint32_t head, u, token;
+    p.per_head.divmod(static_cast<uint32_t>(n - place * per_token), head, u);
+    const int64_t page = place / p.tokens.d;
+    token = static_cast<uint32_t>(place - page * p.tokens.d);
+    const uint8_t* const unit = p.pages + page * p.page_bytes + (static_cast<int64_t>(head) * (p.tokens.d / kFp4Tokens) + token / kFp4Tokens) * (kFp4Unit * D);
+    token %= kFp4Tokens;
+    const uint2 codes = *reinterpret_cast<const uint2*>(unit + token * (D / 2) + u * 8);
+    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(e4m3_as_half(unit[8 * D + token * (D / 16) + u])))) * 256.0f * p.scale;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t two = (j < 4 ? codes.x : codes.y) >> (8 * (j & 3)) & 0xffu;
+      float v[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // (sign, two bits of exponent, one of significand: as fp16 bits the value over 2^14)
+        const uint32_t c = two >> (4 * e);
+        v[e] = __half2float(__ushort_as_half(static_cast<unsigned short>((c & 8) << 12 | (c & 7) << 9))) * 16384.0f * s;
+      }
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    uint4* const dst = reinterpret_cast<uint4*>(p.out + n * 16);
+    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+}  // namespace
+}  // namespace vx
+
+extern "C" int vx_kv_append(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_kv_append_desc* d, void* stream) {
+  using namespace vx;
+  AppendParams p{};
+  const int rc = check_paged(cache, rows, p.cache, p.rows);
+  return rc ? rc : append<false>(p, d, cache->head_dim, cache->kv_heads, stream);
+}
+
+extern "C" int vx_kv_append_fp4(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_kv_append_desc* d, void* stream) {
+  using namespace vx;
+  AppendParams p{};
+  const int rc = check_paged(cache, rows, p.fp4, p.rows);
+  return rc ? rc : append<true>(p, d, cache->head_dim, cache->kv_heads, stream);
+}
+
+extern "C" int vx_kv_values_fp4(const void* pages, int64_t n_pages, int64_t page_bytes, int page_size, int kv_heads, int head_dim, float scale, void* out,
+                                void* stream) {
+  using namespace vx;
+  vx_kv_cache_fp4 cache{};
+  cache.struct_size = sizeof(cache);
+  cache.page_size = page_size;
+  cache.pages = n_pages;
+  cache.kv_heads = kv_heads;
+  cache.head_dim = head_dim;
+  cache.k = cache.v = const_cast<void*>(pages);
+  cache.k_page = cache.v_page = page_bytes;
+  cache.k_scale = cache.v_scale = scale;
+  vx_kv_rows rows{};
+  rows.struct_size = sizeof(rows);
+  Fp4Cache c;
+  KvRows r;
+  if (const int rc = check_paged(&cache, &rows, c, r)) return rc;
+  if (n_pages == 0) return 0;
+  if (!out || !aligned16(out)) return fail(-1, "out must be 16-byte aligned");
+  ValuesParams p{c.k, page_bytes, n_pages * page_size * kv_heads * (head_dim / 16), scale, head_dim, FastDiv(static_cast<uint32_t>(head_dim / 16)),
+                 FastDiv(static_cast<uint32_t>(kv_heads)), FastDiv(static_cast<uint32_t>(page_size)), static_cast<__nv_bfloat16*>(out)};
+  const int64_t blocks = (p.total + 255) / 256, most = 16 * static_cast<int64_t>(sm_count());
+  VX_CUDA_OK(launch_dependent(kv_values_kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
   return 0;
 }

@@ -105,8 +105,23 @@ __device__ __forceinline__ int page_of(const PagedTable& t, int owner, uint32_t 
   return page >= 0 && page < pages ? page : -1;
 }
 
+// A cache in 4 bits: bytes of its pages, units of 16 tokens of a head (kFp4Unit bytes per value of a token).
+struct Fp4Cache {
+  uint8_t *k, *v;
+  int64_t k_page, v_page;
+  float k_scale, v_scale;
+  FastDiv page_units;   // units of a head per page
+  int32_t pages;
+};
+constexpr int kFp4Tokens = 16, kFp4Unit = 9;  // of a unit; bytes per value of a token: eight of codes, one of scales
+
+// The value of an E4M3 scale byte over 256 as fp16: its exponent and significand where fp16 has them (exponents differ by 7 - 15), subnormals
+// included.  The sign bit is dropped; 0x7f gives 480 / 256.
+__device__ __forceinline__ uint32_t e4m3_as_half(uint32_t byte) { return (byte & 0x7fu) << 7; }
+
 // Checks of the descriptors that both entry points make; 0 or an error code.
 int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c, KvRows& r);
+int check_paged(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, Fp4Cache& c, KvRows& r);
 // Element strides and address of a bf16 / fp32 operand whose 16-byte pieces are read whole.
 inline bool pieces_ok(const void* p, int64_t a, int64_t b, int elem) { return aligned16(p) && a * elem % 16 == 0 && b * elem % 16 == 0; }
 // A result [rows, heads, head_dim] whose rows or heads lie in one place.

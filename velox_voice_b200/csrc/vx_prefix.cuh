@@ -20,7 +20,8 @@
 namespace vx {
 
 struct PrefixParams {
-  PagedCache cache;
+  PagedCache cache;               // (a cache in 4 bits: page size and number of pages only)
+  Fp4Cache fp4;
   KvRows rows;
   const __nv_bfloat16* q;
   int64_t q_row, q_head;
@@ -32,7 +33,8 @@ struct PrefixParams {
   const int32_t* group_offsets;
   PagedTable prefix;
   const int32_t* prefix_lengths;
-  float scale2;                   // scale log2(e)
+  float scale2;                   // scale log2(e); a cache in 4 bits: times 256 k_scale, see e4m3_as_half
+  float v_factor;                 // of a cache in 4 bits: 256 v_scale
   float2* part_ml;                // [parts][rows][q_heads]
   float* part_o;                  // [parts][rows][q_heads][head_dim]
   int* status;
@@ -212,6 +214,19 @@ __device__ __forceinline__ bool find_tile(const PrefixParams& p, const Span& sp,
 // Not 0 if one of the two bf16 values of a word is an infinity or NaN, gathered in `sum` (0 x is 0 or NaN).
 __device__ __forceinline__ void note_not_finite(uint32_t& sum, uint32_t two) { asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(two), "r"(0u)); }
 __device__ __forceinline__ bool any_not_finite(uint32_t sum) { return (sum & 0x7fff7fffu) != 0; }
+
+// What the kernels for few rows walk.
+struct RowsParams {
+  PrefixParams p;
+  Span span[2];
+  int32_t warps[2];      // of a CTA per item of the span: 1, 2 or 4
+  int32_t first_blocks;  // CTAs of span[0]; those of span[1] follow
+  int32_t beside;        // the launch in front is the tile kernel of this call, see prefix_rows_kernel
+};
+constexpr int PR_WARPS = 4;
+// Launches prefix_rows_fp4_kernel with `blocks` CTAs of RB blocks of eight rows.
+int launch_rows_fp4(const RowsParams& rp, int head_dim, int rb, int64_t blocks, void* stream);
+int rows_fp4_ctas(int rb, int head_dim);  // per SM
 
 // Launches prefix_tiles_kernel on the spans that have chunks.
 constexpr int kSlotRows = 128;  // rows of a slot of prefix_tiles_kernel

@@ -30,6 +30,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "vx_common.cuh"
 #include "vx_prefix.cuh"
@@ -38,19 +39,9 @@
 namespace vx {
 namespace {
 
-constexpr int PR_WARPS = 4;
-
 // CTAs of prefix_rows_kernel per SM, as many as its registers allow: what a CTA needs before and behind its keys passes under the others'
 // keys.  (16 groups of ten hypotheses, head_dim 64: over 64 frames 8.5 us with 2 or 3, 6.7 with 4, over 1,000 16 with any, over 3,750 37.5, 37.5 and 33.6.)
 constexpr int rows_ctas(int blocks, int head_dim) { return head_dim == 64 ? 4 : (blocks == 2 ? 2 : 3); }
-
-struct RowsParams {
-  PrefixParams p;
-  Span span[2];
-  int32_t warps[2];      // of a CTA per item of the span: 1, 2 or 4
-  int32_t first_blocks;  // CTAs of span[0]; those of span[1] follow
-  int32_t beside;        // the launch in front is the tile kernel of this call, see below
-};
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -615,10 +606,21 @@ int tile_chunk_keys(int64_t capacity, int64_t items, int64_t streams, int64_t un
   return static_cast<int>(best);
 }
 
-int64_t rows_resident(int blocks, int head_dim) { return static_cast<int64_t>(rows_ctas(blocks, head_dim)) * sm_count(); }
+int64_t rows_resident(int blocks, int head_dim, bool fp4) { return static_cast<int64_t>(fp4 ? rows_fp4_ctas(blocks, head_dim) : rows_ctas(blocks, head_dim)) * sm_count(); }
 
-int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, PrefixParams& p, Plan& plan) {
-  const int rc = check_paged(cache, rows, p.cache, p.rows);
+int check_cache(const vx_kv_cache* cache, const vx_kv_rows* rows, PrefixParams& p) { return check_paged(cache, rows, p.cache, p.rows); }
+int check_cache(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, PrefixParams& p) {
+  const int rc = check_paged(cache, rows, p.fp4, p.rows);
+  if (rc) return rc;
+  p.cache.page_size = FastDiv(static_cast<uint32_t>(cache->page_size));
+  p.cache.pages = p.fp4.pages;
+  return 0;
+}
+
+template <class Cache>
+int check_prefix(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, PrefixParams& p, Plan& plan) {
+  constexpr bool FP4 = std::is_same<Cache, vx_kv_cache_fp4>::value;
+  const int rc = check_cache(cache, rows, p);
   if (rc) return rc;
   if (!d || d->struct_size != static_cast<int32_t>(sizeof(vx_prefix_attention_desc))) return fail(-1, "vx_prefix_attention_desc: struct_size");
   if (d->reserved != 0) return fail(-1, "vx_prefix_attention_desc: reserved must be 0");
@@ -635,7 +637,9 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
       return fail(-1, "prefix_lengths or prefix_table is NULL, or its rows are too short");
   }
   p.scale2 = d->scale * 1.4426950408889634f;
-  if (!(d->scale > 0.0f) || !(p.scale2 < INFINITY)) return fail(-1, "scale must be positive and finite, scale log2(e) too");
+  if (FP4) p.scale2 *= 256.0f * p.fp4.k_scale;
+  p.v_factor = FP4 ? 256.0f * p.fp4.v_scale : 1.0f;
+  if (!(d->scale > 0.0f) || !(p.scale2 < INFINITY)) return fail(-1, FP4 ? "scale must be positive and finite, 256 scale k_scale log2(e) too" : "scale must be positive and finite, scale log2(e) too");
   const int per = d->q_heads / cache->kv_heads;
   p.q_heads = d->q_heads;
   p.kv_heads = cache->kv_heads;
@@ -668,10 +672,16 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
       const bool paired = kernel == Plan::kPairs;
       sp.chunk = tile_chunk_keys(cap, n, paired ? sms : 2 * sms, paired ? 256 : 128, paired && cache->head_dim == 64 ? 1.4 : 2.0, cache->head_dim, R * d->q_heads, kind == kSpanJoint);
     }
-    else sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim), 16 * PR_WARPS, cache->head_dim == 64 ? 1024 : 256, 3);
+    else sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim, FP4), 16 * PR_WARPS, cache->head_dim == 64 ? 1024 : 256, 3);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
-  if (rows_o > kSlotRows) {
+  if (FP4) {
+    plan.kernel[0] = plan.kernel[1] = Plan::kRows;
+    plan.blocks = rows_p > 8 || rows_o > 8 ? 2 : 1;
+    cut(plan.span[0], kSpanPrefix, plan.kernel[0], G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
+    cut(plan.span[1], kSpanOwn, plan.kernel[1], S, cap_o, single ? per : 0);
+    plan.span[1].part0 = plan.span[0].chunks;
+  } else if (rows_o > kSlotRows) {
     // Whole prompts or long chunks: prefix and own tokens in a row, no joining of the two, but a walk of the prefix per sequence.  8 key heads,
     // prompts without a history, the two apart (prefix by groups) against in a row, in us:
     //   head_dim 64    130 rows  4 sequences, one prefix of 1,000 keys 42 : 26   of 8,000 62 : 54     64 sequences, 1,000 133 : 120   8,000 349 : 514
@@ -720,19 +730,16 @@ int check_prefix(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_pref
   return 0;
 }
 
-}  // namespace
-}  // namespace vx
-
-extern "C" int64_t vx_prefix_attention_scratch(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
-  using namespace vx;
+template <class Cache>
+int64_t scratch_bytes(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
   PrefixParams p{};
   Plan plan;
   const int rc = check_prefix(cache, rows, d, p, plan);
   return rc ? rc : plan.bytes;
 }
 
-extern "C" int vx_prefix_attention_launches(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
-  using namespace vx;
+template <class Cache>
+int launches(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
   PrefixParams p{};
   Plan plan;
   const int rc = check_prefix(cache, rows, d, p, plan);
@@ -742,8 +749,9 @@ extern "C" int vx_prefix_attention_launches(const vx_kv_cache* cache, const vx_k
   return n;
 }
 
-extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, void* stream) {
-  using namespace vx;
+template <class Cache>
+int attention(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, void* stream) {
+  constexpr bool FP4 = std::is_same<Cache, vx_kv_cache_fp4>::value;
   PrefixParams p{};
   Plan plan;
   const int rc = check_prefix(cache, rows, d, p, plan);
@@ -774,16 +782,39 @@ extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* r
       const int64_t items = static_cast<int64_t>(sp.slots) * sp.chunks * p.kv_heads;
       // All four warps of a CTA on an item while one round of CTAs takes them all, else so many that each has about 128 keys: twice as many take
       // 28 us for 27 (64 hypotheses of 102 to 198 tokens, four utterances of 1,005 to 1,792 frames) and 37 for 32 (124 of 30 to 60 tokens), half as many 29 and 32.
-      rp.warps[i] = items <= rows_resident(plan.blocks, cache->head_dim) || sp.chunk > 256 ? 4 : (sp.chunk > 128 ? 2 : 1);
+      rp.warps[i] = items <= rows_resident(plan.blocks, cache->head_dim, FP4) || sp.chunk > 256 ? 4 : (sp.chunk > 128 ? 2 : 1);
       blocks += (items * rp.warps[i] + PR_WARPS - 1) / PR_WARPS;
       if (i == 0) rp.first_blocks = static_cast<int32_t>(blocks);
     }
     if (blocks >= (1ll << 31)) return fail(-1, "too much work for one call (%lld blocks)", (long long)blocks);
-    const int e = d64 ? (plan.blocks == 2 ? launch_rows<64, 2>(rp, blocks, st) : launch_rows<64, 1>(rp, blocks, st))
+    const int e = FP4 ? launch_rows_fp4(rp, cache->head_dim, plan.blocks, blocks, stream)
+                  : d64 ? (plan.blocks == 2 ? launch_rows<64, 2>(rp, blocks, st) : launch_rows<64, 1>(rp, blocks, st))
                       : (plan.blocks == 2 ? launch_rows<128, 2>(rp, blocks, st) : launch_rows<128, 1>(rp, blocks, st));
     if (e) return e;
   }
   JoinParams jp{p, {plan.span[0], plan.span[1]}, plan.parts == 0 && plan.span[0].part0 >= 0 ? 1 : 0};
   VX_CUDA_OK(d64 ? launch_join<64>(jp, plan.parts, st) : launch_join<128>(jp, plan.parts, st));
   return 0;
+}
+
+}  // namespace
+}  // namespace vx
+
+extern "C" int64_t vx_prefix_attention_scratch(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
+  return vx::scratch_bytes(cache, rows, d);
+}
+extern "C" int vx_prefix_attention_launches(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
+  return vx::launches(cache, rows, d);
+}
+extern "C" int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, void* stream) {
+  return vx::attention(cache, rows, d, stream);
+}
+extern "C" int64_t vx_prefix_attention_fp4_scratch(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
+  return vx::scratch_bytes(cache, rows, d);
+}
+extern "C" int vx_prefix_attention_fp4_launches(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d) {
+  return vx::launches(cache, rows, d);
+}
+extern "C" int vx_prefix_attention_fp4(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* d, void* stream) {
+  return vx::attention(cache, rows, d, stream);
 }

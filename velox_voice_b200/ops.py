@@ -18,6 +18,7 @@ Everything runs on torch's current CUDA stream; nothing synchronises; there is n
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -764,7 +765,42 @@ def _in_pieces(t: torch.Tensor) -> bool:
             and all(_step(t, i) * e % 16 == 0 for i in range(t.dim() - 1)))
 
 
-def _kv_cache(k_pages: torch.Tensor, v_pages: torch.Tensor):
+def fp4_pages(pages: int, page_size: int, kv_heads: int, head_dim: int, *, device="cuda") -> torch.Tensor:
+    """Pages of keys or of values in 4 bits for :func:`kv_append` and :func:`prefix_attention`, zeros: u8 [pages, kv_heads, page_size / 16,
+    9 head_dim].  The last dimension is a unit of 16 tokens of a head: ``codes [16, head_dim / 2]`` (two E2M1 values a byte, the even one in the
+    low half), then ``scales [16, head_dim / 16]`` (E4M3, one for 16 values of a token): 4.5 bits a value.  page_size and head_dim multiples of 16."""
+    if pages < 0 or kv_heads < 1 or page_size < 16 or page_size % 16 != 0 or head_dim % 16 != 0 or not 16 <= head_dim <= 256:
+        raise ValueError(f"pages of 16 n tokens and heads of 16 n values up to 256 wanted, got {pages} of {page_size} tokens, {kv_heads} heads of {head_dim}")
+    return torch.zeros((pages, kv_heads, page_size // 16, 9 * head_dim), dtype=torch.uint8, device=device)
+
+
+def _fp4_tensor(t, name: str) -> None:
+    _require_cuda(t, name)
+    if t.dtype != torch.uint8 or t.dim() != 4 or t.shape[3] % 144 != 0 or not 144 <= t.shape[3] <= 2304 or t.shape[1] < 1 or t.shape[2] < 1:
+        raise ValueError(f"{name} must be uint8 [pages, kv_heads, page_size / 16, 9 head_dim], got {t.dtype} {tuple(t.shape)}")
+    page = t[0].numel() if t.shape[0] else 0
+    if t.data_ptr() % 16 != 0 or (t.shape[0] and not t[0].is_contiguous()) or _step(t, 0) % 16 != 0 or (t.shape[0] > 1 and t.stride(0) < page):
+        raise ValueError(f"{name} must have contiguous pages at 16-byte aligned addresses (strides {t.stride()})")
+
+
+def _power_of_two(x: float, name: str) -> float:
+    x = float(x)
+    if not 2.0 ** -32 <= x <= 2.0 ** 32 or math.frexp(x)[0] != 0.5:
+        raise ValueError(f"{name} must be a power of two from 2^-32 to 2^32, got {x}")
+    return x
+
+
+def _kv_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: float = 1.0, v_scale: float = 1.0):
+    if isinstance(k_pages, torch.Tensor) and k_pages.dtype == torch.uint8:
+        _fp4_tensor(k_pages, "k_pages")
+        _fp4_tensor(v_pages, "v_pages")
+        if v_pages.shape != k_pages.shape or v_pages.device != k_pages.device:
+            raise ValueError("k_pages and v_pages must be uint8 tensors of one shape on one device")
+        pages, heads, units, unit = k_pages.shape
+        return _lib.KvCacheFp4(C.sizeof(_lib.KvCacheFp4), 16 * units, pages, heads, unit // 9, k_pages.data_ptr(), v_pages.data_ptr(), _step(k_pages, 0),
+                               _step(v_pages, 0), _power_of_two(k_scale, "k_scale"), _power_of_two(v_scale, "v_scale"))
+    if k_scale != 1.0 or v_scale != 1.0:
+        raise ValueError("k_scale and v_scale belong to pages in 4 bits")
     for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         _require_cuda(t, n)
         if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape != k_pages.shape or t.device != k_pages.device:
@@ -793,13 +829,13 @@ def _kv_rows(rows: int, page_table, lengths, row_offsets, dev):
     return d, (page_table, lengths, row_offsets)
 
 
-def _heads3d(t, name: str, rows, heads, k_pages, dtypes) -> torch.Tensor:
+def _heads3d(t, name: str, rows, heads, dim, dev, dtypes) -> torch.Tensor:
     """[rows, heads, head_dim] operand on the cache's device; copied where its rows are not at 16-byte addresses."""
     _require_cuda(t, name)
-    if t.device != k_pages.device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {k_pages.device}")
-    if t.dim() != 3 or t.shape[2] != k_pages.shape[3] or (rows is not None and t.shape[0] != rows) or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {k_pages.shape[3]}], got {tuple(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    if t.dim() != 3 or t.shape[2] != dim or (rows is not None and t.shape[0] != rows) or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
     return t if _in_pieces(t) else t.clone(memory_format=torch.contiguous_format)
@@ -808,7 +844,7 @@ def _heads3d(t, name: str, rows, heads, k_pages, dtypes) -> torch.Tensor:
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
               lengths: torch.Tensor, *, q: Optional[torch.Tensor] = None, rotary: Optional[torch.Tensor] = None,
               interleaved: bool = False, row_offsets: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
-              q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+              q_out: Optional[torch.Tensor] = None, k_scale: float = 1.0, v_scale: float = 1.0) -> Optional[torch.Tensor]:
     """Keys and values of new tokens into their pages, rotated by position on the way, and the queries rotated with them
     (``vx_kv_append``, one launch).  Returns the rotated queries bf16 [rows, heads, head_dim] (None without ``q``).
 
@@ -821,22 +857,26 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
 
     Left out, with zero queries: rows of no sequence, of one of negative length, at a position that the table does not have.  Not
     stored: tokens whose page is not there (an entry outside [0, pages), or none).  ``lengths`` stays as it is: the same call of
-    :func:`prefix_attention` takes it, and the program then moves it on."""
-    r = (_native or _host()).kv_append(k, v, k_pages, v_pages, page_table, lengths, q, rotary, interleaved, row_offsets, starts, q_out)
+    :func:`prefix_attention` takes it, and the program then moves it on.
+
+    Pages in 4 bits (:func:`fp4_pages`): keys, once rotated, and values are quantized.  Of 16 values of a token, the scale is the E4M3 number nearest to
+    a sixth of the largest (at most 448), a code the E2M1 number (up to 6) nearest to value / scale, ties to even codes (``vx_kv_append_fp4``).
+    ``k_scale`` and ``v_scale``, powers of two, stand in front of all keys and all values: 1 serves values whose largest of 16 is between 0.1 and 2688."""
+    r = (_native or _host()).kv_append(k, v, k_pages, v_pages, page_table, lengths, q, rotary, interleaved, row_offsets, starts, q_out, k_scale, v_scale)
     if r is not None:
         return None if r is True else r
-    cache = _kv_cache(k_pages, v_pages)
-    dev, kv = k_pages.device, k_pages.shape[2]
+    cache = _kv_cache(k_pages, v_pages, k_scale, v_scale)
+    dev, kv, dim = k_pages.device, cache.kv_heads, cache.head_dim
     kinds = (torch.float32, torch.bfloat16)
-    k = _heads3d(k, "k", None, kv, k_pages, kinds)
+    k = _heads3d(k, "k", None, kv, dim, dev, kinds)
     rows = k.shape[0]
-    v = _heads3d(v, "v", rows, kv, k_pages, (k.dtype,))
+    v = _heads3d(v, "v", rows, kv, dim, dev, (k.dtype,))
     d = _lib.KvAppendDesc(struct_size=C.sizeof(_lib.KvAppendDesc), dtype=_dt(k, "k"))
     d.k, d.k_row, d.k_head = k.data_ptr(), _step(k, 0), _step(k, 1)
     d.v, d.v_row, d.v_head = v.data_ptr(), _step(v, 0), _step(v, 1)
     if q is not None:
         given = q
-        q = _heads3d(q, "q", rows, None, k_pages, (k.dtype,))
+        q = _heads3d(q, "q", rows, None, dim, dev, (k.dtype,))
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
         else:
@@ -864,16 +904,38 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     if starts is not None:
         starts = _int32_on(starts, "starts", (r.sequences,), dev)
         d.starts = starts.data_ptr()
-    _lib.check(_lib.load().vx_kv_append(C.byref(cache), C.byref(r), C.byref(d), _stream()), "vx_kv_append")
+    name = "vx_kv_append_fp4" if isinstance(cache, _lib.KvCacheFp4) else "vx_kv_append"
+    _lib.check(getattr(_lib.load(), name)(C.byref(cache), C.byref(r), C.byref(d), _stream()), name)
     _count(1 if rows else 0)
     del keep
     return q_out
 
 
+def kv_values(pages: torch.Tensor, scale: float = 1.0, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What pages in 4 bits (:func:`fp4_pages`) stand for, exactly: bf16 [pages, page_size, kv_heads, head_dim], the form of a bf16 cache
+    (``vx_kv_values_fp4``, one launch).  ``scale``: the ``k_scale`` or ``v_scale`` that they were written with."""
+    r = (_native or _host()).kv_values(pages, scale, out)
+    if r is not None:
+        return r
+    _fp4_tensor(pages, "pages")
+    n, heads, units, unit = pages.shape
+    scale = _power_of_two(scale, "scale")
+    shape = (n, 16 * units, heads, unit // 9)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=pages.device)
+    else:
+        _require_cuda(out, "out")
+        if out.dtype != torch.bfloat16 or tuple(out.shape) != shape or out.device != pages.device or not out.is_contiguous() or out.data_ptr() % 16 != 0:
+            raise ValueError(f"out must be contiguous bfloat16 {list(shape)} at a 16-byte aligned address")
+    _lib.check(_lib.load().vx_kv_values_fp4(pages.data_ptr(), n, _step(pages, 0), 16 * units, heads, unit // 9, scale, out.data_ptr(), _stream()), "vx_kv_values_fp4")
+    _count(1 if n else 0)
+    return out
+
+
 def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                      prefix_table: Optional[torch.Tensor] = None, prefix_lengths: Optional[torch.Tensor] = None, *,
                      row_offsets: Optional[torch.Tensor] = None, group_offsets: Optional[torch.Tensor] = None,
-                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None, k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
     """Attention of new tokens over a prefix that the sequences of a group share and read together (whole prompts: one by one), and
     over their own tokens (``vx_prefix_attention``).  q bf16 [rows, heads, head_dim] -> bf16 [rows, heads, head_dim]; heads a
     multiple of kv_heads, head_dim 64 or 128.
@@ -883,14 +945,16 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     [0, prefix_lengths[g]) of the pages ``prefix_table[g]`` (int32 [groups, pages]).  ``group_offsets`` int32 [groups + 1]: sequences
     [o_g, o_{g+1}) are group g; without it the groups are of one size.  Without ``prefix_table`` there is no prefix.  Keys on pages
     that are not there (entries outside [0, pages)) are not attended; a row that has no key, or whose sequence has a negative
-    length, gets zeros.  ``scale``: positive, head_dim ** -0.5 unless given."""
+    length, gets zeros.  ``scale``: positive, head_dim ** -0.5 unless given.
+
+    Pages in 4 bits (:func:`fp4_pages`, ``k_scale`` and ``v_scale`` those of :func:`kv_append`) are read as they are (``vx_prefix_attention_fp4``)."""
     r = (_native or _host()).prefix_attention(q, k_pages, v_pages, page_table, lengths, prefix_table, prefix_lengths, row_offsets, group_offsets,
-                                              scale, out)
+                                              scale, out, k_scale, v_scale)
     if r is not None:
         return r
-    cache = _kv_cache(k_pages, v_pages)
-    dev, kv, dim = k_pages.device, k_pages.shape[2], k_pages.shape[3]
-    q = _heads3d(q, "q", None, None, k_pages, (torch.bfloat16,))
+    cache = _kv_cache(k_pages, v_pages, k_scale, v_scale)
+    dev, kv, dim = k_pages.device, cache.kv_heads, cache.head_dim
+    q = _heads3d(q, "q", None, None, dim, dev, (torch.bfloat16,))
     if dim not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {dim}")
     rows, heads = q.shape[0], q.shape[1]
@@ -921,13 +985,14 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
             raise ValueError("out must be bfloat16 of q's shape with contiguous heads at 16-byte aligned addresses")
     d.out, d.o_row, d.o_head = out.data_ptr(), _step(out, 0), _step(out, 1)
     lib = _lib.load()
-    size = int(lib.vx_prefix_attention_scratch(C.byref(cache), C.byref(r), C.byref(d)))
+    name = "vx_prefix_attention_fp4" if isinstance(cache, _lib.KvCacheFp4) else "vx_prefix_attention"
+    size = int(getattr(lib, name + "_scratch")(C.byref(cache), C.byref(r), C.byref(d)))
     if size < 0:
-        _lib.check(size, "vx_prefix_attention")
+        _lib.check(size, name)
     scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     d.scratch, d.scratch_bytes = _ptr(scratch), size
-    _lib.check(lib.vx_prefix_attention(C.byref(cache), C.byref(r), C.byref(d), _stream()), "vx_prefix_attention")
-    _count(int(lib.vx_prefix_attention_launches(C.byref(cache), C.byref(r), C.byref(d))))
+    _lib.check(getattr(lib, name)(C.byref(cache), C.byref(r), C.byref(d), _stream()), name)
+    _count(int(getattr(lib, name + "_launches")(C.byref(cache), C.byref(r), C.byref(d))))
     del keep, prefix_table, prefix_lengths, group_offsets
     return out
 
