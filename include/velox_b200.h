@@ -481,6 +481,41 @@ int64_t vx_prefix_attention_fp4_scratch(const vx_kv_cache_fp4* cache, const vx_k
 int vx_prefix_attention_fp4_launches(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
 int vx_prefix_attention_fp4(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc, void* stream);
 
+/* Drafted tokens against the target's probabilities, as a drafted decoding step ends: which drafts stand, and the token behind them.
+ * Sequence s has rows [o_s, o_{s+1}) (row_offsets as in vx_kv_rows; NULL: one row each, so nothing drafted): row r's logits are the target's for the token behind
+ * ids[r], which for all rows but a sequence's last is the draft d = ids[r + 1].  With p = softmax(logits[r] / temperature) and q = softmax(draft_logits[r] /
+ * temperature) (NULL: the drafter was sure, q is 1 at d), row after row:
+ *   the draft stands where uniforms[r][0] q(d) < p(d);
+ *   at the first that does not, next is drawn from max(p - q, 0), behind the last draft from p: the first token v with
+ *   sum_{u <= v} w_u > uniforms[r][1] sum_u w_u, w those weights (p where max(p - q, 0) is 0 everywhere).
+ * temperature 0: a draft stands where it is the first of the largest logits, next is that of its row.
+ * accepted i32 [sequences]: drafts that stand; next i32 [sequences], -1 where the row has no finite logit, or one that is NaN or +infinity, or the
+ * drafter's row where it counts (such a row's draft does not stand either), or where the sequence has no row.  An id outside [0, vocab) does not stand.  Logits of -infinity have probability 0.
+ * What decides is computed in 64 bits, or in 32 where a bound of their error leaves no doubt; probabilities below 2^-1020 count as 0.  Rows behind the last
+ * sequence are not looked at. */
+typedef struct {
+  int32_t struct_size; /* sizeof(vx_verify_desc) */
+  int32_t dtype;       /* of logits and draft_logits: VX_F32 or VX_BF16 */
+  int64_t rows, vocab, sequences; /* vocab: 1 to 2^24 */
+  const void* logits;       /* [rows][vocab], row stride in elements */
+  int64_t ld_logits;
+  const void* draft_logits; /* the same, or NULL */
+  int64_t ld_draft;
+  const void* ids;          /* [rows], i32 or i64 */
+  int32_t ids_bytes;        /* 4 or 8 */
+  int32_t reserved;         /* 0 */
+  const float* uniforms;    /* [rows][2], in [0, 1) */
+  const int32_t* row_offsets;
+  double temperature;       /* 0, or 2^-20 to 2^20 */
+  int32_t* accepted;
+  int32_t* next;
+  void* scratch;            /* vx_verify_drafts_scratch bytes, 16-byte aligned */
+  int64_t scratch_bytes;
+} vx_verify_desc;
+int64_t vx_verify_drafts_scratch(int64_t rows);
+/* Two launches (none without sequences). */
+int vx_verify_drafts(const vx_verify_desc* desc, void* stream);
+
 /* Block-scaled FP4 GEMM for callers that cannot allocate device memory.  (No counterpart in
  * the reference: its Python wrappers allocate through torch.)
  *

@@ -83,6 +83,8 @@ EXPORTS = (
     "vx_prefix_attention_fp4",
     "vx_prefix_attention_fp4_scratch",
     "vx_prefix_attention_fp4_launches",
+    "vx_verify_drafts",
+    "vx_verify_drafts_scratch",
 )
 
 
@@ -240,6 +242,32 @@ class PrefixAttentionDesc(C.Structure):
     ]
 
 
+class VerifyDesc(C.Structure):
+    """``vx_verify_desc``."""
+
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("dtype", C.c_int32),
+        ("rows", C.c_int64),
+        ("vocab", C.c_int64),
+        ("sequences", C.c_int64),
+        ("logits", C.c_void_p),
+        ("ld_logits", C.c_int64),
+        ("draft_logits", C.c_void_p),
+        ("ld_draft", C.c_int64),
+        ("ids", C.c_void_p),
+        ("ids_bytes", C.c_int32),
+        ("reserved", C.c_int32),
+        ("uniforms", C.c_void_p),
+        ("row_offsets", C.c_void_p),
+        ("temperature", C.c_double),
+        ("accepted", C.c_void_p),
+        ("next", C.c_void_p),
+        ("scratch", C.c_void_p),
+        ("scratch_bytes", C.c_int64),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -351,6 +379,10 @@ def load(build_if_missing: bool = True) -> C.CDLL:
         lib.vx_prefix_attention_fp4_launches.argtypes = [C.POINTER(KvCacheFp4), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc)]
         lib.vx_prefix_attention_fp4.restype = i32
         lib.vx_prefix_attention_fp4.argtypes = [C.POINTER(KvCacheFp4), C.POINTER(KvRows), C.POINTER(PrefixAttentionDesc), vp]
+        lib.vx_verify_drafts_scratch.restype = i64
+        lib.vx_verify_drafts_scratch.argtypes = [i64]
+        lib.vx_verify_drafts.restype = i32
+        lib.vx_verify_drafts.argtypes = [C.POINTER(VerifyDesc), vp]
         lib.vx_ctc_topk_threshold.restype = i32
         lib.vx_ctc_topk_threshold.argtypes = [vp, i64, i64, i32, vp, vp]
         lib.vx_ctc_topk_finish.restype = i32

@@ -19,7 +19,7 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libvelox_b200.so")
 STAMP = os.path.join(LIB_DIR, "libvelox_b200.stamp")
 SOURCES = ("vx_api.cu", "vx_quant.cu", "vx_gemm.cu", "vx_noalloc.cu", "vx_pack.cu", "vx_mel.cu", "vx_attn.cu", "vx_gemm_ln.cu", "vx_pass.cu", "vx_topk.cu", "vx_rowscale.cu",
-           "vx_kv_append.cu", "vx_prefix_attn.cu", "vx_prefix_tiles.cu", "vx_prefix_fp4.cu")
+           "vx_kv_append.cu", "vx_prefix_attn.cu", "vx_prefix_tiles.cu", "vx_prefix_fp4.cu", "vx_verify.cu")
 # native host path of the Python operators: a CPython extension against torch's headers (g++, no device code)
 HOST_SOURCE = "vx_host.cpp"
 HOST_PATH = os.path.join(LIB_DIR, "_vx_host.so")

@@ -12,6 +12,7 @@
 // The C-ABI entry points are taken from the library that ctypes loaded (init(path)); nothing is linked against it.
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Dtype.h>
@@ -33,7 +34,8 @@ namespace {
   X(vx_bsgemm_natural_sf_supported) X(vx_bsgemm_residual_ln_supported) X(vx_bsgemm_residual_ln) X(vx_bsgemm_residual_ln2) X(vx_argmax_ids) X(vx_relpos_attention)   \
   X(vx_power_mel_log) X(vx_power_mel_log_supported) X(vx_sf_from_natural_pair) X(vx_rowscale_linear) X(vx_rowscale_linear_scratch) X(vx_ctc_topk_rows) X(vx_ctc_topk)        \
   X(vx_conformer_pass_supported) X(vx_conformer_pass_scratch) X(vx_conformer_pass) X(vx_kv_append) X(vx_prefix_attention) X(vx_prefix_attention_scratch) X(vx_prefix_attention_launches)        \
-  X(vx_kv_append_fp4) X(vx_kv_values_fp4) X(vx_prefix_attention_fp4) X(vx_prefix_attention_fp4_scratch) X(vx_prefix_attention_fp4_launches)
+  X(vx_kv_append_fp4) X(vx_kv_values_fp4) X(vx_prefix_attention_fp4) X(vx_prefix_attention_fp4_scratch) X(vx_prefix_attention_fp4_launches)        \
+  X(vx_verify_drafts) X(vx_verify_drafts_scratch)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   VX_FUNCS(X)
@@ -1401,6 +1403,62 @@ PyObject* py_kv_values(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
   VX_END
 }
 
+// logits [rows, vocab], rows in a row and apart
+bool logits_arg(PyObject* o, const at::Tensor** t) {
+  if (!is_cuda_tensor(o)) return false;
+  const at::Tensor& x = THPVariable_Unpack(o);
+  *t = &x;
+  return dtype_code(x) >= 0 && x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= (1 << 24) && (x.size(1) == 1 || x.stride(1) == 1) && rows_apart(x);
+}
+// verify_drafts(logits, ids, uniforms, draft_logits | None, row_offsets | None, temperature) -> (accepted, next) | None
+PyObject* py_verify_drafts(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
+  VX_BEGIN
+  VX_ARGS(6)
+  const at::Tensor *x, *y = nullptr, *o = nullptr;
+  if (!logits_arg(p[0], &x) || !is_cuda_tensor(p[1]) || !is_cuda_tensor(p[2]) || !PyFloat_CheckExact(p[5])) Py_RETURN_NONE;
+  const at::Device dev = x->device();
+  if (p[3] != Py_None && (!logits_arg(p[3], &y) || y->sizes() != x->sizes() || y->scalar_type() != x->scalar_type() || y->device() != dev)) Py_RETURN_NONE;
+  const at::Tensor &ids = THPVariable_Unpack(p[1]), &u = THPVariable_Unpack(p[2]);
+  const int64_t rows = x->size(0);
+  if (ids.device() != dev || ids.dim() != 1 || ids.size(0) != rows || !ids.is_contiguous() || (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong)) Py_RETURN_NONE;
+  if (u.device() != dev || u.dim() != 2 || u.size(0) != rows || u.size(1) != 2 || !u.is_contiguous() || u.scalar_type() != at::kFloat ||
+      (reinterpret_cast<uintptr_t>(u.data_ptr()) & 7) != 0)
+    Py_RETURN_NONE;
+  if (p[4] != Py_None && (!int32_arg(p[4], -1, -1, 1, dev, &o) || o->size(0) < 1)) Py_RETURN_NONE;
+  const double t = PyFloat_AS_DOUBLE(p[5]);
+  if (!(t == 0.0 || (t >= 0x1p-20 && t <= 0x1p20))) Py_RETURN_NONE;
+  vx_verify_desc d{};
+  d.struct_size = sizeof(d);
+  d.dtype = dtype_code(*x);
+  d.rows = rows; d.vocab = x->size(1); d.sequences = o ? o->size(0) - 1 : rows;
+  d.logits = x->data_ptr(); d.ld_logits = rows > 1 ? x->stride(0) : d.vocab;
+  if (y) { d.draft_logits = y->data_ptr(); d.ld_draft = rows > 1 ? y->stride(0) : d.vocab; }
+  d.ids = ids.data_ptr(); d.ids_bytes = static_cast<int>(ids.element_size());
+  d.uniforms = static_cast<const float*>(u.data_ptr());
+  d.row_offsets = o ? int32_ptr(*o) : nullptr;
+  d.temperature = t;
+  at::Tensor accepted, next, scratch;
+  {
+    NoGil nogil;
+    const c10::cuda::CUDAGuard on(dev);
+    accepted = empty({d.sequences}, at::kInt, dev);
+    next = empty({d.sequences}, at::kInt, dev);
+    d.scratch_bytes = g.vx_verify_drafts_scratch(rows);
+    scratch = empty({d.scratch_bytes}, at::kByte, dev);
+    d.accepted = static_cast<int32_t*>(accepted.data_ptr());
+    d.next = static_cast<int32_t*>(next.data_ptr());
+    d.scratch = scratch.data_ptr();
+    check(g.vx_verify_drafts(&d, stream()), "vx_verify_drafts");
+    count(d.sequences == 0 ? 0 : (rows == 0 ? 1 : 2));
+  }
+  PyObject* const r = PyTuple_New(2);
+  if (!r) throw PyFail{};
+  PyTuple_SET_ITEM(r, 0, wrap(accepted));
+  PyTuple_SET_ITEM(r, 1, wrap(next));
+  return r;
+  VX_END
+}
+
 // init(library path, VeloxError, Quantized)
 PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   VX_ARGS(3)
@@ -1441,6 +1499,7 @@ PyMethodDef kMethods[] = {
     VX_METHOD("kv_append", py_kv_append),
     VX_METHOD("prefix_attention", py_prefix_attention),
     VX_METHOD("kv_values", py_kv_values),
+    VX_METHOD("verify_drafts", py_verify_drafts),
     VX_METHOD("stack_plan", py_stack_plan),
     VX_METHOD("stack_plan_current", py_stack_plan_current),
     VX_METHOD("stack_forward", py_stack_forward),

@@ -3,8 +3,9 @@
 Two layers:
 
 * the library's own operators -- :func:`quantize`, :func:`ln_quantize`, :func:`layernorm`,
-  :func:`bsgemm` -- which carry every format and fused epilogue, and the paged cache of a decoder behind the
-  encoder -- :func:`kv_append`, :func:`prefix_attention`;
+  :func:`bsgemm` -- which carry every format and fused epilogue, and those of a decoder behind the encoder: its paged
+  cache -- :func:`kv_append`, :func:`prefix_attention`, in 4 bits :func:`fp4_pages`, :func:`kv_values` -- and its
+  drafts -- :func:`verify_drafts`;
 * the reference's operator names with the reference's signatures
   (``veloxvoice/kernels/ops/triton_ops.py`` and ``veloxvoice/kernels/ops/cuda_ops.py``):
   :func:`per_row_col_quantize`, :func:`triton_quantize_w`, :func:`mxfp4_block_quantize`,
@@ -995,6 +996,65 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     _count(int(getattr(lib, name + "_launches")(C.byref(cache), C.byref(r), C.byref(d))))
     del keep, prefix_table, prefix_lengths, group_offsets
     return out
+
+
+def _rows_of_logits(t, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    _require_cuda(t, name)
+    _dt(t, name)
+    if t.dim() != 2 or t.shape[1] < 1 or t.shape[1] > 2 ** 24:
+        raise ValueError(f"{name} must be [rows, vocab] with a vocabulary of 1 to 2^24, got {tuple(t.shape)}")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must be as logits are: {like.dtype} {tuple(like.shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    ok = (t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+    return t if ok else t.contiguous()
+
+
+def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, uniforms: torch.Tensor, *, draft_logits: Optional[torch.Tensor] = None,
+                  row_offsets: Optional[torch.Tensor] = None, temperature: float = 1.0):
+    """Drafted tokens against the target's probabilities, from given random numbers (``vx_verify_drafts``, two launches): (accepted, next),
+    int32 [sequences] each -- how many drafts of a sequence stand, and the token behind them.
+
+    logits bf16 or f32 [rows, vocab]: rows [o_s, o_{s+1}) (``row_offsets`` int32 [sequences + 1]; without it a row each, and no drafts) are sequence s's; row r's
+    are the target's for the token behind ids[r] (``ids`` int32 or int64 [rows]: the last certain token, then the drafts, as they went into the model).
+    draft_logits: the drafter's, laid out the same (a sequence's last row is not read), or None: it was sure of its drafts.  ``uniforms`` f32 [rows, 2] in
+    [0, 1).  With p and q their softmax at ``temperature``: the draft d of row r stands where uniforms[r, 0] q(d) < p(d); at the first that does
+    not, ``next`` is drawn from max(p - q, 0), behind the last draft from p, by uniforms[r, 1]: the first token whose cumulated weight is above that share of all.
+    temperature 0: a draft stands where it is the first of the largest logits, and ``next`` is that.
+
+    Token logits of -infinity are possible, rows with NaN, +infinity or nothing finite end a sequence's drafts with ``next`` -1, as does a sequence without rows."""
+    r = (_native or _host()).verify_drafts(logits, ids, uniforms, draft_logits, row_offsets, temperature)
+    if r is not None:
+        return r
+    logits = _rows_of_logits(logits, "logits")
+    dev, rows = logits.device, logits.shape[0]
+    if draft_logits is not None:
+        draft_logits = _rows_of_logits(draft_logits, "draft_logits", logits)
+    for t, n, shape, kinds in ((ids, "ids", (rows,), (torch.int32, torch.int64)), (uniforms, "uniforms", (rows, 2), (torch.float32,))):
+        _require_cuda(t, n)
+        if t.device != dev or tuple(t.shape) != shape or t.dtype not in kinds:
+            raise ValueError(f"{n} must be {' or '.join(map(str, kinds))} {list(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    ids, uniforms = ids.contiguous(), uniforms.contiguous()
+    if uniforms.data_ptr() % 8 != 0:
+        uniforms = uniforms.clone()
+    if row_offsets is not None:
+        row_offsets = _int32_on(row_offsets, "row_offsets", (None,), dev)
+        if row_offsets.shape[0] < 1:
+            raise ValueError("row_offsets must have sequences + 1 entries, got none")
+    sequences = rows if row_offsets is None else row_offsets.shape[0] - 1
+    temperature = float(temperature)
+    if not (temperature == 0.0 or 2.0 ** -20 <= temperature <= 2.0 ** 20):
+        raise ValueError(f"temperature must be 0 or from 2^-20 to 2^20, got {temperature}")
+    lib = _lib.load()
+    accepted, follows = torch.empty(sequences, dtype=torch.int32, device=dev), torch.empty(sequences, dtype=torch.int32, device=dev)
+    size = int(lib.vx_verify_drafts_scratch(rows))
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+    d = _lib.VerifyDesc(C.sizeof(_lib.VerifyDesc), _dt(logits, "logits"), rows, logits.shape[1], sequences, _ptr(logits), logits.stride(0) if rows > 1 else logits.shape[1],
+                        _ptr(draft_logits), 0 if draft_logits is None else (draft_logits.stride(0) if rows > 1 else logits.shape[1]), _ptr(ids), ids.element_size(), 0,
+                        _ptr(uniforms), _ptr(row_offsets), temperature, _ptr(accepted), _ptr(follows), _ptr(scratch), size)
+    with torch.cuda.device(dev):
+        _lib.check(lib.vx_verify_drafts(C.byref(d), _stream()), "vx_verify_drafts")
+    _count(0 if sequences == 0 else (1 if rows == 0 else 2))
+    return accepted, follows
 
 
 # ======================================================================================
