@@ -230,6 +230,6 @@ int rows_fp4_ctas(int rb, int head_dim);  // per SM
 
 // Launches prefix_tiles_kernel on the spans that have chunks.
 constexpr int kSlotRows = 128;  // rows of a slot of prefix_tiles_kernel
-int launch_prefix_tiles(const PrefixParams& p, int head_dim, bool paired, const Span& first, const Span& second, void* stream);
+int launch_prefix_tiles(const PrefixParams& p, int head_dim, bool paired, bool fp4, const Span& first, const Span& second, void* stream);
 
 }  // namespace vx

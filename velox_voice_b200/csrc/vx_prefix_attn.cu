@@ -675,13 +675,7 @@ int check_prefix(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_att
     else sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim, FP4), 16 * PR_WARPS, cache->head_dim == 64 ? 1024 : 256, 3);
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
-  if (FP4) {
-    plan.kernel[0] = plan.kernel[1] = Plan::kRows;
-    plan.blocks = rows_p > 8 || rows_o > 8 ? 2 : 1;
-    cut(plan.span[0], kSpanPrefix, plan.kernel[0], G, cap_p, single && p.group_size > 0 ? static_cast<int64_t>(p.group_size) * per : 0);
-    cut(plan.span[1], kSpanOwn, plan.kernel[1], S, cap_o, single ? per : 0);
-    plan.span[1].part0 = plan.span[0].chunks;
-  } else if (rows_o > kSlotRows) {
+  if (rows_o > kSlotRows) {
     // Whole prompts or long chunks: prefix and own tokens in a row, no joining of the two, but a walk of the prefix per sequence.  8 key heads,
     // prompts without a history, the two apart (prefix by groups) against in a row, in us:
     //   head_dim 64    130 rows  4 sequences, one prefix of 1,000 keys 42 : 26   of 8,000 62 : 54     64 sequences, 1,000 133 : 120   8,000 349 : 514
@@ -771,7 +765,7 @@ int attention(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attent
   p.status = device_status_ptr();
   for (const Plan::Kernel k : {Plan::kPairs, Plan::kTiles})
     if (plan.walks(k)) {
-      const int e = launch_prefix_tiles(p, cache->head_dim, k == Plan::kPairs, plan.part(k, 0), plan.part(k, 1), stream);
+      const int e = launch_prefix_tiles(p, cache->head_dim, k == Plan::kPairs, FP4, plan.part(k, 0), plan.part(k, 1), stream);
       if (e) return e;
     }
   if (plan.walks(Plan::kRows)) {

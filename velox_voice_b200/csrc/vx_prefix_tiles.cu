@@ -39,6 +39,7 @@
 // Every wait on a barrier is bounded.
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -59,7 +60,7 @@ constexpr int PT_ITEMS = 4;                // items of a stream that are known a
 constexpr int PT_Q_PANEL = kSlotRows * 128;  // 64 bf16 of every row
 constexpr uint32_t PT_TM_SLOT = 256, PT_TM_O = 128, PT_TM_COLS = 512;
 
-template <int D, bool PAIRED>
+template <int D, bool PAIRED, bool FP4>
 struct TileShape {
   static constexpr int kKeys = PAIRED ? 128 : 64;
   static constexpr int kBuffers = PAIRED ? 1 : 2;             // of S
@@ -67,13 +68,17 @@ struct TileShape {
   static constexpr int kTile = D / 64 * kPanel;               // bytes of a K or V tile
   static constexpr int kQ = D / 64 * PT_Q_PANEL;              // of a slot's queries
   static constexpr int kStreams = PAIRED ? 1 : 2;
-  static constexpr int kParts = PAIRED ? 4 : 1;               // loaders that share a tile
+  static constexpr int kParts = PAIRED ? (FP4 ? 2 : 4) : 1;   // loaders that share a tile (FP4: of K, of V)
   // P of a tile handed over in halves, so that the products of the first run under the exponentials of the second.  Gains where the products are
   // short (16 utterances of 3,116 to 5,510 frames, 9,894 tokens of 66 prompts, head_dim 64: 363 -> 339 us) and loses where an issuer that waits for the
   // second half keeps the other slot's products waiting (6,906 tokens of four prompts behind 16,384, head_dim 128: 1,710 -> 1,755).
   static constexpr bool kHalves = PAIRED && D == 64;
-  static constexpr int kStagesK = D == 128 ? 3 : 5, kStagesV = D == 128 ? 2 : 5;  // of a stream
-  static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + 1024;
+  static constexpr int kStagesK = FP4 ? (D == 128 ? 2 : 3) : (D == 128 ? 3 : 5);  // of a stream
+  static constexpr int kStagesV = FP4 ? (D == 128 ? (PAIRED ? 2 : 1) : 3) : (D == 128 ? 2 : 5);
+  // FP4: tiles of a loader (64 keys or values of them) that are on their way as they lie in the cache, 4 units each
+  static constexpr int kRaw = FP4 ? (D == 128 && PAIRED ? 1 : 3) : 0;
+  static constexpr int kRawTile = 4 * kFp4Unit * D;
+  static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + 4 * kRaw * kRawTile + 1024;
 };
 
 struct TilesParams {
@@ -98,14 +103,15 @@ struct TileBarriers {
   uint64_t p_half[2];  // kHalves: the first half of a tile's P
   uint64_t s_full[2][Shape::kBuffers], p_full[2][Shape::kBuffers], pv_done[2][Shape::kBuffers], q_full[2], q_empty[2];
   uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
+  uint64_t raw_full[4][Shape::kRaw > 0 ? Shape::kRaw : 1];
   alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
   TileItem item[2][PT_ITEMS];
   uint32_t tmem_base;
 };
 
-// bf16 x bf16 -> fp32, A K-major; B K-major or MN-major (b_mn)
-__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+// bf16 x bf16 (or fp16 x fp16) -> fp32, A K-major; B K-major or MN-major (b_mn)
+__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn, bool f16 = false) {
+  return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 __device__ __forceinline__ void mma_bf16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -136,6 +142,34 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+// Eight codes times their scale (fp16 twice, over 256), exactly: as fp16, or as bf16
+template <bool BF16>
+__device__ __forceinline__ void codes_as_16(uint32_t w, uint32_t scale, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(scale));
+    if (BF16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      h[j] = pack_bf16(f.x, f.y);
+    }
+  }
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 // A whole 32-byte sector from one lane: lanes write rows of their own.
 __device__ __forceinline__ void store32(float* dst, const uint32_t* v) {
@@ -272,9 +306,145 @@ __device__ __noinline__ void put_back(const float* o, uint32_t o_tmem) {
   tc_wait_st_all();
 }
 
+// The loaders of a cache in 4 bits: a warp has the keys or the values of its stream, 64 of a tile.  It fetches units as they lie in the cache (a bulk copy each, up
+// to kRaw of its tiles ahead and across items) and writes them as the products read them: keys in bf16, as the queries are, values in fp16, both over 256.
+// A lane takes 32 values, 16 bytes; at head_dim 128 the lanes of the second panel take their halves the other way round, so that eight
+// lanes write to eight different 16-byte columns.  Units that are not there are written as zeros.
 template <int D, bool PAIRED>
+__device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarriers<TileShape<D, PAIRED, true>>& bar, uint8_t* k_ring, uint8_t* v_ring, uint8_t* raw) {
+  using Shape = TileShape<D, PAIRED, true>;
+  constexpr unsigned ALL = 0xffffffffu;
+  constexpr int BN = Shape::kKeys, STREAMS = Shape::kStreams, PARTS = Shape::kParts, RAW = Shape::kRaw, UNIT = kFp4Unit * D, UNITS = 4;
+  const int loader = (threadIdx.x >> 5) - 8, lane = threadIdx.x & 31;
+  const int stream = loader / (4 / STREAMS), local = loader % (4 / STREAMS), part = local % PARTS;
+  const bool values = local >= PARTS;
+  const int stages = values ? Shape::kStagesV : Shape::kStagesK;
+  uint64_t* const full = values ? bar.v_full[stream] : bar.k_full[stream];
+  uint64_t* const empty = values ? bar.v_empty[stream] : bar.k_empty[stream];
+  const uint32_t ring = smem_u32(values ? v_ring : k_ring) + stream * stages * Shape::kTile + part * 64 * 128;
+  const uint8_t* const cache = values ? p.fp4.v : p.fp4.k;
+  const int64_t page_bytes = values ? p.fp4.v_page : p.fp4.k_page;
+  uint64_t* const raw_full = bar.raw_full[loader];
+
+  // the tile that is fetched next: tile `tile` of the item t
+  TileItem t;
+  t.tiles = 0;
+  int at = 0, tile = -1;
+  uint32_t item_phase = 0;
+  bool ended = false, ok = true;
+  auto advance = [&](bool wait) {  // false: not known yet (or the end)
+    if (tile + 1 < t.tiles) {
+      ++tile;
+      return true;
+    }
+    if (ended) return false;
+    const bool there = wait ? mbar_wait_spin(&bar.item_full[stream][at], item_phase, p.status, 57) : mbar_poll(&bar.item_full[stream][at], item_phase);
+    if (!__all_sync(ALL, there)) {
+      if (wait) ok = false;
+      return false;
+    }
+    t = bar.item[stream][at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar.item_empty[stream][at]);
+    if (++at == PT_ITEMS) { at = 0; item_phase ^= 1; }
+    tile = 0;
+    ended = t.tiles == 0;
+    return !ended;
+  };
+  int n_of[RAW], there_of[RAW];  // of the tiles on their way: keys of this lane's unit, which units are there
+  int fetched = 0, done = 0;
+  // where a lane reads a unit and writes it
+  constexpr int LANES = D / 32, TOKENS = 32 / LANES, PIECES = 16 / TOKENS;  // lanes of a token, tokens of a piece
+  const int c = lane % LANES, token = lane / LANES, turned = c >> 1;
+  const uint32_t raw_at = smem_u32(raw);
+  while (ok) {
+    while (fetched - done < RAW && advance(fetched == done)) {
+      const int v = t.v0 + tile * BN;
+      const bool own = v >= t.p128;
+      const int j = v - (own ? t.p128 : 0) + part * 64 + 16 * lane, end = own ? t.o_keys : t.p_keys;
+      const int n = lane < UNITS ? min(max(end - j, 0), 16) : 0;
+      const PagedTable& table = own ? p.rows.table : p.prefix;
+      int page = -1;
+      uint32_t rest = 0;
+      if (n > 0) {
+        uint32_t index;
+        p.fp4.page_units.divmod(static_cast<uint32_t>(j) / kFp4Tokens, index, rest);
+        page = page_of(table, own ? t.sequence : t.group, index, p.cache.pages);
+      }
+      const uint32_t there = __ballot_sync(ALL, page >= 0);
+      const int slot = fetched % RAW;
+      if (lane == 0) mbar_expect_tx(&raw_full[slot], __popc(there) * UNIT);
+      __syncwarp();
+      if (page >= 0)
+        bulk_load(raw + slot * Shape::kRawTile + lane * UNIT, cache + page * page_bytes + (static_cast<int64_t>(t.head) * p.fp4.page_units.d + rest) * UNIT, UNIT, &raw_full[slot]);
+      // (a queue in registers: the tiles before it are its first entries)
+#pragma unroll
+      for (int e = 0; e < RAW; ++e)
+        if (e == fetched - done) {
+          n_of[e] = page >= 0 ? n : 0;
+          there_of[e] = static_cast<int>(there);
+        }
+      ++fetched;
+    }
+    if (!ok || fetched == done) break;
+    const int m = done, stage = m % stages, slot = m % RAW;
+    ok = __all_sync(ALL, mbar_wait(&empty[stage], (m / stages + 1) & 1, p.status, 58) && mbar_wait(&raw_full[slot], (m / RAW) & 1, p.status, 59));
+    if (!ok) break;
+    const uint32_t src = raw_at + slot * Shape::kRawTile, dst = ring + stage * Shape::kTile;
+#pragma unroll 1
+    for (int u = 0; u < UNITS; ++u) {
+      const bool there = (there_of[0] >> u) & 1;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int key = i * TOKENS + token;  // of the unit
+        const uint32_t from = src + u * UNIT + key * (D / 2) + c * 16, scales = src + u * UNIT + 8 * D + key * (D / 16) + c * 2;
+        const uint32_t to = dst + (c >> 1) * Shape::kPanel + (u * 16 + key) * 128;
+        uint32_t w[4] = {0, 0, 0, 0}, two = 0;
+        if (there) {
+          if constexpr (D == 128) {
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from + 8 * turned) : "memory");
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[2]), "=r"(w[3]) : "r"(from + 8 * (1 - turned)) : "memory");
+          } else {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+          }
+          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(two) : "r"(scales) : "memory");
+        }
+        const int swap = D == 128 ? turned : 0;
+        const uint32_t s0 = (__byte_perm(two, 0, swap ? 0x4141 : 0x4040) << 7) & 0x3f803f80u, s1 = (__byte_perm(two, 0, swap ? 0x4040 : 0x4141) << 7) & 0x3f803f80u;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t h[4];
+          if (values) codes_as_16<false>(w[x], x < 2 ? s0 : s1, h);
+          else codes_as_16<true>(w[x], x < 2 ? s0 : s1, h);
+          const int column = (c & 1) * 4 + (x ^ (2 * swap));
+          st_shared16(to + ((column ^ (key & 7)) << 4), h);
+        }
+      }
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(&full[stage]);
+    if (!values) {
+      // (the softmax has read the mask PT_MASKS tiles of the stream before this one, see load of the other cache)
+      uint16_t* const mask = bar.mask[stream][m % PT_MASKS] + part * UNITS;
+      if (lane < UNITS) mask[lane] = static_cast<uint16_t>(low_bits(n_of[0]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.mask_full[stream][m % PT_MASKS]);
+    }
+    __syncwarp();  // every lane has read the slot: it is filled again
+    ++done;
+#pragma unroll
+    for (int e = 0; e + 1 < RAW; ++e) {
+      n_of[e] = n_of[e + 1];
+      there_of[e] = there_of[e + 1];
+    }
+  }
+  // (copies on their way after a limit ran out: each is waited for, with a limit)
+  for (; done < fetched; ++done) mbar_wait(&raw_full[done % RAW], (done / RAW) & 1, p.status, 59);
+}
+
+template <int D, bool PAIRED, bool FP4>
 __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __grid_constant__ TilesParams tp) {
-  using Shape = TileShape<D, PAIRED>;
+  using Shape = TileShape<D, PAIRED, FP4>;
   constexpr int BN = Shape::kKeys, NB = Shape::kBuffers, NK = Shape::kStagesK, NV = Shape::kStagesV;
   constexpr int STREAMS = PAIRED ? 1 : 2;
   constexpr unsigned ALL = 0xffffffffu;
@@ -282,6 +452,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   uint8_t* const q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* const k_ring = q_s + 2 * Shape::kQ;
   uint8_t* const v_ring = k_ring + STREAMS * NK * Shape::kTile;
+  uint8_t* const raw_ring = v_ring + STREAMS * NV * Shape::kTile;
   __shared__ TileBarriers<Shape> bar;
   const PrefixParams& p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -303,6 +474,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       mbar_init(&bar.q_empty[s], 1);
       mbar_init(&bar.p_half[s], 4);
     }
+    if (FP4 && lane < 2 * Shape::kRaw) mbar_init(&bar.raw_full[0][0] + s * 2 * Shape::kRaw + lane, 1);
     if (s < STREAMS && lane < NK) {
       mbar_init(&bar.k_full[s][lane], 32 * Shape::kParts);  // threads of the loaders that share a tile
       mbar_init(&bar.k_empty[s][lane], 1);
@@ -344,6 +516,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   if (warp >= 8 && warp < 12) {
     // =========================== loaders ===========================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - SOFTMAX_REGS));
+    if constexpr (FP4) {
+      load_fp4_tiles<D, PAIRED>(p, bar, k_ring, v_ring, raw_ring + (warp - 8) * Shape::kRaw * Shape::kRawTile);
+    } else {
     constexpr int PARTS = Shape::kParts, TEAM = 4 / STREAMS / PARTS;  // loaders that share a tile, that take tiles in turn
     constexpr int MINE = BN / PARTS, GROUPS = MINE / 16, PER_LANE = MINE / 32;
     const int stream = (warp - 8) / (4 / STREAMS), part = (warp - 8) % PARTS, rank = (warp - 8) / PARTS % TEAM;
@@ -474,6 +649,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     }
     if (PAIRED && ok && first > 0) load_v(first - 1, v_due);
     cp_async_wait_all();
+    }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - SOFTMAX_REGS));
     if (warp == 12 || (warp == 15 && !PAIRED)) {
@@ -483,7 +659,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       // Descriptors: the low word is the shared address >> 4 and, for V (MN-major), the distance of its panels of 64 columns above bit 16; the
       // high word has the distance of 8-row groups, version and swizzle.  Low words come out of a shuffle, so that the compiler knows
       // them to be the same in all lanes and forms the descriptors in uniform registers.
-      const uint32_t idesc_s = idesc_bf16(128, BN, false), idesc_o = idesc_bf16(128, D, true);
+      const uint32_t idesc_s = idesc_bf16(128, BN, false), idesc_o = idesc_bf16(128, D, true, FP4);
       const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
       auto desc = [&](uint32_t lo) { return (static_cast<uint64_t>(desc_hi) << 32) | lo; };
       const uint32_t q_lo = smem_u32(q_s) >> 4, k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
@@ -820,7 +996,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             x0 = ex2(x0);
             x1 = ex2(x1);
             sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], pack_f32x2(x0, x1));
-            pk[e >> 1] = pack_bf16(x0, x1);
+            pk[e >> 1] = FP4 ? pack_f16(x0, x1) : pack_bf16(x0, x1);
           }
           tc_st_x16(tb + 16 * i, pk);  // over S, which is in registers
           if (Shape::kHalves && !LATE && i == W / 2 - 1) {
@@ -835,7 +1011,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         unpack_f32x2(sum[1], b0, b1);
         l += (a0 + a1) + (b0 + b1);
         tc_wait_st_all();
-        if (LATE) {
+        if (LATE && !FP4) {  // (a cache in 4 bits holds finite values only)
           ok = __all_sync(ALL, mbar_wait(&bar.v_full[stream][mk % NV], (mk / NV) & 1, p.status, 54));
           if (!ok) return;
           const uint8_t* const values = v_ring + (stream * NV + mk % NV) * Shape::kTile;
@@ -879,13 +1055,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           uint32_t o[32];
           tc_ld_32x32b_x32(tm + PT_TM_O + 32 * i, o);
           tc_wait_ld();
+          if (FP4) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * p.v_factor);
+          }
           if (there) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) store32(p.part_o + at * D + 32 * i + 8 * e, &o[8 * e]);
           }
         }
       } else {
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l != 0.0f ? (FP4 ? p.v_factor : 1.0f) / l : 0.0f;
         __nv_bfloat16* const dst = p.out + row * p.o_row + qh * p.o_head;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -914,32 +1094,36 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
   }
 }
 
-template <int D, bool PAIRED>
+template <int D, bool PAIRED, bool FP4>
 int launch(const TilesParams& tp, int64_t items, cudaStream_t st) {  // `items`: at most
   int dev = 0;
   VX_CUDA_OK(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_done{0};
   const bool cached = dev >= 0 && dev < 64;
   if (!cached || !(attr_done.load(std::memory_order_acquire) & (1ull << dev))) {
-    VX_CUDA_OK(cudaFuncSetAttribute(prefix_tiles_kernel<D, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<D, PAIRED>::kSmem));
+    VX_CUDA_OK(cudaFuncSetAttribute(prefix_tiles_kernel<D, PAIRED, FP4>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<D, PAIRED, FP4>::kSmem));
     if (cached) attr_done.fetch_or(1ull << dev, std::memory_order_release);
   }
   const int64_t ctas = PAIRED ? items : (items + 1) / 2;
-  VX_CUDA_OK(launch_dependent(prefix_tiles_kernel<D, PAIRED>, dim3(static_cast<unsigned>(ctas < sm_count() ? ctas : sm_count())), dim3(PT_THREADS),
-                              TileShape<D, PAIRED>::kSmem, st, tp));
+  VX_CUDA_OK(launch_dependent(prefix_tiles_kernel<D, PAIRED, FP4>, dim3(static_cast<unsigned>(ctas < sm_count() ? ctas : sm_count())), dim3(PT_THREADS),
+                              TileShape<D, PAIRED, FP4>::kSmem, st, tp));
   return 0;
 }
 
 }  // namespace
 
-int launch_prefix_tiles(const PrefixParams& p, int head_dim, bool paired, const Span& a, const Span& b, void* stream) {
+int launch_prefix_tiles(const PrefixParams& p, int head_dim, bool paired, bool fp4, const Span& a, const Span& b, void* stream) {
   const TilesParams tp{p, {a, b}};
   const int64_t first = static_cast<int64_t>(a.slots) * a.chunks * p.kv_heads;
   const int64_t items = first + static_cast<int64_t>(b.slots) * b.chunks * p.kv_heads;
   if (items >= (1ll << 31)) return fail(-1, "too much work for one call (%lld items)", (long long)items);
   const auto st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 64) return paired ? launch<64, true>(tp, items, st) : launch<64, false>(tp, items, st);
-  return paired ? launch<128, true>(tp, items, st) : launch<128, false>(tp, items, st);
+  if (fp4) {
+    if (head_dim == 64) return paired ? launch<64, true, true>(tp, items, st) : launch<64, false, true>(tp, items, st);
+    return paired ? launch<128, true, true>(tp, items, st) : launch<128, false, true>(tp, items, st);
+  }
+  if (head_dim == 64) return paired ? launch<64, true, false>(tp, items, st) : launch<64, false, false>(tp, items, st);
+  return paired ? launch<128, true, false>(tp, items, st) : launch<128, false, false>(tp, items, st);
 }
 
 }  // namespace vx
