@@ -104,6 +104,7 @@ struct TileBarriers {
   uint64_t s_full[2][Shape::kBuffers], p_full[2][Shape::kBuffers], pv_done[2][Shape::kBuffers], q_full[2], q_empty[2];
   uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
   uint64_t raw_full[4][Shape::kRaw > 0 ? Shape::kRaw : 1];
+  float q_scale[Shape::kRaw > 0 ? 2 : 1][PT_ITEMS][Shape::kRaw > 0 ? kSlotRows : 1];  // FP4: factors of the scores of a slot's rows, by the place of their item
   alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
   TileItem item[2][PT_ITEMS];
   uint32_t tmem_base;
@@ -148,9 +149,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
   return r;
 }
-// Eight codes times their scale (fp16 twice, over 256), exactly: as fp16, or as bf16
-template <bool BF16>
-__device__ __forceinline__ void codes_as_16(uint32_t w, uint32_t scale, uint32_t (&h)[4]) {
+// Eight codes times their scale (fp16 twice, over 256), exactly
+__device__ __forceinline__ void codes_as_half(uint32_t w, uint32_t scale, uint32_t (&h)[4]) {
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
       "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
@@ -160,13 +160,7 @@ __device__ __forceinline__ void codes_as_16(uint32_t w, uint32_t scale, uint32_t
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
       : "r"(w));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(scale));
-    if (BF16) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-      h[j] = pack_bf16(f.x, f.y);
-    }
-  }
+  for (int j = 0; j < 4; ++j) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(scale));
 }
 __device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t (&v)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
@@ -307,7 +301,8 @@ __device__ __noinline__ void put_back(const float* o, uint32_t o_tmem) {
 }
 
 // The loaders of a cache in 4 bits: a warp has the keys or the values of its stream, 64 of a tile.  It fetches units as they lie in the cache (a bulk copy each, up
-// to kRaw of its tiles ahead and across items) and writes them as the products read them: keys in bf16, as the queries are, values in fp16, both over 256.
+// to kRaw of its tiles ahead and across items) and writes them as the products read them, in fp16 over 256, which is exact.  (Keys in bf16, as the queries
+// come: three more instructions for two values, and the loader of the keys was the bound: 127 us for 80 over an hour of prefix.)
 // A lane takes 32 values, 16 bytes; at head_dim 128 the lanes of the second panel take their halves the other way round, so that eight
 // lanes write to eight different 16-byte columns.  Units that are not there are written as zeros.
 template <int D, bool PAIRED>
@@ -332,6 +327,22 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
   int at = 0, tile = -1;
   uint32_t item_phase = 0;
   bool ended = false, ok = true;
+  // Where a lane's unit (of lanes 0 to 3) of tile x is: table entry as it stands there, place on the page, keys.  Asked for a tile ahead within an item.
+  int entry = -1, n = 0;
+  uint32_t rest = 0;
+  auto look_up = [&](int x) {
+    const int v = t.v0 + x * BN;
+    const bool own = v >= t.p128;
+    const int j = v - (own ? t.p128 : 0) + part * 64 + 16 * lane, end = own ? t.o_keys : t.p_keys;
+    n = lane < UNITS && x < t.tiles ? min(max(end - j, 0), 16) : 0;
+    entry = -1;
+    if (n > 0) {
+      const PagedTable& table = own ? p.rows.table : p.prefix;
+      uint32_t index;
+      p.fp4.page_units.divmod(static_cast<uint32_t>(j) / kFp4Tokens, index, rest);
+      entry = table.table[static_cast<int64_t>(own ? t.sequence : t.group) * table.ld + index];  // (keys end where the table does)
+    }
+  };
   auto advance = [&](bool wait) {  // false: not known yet (or the end)
     if (tile + 1 < t.tiles) {
       ++tile;
@@ -349,34 +360,27 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
     if (++at == PT_ITEMS) { at = 0; item_phase ^= 1; }
     tile = 0;
     ended = t.tiles == 0;
+    look_up(0);
     return !ended;
   };
   int n_of[RAW], there_of[RAW];  // of the tiles on their way: keys of this lane's unit, which units are there
-  int fetched = 0, done = 0;
+  int fetched = 0, done = 0, fetch_slot = 0, stage = 0, slot = 0;
+  uint32_t stage_phase = 1, slot_phase = 0;
   // where a lane reads a unit and writes it
   constexpr int LANES = D / 32, TOKENS = 32 / LANES, PIECES = 16 / TOKENS;  // lanes of a token, tokens of a piece
-  const int c = lane % LANES, token = lane / LANES, turned = c >> 1;
-  const uint32_t raw_at = smem_u32(raw);
+  const int c = lane % LANES, token = lane / LANES, turned = D == 128 ? c >> 1 : 0;
+  const uint32_t raw_at = smem_u32(raw) + token * (D / 2) + c * 16 + 8 * turned, scale_at = smem_u32(raw) + 8 * D + token * (D / 16) + c * 2;
+  const uint32_t low = turned ? 0x4141 : 0x4040, high = turned ? 0x4040 : 0x4141;
+  const uint32_t to_at = ring + (c >> 1) * Shape::kPanel + token * 128;
   while (ok) {
     while (fetched - done < RAW && advance(fetched == done)) {
-      const int v = t.v0 + tile * BN;
-      const bool own = v >= t.p128;
-      const int j = v - (own ? t.p128 : 0) + part * 64 + 16 * lane, end = own ? t.o_keys : t.p_keys;
-      const int n = lane < UNITS ? min(max(end - j, 0), 16) : 0;
-      const PagedTable& table = own ? p.rows.table : p.prefix;
-      int page = -1;
-      uint32_t rest = 0;
-      if (n > 0) {
-        uint32_t index;
-        p.fp4.page_units.divmod(static_cast<uint32_t>(j) / kFp4Tokens, index, rest);
-        page = page_of(table, own ? t.sequence : t.group, index, p.cache.pages);
-      }
+      const int page = entry >= 0 && entry < p.cache.pages ? entry : -1;
       const uint32_t there = __ballot_sync(ALL, page >= 0);
-      const int slot = fetched % RAW;
-      if (lane == 0) mbar_expect_tx(&raw_full[slot], __popc(there) * UNIT);
+      if (lane == 0) mbar_expect_tx(&raw_full[fetch_slot], __popc(there) * UNIT);
       __syncwarp();
       if (page >= 0)
-        bulk_load(raw + slot * Shape::kRawTile + lane * UNIT, cache + page * page_bytes + (static_cast<int64_t>(t.head) * p.fp4.page_units.d + rest) * UNIT, UNIT, &raw_full[slot]);
+        bulk_load(raw + fetch_slot * Shape::kRawTile + lane * UNIT, cache + page * page_bytes + (static_cast<int64_t>(t.head) * p.fp4.page_units.d + rest) * UNIT, UNIT,
+                  &raw_full[fetch_slot]);
       // (a queue in registers: the tiles before it are its first entries)
 #pragma unroll
       for (int e = 0; e < RAW; ++e)
@@ -385,53 +389,62 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
           there_of[e] = static_cast<int>(there);
         }
       ++fetched;
+      if (++fetch_slot == RAW) fetch_slot = 0;
+      look_up(tile + 1);
     }
     if (!ok || fetched == done) break;
-    const int m = done, stage = m % stages, slot = m % RAW;
-    ok = __all_sync(ALL, mbar_wait(&empty[stage], (m / stages + 1) & 1, p.status, 58) && mbar_wait(&raw_full[slot], (m / RAW) & 1, p.status, 59));
+    ok = __all_sync(ALL, mbar_wait(&raw_full[slot], slot_phase, p.status, 59) && mbar_wait(&empty[stage], stage_phase, p.status, 58));
     if (!ok) break;
-    const uint32_t src = raw_at + slot * Shape::kRawTile, dst = ring + stage * Shape::kTile;
+    const uint32_t dst = to_at + stage * Shape::kTile;
+    // units two at a time: all that is read of them, then what is written
 #pragma unroll 1
-    for (int u = 0; u < UNITS; ++u) {
-      const bool there = (there_of[0] >> u) & 1;
+    for (int u = 0; u < UNITS; u += 2) {
+      uint32_t w[2][PIECES][4], two[2][PIECES];
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int key = i * TOKENS + token;  // of the unit
-        const uint32_t from = src + u * UNIT + key * (D / 2) + c * 16, scales = src + u * UNIT + 8 * D + key * (D / 16) + c * 2;
-        const uint32_t to = dst + (c >> 1) * Shape::kPanel + (u * 16 + key) * 128;
-        uint32_t w[4] = {0, 0, 0, 0}, two = 0;
-        if (there) {
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const uint32_t at = slot * Shape::kRawTile + (u + f) * UNIT;
           if constexpr (D == 128) {
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from + 8 * turned) : "memory");
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[2]), "=r"(w[3]) : "r"(from + 8 * (1 - turned)) : "memory");
+            const uint32_t from = raw_at + at + i * TOKENS * (D / 2);
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[f][i][0]), "=r"(w[f][i][1]) : "r"(from));
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[f][i][2]), "=r"(w[f][i][3]) : "r"(from ^ 8));
           } else {
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[f][i][0]), "=r"(w[f][i][1]), "=r"(w[f][i][2]), "=r"(w[f][i][3]) : "r"(raw_at + at));
           }
-          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(two) : "r"(scales) : "memory");
+          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(two[f][i]) : "r"(scale_at + at + i * TOKENS * (D / 16)));
         }
-        const int swap = D == 128 ? turned : 0;
-        const uint32_t s0 = (__byte_perm(two, 0, swap ? 0x4141 : 0x4040) << 7) & 0x3f803f80u, s1 = (__byte_perm(two, 0, swap ? 0x4040 : 0x4141) << 7) & 0x3f803f80u;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t h[4];
-          if (values) codes_as_16<false>(w[x], x < 2 ? s0 : s1, h);
-          else codes_as_16<true>(w[x], x < 2 ? s0 : s1, h);
-          const int column = (c & 1) * 4 + (x ^ (2 * swap));
-          st_shared16(to + ((column ^ (key & 7)) << 4), h);
+      for (int f = 0; f < 2; ++f) {
+        const bool there = (there_of[0] >> (u + f)) & 1;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const uint32_t pair = there ? two[f][i] : 0;  // (codes times 0)
+          const uint32_t s0 = (__byte_perm(pair, 0, low) << 7) & 0x3f803f80u, s1 = (__byte_perm(pair, 0, high) << 7) & 0x3f803f80u;
+          const uint32_t to = dst + ((u + f) * 16 + i * TOKENS) * 128;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t h[4];
+            codes_as_half(w[f][i][x], x < 2 ? s0 : s1, h);
+            const int column = (c & 1) * 4 + (x ^ (2 * turned));
+            st_shared16(to + ((column ^ ((i * TOKENS + token) & 7)) << 4), h);
+          }
         }
       }
     }
     fence_proxy_async_smem();
     mbar_arrive(&full[stage]);
     if (!values) {
-      // (the softmax has read the mask PT_MASKS tiles of the stream before this one, see load of the other cache)
-      uint16_t* const mask = bar.mask[stream][m % PT_MASKS] + part * UNITS;
+      // (the softmax has read the mask PT_MASKS tiles of the stream before this one, see the loaders of the other cache)
+      uint16_t* const mask = bar.mask[stream][done % PT_MASKS] + part * UNITS;
       if (lane < UNITS) mask[lane] = static_cast<uint16_t>(low_bits(n_of[0]));
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.mask_full[stream][m % PT_MASKS]);
+      if (lane == 0) mbar_arrive(&bar.mask_full[stream][done % PT_MASKS]);
     }
     __syncwarp();  // every lane has read the slot: it is filled again
     ++done;
+    if (++stage == stages) { stage = 0; stage_phase ^= 1; }
+    if (++slot == RAW) { slot = 0; slot_phase ^= 1; }
 #pragma unroll
     for (int e = 0; e + 1 < RAW; ++e) {
       n_of[e] = n_of[e + 1];
@@ -439,7 +452,10 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
     }
   }
   // (copies on their way after a limit ran out: each is waited for, with a limit)
-  for (; done < fetched; ++done) mbar_wait(&raw_full[done % RAW], (done / RAW) & 1, p.status, 59);
+  for (; done < fetched; ++done) {
+    mbar_wait(&raw_full[slot], slot_phase, p.status, 59);
+    if (++slot == RAW) { slot = 0; slot_phase ^= 1; }
+  }
 }
 
 template <int D, bool PAIRED, bool FP4>
@@ -659,7 +675,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       // Descriptors: the low word is the shared address >> 4 and, for V (MN-major), the distance of its panels of 64 columns above bit 16; the
       // high word has the distance of 8-row groups, version and swizzle.  Low words come out of a shuffle, so that the compiler knows
       // them to be the same in all lanes and forms the descriptors in uniform registers.
-      const uint32_t idesc_s = idesc_bf16(128, BN, false), idesc_o = idesc_bf16(128, D, true, FP4);
+      const uint32_t idesc_s = idesc_bf16(128, BN, false, FP4), idesc_o = idesc_bf16(128, D, true, FP4);
       const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
       auto desc = [&](uint32_t lo) { return (static_cast<uint64_t>(desc_hi) << 32) | lo; };
       const uint32_t q_lo = smem_u32(q_s) >> 4, k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
@@ -800,7 +816,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       uint32_t q_phase = 0;
       bool ok = true;
       // The queries of the slot's rows [rho0, rho0 + 128) of `rows`, by whole warps of them: rows that do not exist are zeros.
-      auto load_q = [&](int row0, int rows, int rho0, int head) {
+      auto load_q = [&](int row0, int rows, int rho0, int head, int place) {
         ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
         if (!ok) return;
         q_phase ^= 1;
@@ -814,15 +830,41 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           p.per_kv.divmod(static_cast<uint32_t>(there ? rho0 + r : 0), tok, hq);
           cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4), src + tok * p.q_row + hq * p.q_head, there);
         }
-        cp_async_arrive(&bar.q_full[stream]);
+        if constexpr (FP4) {
+          // To fp16 where they lie, by a power of two of the row, which puts its largest value in [1, 2) (queries between 2^-100 and 2^100): a
+          // lane has read and written the same pieces, the lanes of a row agree on the power.
+          cp_async_wait_all();
+          __syncwarp();
+#pragma unroll 4
+          for (int r = sub; r < n_rows; r += ROWS) {
+            const uint32_t at = dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+            uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll
+            for (int x = 1; x < LANES; x <<= 1) most = __vmaxu2(most, __shfl_xor_sync(ALL, most, x));
+            const int e = static_cast<int>(min(max(max(most >> 16, most & 0xffffu) >> 7, 27u), 227u));
+            const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xffff0000u) * down);
+            st_shared16(at, h);
+            if (piece == 0) bar.q_scale[slot][place][r] = fminf(p.scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(&bar.q_full[stream]);
+        } else {
+          cp_async_arrive(&bar.q_full[stream]);
+        }
       };
       if (PAIRED && slot == 1) {  // the second slot's
         Items items;
         TileItem t;
         while (ok) {
+          const int place = items.at;
           ok = next_item(stream, items, t);
           if (!ok || t.tiles == 0) break;
-          load_q(t.row0, t.rows, t.rho0 + kSlotRows, t.head);
+          load_q(t.row0, t.rows, t.rho0 + kSlotRows, t.head, place);
         }
         cp_async_wait_all();
       } else {
@@ -856,8 +898,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           const bool second = n >= items0;
           TileItem t;
           if (!find_tile_item<PAIRED, BN>(p, tp.span[second], second ? st1 : st0, second ? n - items0 : n, t)) continue;
+          const int place = at;
           hand_out(t, lane == 0);
-          if (ok) load_q(t.row0, t.rows, t.rho0, t.head);
+          if (ok) load_q(t.row0, t.rows, t.rho0, t.head, place);
         }
         TileItem end;
         end.tiles = 0;
@@ -878,6 +921,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     uint32_t units = 0, mine_done = 0;      // tiles of the slot so far: unit n has buffer n % NB, phase n / NB; its items so far
     bool ok = true;
     while (true) {
+      [[maybe_unused]] const int place = items.at;
       ok = next_item(stream, items, t);
       if (!ok || t.tiles == 0) break;
       const int rho = t.rho0 + (PAIRED ? slot * kSlotRows : 0) + quad * 32 + lane;
@@ -887,7 +931,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const bool idle = rho - lane >= t.rows;  // a warp without rows: whatever its P holds stays in its own rows of O
       const int limit = there ? own_keys(p, t.length, static_cast<int>(tok)) : t.o_keys;
       const int warp_limit = __shfl_sync(ALL, limit, 0);  // limits ascend with the rows
-      float factor = p.scale2, m_ref = NEG_INF, l = 0.0f;
+      float scale2 = p.scale2, factor = scale2, m_ref = NEG_INF, l = 0.0f;
       float o_apart[D];    // O behind the tile before, where that was formed apart (in local memory)
       bool apart = false;
       const int mine = PAIRED ? (slot ? t.n[1] : t.n[0]) : t.tiles;
@@ -958,8 +1002,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         if (__any_sync(ALL, moves || (LATE && apart))) {
           float alpha = 1.0f;
           if (moves) {
-            const float before = in_log2(m_ref, factor, p.scale2);
-            factor = p.scale2;
+            const float before = in_log2(m_ref, factor, scale2);
+            factor = scale2;
             m_ref = mx * factor;
             alpha = ex2(before - m_ref);  // 0 for -inf
             if (fabsf(m_ref) >= PT_LARGE) {
@@ -1032,7 +1076,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const int first_late = warp_limit >= t.o_keys ? mine : min(max(t.p128 + warp_limit - t.v0, 0) / BN, mine);
       // A slot that took none of the last tiles may be far ahead of the loaders, where the phase of a mask says nothing yet: its first S tells
       // that they have come here.
-      if (PAIRED && mine > 0 && !idle) ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][units % NB], (units / NB) & 1, p.status, 55));
+      if ((PAIRED || FP4) && mine > 0 && !idle) ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][units % NB], (units / NB) & 1, p.status, 55));
+      if constexpr (FP4) {  // (with S, the queries it is of are there)
+        if (!idle) scale2 = factor = bar.q_scale[slot][place][quad * 32 + lane];
+      }
       int u = 0;
       for (; ok && u < first_late; ++u, ++units) do_tile(std::false_type{}, u);
       for (; ok && u < mine; ++u, ++units) do_tile(std::true_type{}, u);
@@ -1049,7 +1096,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const int64_t row = t.row0 + static_cast<int>(tok), qh = t.head * static_cast<int64_t>(p.per_kv.d) + hq;
       if (t.part >= 0) {
         const int64_t at = (static_cast<int64_t>(t.part) * p.rows.rows + row) * p.q_heads + qh;
-        if (there) p.part_ml[at] = make_float2(in_log2(m_ref, factor, p.scale2), l);
+        if (there) p.part_ml[at] = make_float2(in_log2(m_ref, factor, scale2), l);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
