@@ -75,10 +75,10 @@ struct TileShape {
   static constexpr bool kHalves = PAIRED && D == 64;
   static constexpr int kStagesK = FP4 ? (D == 128 ? 2 : 3) : (D == 128 ? 3 : 5);  // of a stream
   static constexpr int kStagesV = FP4 ? (D == 128 ? (PAIRED ? 2 : 1) : 3) : (D == 128 ? 2 : 5);
-  // FP4: tiles of a loader (64 keys or values of them) that are on their way as they lie in the cache, 4 units each
-  static constexpr int kRaw = FP4 ? (D == 128 && PAIRED ? 1 : 3) : 0;
-  static constexpr int kRawTile = 4 * kFp4Unit * D;
-  static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + 4 * kRaw * kRawTile + 1024;
+  // FP4: tiles of a stream that are on their way as they lie in the cache, units of their keys, then of their values
+  static constexpr int kRaw = FP4 ? (D == 128 ? (PAIRED ? 1 : 3) : (PAIRED ? 3 : 6)) : 0;
+  static constexpr int kUnits = kKeys / 16, kRawTile = 2 * kUnits * kFp4Unit * D;
+  static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + kStreams * kRaw * kRawTile + 1024;
 };
 
 struct TilesParams {
@@ -96,6 +96,8 @@ struct TileItem {
   int part;
 };
 
+constexpr uint32_t kRawEnd = 0xffffffffu;
+
 template <class Shape>
 struct TileBarriers {
   uint64_t k_full[Shape::kStreams][Shape::kStagesK], k_empty[Shape::kStreams][Shape::kStagesK];
@@ -103,7 +105,8 @@ struct TileBarriers {
   uint64_t p_half[2];  // kHalves: the first half of a tile's P
   uint64_t s_full[2][Shape::kBuffers], p_full[2][Shape::kBuffers], pv_done[2][Shape::kBuffers], q_full[2], q_empty[2];
   uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
-  uint64_t raw_full[4][Shape::kRaw > 0 ? Shape::kRaw : 1];
+  uint64_t raw_full[2][Shape::kRaw > 0 ? Shape::kRaw : 1], raw_empty[2][Shape::kRaw > 0 ? Shape::kRaw : 1];
+  uint32_t raw_there[2][Shape::kRaw > 0 ? Shape::kRaw : 1];  // FP4: which units of a tile there are; kRawEnd: no tile, the stream ends
   float q_scale[Shape::kRaw > 0 ? 2 : 1][PT_ITEMS][Shape::kRaw > 0 ? kSlotRows : 1];  // FP4: factors of the scores of a slot's rows, by the place of their item
   alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
   TileItem item[2][PT_ITEMS];
@@ -300,101 +303,35 @@ __device__ __noinline__ void put_back(const float* o, uint32_t o_tmem) {
   tc_wait_st_all();
 }
 
-// The loaders of a cache in 4 bits: a warp has the keys or the values of its stream, 64 of a tile.  It fetches units as they lie in the cache (a bulk copy each, up
-// to kRaw of its tiles ahead and across items) and writes them as the products read them, in fp16 over 256, which is exact.  (Keys in bf16, as the queries
-// come: three more instructions for two values, and the loader of the keys was the bound: 127 us for 80 over an hour of prefix.)
-// A lane takes 32 values, 16 bytes; at head_dim 128 the lanes of the second panel take their halves the other way round, so that eight
-// lanes write to eight different 16-byte columns.  Units that are not there are written as zeros.
+// The loaders of a cache in 4 bits: a warp has the keys or the values of its stream, 64 of a tile.  It writes units, which lie in shared memory as in the
+// cache, as the products read them: fp16 over 256, which is exact.  (Keys in bf16, as the queries come: three more instructions for two
+// values, and the loader of the keys was the bound: 127 us for 80 over an hour of prefix.)  A lane takes 32 values, 16 bytes; at head_dim
+// 128 the lanes of the second panel take their halves the other way round, so that eight lanes write to eight different 16-byte
+// columns.  Units that are not there are written as zeros.
 template <int D, bool PAIRED>
 __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarriers<TileShape<D, PAIRED, true>>& bar, uint8_t* k_ring, uint8_t* v_ring, uint8_t* raw) {
   using Shape = TileShape<D, PAIRED, true>;
   constexpr unsigned ALL = 0xffffffffu;
-  constexpr int BN = Shape::kKeys, STREAMS = Shape::kStreams, PARTS = Shape::kParts, RAW = Shape::kRaw, UNIT = kFp4Unit * D, UNITS = 4;
+  constexpr int STREAMS = Shape::kStreams, PARTS = Shape::kParts, RAW = Shape::kRaw, UNIT = kFp4Unit * D, UNITS = 4;
   const int loader = (threadIdx.x >> 5) - 8, lane = threadIdx.x & 31;
   const int stream = loader / (4 / STREAMS), local = loader % (4 / STREAMS), part = local % PARTS;
   const bool values = local >= PARTS;
   const int stages = values ? Shape::kStagesV : Shape::kStagesK;
   uint64_t* const full = values ? bar.v_full[stream] : bar.k_full[stream];
   uint64_t* const empty = values ? bar.v_empty[stream] : bar.k_empty[stream];
-  const uint32_t ring = smem_u32(values ? v_ring : k_ring) + stream * stages * Shape::kTile + part * 64 * 128;
-  const uint8_t* const cache = values ? p.fp4.v : p.fp4.k;
-  const int64_t page_bytes = values ? p.fp4.v_page : p.fp4.k_page;
-  uint64_t* const raw_full = bar.raw_full[loader];
-
-  // the tile that is fetched next: tile `tile` of the item t
-  TileItem t;
-  t.tiles = 0;
-  int at = 0, tile = -1;
-  uint32_t item_phase = 0;
-  bool ended = false, ok = true;
-  // Where a lane's unit (of lanes 0 to 3) of tile x is: table entry as it stands there, place on the page, keys.  Asked for a tile ahead within an item.
-  int entry = -1, n = 0;
-  uint32_t rest = 0;
-  auto look_up = [&](int x) {
-    const int v = t.v0 + x * BN;
-    const bool own = v >= t.p128;
-    const int j = v - (own ? t.p128 : 0) + part * 64 + 16 * lane, end = own ? t.o_keys : t.p_keys;
-    n = lane < UNITS && x < t.tiles ? min(max(end - j, 0), 16) : 0;
-    entry = -1;
-    if (n > 0) {
-      const PagedTable& table = own ? p.rows.table : p.prefix;
-      uint32_t index;
-      p.fp4.page_units.divmod(static_cast<uint32_t>(j) / kFp4Tokens, index, rest);
-      entry = table.table[static_cast<int64_t>(own ? t.sequence : t.group) * table.ld + index];  // (keys end where the table does)
-    }
-  };
-  auto advance = [&](bool wait) {  // false: not known yet (or the end)
-    if (tile + 1 < t.tiles) {
-      ++tile;
-      return true;
-    }
-    if (ended) return false;
-    const bool there = wait ? mbar_wait_spin(&bar.item_full[stream][at], item_phase, p.status, 57) : mbar_poll(&bar.item_full[stream][at], item_phase);
-    if (!__all_sync(ALL, there)) {
-      if (wait) ok = false;
-      return false;
-    }
-    t = bar.item[stream][at];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bar.item_empty[stream][at]);
-    if (++at == PT_ITEMS) { at = 0; item_phase ^= 1; }
-    tile = 0;
-    ended = t.tiles == 0;
-    look_up(0);
-    return !ended;
-  };
-  int n_of[RAW], there_of[RAW];  // of the tiles on their way: keys of this lane's unit, which units are there
-  int fetched = 0, done = 0, fetch_slot = 0, stage = 0, slot = 0;
-  uint32_t stage_phase = 1, slot_phase = 0;
   // where a lane reads a unit and writes it
   constexpr int LANES = D / 32, TOKENS = 32 / LANES, PIECES = 16 / TOKENS;  // lanes of a token, tokens of a piece
   const int c = lane % LANES, token = lane / LANES, turned = D == 128 ? c >> 1 : 0;
-  const uint32_t raw_at = smem_u32(raw) + token * (D / 2) + c * 16 + 8 * turned, scale_at = smem_u32(raw) + 8 * D + token * (D / 16) + c * 2;
+  const uint32_t unit0 = smem_u32(raw) + stream * RAW * Shape::kRawTile + ((values ? Shape::kUnits : 0) + part * UNITS) * UNIT;
+  const uint32_t raw_at = unit0 + token * (D / 2) + c * 16 + 8 * turned, scale_at = unit0 + 8 * D + token * (D / 16) + c * 2;
   const uint32_t low = turned ? 0x4141 : 0x4040, high = turned ? 0x4040 : 0x4141;
-  const uint32_t to_at = ring + (c >> 1) * Shape::kPanel + token * 128;
-  while (ok) {
-    while (fetched - done < RAW && advance(fetched == done)) {
-      const int page = entry >= 0 && entry < p.cache.pages ? entry : -1;
-      const uint32_t there = __ballot_sync(ALL, page >= 0);
-      if (lane == 0) mbar_expect_tx(&raw_full[fetch_slot], __popc(there) * UNIT);
-      __syncwarp();
-      if (page >= 0)
-        bulk_load(raw + fetch_slot * Shape::kRawTile + lane * UNIT, cache + page * page_bytes + (static_cast<int64_t>(t.head) * p.fp4.page_units.d + rest) * UNIT, UNIT,
-                  &raw_full[fetch_slot]);
-      // (a queue in registers: the tiles before it are its first entries)
-#pragma unroll
-      for (int e = 0; e < RAW; ++e)
-        if (e == fetched - done) {
-          n_of[e] = page >= 0 ? n : 0;
-          there_of[e] = static_cast<int>(there);
-        }
-      ++fetched;
-      if (++fetch_slot == RAW) fetch_slot = 0;
-      look_up(tile + 1);
-    }
-    if (!ok || fetched == done) break;
-    ok = __all_sync(ALL, mbar_wait(&raw_full[slot], slot_phase, p.status, 59) && mbar_wait(&empty[stage], stage_phase, p.status, 58));
-    if (!ok) break;
+  const uint32_t to_at = smem_u32(values ? v_ring : k_ring) + stream * stages * Shape::kTile + part * 64 * 128 + (c >> 1) * Shape::kPanel + token * 128;
+  int stage = 0, slot = 0;
+  uint32_t stage_phase = 1, slot_phase = 0;
+  while (true) {
+    if (!__all_sync(ALL, mbar_wait(&bar.raw_full[stream][slot], slot_phase, p.status, 59))) break;
+    const uint32_t there = bar.raw_there[stream][slot];
+    if (there == kRawEnd || !__all_sync(ALL, mbar_wait(&empty[stage], stage_phase, p.status, 58))) break;
     const uint32_t dst = to_at + stage * Shape::kTile;
     // units two at a time: all that is read of them, then what is written
 #pragma unroll 1
@@ -416,10 +353,10 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
         }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const bool there = (there_of[0] >> (u + f)) & 1;
+        const bool is = (there >> (part * UNITS + u + f)) & 1;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const uint32_t pair = there ? two[f][i] : 0;  // (codes times 0)
+          const uint32_t pair = is ? two[f][i] : 0;  // (codes times 0)
           const uint32_t s0 = (__byte_perm(pair, 0, low) << 7) & 0x3f803f80u, s1 = (__byte_perm(pair, 0, high) << 7) & 0x3f803f80u;
           const uint32_t to = dst + ((u + f) * 16 + i * TOKENS) * 128;
 #pragma unroll
@@ -434,26 +371,9 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
     }
     fence_proxy_async_smem();
     mbar_arrive(&full[stage]);
-    if (!values) {
-      // (the softmax has read the mask PT_MASKS tiles of the stream before this one, see the loaders of the other cache)
-      uint16_t* const mask = bar.mask[stream][done % PT_MASKS] + part * UNITS;
-      if (lane < UNITS) mask[lane] = static_cast<uint16_t>(low_bits(n_of[0]));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.mask_full[stream][done % PT_MASKS]);
-    }
-    __syncwarp();  // every lane has read the slot: it is filled again
-    ++done;
+    __syncwarp();  // every lane has read the slot
+    if (lane == 0) mbar_arrive(&bar.raw_empty[stream][slot]);
     if (++stage == stages) { stage = 0; stage_phase ^= 1; }
-    if (++slot == RAW) { slot = 0; slot_phase ^= 1; }
-#pragma unroll
-    for (int e = 0; e + 1 < RAW; ++e) {
-      n_of[e] = n_of[e + 1];
-      there_of[e] = there_of[e + 1];
-    }
-  }
-  // (copies on their way after a limit ran out: each is waited for, with a limit)
-  for (; done < fetched; ++done) {
-    mbar_wait(&raw_full[slot], slot_phase, p.status, 59);
     if (++slot == RAW) { slot = 0; slot_phase ^= 1; }
   }
 }
@@ -475,10 +395,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 
   if (warp < 2) {  // each lane some barriers
     const int s = warp;  // slot, stream
-    for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], Shape::kParts);
+    for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], FP4 ? 1 : Shape::kParts);
     if (lane < PT_ITEMS) {
       mbar_init(&bar.item_full[s][lane], 1);
-      mbar_init(&bar.item_empty[s][lane], 4 / STREAMS + 1 + 8 / STREAMS + (PAIRED ? 1 : 0));  // warps that read an item: loaders, MMA issuer, softmax, the second slot's queries
+      mbar_init(&bar.item_empty[s][lane], (FP4 ? 0 : 4 / STREAMS) + 1 + 8 / STREAMS + (PAIRED ? 1 : 0));  // warps that read an item: loaders, MMA issuer, softmax, the second slot's queries
     }
     if (lane < NB) {
       mbar_init(&bar.s_full[s][lane], 1);
@@ -490,7 +410,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       mbar_init(&bar.q_empty[s], 1);
       mbar_init(&bar.p_half[s], 4);
     }
-    if (FP4 && lane < 2 * Shape::kRaw) mbar_init(&bar.raw_full[0][0] + s * 2 * Shape::kRaw + lane, 1);
+    if (FP4 && s < STREAMS && lane < Shape::kRaw) {
+      mbar_init(&bar.raw_full[s][lane], 1);
+      mbar_init(&bar.raw_empty[s][lane], 4 / STREAMS);  // loaders of the stream
+    }
     if (s < STREAMS && lane < NK) {
       mbar_init(&bar.k_full[s][lane], 32 * Shape::kParts);  // threads of the loaders that share a tile
       mbar_init(&bar.k_empty[s][lane], 1);
@@ -533,7 +456,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     // =========================== loaders ===========================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - SOFTMAX_REGS));
     if constexpr (FP4) {
-      load_fp4_tiles<D, PAIRED>(p, bar, k_ring, v_ring, raw_ring + (warp - 8) * Shape::kRaw * Shape::kRawTile);
+      load_fp4_tiles<D, PAIRED>(p, bar, k_ring, v_ring, raw_ring);
     } else {
     constexpr int PARTS = Shape::kParts, TEAM = 4 / STREAMS / PARTS;  // loaders that share a tile, that take tiles in turn
     constexpr int MINE = BN / PARTS, GROUPS = MINE / 16, PER_LANE = MINE / 32;
@@ -831,25 +754,39 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4), src + tok * p.q_row + hq * p.q_head, there);
         }
         if constexpr (FP4) {
-          // To fp16 where they lie, by a power of two of the row, which puts its largest value in [1, 2) (queries between 2^-100 and 2^100): a
-          // lane has read and written the same pieces, the lanes of a row agree on the power.
+          // To fp16 where they lie, by a power of two of the row, which puts its largest value in [1, 2) (queries between 2^-100 and 2^100); a row
+          // per lane.  (By the lanes that copied its pieces, with shuffles: 270 cycles for two rows, 17,000 ahead of the first product.)
           cp_async_wait_all();
           __syncwarp();
-#pragma unroll 4
-          for (int r = sub; r < n_rows; r += ROWS) {
-            const uint32_t at = dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
-            uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll 1
+          for (int r = lane; r < n_rows; r += 32) {
+            const uint32_t row = smem_u32(q_s) + slot * Shape::kQ + r * 128, swz = (r & 7) << 4;
+            uint32_t most = 0;
 #pragma unroll
-            for (int x = 1; x < LANES; x <<= 1) most = __vmaxu2(most, __shfl_xor_sync(ALL, most, x));
+            for (int i = 0; i < D / 8; ++i) {
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(row + (i >> 3) * PT_Q_PANEL + (((i & 7) << 4) ^ swz)));
+              most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu)));
+            }
             const int e = static_cast<int>(min(max(max(most >> 16, most & 0xffffu) >> 7, 27u), 227u));
             const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-            uint32_t h[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xffff0000u) * down);
-            st_shared16(at, h);
-            if (piece == 0) bar.q_scale[slot][place][r] = fminf(p.scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f);
+            for (int i0 = 0; i0 < D / 8; i0 += 4) {
+              uint32_t w[4][4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                             : "r"(row + ((i0 + i) >> 3) * PT_Q_PANEL + ((((i0 + i) & 7) << 4) ^ swz)));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t h[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(w[i][k] << 16) * down, __uint_as_float(w[i][k] & 0xffff0000u) * down);
+                st_shared16(row + ((i0 + i) >> 3) * PT_Q_PANEL + ((((i0 + i) & 7) << 4) ^ swz), h);
+              }
+            }
+            bar.q_scale[slot][place][r] = fminf(p.scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f);
           }
           fence_proxy_async_smem();
           mbar_arrive(&bar.q_full[stream]);
@@ -879,6 +816,53 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           if (lane == 0) mbar_arrive(&bar.item_full[stream][at]);
           if (++at == PT_ITEMS) { at = 0; phase ^= 1; }
         };
+        // FP4: units of tiles to shared memory as they lie in the cache, those of keys by the lower lanes, those of values by lanes 16 on.  The table is
+        // read a tile ahead.
+        [[maybe_unused]] int entry = -1, keys_there = 0, raw_slot = 0, fetched = 0;
+        [[maybe_unused]] uint32_t rest = 0, raw_phase = 0;
+        [[maybe_unused]] auto look_up = [&](const TileItem& t, int x) {
+          const int v = t.v0 + x * BN;
+          const bool own = v >= t.p128;
+          const int unit = lane & 15, j = v - (own ? t.p128 : 0) + 16 * unit, end = own ? t.o_keys : t.p_keys;
+          keys_there = unit < Shape::kUnits && x < t.tiles ? min(max(end - j, 0), 16) : 0;
+          entry = -1;
+          if (keys_there > 0) {
+            const PagedTable& table = own ? p.rows.table : p.prefix;
+            uint32_t index;
+            p.fp4.page_units.divmod(static_cast<uint32_t>(j) / kFp4Tokens, index, rest);
+            entry = table.table[static_cast<int64_t>(own ? t.sequence : t.group) * table.ld + index];  // (keys end where the table does)
+          }
+        };
+        [[maybe_unused]] auto fetch = [&](const TileItem& t, int from, int to) {
+          constexpr int UNIT = kFp4Unit * D;
+          const bool values = lane >= 16;
+          const int64_t page_bytes = values ? p.fp4.v_page : p.fp4.k_page;
+          const uint8_t* const base = (values ? p.fp4.v : p.fp4.k) + static_cast<int64_t>(t.head) * p.fp4.page_units.d * UNIT;
+          uint8_t* const raw = raw_ring + stream * Shape::kRaw * Shape::kRawTile + ((values ? Shape::kUnits : 0) + (lane & 15)) * UNIT;
+#pragma unroll 1
+          for (int x = from; x < to && ok; ++x) {
+            const bool is = entry >= 0 && entry < p.cache.pages;
+            const uint32_t there = __ballot_sync(ALL, is);
+            const uint8_t* const src = base + (is ? entry : 0) * page_bytes + static_cast<int64_t>(rest) * UNIT;
+            const int keys = is ? keys_there : 0;
+            look_up(t, x + 1);
+            ok = __all_sync(ALL, mbar_wait(&bar.raw_empty[stream][raw_slot], raw_phase ^ 1, p.status, 57));
+            if (!ok) return;
+            // (the softmax has read the mask PT_MASKS tiles of the stream before this one: PT_MASKS is more than the rings hold and a slot has begun)
+            static_assert(Shape::kRaw + Shape::kStagesK + 2 * NB + 1 < PT_MASKS, "");
+            uint16_t* const mask = bar.mask[stream][fetched % PT_MASKS];
+            if (lane < Shape::kUnits) mask[lane] = static_cast<uint16_t>(low_bits(keys));
+            if (lane == 0) {
+              bar.raw_there[stream][raw_slot] = there & 0xffffu;
+              mbar_expect_tx(&bar.raw_full[stream][raw_slot], __popc(there) * UNIT);
+            }
+            __syncwarp();
+            if (is) bulk_load(raw + raw_slot * Shape::kRawTile, src, UNIT, &bar.raw_full[stream][raw_slot]);
+            if (lane == 0) mbar_arrive(&bar.mask_full[stream][fetched % PT_MASKS]);
+            ++fetched;
+            if (++raw_slot == Shape::kRaw) { raw_slot = 0; raw_phase ^= 1; }
+          }
+        };
         // A stream has an item of every round, in turn from both ends of it: with causal rows the later tiles have more keys.  (The host saw to
         // it that items are below 2^31.)
         constexpr int TM = PAIRED ? 2 * kSlotRows : kSlotRows;
@@ -900,11 +884,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           if (!find_tile_item<PAIRED, BN>(p, tp.span[second], second ? st1 : st0, second ? n - items0 : n, t)) continue;
           const int place = at;
           hand_out(t, lane == 0);
-          if (ok) load_q(t.row0, t.rows, t.rho0, t.head, place);
+          if constexpr (FP4) {  // the first tiles on their way, the queries, the other tiles
+            look_up(t, 0);
+            const int ahead = min(t.tiles, Shape::kRaw);
+            fetch(t, 0, ahead);
+            if (ok) load_q(t.row0, t.rows, t.rho0, t.head, place);
+            fetch(t, ahead, t.tiles);
+          } else {
+            if (ok) load_q(t.row0, t.rows, t.rho0, t.head, place);
+          }
         }
         TileItem end;
         end.tiles = 0;
         if (ok) hand_out(end, lane == 0);
+        if constexpr (FP4) {
+          ok = ok && __all_sync(ALL, mbar_wait(&bar.raw_empty[stream][raw_slot], raw_phase ^ 1, p.status, 57));
+          if (ok && lane == 0) {
+            bar.raw_there[stream][raw_slot] = kRawEnd;
+            mbar_arrive(&bar.raw_full[stream][raw_slot]);
+          }
+          // (copies on their way after a limit ran out: each is waited for, with a limit)
+          if (!ok)
+            for (int i = 0; i < Shape::kRaw && i < fetched; ++i) {
+              raw_slot = (raw_slot == 0 ? Shape::kRaw : raw_slot) - 1;
+              if (raw_slot == Shape::kRaw - 1) raw_phase ^= 1;
+              mbar_wait(&bar.raw_full[stream][raw_slot], raw_phase, p.status, 59);
+            }
+        }
         cp_async_wait_all();
       }
     }
