@@ -107,7 +107,6 @@ struct TileBarriers {
   uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
   uint64_t raw_full[2][Shape::kRaw > 0 ? Shape::kRaw : 1], raw_empty[2][Shape::kRaw > 0 ? Shape::kRaw : 1];
   uint32_t raw_there[2][Shape::kRaw > 0 ? Shape::kRaw : 1];  // FP4: which units of a tile there are; kRawEnd: no tile, the stream ends
-  float q_scale[Shape::kRaw > 0 ? 2 : 1][PT_ITEMS][Shape::kRaw > 0 ? kSlotRows : 1];  // FP4: factors of the scores of a slot's rows, by the place of their item
   alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
   TileItem item[2][PT_ITEMS];
   uint32_t tmem_base;
@@ -398,7 +397,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], FP4 ? 1 : Shape::kParts);
     if (lane < PT_ITEMS) {
       mbar_init(&bar.item_full[s][lane], 1);
-      mbar_init(&bar.item_empty[s][lane], (FP4 ? 0 : 4 / STREAMS) + 1 + 8 / STREAMS + (PAIRED ? 1 : 0));  // warps that read an item: loaders, MMA issuer, softmax, the second slot's queries
+      mbar_init(&bar.item_empty[s][lane], (FP4 ? 0 : 4 / STREAMS) + 1 + 8 / STREAMS + (PAIRED && !FP4 ? 1 : 0));  // warps that read an item: loaders, MMA issuer, softmax, the second slot's queries
     }
     if (lane < NB) {
       mbar_init(&bar.s_full[s][lane], 1);
@@ -406,7 +405,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       mbar_init(&bar.pv_done[s][lane], 1);
     }
     if (lane == 0) {
-      mbar_init(&bar.q_full[s], 64 / STREAMS);  // threads that load queries
+      mbar_init(&bar.q_full[s], (FP4 ? 256 : 64) / STREAMS);  // threads that load queries
       mbar_init(&bar.q_empty[s], 1);
       mbar_init(&bar.p_half[s], 4);
     }
@@ -663,13 +662,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             ok = take_p(0, vs, fresh);
             if (ok && last[0] && leader) tc_commit(&bar.pv_done[0][0]);
           }
+          auto second_p = [&] {
+            ok = take_p(1, vs, fresh);
+            if (ok && last[1] && leader) tc_commit(&bar.pv_done[1][0]);
+          };
+          // FP4: the softmax of a slot loads its queries behind its last O of the item before, so that has to be on its way here
+          const bool early = FP4 && first;
+          if (ok && early && has[1]) second_p();
           if (ok && first) ok = wait_q(0);
           if (ok && more) ok = landed(bar.k_full[0], ks, k_phase);
           if (ok && has0) issue_s(0, 0, ks);
-          if (ok && has[1]) {
-            ok = take_p(1, vs, fresh);
-            if (ok && last[1] && leader) tc_commit(&bar.pv_done[1][0]);
-          }
+          if (ok && !early && has[1]) second_p();
           if (!ok) return;
           if (has1) issue_s(1, 0, ks);
           if (leader) {
@@ -739,7 +742,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       uint32_t q_phase = 0;
       bool ok = true;
       // The queries of the slot's rows [rho0, rho0 + 128) of `rows`, by whole warps of them: rows that do not exist are zeros.
-      auto load_q = [&](int row0, int rows, int rho0, int head, int place) {
+      auto load_q = [&](int row0, int rows, int rho0, int head) {
         ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
         if (!ok) return;
         q_phase ^= 1;
@@ -753,55 +756,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           p.per_kv.divmod(static_cast<uint32_t>(there ? rho0 + r : 0), tok, hq);
           cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4), src + tok * p.q_row + hq * p.q_head, there);
         }
-        if constexpr (FP4) {
-          // To fp16 where they lie, by a power of two of the row, which puts its largest value in [1, 2) (queries between 2^-100 and 2^100); a row
-          // per lane.  (By the lanes that copied its pieces, with shuffles: 270 cycles for two rows, 17,000 ahead of the first product.)
-          cp_async_wait_all();
-          __syncwarp();
-#pragma unroll 1
-          for (int r = lane; r < n_rows; r += 32) {
-            const uint32_t row = smem_u32(q_s) + slot * Shape::kQ + r * 128, swz = (r & 7) << 4;
-            uint32_t most = 0;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(row + (i >> 3) * PT_Q_PANEL + (((i & 7) << 4) ^ swz)));
-              most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu)));
-            }
-            const int e = static_cast<int>(min(max(max(most >> 16, most & 0xffffu) >> 7, 27u), 227u));
-            const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-#pragma unroll
-            for (int i0 = 0; i0 < D / 8; i0 += 4) {
-              uint32_t w[4][4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
-                             : "r"(row + ((i0 + i) >> 3) * PT_Q_PANEL + ((((i0 + i) & 7) << 4) ^ swz)));
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t h[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(w[i][k] << 16) * down, __uint_as_float(w[i][k] & 0xffff0000u) * down);
-                st_shared16(row + ((i0 + i) >> 3) * PT_Q_PANEL + ((((i0 + i) & 7) << 4) ^ swz), h);
-              }
-            }
-            bar.q_scale[slot][place][r] = fminf(p.scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f);
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(&bar.q_full[stream]);
-        } else {
-          cp_async_arrive(&bar.q_full[stream]);
-        }
+        cp_async_arrive(&bar.q_full[stream]);
       };
-      if (PAIRED && slot == 1) {  // the second slot's
+      if (PAIRED && FP4 && slot == 1) {  // (the softmax loads its queries)
+      } else if (PAIRED && slot == 1) {  // the second slot's
         Items items;
         TileItem t;
         while (ok) {
-          const int place = items.at;
           ok = next_item(stream, items, t);
           if (!ok || t.tiles == 0) break;
-          load_q(t.row0, t.rows, t.rho0 + kSlotRows, t.head, place);
+          load_q(t.row0, t.rows, t.rho0 + kSlotRows, t.head);
         }
         cp_async_wait_all();
       } else {
@@ -833,14 +797,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             entry = table.table[static_cast<int64_t>(own ? t.sequence : t.group) * table.ld + index];  // (keys end where the table does)
           }
         };
-        [[maybe_unused]] auto fetch = [&](const TileItem& t, int from, int to) {
+        [[maybe_unused]] auto fetch = [&](const TileItem& t) {
           constexpr int UNIT = kFp4Unit * D;
           const bool values = lane >= 16;
           const int64_t page_bytes = values ? p.fp4.v_page : p.fp4.k_page;
           const uint8_t* const base = (values ? p.fp4.v : p.fp4.k) + static_cast<int64_t>(t.head) * p.fp4.page_units.d * UNIT;
           uint8_t* const raw = raw_ring + stream * Shape::kRaw * Shape::kRawTile + ((values ? Shape::kUnits : 0) + (lane & 15)) * UNIT;
+          look_up(t, 0);
 #pragma unroll 1
-          for (int x = from; x < to && ok; ++x) {
+          for (int x = 0; x < t.tiles && ok; ++x) {
             const bool is = entry >= 0 && entry < p.cache.pages;
             const uint32_t there = __ballot_sync(ALL, is);
             const uint8_t* const src = base + (is ? entry : 0) * page_bytes + static_cast<int64_t>(rest) * UNIT;
@@ -882,17 +847,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           const bool second = n >= items0;
           TileItem t;
           if (!find_tile_item<PAIRED, BN>(p, tp.span[second], second ? st1 : st0, second ? n - items0 : n, t)) continue;
-          const int place = at;
           hand_out(t, lane == 0);
-          if constexpr (FP4) {  // the first tiles on their way, the queries, the other tiles
-            look_up(t, 0);
-            const int ahead = min(t.tiles, Shape::kRaw);
-            fetch(t, 0, ahead);
-            if (ok) load_q(t.row0, t.rows, t.rho0, t.head, place);
-            fetch(t, ahead, t.tiles);
-          } else {
-            if (ok) load_q(t.row0, t.rows, t.rho0, t.head, place);
-          }
+          if constexpr (FP4) fetch(t);
+          else if (ok) load_q(t.row0, t.rows, t.rho0, t.head);
         }
         TileItem end;
         end.tiles = 0;
@@ -924,10 +881,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     Items items;
     TileItem t;
     int masks = 0;                          // tiles of the stream up to this item
+    [[maybe_unused]] uint32_t q_phase = 0;
     uint32_t units = 0, mine_done = 0;      // tiles of the slot so far: unit n has buffer n % NB, phase n / NB; its items so far
     bool ok = true;
     while (true) {
-      [[maybe_unused]] const int place = items.at;
       ok = next_item(stream, items, t);
       if (!ok || t.tiles == 0) break;
       const int rho = t.rho0 + (PAIRED ? slot * kSlotRows : 0) + quad * 32 + lane;
@@ -937,7 +894,40 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const bool idle = rho - lane >= t.rows;  // a warp without rows: whatever its P holds stays in its own rows of O
       const int limit = there ? own_keys(p, t.length, static_cast<int>(tok)) : t.o_keys;
       const int warp_limit = __shfl_sync(ALL, limit, 0);  // limits ascend with the rows
-      float scale2 = p.scale2, factor = scale2, m_ref = NEG_INF, l = 0.0f;
+      float scale2 = p.scale2;
+      if constexpr (FP4) {
+        // The thread's query, in fp16 by a power of two, which puts its largest value in [1, 2) (queries between 2^-100 and 2^100).  (By the warps that hand
+        // out items 15,000 cycles ahead of the first product, by these 3,000, of which none pass under the item before.)
+        ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
+        if (!ok) break;
+        q_phase ^= 1;
+        if (!idle) {
+          uint4 w[D / 8];
+          const __nv_bfloat16* const src = p.q + (t.row0 + static_cast<int64_t>(tok)) * p.q_row + (t.head * static_cast<int64_t>(p.per_kv.d) + hq) * p.q_head;
+          uint32_t most = 0;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) w[i] = there ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+            most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu), __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu)));
+          const int e = static_cast<int>(min(max(max(most >> 16, most & 0xffffu) >> 7, 27u), 227u));
+          const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          scale2 = fminf(scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f);
+          const int r = quad * 32 + lane;
+          const uint32_t row = smem_u32(q_s) + slot * Shape::kQ + r * 128;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
+            st_shared16(row + (i >> 3) * PT_Q_PANEL + (((i ^ r) & 7) << 4), h);
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&bar.q_full[stream]);
+      }
+      float factor = scale2, m_ref = NEG_INF, l = 0.0f;
       float o_apart[D];    // O behind the tile before, where that was formed apart (in local memory)
       bool apart = false;
       const int mine = PAIRED ? (slot ? t.n[1] : t.n[0]) : t.tiles;
@@ -1082,10 +1072,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const int first_late = warp_limit >= t.o_keys ? mine : min(max(t.p128 + warp_limit - t.v0, 0) / BN, mine);
       // A slot that took none of the last tiles may be far ahead of the loaders, where the phase of a mask says nothing yet: its first S tells
       // that they have come here.
-      if ((PAIRED || FP4) && mine > 0 && !idle) ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][units % NB], (units / NB) & 1, p.status, 55));
-      if constexpr (FP4) {  // (with S, the queries it is of are there)
-        if (!idle) scale2 = factor = bar.q_scale[slot][place][quad * 32 + lane];
-      }
+      if (PAIRED && mine > 0 && !idle) ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][units % NB], (units / NB) & 1, p.status, 55));
       int u = 0;
       for (; ok && u < first_late; ++u, ++units) do_tile(std::false_type{}, u);
       for (; ok && u < mine; ++u, ++units) do_tile(std::true_type{}, u);
