@@ -8,12 +8,12 @@
 //                        sums of both rows, then of max(p - q, 0) in ascending order -- CTA, thread, token -- in fp64, since a token stands or falls with
 //                        one comparison of a sum over the vocabulary: with 131,071 tokens and fp32 sums one draw of ten would be near a border.
 //
-// 2^y in fp64: y = n / 64 + r, |r| <= 1 / 128, 2^(n mod 64 / 64) from a table, 2^r by its Taylor series to r^5 (the next term is below 2^-54).
-
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "vx_common.cuh"
 #include "vx_paged.cuh"
@@ -24,13 +24,19 @@ namespace {
 
 constexpr int VR_THREADS = 256;
 constexpr int VN_THREADS = 512;
+#ifndef VR_LEAST
+#define VR_LEAST 4096
+#endif
+#ifndef VN_LEAST
+#define VN_LEAST 4096
+#endif
 constexpr unsigned ALL = 0xffffffffu;
 
 enum Draft : int32_t { kFalls = 0, kStands = 1, kOpen = 2 };
 
 // What the first launch leaves of a row.
 struct RowFinding {
-  float most, draft_most;  // largest logits
+  float most, draft_most;  // largest logits; most NaN: nothing is drawn from the row
   int32_t draft;           // Draft
   int32_t best;            // temperature 0: its first largest token, -1: none
 };
@@ -231,16 +237,18 @@ __global__ void __launch_bounds__(VR_THREADS) verify_rows_kernel(const __grid_co
       }
     }
     RowFinding f{a[0].m, a[1].m, kFalls, -1};
+    auto sound = [](const Running& r) { return r.sum > 0.0f && r.sum < INFINITY && fabsf(r.m) < INFINITY; };  // (NaN among the logits: the sum is)
+    if (!GREEDY && !(sound(a[0]) && (!drafter || sound(a[1])))) f.most = NAN;  // nothing is drawn from this row
     const int64_t d = last ? -1 : id_at(p, row + 1);
     const bool known = d >= 0 && d < p.vocab;
     if (GREEDY) {
       // (a maximum that is not finite, or NaN among the logits: none)
       f.best = a[0].sum == 0.0f && fabsf(a[0].m) < INFINITY ? a[0].at : -1;
       if (known && f.best == d) f.draft = kStands;
-    } else if (known) {
+    } else if (known && f.most == f.most) {
       const float pt = ex2((to_float(row_t[d]) - a[0].m) * c), qd = drafter ? ex2((to_float(row_d[d]) - a[1].m) * c) : 1.0f;
       const float left = p.uniforms[row].x * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * 0x1p-12f;
-      // (anything that is NaN, infinite or near the end of the range is open)
+      // (anything near the end of the range is open)
       if (!(left > 1e-30f && right > 1e-30f && left < 1e30f && right < 1e30f) || fabsf(left - right) <= gap) f.draft = kOpen;
       else f.draft = left < right ? kStands : kFalls;
     }
@@ -251,35 +259,61 @@ __global__ void __launch_bounds__(VR_THREADS) verify_rows_kernel(const __grid_co
 
 // ---------------------------------------------------------------- the token behind
 
-struct Exp2Table {
-  double t[64];
+// 2^y = 2^floor(n / 1024) 2^(n mod 1024 / 1024) 2^r with n = 1024 y rounded, |r| <= 1 / 2048: the second factor from a table, which a block makes of two of
+// 32, the third by its Taylor series to r^3 (the next term is below 2^-50).  (A table of 64 and a series to r^5: three of eleven fp64 operations more.)
+constexpr int kExpTable = 1024;
+__device__ const double kCoarse[32] = {  // 2^(k / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+__device__ const double kFine[32] = {  // 2^(k / 1024)
+    1.0, 1.0006771306930664, 1.0013547198921082, 1.002032767907594, 1.0027112750502025, 1.0033902416308227, 1.004069667960554, 1.0047495543507072,
+    1.0054299011128027, 1.006110708558573, 1.0067919769999607, 1.0074737067491204, 1.0081558981184175, 1.0088385514204294, 1.0095216669679448, 1.0102052450739643,
+    1.0108892860517005, 1.011573790214578, 1.0122587578762337, 1.0129441893505169, 1.0136300849514894, 1.0143164449934257, 1.0150032697908125, 1.0156905596583505,
+    1.016378314910953, 1.0170665358637463, 1.0177552228320703, 1.0184443761314785, 1.019133996077738, 1.0198240829868295, 1.0205146371749483, 1.0212056589585028};
+
+// 2^((x - at) c) for x <= at; 0 below 2^-1000
+struct Weight {
+  double c, from;  // from: at c
+  float c32, at;
+  __device__ __forceinline__ double operator()(const double* tab, float x) const {
+    constexpr double big = 6755399441055744.0 / kExpTable;  // 1.5 2^52 / 1024: the last bit of a sum is 1 / 1024
+    const double y = fma(static_cast<double>(x), c, -from), t = y + big, r = y - (t - big);
+    const int n = __double2loint(t);
+    constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3;
+    const double s = tab[n & (kExpTable - 1)], v = fma(s, fma(fma(c3, r, c2), r, c1) * r, s);
+    const int high = __double2hiint(v) + ((n >> 10) << 20);
+    return (x - at) * c32 >= -1000.0f ? __hiloint2double(high, __double2loint(v)) : 0.0;
+  }
 };
-// 2^y for y <= 0
-__device__ __forceinline__ double exp2_fp64(const Exp2Table& tab, double y) {
-  if (!(y >= -1020.0)) return y != y ? y : 0.0;
-  const double big = 6755399441055744.0 / 64.0;  // 1.5 2^52 / 64: the last bit of a sum is 1 / 64
-  const double t = y + big, r = y - (t - big);
-  const int n = __double2loint(t);
-  constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5;
-  const double s = tab.t[n & 63], q = fma(fma(fma(fma(c5, r, c4), r, c3), r, c2), r, c1) * r, v = fma(s, q, s);
-  return __hiloint2double(__double2hiint(v) + ((n >> 6) << 20), __double2loint(v));
-}
 
 __device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
   return x;
 }
+__device__ __forceinline__ double warp_scan(double x) {  // the sum up to this lane, its own included
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(ALL, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
 
+// The tokens of a CTA are a run of the vocabulary, those of its warps runs of that, and a warp takes 32 neighbours at a time: sums by warps are sums in
+// ascending order, whose first to pass a number tells the warp that has the token.
 template <typename T>
-__global__ void __launch_bounds__(VN_THREADS) verify_next_kernel(const __grid_constant__ VerifyParams p, int ctas) {
+__global__ void __launch_bounds__(VN_THREADS, 2) verify_next_kernel(const __grid_constant__ VerifyParams p, int ctas) {
   pdl_launch_dependents();
-  __shared__ Exp2Table tab;
-  __shared__ double warp_s[2][VN_THREADS / 32], cta_s[2][2];  // cta_s: in turn, so that one cluster barrier per exchange is enough
+  constexpr int WARPS = VN_THREADS / 32, AHEAD = 4;
+  __shared__ double tab[kExpTable];
+  __shared__ double warp_s[2][2][WARPS], cta_s[2][2];  // each in turn, so that one barrier per exchange is enough
   const int s = static_cast<int>(blockIdx.x) / ctas, rank = static_cast<int>(blockIdx.x) - s * ctas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x < 64) tab.t[threadIdx.x] = exp2(threadIdx.x / 64.0);
-  __syncthreads();
+  for (int i = threadIdx.x; i < kExpTable; i += VN_THREADS) tab[i] = kCoarse[i >> 5] * kFine[i & 31];
   pdl_wait();
   const int row0 = first_row_of(p, s), row1 = first_row_of(p, s + 1), drafts = row1 - row0 - 1;
   const bool writer = rank == 0 && threadIdx.x == 0;
@@ -290,35 +324,52 @@ __global__ void __launch_bounds__(VN_THREADS) verify_next_kernel(const __grid_co
     }
     return;
   }
+  // The first draft from one on that does not stand for certain, and what was found of its row: 32 rows at a time, a lane each.
+  RowFinding found;
+  auto first_doubt = [&](int from) {
+    while (true) {
+      const int n = min(drafts - from + 1, 32);  // (with the row behind the last draft)
+      const RowFinding f = p.found[row0 + from + min(lane, n - 1)];
+      const unsigned doubt = __ballot_sync(ALL, lane < n && (f.draft != kStands || from + lane == drafts));
+      if (doubt) {
+        const int at = __ffs(doubt) - 1;
+        found.most = __shfl_sync(ALL, f.most, at);
+        found.draft_most = __shfl_sync(ALL, f.draft_most, at);
+        found.draft = __shfl_sync(ALL, f.draft, at);
+        found.best = __shfl_sync(ALL, f.best, at);
+        return from + at;
+      }
+      from += n;
+    }
+  };
   if (p.greedy) {
-    if (writer) {
-      int i = 0;
-      while (i < drafts && p.found[row0 + i].draft == kStands) ++i;
-      p.accepted[s] = i;
-      p.next[s] = p.found[row0 + i].best;
+    if (warp == 0 && rank == 0) {
+      const int i = first_doubt(0);
+      if (lane == 0) {
+        p.accepted[s] = i;
+        p.next[s] = found.best;
+      }
     }
     return;
   }
-  // this thread's tokens, in a row
-  const int each = (p.vocab + ctas * VN_THREADS - 1) / (ctas * VN_THREADS);
-  const int v0 = min((rank * VN_THREADS + static_cast<int>(threadIdx.x)) * each, p.vocab), v1 = min(v0 + each, p.vocab);
+  // this warp's tokens
+  const int each = ((p.vocab + ctas * WARPS - 1) / (ctas * WARPS) + 31) / 32 * 32;
+  const int v0 = min((rank * WARPS + warp) * each, p.vocab), v1 = min(v0 + each, p.vocab);
   int turn = 0;
-  // a and b summed over the cluster, the CTAs' a in front of this one in `before`
+  // a and b, the warps' own, summed over the cluster; the sums of a in front of this warp in `before`
   auto sum_all = [&](double& a, double& b, double& before) {
-    a = warp_sum(a);
-    b = warp_sum(b);
+    turn ^= 1;
     if (lane == 0) {
-      warp_s[0][warp] = a;
-      warp_s[1][warp] = b;
+      warp_s[turn][0][warp] = a;
+      warp_s[turn][1][warp] = b;
     }
     __syncthreads();
-    a = b = before = 0.0;
-    for (int w = 0; w < VN_THREADS / 32; ++w) {
-      a += warp_s[0][w];
-      b += warp_s[1][w];
-    }
+    const double up = warp_scan(lane < WARPS ? warp_s[turn][0][lane] : 0.0);
+    a = __shfl_sync(ALL, up, 31);
+    before = __shfl_sync(ALL, up, (warp + 31) & 31);
+    if (warp == 0) before = 0.0;
+    b = warp_sum(lane < WARPS ? warp_s[turn][1][lane] : 0.0);
     if (ctas > 1) {
-      turn ^= 1;
       if (threadIdx.x == 0) {
         cta_s[turn][0] = a;
         cta_s[turn][1] = b;
@@ -326,143 +377,176 @@ __global__ void __launch_bounds__(VN_THREADS) verify_next_kernel(const __grid_co
       cluster_sync_all();
       a = b = 0.0;
       for (int k = 0; k < ctas; ++k) {
-        if (k == rank) before = a;
+        if (k == rank) before += a;
         a += ld_cluster(&cta_s[turn][0], k);
         b += ld_cluster(&cta_s[turn][1], k);
       }
     }
-    __syncthreads();
   };
-  struct Row {
-    const T *t, *d;
-    double mt, md, zt, zd;
-    int64_t draft;  // the token, where the drafter was sure; -1: none
-  };
-  auto weight_t = [&](const Row& r, int v) { return exp2_fp64(tab, (static_cast<double>(to_float(r.t[v])) - r.mt) * p.log2e_t); };
-  auto weight_d = [&](const Row& r, int v) { return exp2_fp64(tab, (static_cast<double>(to_float(r.d[v])) - r.md) * p.log2e_t); };
-  auto open_row = [&](int row, bool last) {  // with the sums of both sides
-    Row r{static_cast<const T*>(p.logits) + row * p.ld, nullptr, p.found[row].most, 0.0, 0.0, 0.0, -1};
-    if (!last && p.draft_logits) {
-      r.d = static_cast<const T*>(p.draft_logits) + row * p.ld_draft;
-      r.md = p.found[row].draft_most;
-    } else if (!last) {
-      r.draft = id_at(p, row + 1);
+  // The row that is looked at: weights of its tokens, times 2^(largest logit c); the drafter's
+  const double c = p.log2e_t;
+  const T *t, *d;   // d: NULL without a drafter
+  Weight wt, wd;
+  int sure;         // the draft, where the drafter was sure of it; -1: none
+  auto begin_row = [&](int i) {
+    const int row = row0 + i;
+    t = static_cast<const T*>(p.logits) + row * p.ld;
+    d = i < drafts && p.draft_logits ? static_cast<const T*>(p.draft_logits) + row * p.ld_draft : nullptr;
+    wt = {c, static_cast<double>(found.most) * c, static_cast<float>(c), found.most};
+    wd = {c, static_cast<double>(found.draft_most) * c, static_cast<float>(c), found.draft_most};
+    sure = -1;
+    if (i < drafts && !p.draft_logits) {
+      const int64_t id = id_at(p, row + 1);
+      if (id >= 0 && id < p.vocab) sure = static_cast<int>(id);
     }
-    double a = 0.0, b = 0.0, before;
-#pragma unroll 4
-    for (int v = v0; v < v1; ++v) {
-      a += weight_t(r, v);
-      if (r.d) b += weight_d(r, v);
+  };
+  // What is left of a token's weight: the target's less `ratio` of the drafter's, where that is above 0, nothing for the token `out`.  One body for the sums
+  // (ratio 0) and for what is drawn from: what is fetched for the first time costs here.  BOTH: there is a drafter.
+  double ratio = 0.0;
+  int out = -1;
+  auto left_of = [&](auto both, int v, float x, float y, double& drafter) {
+    double w = wt(tab, x);
+    if (decltype(both)::value) {
+      drafter = wd(tab, y);
+      w = fma(drafter, -ratio, w);
+      if (__double2hiint(w) < 0) w = 0.0;
     }
-    sum_all(a, b, before);
-    r.zt = a;
-    r.zd = b;
-    return r;
+    return v == out ? 0.0 : w;
   };
-  int i = 0;
-  Row r;
-  bool opened = false;
-  for (; i < drafts; ++i) {
-    const int found = p.found[row0 + i].draft;
-    opened = false;
-    if (found == kStands) continue;
-    if (found == kFalls) break;
-    r = open_row(row0 + i, false);
-    opened = true;
-    const int64_t d = id_at(p, row0 + i + 1);
-    if (d < 0 || d >= p.vocab) break;
-    const double left = static_cast<double>(p.uniforms[row0 + i].x) * (r.d ? weight_d(r, static_cast<int>(d)) / r.zd : 1.0);
-    if (!(left < weight_t(r, static_cast<int>(d)) / r.zt)) break;
-  }
-  const int row = row0 + i;
-  if (!(opened && i < drafts)) r = open_row(row, i == drafts);
-  // what is drawn from
-  const bool rest = r.d != nullptr || r.draft >= 0;
-  const double inv_t = 1.0 / r.zt, inv_d = r.d ? 1.0 / r.zd : 0.0;
-  auto left_at = [&](int v, bool rest) {
-    double x = weight_t(r, v) * inv_t;
-    if (rest && r.d) x = fmax(x - weight_d(r, v) * inv_d, 0.0);
-    else if (rest && v == r.draft) x = 0.0;
-    return x;
-  };
-  int chosen = -1;
-  const bool sound = r.zt > 0.0 && r.zt < INFINITY && (!r.d || (r.zd > 0.0 && r.zd < INFINITY));
-  for (int pass = rest ? 0 : 1; sound && pass < 2; ++pass) {  // (uniform over the cluster)
-    double mine = 0.0, unused = 0.0, before;
-#pragma unroll 4
-    for (int v = v0; v < v1; ++v) mine += left_at(v, pass == 0);
-    // sums in front of this thread
-    double up = mine;
+  // sums over this warp's tokens, 32 at a time in ascending order, the next AHEAD groups on their way
+  auto walk_row = [&](auto both, double& a, double& b) {
+    constexpr bool BOTH = decltype(both)::value;
+    float x[AHEAD], y[AHEAD];
+    auto load = [&](int v) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(ALL, up, o);
-      if (lane >= o) up += y;
+      for (int e = 0; e < AHEAD; ++e) {  // (behind the end: of no weight)
+        x[e] = v + 32 * e < v1 ? to_float(t[v + 32 * e]) : -INFINITY;
+        y[e] = BOTH && v + 32 * e < v1 ? to_float(d[v + 32 * e]) : -INFINITY;
+      }
+    };
+    double sum[2] = {0.0, 0.0}, other[2] = {0.0, 0.0};
+    load(v0 + lane);
+#pragma unroll 1
+    for (int v = v0 + lane; v - lane < v1; v += 32 * AHEAD) {
+      float x0[AHEAD], y0[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        x0[e] = x[e];
+        y0[e] = y[e];
+      }
+      load(v + 32 * AHEAD);
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        double drafter = 0.0;
+        sum[e & 1] += left_of(both, v + 32 * e, x0[e], y0[e], drafter);
+        other[e & 1] += drafter;
+      }
     }
-    double all = mine;
-    sum_all(all, unused, before);
-    if (!(all > 0.0)) continue;
-    for (int w = 0; w < warp; ++w) before += warp_s[0][w];
-    const double target = static_cast<double>(p.uniforms[row].y) * all;
-    // The first thread whose sum passes the target has the token; rounding, or a number that is not below 1, can leave none: then the last with a weight.
-    const bool passes = before + up > target, weighs = mine > 0.0;
-    __shared__ int first_s[2], seen_s[2][2];
+    a = warp_sum(sum[0] + sum[1]);
+    b = BOTH ? warp_sum(other[0] + other[1]) : 0.0;
+  };
+  __syncthreads();  // (the table)
+  int i = first_doubt(0), chosen = -1;
+  bool mine = false;                            // this warp has the token
+  enum { kSums, kRest, kAll } what = kSums;     // what is summed up
+  if (found.most == found.most) begin_row(i);
+#pragma unroll 1
+  while (found.most == found.most) {            // (uniform over the cluster; NaN: nothing is drawn from the row)
+    double own, all, others, before;
+    if (d) walk_row(std::true_type{}, own, others);
+    else walk_row(std::false_type{}, own, others);
+    all = own;
+    sum_all(all, others, before);
+    if (what == kSums) {
+      if (i < drafts && found.draft == kOpen) {
+        const int64_t id = id_at(p, row0 + i + 1);
+        if (id >= 0 && id < p.vocab) {
+          const double left = static_cast<double>(p.uniforms[row0 + i].x) * (d ? wd(tab, to_float(d[id])) / others : 1.0);
+          if (left < wt(tab, to_float(t[id])) / all) {
+            i = first_doubt(i + 1);
+            begin_row(i);
+            continue;
+          }
+        }
+      }
+      what = kAll;
+      if (d || sure >= 0) {
+        what = kRest;
+        ratio = d ? all / others : 0.0;
+        out = sure;
+        continue;
+      }
+    } else if (what == kRest && !(all > 0.0)) {  // nothing is left: p
+      what = kAll;
+      ratio = 0.0;
+      out = -1;
+      continue;
+    }
+    const double target = static_cast<double>(p.uniforms[row0 + i].y) * all;
+    // The first warp whose sum passes the target has the token; a number that is not below 1 (or rounding) can leave none: then the last with a weight.
+    __shared__ int first_s[2], seen_s[2];
     if (threadIdx.x == 0) first_s[0] = 0x7fffffff, first_s[1] = -1;
     __syncthreads();
-    const unsigned who = __ballot_sync(ALL, passes && weighs), weigh = __ballot_sync(ALL, weighs);
-    if (lane == 0) {
-      if (who) atomicMin(&first_s[0], warp * 32 + __ffs(who) - 1);
-      if (weigh) atomicMax(&first_s[1], warp * 32 + 31 - __clz(weigh));
+    if (lane == 0 && own > 0.0) {
+      if (before + own > target) atomicMin(&first_s[0], warp);
+      atomicMax(&first_s[1], warp);
     }
     __syncthreads();
-    int from = first_s[0], lastly = first_s[1], owner = from != 0x7fffffff ? rank : -1;
-    bool exact = from != 0x7fffffff;
+    int from = first_s[0], owner = from != 0x7fffffff ? rank : -1;
     if (ctas > 1) {
-      if (threadIdx.x == 0) seen_s[pass][0] = from, seen_s[pass][1] = lastly;
+      if (threadIdx.x < 2) seen_s[threadIdx.x] = first_s[threadIdx.x];
       cluster_sync_all();
       owner = -1;
       int fallback = -1;
       for (int k = ctas - 1; k >= 0; --k) {
-        if (ld_cluster(&seen_s[pass][0], k) != 0x7fffffff) owner = k;
-        if (fallback < 0 && ld_cluster(&seen_s[pass][1], k) >= 0) fallback = k;
+        if (ld_cluster(&seen_s[0], k) != 0x7fffffff) owner = k;
+        if (fallback < 0 && ld_cluster(&seen_s[1], k) >= 0) fallback = k;
       }
-      exact = owner >= 0;
-      if (!exact) owner = fallback;
-    } else if (!exact) {
+      if (owner < 0) {
+        owner = fallback;
+        from = 0x7fffffff;
+      }
+    } else {
       owner = 0;
     }
-    if (owner == rank) {
-      const int thread = exact ? from : lastly;
-      if (warp == thread >> 5) {  // its tokens by the lanes of the warp
-        const double base = __shfl_sync(ALL, before + up - mine, thread & 31);
-        const int a0 = __shfl_sync(ALL, v0, thread & 31), a1 = __shfl_sync(ALL, v1, thread & 31);
-        double sum = base;
-        int pick = -1, heavy = -1;
-        for (int v = a0; v < a1 && pick < 0; v += 32) {
-          double x = v + lane < a1 ? left_at(v + lane, pass == 0) : 0.0;
-          const unsigned has = __ballot_sync(ALL, x > 0.0);
-          if (has) heavy = v + 31 - __clz(has);
+    const bool exact = from != 0x7fffffff;
+    mine = owner == rank && warp == (exact ? from : first_s[1]);
+    if (mine) {
+      // groups of 32 neighbours, four at a time: their sums, the first that passes the target, its lanes
+      double sum = before;
+      int pick = -1, heavy = -1;
+#pragma unroll 1
+      for (int v = v0; v < v1 && pick < 0; v += 32 * AHEAD) {
+        double x[AHEAD], group[AHEAD];
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(ALL, x, o);
-            if (lane >= o) x += y;
-          }
-          const unsigned over = __ballot_sync(ALL, sum + x > target) & has;
-          if (over && exact) pick = v + __ffs(over) - 1;
-          sum += __shfl_sync(ALL, x, 31);
+        for (int e = 0; e < AHEAD; ++e) {
+          const int at = v + 32 * e + lane;
+          double drafter;
+          const float l = at < v1 ? to_float(t[at]) : -INFINITY;
+          x[e] = d ? left_of(std::true_type{}, at, l, at < v1 ? to_float(d[at]) : -INFINITY, drafter) : left_of(std::false_type{}, at, l, 0.0f, drafter);
         }
-        chosen = pick >= 0 ? pick : heavy;
-        if (lane == 0) {
-          p.accepted[s] = i;
-          p.next[s] = chosen;
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+          const unsigned has = __ballot_sync(ALL, x[e] > 0.0);
+          if (has) heavy = v + 32 * e + 31 - __clz(has);
+          group[e] = warp_sum(x[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+          if (exact && pick < 0 && sum + group[e] > target) {
+            const unsigned has = __ballot_sync(ALL, x[e] > 0.0), over = __ballot_sync(ALL, sum + warp_scan(x[e]) > target) & has;
+            pick = v + 32 * e + (over ? __ffs(over) - 1 : 31 - __clz(has));  // (a group of no weight does not pass)
+          }
+          sum += group[e];
         }
       }
+      chosen = pick >= 0 ? pick : heavy;
     }
-    if (ctas > 1) cluster_sync_all();
-    return;
+    break;
   }
-  if (writer) {
+  if (chosen < 0 ? writer && found.most != found.most : lane == 0) {
     p.accepted[s] = i;
-    p.next[s] = -1;
+    p.next[s] = chosen;
   }
   if (ctas > 1) cluster_sync_all();  // (shared memory of a CTA that ended is not read)
 }
@@ -490,10 +574,10 @@ cudaError_t launch_clusters(K kernel, int64_t owners, int ctas, int threads, cud
   cfg.numAttrs = static_cast<unsigned>(n);
   return cudaLaunchKernelEx(&cfg, kernel, p, ctas);
 }
-// CTAs per owner: while SMs would be left without one and each has `least` values
-int cluster_size(int64_t owners, int64_t values, int64_t least) {
+// CTAs per owner: while there are fewer than `wanted` of them in all and each has `least` values or more
+int cluster_size(int64_t owners, int64_t wanted, int64_t values, int64_t least) {
   int c = 1;
-  while (c < 8 && 2 * c * owners <= 2 * static_cast<int64_t>(sm_count()) && values >= 2 * c * least) c *= 2;
+  while (c < 8 && c * owners < wanted && values >= 2 * c * least) c *= 2;
   return c;
 }
 
@@ -540,12 +624,12 @@ extern "C" int vx_verify_drafts(const vx_verify_desc* d, void* stream) {
   const auto st = static_cast<cudaStream_t>(stream);
   const bool f32 = d->dtype == VX_F32;
   if (d->rows > 0) {
-    const int ctas = cluster_size(d->rows, d->vocab, 2048);
+    const int ctas = cluster_size(d->rows, 6 * static_cast<int64_t>(sm_count()), d->vocab, VR_LEAST);
     auto kernel = p.greedy ? (f32 ? verify_rows_kernel<float, true> : verify_rows_kernel<__nv_bfloat16, true>)
                            : (f32 ? verify_rows_kernel<float, false> : verify_rows_kernel<__nv_bfloat16, false>);
     VX_CUDA_OK(launch_clusters(kernel, d->rows, ctas, VR_THREADS, st, p));
   }
-  const int ctas = p.greedy ? 1 : cluster_size(d->sequences, d->vocab, VN_THREADS);
+  const int ctas = p.greedy ? 1 : cluster_size(d->sequences, 3 * static_cast<int64_t>(sm_count()), d->vocab, VN_LEAST);
   VX_CUDA_OK(launch_clusters(f32 ? verify_next_kernel<float> : verify_next_kernel<__nv_bfloat16>, d->sequences, ctas, VN_THREADS, st, p));
   return 0;
 }
