@@ -95,7 +95,7 @@ namespace {
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_BLOCKS = 6;     // per SM, at 40 registers a thread: five of 46 take 375 us at the size above, seven or eight, which spill, 507
-constexpr int AP_BLOCKS_FP4 = 4;
+constexpr int AP_BLOCKS_FP4 = 5;  // at 48 registers: 384 us for four of 62 389, six 399 (and with 17 divisions for 16 values, four of them, 418)
 constexpr int AP_UNITS = 16;     // of a thread in large calls, since a block looks its rows up before it moves any: 4 take 422 us there, 8 391, 16 375 (of five blocks)
 constexpr int AP_MAX_ROWS = 32;  // rows of a block at most
 
@@ -183,20 +183,32 @@ __device__ __forceinline__ void rotated8(const AppendParams& p, const T* src, co
   }
 }
 
-// Sixteen values to codes and their scale.  Divided by 16 values' scale the quotient is rounded to fp32 first: a value whose significand has 24 bits at most,
-// over a scale whose significand has 4, is a border between two codes exactly or is off it by more than half a unit, so the code is that of the
-// exact quotient.  (A quotient in the range of fp32's subnormals is far below the first border.)
+// Sixteen values to codes and their scale.  The quotient by the scale is rounded to fp32 first: a value whose significand has 24 bits at most, over a scale whose
+// significand has 4, is a border between two codes exactly or is off it by more than half a unit, so the code is that of the exact quotient.  A
+// quotient is formed from the correctly rounded reciprocal and one remainder step (Markstein, IBM J. Res. Dev. 34(1), 1990, see Nv16Tensor); below fp32's
+// normal range it is far below the first border.  (17 divisions instead: see AP_BLOCKS_FP4.)
 __device__ __forceinline__ uint2 quantize16(const float (&a)[8], const float (&b)[8], float inv_g, uint32_t& byte) {
   const float most = __fmul_rn(fmaxf(amax8(a), amax8(b)), inv_g);
-  byte = __nv_cvt_float_to_fp8(__fdiv_rn(most, 6.0f), __NV_SATFINITE, __NV_E4M3) & 0x7fu;
+  constexpr float kSixth = 1.0f / 6.0f;  // correctly rounded
+  const float sixth = __fmul_rn(most, kSixth);
+  byte = __nv_cvt_float_to_fp8(most < 1e30f ? __fmaf_rn(__fmaf_rn(-sixth, 6.0f, most), kSixth, sixth) : most, __NV_SATFINITE, __NV_E4M3) & 0x7fu;
   const float s = e4m3_to_float(byte);
   if (byte == 0) return make_uint2(0, 0);
+  const float r = __frcp_rn(s);
+  const uint64_t g2 = pack_f32x2(inv_g, inv_g), r2 = pack_f32x2(r, r), s2 = pack_f32x2(-s, -s);
   uint32_t w[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     float q[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(__fmul_rn(e ? b[j] : a[j], inv_g), s);
+    for (int j = 0; j < 8; j += 2) {
+      const uint64_t x = mul_f32x2(e ? pack_f32x2(b[j], b[j + 1]) : pack_f32x2(a[j], a[j + 1]), g2), q0 = mul_f32x2(x, r2);
+      unpack_f32x2(fma_f32x2(fma_f32x2(q0, s2, x), r2, q0), q[j], q[j + 1]);
+    }
+    if (!(most < 1e30f)) {  // (infinities: to the largest codes of their signs)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = __fmul_rn(e ? b[j] : a[j], inv_g) * r;
+    }
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"

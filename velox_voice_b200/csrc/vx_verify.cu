@@ -574,10 +574,10 @@ cudaError_t launch_clusters(K kernel, int64_t owners, int ctas, int threads, cud
   cfg.numAttrs = static_cast<unsigned>(n);
   return cudaLaunchKernelEx(&cfg, kernel, p, ctas);
 }
-// CTAs per owner: while there are fewer than `wanted` of them in all and each has `least` values or more
-int cluster_size(int64_t owners, int64_t wanted, int64_t values, int64_t least) {
+// CTAs per owner: as many as leave no more than `most` in all and each `least` values or more
+int cluster_size(int64_t owners, int64_t most, int64_t values, int64_t least) {
   int c = 1;
-  while (c < 8 && c * owners < wanted && values >= 2 * c * least) c *= 2;
+  while (c < 8 && 2 * c * owners <= most && values >= 2 * c * least) c *= 2;
   return c;
 }
 
@@ -624,12 +624,12 @@ extern "C" int vx_verify_drafts(const vx_verify_desc* d, void* stream) {
   const auto st = static_cast<cudaStream_t>(stream);
   const bool f32 = d->dtype == VX_F32;
   if (d->rows > 0) {
-    const int ctas = cluster_size(d->rows, 6 * static_cast<int64_t>(sm_count()), d->vocab, VR_LEAST);
+    const int ctas = cluster_size(d->rows, 12 * static_cast<int64_t>(sm_count()), d->vocab, VR_LEAST);
     auto kernel = p.greedy ? (f32 ? verify_rows_kernel<float, true> : verify_rows_kernel<__nv_bfloat16, true>)
                            : (f32 ? verify_rows_kernel<float, false> : verify_rows_kernel<__nv_bfloat16, false>);
     VX_CUDA_OK(launch_clusters(kernel, d->rows, ctas, VR_THREADS, st, p));
   }
-  const int ctas = p.greedy ? 1 : cluster_size(d->sequences, 3 * static_cast<int64_t>(sm_count()), d->vocab, VN_LEAST);
+  const int ctas = p.greedy ? 1 : cluster_size(d->sequences, 2 * static_cast<int64_t>(sm_count()), d->vocab, VN_LEAST);
   VX_CUDA_OK(launch_clusters(f32 ? verify_next_kernel<float> : verify_next_kernel<__nv_bfloat16>, d->sequences, ctas, VN_THREADS, st, p));
   return 0;
 }
