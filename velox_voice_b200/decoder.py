@@ -9,9 +9,11 @@ once and become a prefix that all of its hypotheses share; each hypothesis then 
 
 in three uses of the same two operators (:func:`ops.kv_append`, :func:`ops.prefix_attention`): :meth:`HypothesisDecoder.read`
 (frames, many rows of a sequence, no prefix), :meth:`~HypothesisDecoder.step` (a token per hypothesis) and
-:meth:`~HypothesisDecoder.score` (whole hypotheses at once).
+:meth:`~HypothesisDecoder.score` (whole hypotheses at once).  :meth:`~HypothesisDecoder.verify` scores drafts and keeps those that stand
+(:func:`ops.verify_drafts`).  The cache is bf16, or 4 bits a value and a scale for 16 (``DecoderConfig(cache="fp4")``).
 
-``python -m velox_voice_b200.decoder`` reads an utterance and decodes ten hypotheses of it, with random weights.
+``python -m velox_voice_b200.decoder`` reads an utterance and decodes ten hypotheses of it, with random weights; ``--cache fp4`` with a cache in 4
+bits, ``--drafts 4`` with four drafts a step, from a decoder of the first blocks.
 """
 
 from __future__ import annotations
@@ -37,6 +39,7 @@ class DecoderConfig:
     page_size: int = 16
     positions: int = 8192  # frames and tokens of a hypothesis together
     eps: float = 1e-5
+    cache: str = "bf16"  # or "fp4": page_size a multiple of 16
 
     @property
     def head_dim(self) -> int:
@@ -113,9 +116,15 @@ class HypothesisDecoder:
         self.after, self.head = norm("after"), pack("head")
         self.embed = weights["embed"].to(dev).bfloat16()
         self.rotary = ops.rotary_table(cfg.positions, cfg.head_dim, device=dev)
-        shape = (cfg.blocks, pages, cfg.page_size, cfg.kv_heads, cfg.head_dim)
-        self.k_pages = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-        self.v_pages = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        # [blocks, pages, ...]
+        if cfg.cache == "fp4":
+            self.k_pages, self.v_pages = (ops.fp4_pages(cfg.blocks * pages, cfg.page_size, cfg.kv_heads, cfg.head_dim, device=dev).unflatten(0, (cfg.blocks, pages))
+                                          for _ in range(2))
+        elif cfg.cache == "bf16":
+            shape = (cfg.blocks, pages, cfg.page_size, cfg.kv_heads, cfg.head_dim)
+            self.k_pages, self.v_pages = (torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        else:
+            raise ValueError(f"cache must be 'bf16' or 'fp4', got {cfg.cache!r}")
         self._free = list(range(pages))
 
     # ---- pages
@@ -214,6 +223,23 @@ class HypothesisDecoder:
 
     def score(self, hyp: Hypotheses, ids: torch.Tensor, counts: Sequence[int]) -> torch.Tensor:
         """Whole continuations at once: ids [sum(counts)], hypothesis after hypothesis -> bf16 logits [sum(counts), vocab]."""
+        return self._score(hyp, ids, counts)[0]
+
+    def verify(self, hyp: Hypotheses, ids: torch.Tensor, counts: Sequence[int], uniforms: torch.Tensor, *, draft_logits=None, temperature: float = 1.0):
+        """Drafts: ids [sum(counts)] are, hypothesis after hypothesis, the token that :meth:`step` or this gave last and the drafts behind it; arguments and
+        results (accepted, next) of :func:`ops.verify_drafts`.  The cache keeps the first token of a hypothesis and its drafts that stand.  (A hypothesis of
+        no ids, or one that has finished, stays as it is, whatever the results say.)  `hyp.tokens` counts all drafts: :meth:`settle` after some calls."""
+        logits, offsets, n = self._score(hyp, ids, counts)
+        accepted, following = ops.verify_drafts(logits, ids, uniforms, draft_logits=draft_logits, row_offsets=offsets, temperature=temperature)
+        hyp.lengths.sub_(torch.where((hyp.lengths >= 0) & (n > 0), n - 1 - accepted, 0))
+        return accepted, following
+
+    def settle(self, hyp: Hypotheses) -> None:
+        """Counts the tokens of the hypotheses as they are on the device (waits for it): drafts that did not stand give their room back."""
+        self._held(hyp)
+        hyp.tokens = [min(t, m) if m >= 0 else t for t, m in zip(hyp.tokens, hyp.lengths.tolist())]
+
+    def _score(self, hyp: Hypotheses, ids: torch.Tensor, counts: Sequence[int]):
         counts = list(counts)
         if len(counts) != len(hyp.tokens) or min(counts) < 0 or sum(counts) != ids.numel():
             raise ValueError(f"counts must be those of {len(hyp.tokens)} hypotheses and sum to {ids.numel()} ids, got {counts}")
@@ -224,7 +250,7 @@ class HypothesisDecoder:
         x = self._hidden(hyp, ids, offsets)
         hyp.lengths.add_(torch.where(hyp.lengths >= 0, n, 0))
         hyp.tokens = tokens
-        return self.head(ops.ln_quantize(x, *self.after, self.cfg.eps, self.cfg.fmt))
+        return self.head(ops.ln_quantize(x, *self.after, self.cfg.eps, self.cfg.fmt)), offsets, n
 
     def compile_step(self, hyp: Hypotheses):
         """``step`` as a CUDA graph: a function of ids (copied in) that returns the graph's own output."""
@@ -251,6 +277,29 @@ class HypothesisDecoder:
         return run
 
 
+def _drafted(o, cfg: DecoderConfig, weights, pages: int, frames: torch.Tensor, dec: HypothesisDecoder, hyp: Hypotheses, ids: torch.Tensor) -> None:
+    """Decodes with drafts of a decoder of the first blocks, which takes back what did not stand, until each hypothesis has its tokens."""
+    small = HypothesisDecoder(DecoderConfig(**{**vars(cfg), "blocks": max(1, cfg.blocks // 3)}), weights, pages=pages)
+    guess = small.begin(small.read(frames, [o.frames] * o.utterances), o.beams, hyp.max_tokens)
+    n, rows, rounds, stood = ids.numel(), o.drafts + 1, 0, 0
+    while min(hyp.tokens) < o.tokens:
+        drafts, logits = [ids], []
+        for _ in range(rows):  # (the last one only for its place in the small decoder's cache)
+            logits.append(small.score(guess, drafts[-1], [1] * n))
+            drafts.append(torch.distributions.Categorical(logits=logits[-1].float()).sample())
+        given = torch.stack(drafts[:rows], 1).flatten()
+        live = hyp.lengths >= 0
+        accepted, following = dec.verify(hyp, given, [rows] * n, torch.rand(n * rows, 2, device=ids.device), draft_logits=torch.stack(logits, 1).flatten(0, 1))
+        guess.lengths.copy_(hyp.lengths)
+        for x in (hyp, guess):
+            (dec if x is hyp else small).settle(x)
+            x.lengths.masked_fill_(x.lengths >= o.tokens, -1)  # finished: takes no more part
+            x.tokens = [min(t, o.tokens) for t in x.tokens]
+        ids, rounds, stood = following.long(), rounds + 1, stood + int((accepted * live).sum())
+    print(f"{o.utterances} x {o.beams} hypotheses over {o.frames} frames, {o.drafts} drafts a step: {rounds} steps for {o.tokens} tokens, "
+          f"{stood / rounds / n:.2f} drafts stood in one")
+
+
 def main() -> None:
     import argparse
 
@@ -259,15 +308,22 @@ def main() -> None:
     a.add_argument("--utterances", type=int, default=1)
     a.add_argument("--beams", type=int, default=10)
     a.add_argument("--tokens", type=int, default=32)
+    a.add_argument("--cache", choices=("bf16", "fp4"), default="bf16")
+    a.add_argument("--drafts", type=int, default=0)
     o = a.parse_args()
-    cfg = DecoderConfig(positions=o.frames + o.tokens)
+    room = o.tokens + o.drafts + 1 if o.drafts > 0 else o.tokens  # (the last drafts may reach beyond)
+    cfg = DecoderConfig(positions=o.frames + room, cache=o.cache)
     ps = cfg.page_size
-    dec = HypothesisDecoder(cfg, make_weights(cfg), pages=o.utterances * (-(-o.frames // ps) + o.beams * -(-o.tokens // ps)))
+    pages = o.utterances * (-(-o.frames // ps) + o.beams * -(-room // ps))
+    weights = make_weights(cfg)
+    dec = HypothesisDecoder(cfg, weights, pages=pages)
     frames = torch.randn(o.utterances * o.frames, cfg.d_model, device="cuda").bfloat16()
     utt = dec.read(frames, [o.frames] * o.utterances)
-    hyp = dec.begin(utt, o.beams, o.tokens)
-    step = dec.compile_step(hyp)
+    hyp = dec.begin(utt, o.beams, room)
     ids = torch.arange(o.utterances * o.beams, device="cuda") % cfg.vocab
+    if o.drafts > 0:
+        return _drafted(o, cfg, weights, pages, frames, dec, hyp, ids)
+    step = dec.compile_step(hyp)
     e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     said = [ids]
     e0.record()
