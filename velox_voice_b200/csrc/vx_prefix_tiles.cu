@@ -75,10 +75,10 @@ struct TileShape {
   static constexpr bool kHalves = PAIRED && D == 64;
   static constexpr int kStagesK = FP4 ? (D == 128 ? 2 : 3) : (D == 128 ? 3 : 5);  // of a stream
   static constexpr int kStagesV = FP4 ? (D == 128 ? (PAIRED ? 2 : 1) : 3) : (D == 128 ? 2 : 5);
-  // FP4: tiles of a stream that are on their way as they lie in the cache, units of their keys, then of their values
-  static constexpr int kRaw = FP4 ? (D == 128 ? (PAIRED ? 1 : 3) : (PAIRED ? 3 : 6)) : 0;
-  static constexpr int kUnits = kKeys / 16, kRawTile = 2 * kUnits * kFp4Unit * D;
-  static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + kStreams * kRaw * kRawTile + 1024;
+  // FP4: keys and values of tiles of a stream that are on their way as they lie in the cache
+  static constexpr int kRawK = FP4 ? (D == 128 ? (PAIRED ? 2 : 3) : (PAIRED ? 3 : 6)) : 1, kRawV = FP4 && D == 128 && PAIRED ? 1 : kRawK;
+  static constexpr int kUnits = kKeys / 16, kRawHalf = FP4 ? kUnits * kFp4Unit * D : 0;  // units of a tile's keys, bytes
+  static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + kStreams * (kRawK + kRawV) * kRawHalf + 1024;
 };
 
 struct TilesParams {
@@ -105,8 +105,10 @@ struct TileBarriers {
   uint64_t p_half[2];  // kHalves: the first half of a tile's P
   uint64_t s_full[2][Shape::kBuffers], p_full[2][Shape::kBuffers], pv_done[2][Shape::kBuffers], q_full[2], q_empty[2];
   uint64_t mask_full[2][PT_MASKS], item_full[2][PT_ITEMS], item_empty[2][PT_ITEMS];
-  uint64_t raw_full[2][Shape::kRaw > 0 ? Shape::kRaw : 1], raw_empty[2][Shape::kRaw > 0 ? Shape::kRaw : 1];
-  uint32_t raw_there[2][Shape::kRaw > 0 ? Shape::kRaw : 1];  // FP4: which units of a tile there are; kRawEnd: no tile, the stream ends
+  struct Raw {  // FP4, of the keys or the values of a stream
+    uint64_t full[Shape::kRawK], empty[Shape::kRawK];
+    uint32_t there[Shape::kRawK];  // which units of a tile there are; kRawEnd: no tile, the stream ends
+  } raw[2][2];
   alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
   TileItem item[2][PT_ITEMS];
   uint32_t tmem_base;
@@ -311,25 +313,26 @@ template <int D, bool PAIRED>
 __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarriers<TileShape<D, PAIRED, true>>& bar, uint8_t* k_ring, uint8_t* v_ring, uint8_t* raw) {
   using Shape = TileShape<D, PAIRED, true>;
   constexpr unsigned ALL = 0xffffffffu;
-  constexpr int STREAMS = Shape::kStreams, PARTS = Shape::kParts, RAW = Shape::kRaw, UNIT = kFp4Unit * D, UNITS = 4;
+  constexpr int STREAMS = Shape::kStreams, PARTS = Shape::kParts, UNIT = kFp4Unit * D, UNITS = 4;
   const int loader = (threadIdx.x >> 5) - 8, lane = threadIdx.x & 31;
   const int stream = loader / (4 / STREAMS), local = loader % (4 / STREAMS), part = local % PARTS;
   const bool values = local >= PARTS;
-  const int stages = values ? Shape::kStagesV : Shape::kStagesK;
+  const int stages = values ? Shape::kStagesV : Shape::kStagesK, slots = values ? Shape::kRawV : Shape::kRawK;
+  auto& raw_bar = bar.raw[stream][values];
   uint64_t* const full = values ? bar.v_full[stream] : bar.k_full[stream];
   uint64_t* const empty = values ? bar.v_empty[stream] : bar.k_empty[stream];
   // where a lane reads a unit and writes it
   constexpr int LANES = D / 32, TOKENS = 32 / LANES, PIECES = 16 / TOKENS;  // lanes of a token, tokens of a piece
   const int c = lane % LANES, token = lane / LANES, turned = D == 128 ? c >> 1 : 0;
-  const uint32_t unit0 = smem_u32(raw) + stream * RAW * Shape::kRawTile + ((values ? Shape::kUnits : 0) + part * UNITS) * UNIT;
+  const uint32_t unit0 = smem_u32(raw) + (stream * (Shape::kRawK + Shape::kRawV) + (values ? Shape::kRawK : 0)) * Shape::kRawHalf + part * UNITS * UNIT;
   const uint32_t raw_at = unit0 + token * (D / 2) + c * 16 + 8 * turned, scale_at = unit0 + 8 * D + token * (D / 16) + c * 2;
   const uint32_t low = turned ? 0x4141 : 0x4040, high = turned ? 0x4040 : 0x4141;
   const uint32_t to_at = smem_u32(values ? v_ring : k_ring) + stream * stages * Shape::kTile + part * 64 * 128 + (c >> 1) * Shape::kPanel + token * 128;
   int stage = 0, slot = 0;
   uint32_t stage_phase = 1, slot_phase = 0;
   while (true) {
-    if (!__all_sync(ALL, mbar_wait(&bar.raw_full[stream][slot], slot_phase, p.status, 59))) break;
-    const uint32_t there = bar.raw_there[stream][slot];
+    if (!__all_sync(ALL, mbar_wait(&raw_bar.full[slot], slot_phase, p.status, 59))) break;
+    const uint32_t there = raw_bar.there[slot];
     if (there == kRawEnd || !__all_sync(ALL, mbar_wait(&empty[stage], stage_phase, p.status, 58))) break;
     const uint32_t dst = to_at + stage * Shape::kTile;
     // units two at a time: all that is read of them, then what is written
@@ -340,7 +343,7 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const uint32_t at = slot * Shape::kRawTile + (u + f) * UNIT;
+          const uint32_t at = slot * Shape::kRawHalf + (u + f) * UNIT;
           if constexpr (D == 128) {
             const uint32_t from = raw_at + at + i * TOKENS * (D / 2);
             asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[f][i][0]), "=r"(w[f][i][1]) : "r"(from));
@@ -371,9 +374,9 @@ __device__ __forceinline__ void load_fp4_tiles(const PrefixParams& p, TileBarrie
     fence_proxy_async_smem();
     mbar_arrive(&full[stage]);
     __syncwarp();  // every lane has read the slot
-    if (lane == 0) mbar_arrive(&bar.raw_empty[stream][slot]);
+    if (lane == 0) mbar_arrive(&raw_bar.empty[slot]);
     if (++stage == stages) { stage = 0; stage_phase ^= 1; }
-    if (++slot == RAW) { slot = 0; slot_phase ^= 1; }
+    if (++slot == slots) { slot = 0; slot_phase ^= 1; }
   }
 }
 
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 
   if (warp < 2) {  // each lane some barriers
     const int s = warp;  // slot, stream
-    for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], FP4 ? 1 : Shape::kParts);
+    for (int i = lane; i < PT_MASKS; i += 32) mbar_init(&bar.mask_full[s][i], Shape::kParts);
     if (lane < PT_ITEMS) {
       mbar_init(&bar.item_full[s][lane], 1);
       mbar_init(&bar.item_empty[s][lane], (FP4 ? 0 : 4 / STREAMS) + 1 + 8 / STREAMS + (PAIRED && !FP4 ? 1 : 0));  // warps that read an item: loaders, MMA issuer, softmax, the second slot's queries
@@ -409,9 +412,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       mbar_init(&bar.q_empty[s], 1);
       mbar_init(&bar.p_half[s], 4);
     }
-    if (FP4 && s < STREAMS && lane < Shape::kRaw) {
-      mbar_init(&bar.raw_full[s][lane], 1);
-      mbar_init(&bar.raw_empty[s][lane], 4 / STREAMS);  // loaders of the stream
+    if (FP4 && s < STREAMS && lane < 2 * Shape::kRawK) {
+      auto& raw = bar.raw[s][lane & 1];
+      mbar_init(&raw.full[lane >> 1], 1);
+      mbar_init(&raw.empty[lane >> 1], Shape::kParts);  // loaders that share a tile
     }
     if (s < STREAMS && lane < NK) {
       mbar_init(&bar.k_full[s][lane], 32 * Shape::kParts);  // threads of the loaders that share a tile
@@ -782,8 +786,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         };
         // FP4: units of tiles to shared memory as they lie in the cache, those of keys by the lower lanes, those of values by lanes 16 on.  The table is
         // read a tile ahead.
-        [[maybe_unused]] int entry = -1, keys_there = 0, raw_slot = 0, fetched = 0;
-        [[maybe_unused]] uint32_t rest = 0, raw_phase = 0;
+        [[maybe_unused]] int entry = -1, keys_there = 0, raw_slot[2] = {0, 0}, fetched = 0;
+        [[maybe_unused]] uint32_t rest = 0, raw_phase[2] = {0, 0};
+        // the next slot of the keys or of the values, when the loaders have it free
+        [[maybe_unused]] auto next_raw = [&](int e, uint32_t there, uint32_t bytes) {
+          ok = __all_sync(ALL, mbar_wait(&bar.raw[stream][e].empty[raw_slot[e]], raw_phase[e] ^ 1, p.status, 57));
+          const int slot = raw_slot[e];
+          if (ok && lane == 0) {
+            bar.raw[stream][e].there[slot] = there;
+            if (there == kRawEnd) mbar_arrive(&bar.raw[stream][e].full[slot]);
+            else mbar_expect_tx(&bar.raw[stream][e].full[slot], bytes);
+          }
+          __syncwarp();
+          if (++raw_slot[e] == (e ? Shape::kRawV : Shape::kRawK)) { raw_slot[e] = 0; raw_phase[e] ^= 1; }
+          return slot;
+        };
         [[maybe_unused]] auto look_up = [&](const TileItem& t, int x) {
           const int v = t.v0 + x * BN;
           const bool own = v >= t.p128;
@@ -802,7 +819,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           const bool values = lane >= 16;
           const int64_t page_bytes = values ? p.fp4.v_page : p.fp4.k_page;
           const uint8_t* const base = (values ? p.fp4.v : p.fp4.k) + static_cast<int64_t>(t.head) * p.fp4.page_units.d * UNIT;
-          uint8_t* const raw = raw_ring + stream * Shape::kRaw * Shape::kRawTile + ((values ? Shape::kUnits : 0) + (lane & 15)) * UNIT;
+          uint8_t* const raw = raw_ring + (stream * (Shape::kRawK + Shape::kRawV) + (values ? Shape::kRawK : 0)) * Shape::kRawHalf + (lane & 15) * UNIT;
           look_up(t, 0);
 #pragma unroll 1
           for (int x = 0; x < t.tiles && ok; ++x) {
@@ -811,21 +828,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             const uint8_t* const src = base + (is ? entry : 0) * page_bytes + static_cast<int64_t>(rest) * UNIT;
             const int keys = is ? keys_there : 0;
             look_up(t, x + 1);
-            ok = __all_sync(ALL, mbar_wait(&bar.raw_empty[stream][raw_slot], raw_phase ^ 1, p.status, 57));
-            if (!ok) return;
             // (the softmax has read the mask PT_MASKS tiles of the stream before this one: PT_MASKS is more than the rings hold and a slot has begun)
-            static_assert(Shape::kRaw + Shape::kStagesK + 2 * NB + 1 < PT_MASKS, "");
+            static_assert(1 + Shape::kRawK + Shape::kStagesK + 2 * NB + 1 < PT_MASKS, "");  // (one that waits for its slot)
             uint16_t* const mask = bar.mask[stream][fetched % PT_MASKS];
-            if (lane < Shape::kUnits) mask[lane] = static_cast<uint16_t>(low_bits(keys));
-            if (lane == 0) {
-              bar.raw_there[stream][raw_slot] = there & 0xffffu;
-              mbar_expect_tx(&bar.raw_full[stream][raw_slot], __popc(there) * UNIT);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (e == 0 && lane < Shape::kUnits) mask[lane] = static_cast<uint16_t>(low_bits(keys));
+              __syncwarp();
+              const int slot = next_raw(e, there & 0xffffu, __popc(there & 0xffffu) * UNIT);
+              if (!ok) return;
+              if (is && values == (e == 1)) bulk_load(raw + slot * Shape::kRawHalf, src, UNIT, &bar.raw[stream][e].full[slot]);
             }
-            __syncwarp();
-            if (is) bulk_load(raw + raw_slot * Shape::kRawTile, src, UNIT, &bar.raw_full[stream][raw_slot]);
-            if (lane == 0) mbar_arrive(&bar.mask_full[stream][fetched % PT_MASKS]);
             ++fetched;
-            if (++raw_slot == Shape::kRaw) { raw_slot = 0; raw_phase ^= 1; }
           }
         };
         // A stream has an item of every round, in turn from both ends of it: with causal rows the later tiles have more keys.  (The host saw to
@@ -855,17 +869,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         end.tiles = 0;
         if (ok) hand_out(end, lane == 0);
         if constexpr (FP4) {
-          ok = ok && __all_sync(ALL, mbar_wait(&bar.raw_empty[stream][raw_slot], raw_phase ^ 1, p.status, 57));
-          if (ok && lane == 0) {
-            bar.raw_there[stream][raw_slot] = kRawEnd;
-            mbar_arrive(&bar.raw_full[stream][raw_slot]);
-          }
+          for (int e = 0; e < 2 && ok; ++e) next_raw(e, kRawEnd, 0);
           // (copies on their way after a limit ran out: each is waited for, with a limit)
-          if (!ok)
-            for (int i = 0; i < Shape::kRaw && i < fetched; ++i) {
-              raw_slot = (raw_slot == 0 ? Shape::kRaw : raw_slot) - 1;
-              if (raw_slot == Shape::kRaw - 1) raw_phase ^= 1;
-              mbar_wait(&bar.raw_full[stream][raw_slot], raw_phase, p.status, 59);
+          for (int e = 0; e < 2 && !ok; ++e)
+            for (int i = 0; i < (e ? Shape::kRawV : Shape::kRawK) && i < fetched; ++i) {
+              if (raw_slot[e] == 0) raw_phase[e] ^= 1;
+              raw_slot[e] = (raw_slot[e] == 0 ? (e ? Shape::kRawV : Shape::kRawK) : raw_slot[e]) - 1;
+              mbar_wait(&bar.raw[stream][e].full[raw_slot[e]], raw_phase[e], p.status, 59);
             }
         }
         cp_async_wait_all();
@@ -946,7 +956,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         }
         // which keys of the tile this row sees: as a rule all of them
         const int mk = masks + u;
-        const bool marked = mbar_wait(&bar.mask_full[stream][mk % PT_MASKS], (mk / PT_MASKS) & 1, p.status, 44);
+        // (FP4: the mask of a tile was written before its keys were fetched, so S tells of it)
+        const bool marked = FP4 || mbar_wait(&bar.mask_full[stream][mk % PT_MASKS], (mk / PT_MASKS) & 1, p.status, 44);
+        bool formed = true;
+        if (FP4) formed = mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 45);
         const uint32_t* const words = reinterpret_cast<const uint32_t*>(bar.mask[stream][mk % PT_MASKS]);
         const int v = t.v0 + u * BN;
         uint32_t seen[W], both = 0xffffffffu;
@@ -961,7 +974,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < W; ++i) seen[i] &= low_bits(limit - (v - t.p128) - 32 * i);
         }
-        const bool formed = mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 45);
+        if (!FP4) formed = mbar_wait(&bar.s_full[slot][buffer], parity, p.status, 45);
         ok = __all_sync(ALL, marked && formed);
         if (!ok) return;
         tc_fence_after();
@@ -1032,7 +1045,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             float x0, x1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1])), k2, n2), x0, x1);
+            const uint64_t x2 = fma_f32x2(pack_f32x2(__uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1])), k2, n2);
+            unpack_f32x2(x2, x0, x1);
             x0 = ex2(x0);
             x1 = ex2(x1);
             sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], pack_f32x2(x0, x1));
