@@ -400,4 +400,6 @@ def test_launches_are_counted(ops):
     ops.kv_append(k, k, kp, vp, t, n)
     ops.prefix_attention(q, kp, vp, t, n)
     ops.kv_values(kp)
-    assert ops.launch_count() == 4
+    assert ops.launch_count() == 3  # (few keys: attention is one launch)
+    ops.prefix_attention(q, kp, vp, t.expand(2, 1).repeat(1, 900), n)
+    assert ops.launch_count() == 5

@@ -219,7 +219,7 @@ __device__ __forceinline__ bool any_not_finite(uint32_t sum) { return (sum & 0x7
 struct RowsParams {
   PrefixParams p;
   Span span[2];
-  int32_t warps[2];      // of a CTA per item of the span: 1, 2 or 4
+  int32_t warps[2];      // of a CTA per item of the span: 1, 2 or 4; a cache in 4 bits, one span: 8 or 16 too, a CTA of so many
   int32_t first_blocks;  // CTAs of span[0]; those of span[1] follow
   int32_t beside;        // the launch in front is the tile kernel of this call, see prefix_rows_kernel
 };

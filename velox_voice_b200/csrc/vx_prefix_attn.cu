@@ -551,10 +551,12 @@ struct Plan {
   Span span[2];
   enum Kernel { kRows, kTiles, kPairs } kernel[2];  // that walks the span
   int blocks;                                       // of eight rows, of the kernel for few rows
+  int warps[2];                                     // of that kernel per item; 0: by the rule of the launch
   int parts;
   int64_t ml_bytes, bytes;
 
   Span part(Kernel k, int i) const { return kernel[i] == k ? span[i] : kNoSpan; }  // the span, where kernel k walks it
+  bool whole_rows() const { return kernel[0] == kRows && span[0].part0 < 0 && span[0].chunks > 0; }  // the kernel for few rows writes the result itself
   bool walks(Kernel k) const { return part(k, 0).chunks > 0 || part(k, 1).chunks > 0; }
 };
 
@@ -672,10 +674,42 @@ int check_prefix(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_att
       const bool paired = kernel == Plan::kPairs;
       sp.chunk = tile_chunk_keys(cap, n, paired ? sms : 2 * sms, paired ? 256 : 128, paired && cache->head_dim == 64 ? 1.4 : 2.0, cache->head_dim, R * d->q_heads, kind == kSpanJoint);
     }
-    else sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim, FP4), 16 * PR_WARPS, cache->head_dim == 64 ? 1024 : 256, 3);
+    else if (!FP4) sp.chunk = chunk_keys(cap, items, rows_resident(plan.blocks, cache->head_dim, FP4), 16 * PR_WARPS, cache->head_dim == 64 ? 1024 : 256, 3);
+    else {
+      // In 4 bits 256 keys of a warp are few: what it costs to begin passes under fewer bytes.  With much to walk the warps take items of their own; long runs
+      // are walked by the four of a CTA, which leave a fourth of the parts.  Own tokens, 8 key heads of 128, four query heads each, keys a chunk x warps, in us:
+      //   128 sequences of 512 to 1,024 (with the prefixes beside them)   256 x 1  85   512 x 2  88   1,024 x 4  91   512 x 1  95
+      //   64 sequences of 4,000 to 8,000                                  640 x 1  90   1,024 x 2  88   2,048 x 4  86   4,096 x 4  90
+      const int64_t resident = rows_resident(plan.blocks, cache->head_dim, FP4);
+      int& warps = plan.warps[&sp - plan.span];
+      if (cap * items <= 1024 * resident) {
+        sp.chunk = chunk_keys(cap, items, resident, 16 * PR_WARPS, 1024, 3);
+      } else {
+        sp.chunk = chunk_keys(cap, items, PR_WARPS * resident, 16 * PR_WARPS, 256, 3);
+        warps = 1;
+        if (8 * static_cast<int64_t>(sp.chunk) <= cap) {
+          warps = PR_WARPS;
+          sp.chunk = chunk_keys(cap, items, resident, 16 * PR_WARPS, 1024, 3);
+        }
+      }
+    }
     sp.chunks = static_cast<int32_t>((cap + sp.chunk - 1) / sp.chunk);
   };
-  if (rows_o > kSlotRows) {
+  // Few items (sequence and key head) over few keys, in 4 bits: one CTA walks a sequence's prefix and own tokens and writes the rows; the hypotheses of a group read their prefix
+  // each for itself, from L2.  As many warps as leave an SM its sixteen.  Whole against parts and a join, 8 key heads, single tokens, in us:
+  //   head_dim 64    10 sequences   400 own tokens 6.5 : 8.8   700 shared + 24 7.8 : 8.7   1,000 + 60 9.1 : 8.8   1,500 + 60 10.8 : 9.0     32  1,000 own 11.5 : 16.1   70  700 + 50 15.2 : 17.4
+  //   head_dim 128 (4 query heads)  400 7.9 : 9.9              700 + 24 9.7 : 11.5         1,000 + 60 11.5 : 15.5  1,500 + 60 13.9 : 13.1    32  1,000 15.4 : 19.4       70  700 + 50 20.6 : 24.8
+  const int64_t whole_items = (single ? S * ((per + 7) / 8) : R * per / 8 + S) * p.kv_heads, sms = sm_count();
+  const int whole_warps = whole_items <= sms ? 16 : (whole_items <= 2 * sms ? 8 : 4);
+  if (FP4 && rows_o <= 8 && whole_items <= 4 * sms && cap_p + cap_o <= 1024) {
+    plan.kernel[0] = plan.kernel[1] = Plan::kRows;
+    plan.blocks = 1;
+    cut(plan.span[0], kSpanJoint, Plan::kRows, S, cap_p + cap_o > 0 ? cap_p + cap_o : 1, single ? per : 0);
+    plan.span[0].chunk = static_cast<int32_t>(round_up(cap_p + cap_o, 64));
+    plan.span[0].chunks = 1;
+    plan.span[0].part0 = -1;
+    plan.warps[0] = whole_warps;
+  } else if (rows_o > kSlotRows) {
     // Whole prompts or long chunks: prefix and own tokens in a row, no joining of the two, but a walk of the prefix per sequence.  8 key heads,
     // prompts without a history, the two apart (prefix by groups) against in a row, in us:
     //   head_dim 64    130 rows  4 sequences, one prefix of 1,000 keys 42 : 26   of 8,000 62 : 54     64 sequences, 1,000 133 : 120   8,000 349 : 514
@@ -738,7 +772,7 @@ int launches(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attenti
   Plan plan;
   const int rc = check_prefix(cache, rows, d, p, plan);
   if (rc) return rc;
-  int n = p.rows.rows > 0 ? 1 : 0;  // the join
+  int n = p.rows.rows > 0 && !plan.whole_rows() ? 1 : 0;  // the join
   for (const Plan::Kernel k : {Plan::kRows, Plan::kTiles, Plan::kPairs}) n += plan.walks(k) ? 1 : 0;
   return n;
 }
@@ -776,8 +810,9 @@ int attention(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attent
       const int64_t items = static_cast<int64_t>(sp.slots) * sp.chunks * p.kv_heads;
       // All four warps of a CTA on an item while one round of CTAs takes them all, else so many that each has about 128 keys: twice as many take
       // 28 us for 27 (64 hypotheses of 102 to 198 tokens, four utterances of 1,005 to 1,792 frames) and 37 for 32 (124 of 30 to 60 tokens), half as many 29 and 32.
-      rp.warps[i] = items <= rows_resident(plan.blocks, cache->head_dim, FP4) || sp.chunk > 256 ? 4 : (sp.chunk > 128 ? 2 : 1);
-      blocks += (items * rp.warps[i] + PR_WARPS - 1) / PR_WARPS;
+      rp.warps[i] = plan.warps[i] ? plan.warps[i] : items <= rows_resident(plan.blocks, cache->head_dim, FP4) || sp.chunk > 256 ? 4 : (sp.chunk > 128 ? 2 : 1);
+      const int of_cta = rp.warps[i] > PR_WARPS ? rp.warps[i] : PR_WARPS;
+      blocks += (items * rp.warps[i] + of_cta - 1) / of_cta;
       if (i == 0) rp.first_blocks = static_cast<int32_t>(blocks);
     }
     if (blocks >= (1ll << 31)) return fail(-1, "too much work for one call (%lld blocks)", (long long)blocks);
@@ -786,6 +821,7 @@ int attention(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_attent
                       : (plan.blocks == 2 ? launch_rows<128, 2>(rp, blocks, st) : launch_rows<128, 1>(rp, blocks, st));
     if (e) return e;
   }
+  if (plan.whole_rows()) return 0;
   JoinParams jp{p, {plan.span[0], plan.span[1]}, plan.parts == 0 && plan.span[0].part0 >= 0 ? 1 : 0};
   VX_CUDA_OK(d64 ? launch_join<64>(jp, plan.parts, st) : launch_join<128>(jp, plan.parts, st));
   return 0;

@@ -29,6 +29,7 @@
 namespace vx {
 namespace {
 
+// CTAs of four warps per SM; those of eight or sixteen, which take an item each, have as many warps together.
 constexpr int rows4_ctas(int rb, int head_dim) { return head_dim == 64 ? 4 : (rb == 2 ? 3 : 4); }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -92,12 +93,11 @@ struct Rows4Shape {
   static constexpr int kUnit = kFp4Unit * D;
   static constexpr int kStages = D == 128 ? 4 : 6;
   static constexpr int kRing = kStages * 2 * kUnit;  // of a warp
-  static constexpr int kSmem = PR_WARPS * kRing;
 };
 
-// RB blocks of eight rows.
-template <int D, int RB>
-__global__ void __launch_bounds__(PR_WARPS * 32, rows4_ctas(RB, D)) prefix_rows_fp4_kernel(const __grid_constant__ RowsParams rp) {
+// RB blocks of eight rows.  WHOLE: an item has all keys of its rows, those of the prefix and its own (one chunk of a joint span), and writes them to `out`.
+template <int D, int RB, int WARPS, bool WHOLE>
+__global__ void __launch_bounds__(WARPS * 32, rows4_ctas(RB, D) * PR_WARPS / WARPS) prefix_rows_fp4_kernel(const __grid_constant__ RowsParams rp) {
   using Shape = Rows4Shape<D>;
   constexpr int NS = Shape::kStages, UNIT = Shape::kUnit;
   constexpr int KW = D / 32;  // words of a key per lane
@@ -105,9 +105,9 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows4_ctas(RB, D)) prefix_rows_
   constexpr int TM = 8 * RB;
   constexpr unsigned ALL = 0xffffffffu;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 ml_s[PR_WARPS][TM];
-  __shared__ uint64_t full_s[PR_WARPS][NS];
-  __shared__ int first_s[PR_WARPS][NS];  // first key of a stage
+  __shared__ float2 ml_s[WARPS][TM];
+  __shared__ uint64_t full_s[WARPS][NS];
+  __shared__ int first_s[WARPS][NS];  // first key of a stage
   const PrefixParams& p = rp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   if (lane < NS) mbar_init(&full_s[warp][lane], 1);
@@ -127,34 +127,52 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows4_ctas(RB, D)) prefix_rows_
   if (second) n -= rp.first_blocks;
   const Span& sp = rp.span[second];
   const int warps = rp.warps[second], team = warp / warps, rank = warp - team * warps;  // the warps of an item
-  n = n * (PR_WARPS / warps) + team;
+  n = n * (WARPS / warps) + team;
   const int head = n % p.kv_heads;
   n /= p.kv_heads;
   const int chunk = n / sp.slots;
   if (chunk >= sp.chunks) return;
-  const bool own = sp.kind == kSpanOwn;
+  const bool own = WHOLE || sp.kind == kSpanOwn;
+  if (WHOLE && blockIdx.x == 0) {  // rows of no sequence: zeros
+    const int head_pieces = D / 8, pieces = p.q_heads * head_pieces;
+    const int before = owner_row0(p, true, 0), behind = owner_row0(p, true, p.rows.sequences);
+    for (int row = 0; row < p.rows.rows; ++row) {
+      if (row == before) row = max(behind, before);
+      if (row >= p.rows.rows) break;
+      for (int i = threadIdx.x; i < pieces; i += WARPS * 32)
+        *reinterpret_cast<uint4*>(p.out + row * p.o_row + i / head_pieces * p.o_head + i % head_pieces * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
   ItemRows it;
   if (!find_rows<TM>(p, sp, n - chunk * sp.slots, it)) return;
   const int length = own ? tokens_before(p, it.owner) : 0;
-  // keys [key0, keys): those of the chunk that the tile's last row sees
+  // keys [key0, keys): those of the chunk that the tile's last row sees; in front of them, joint, `shared` units of the prefix
   int keys = own ? own_keys(p, length, static_cast<int>(p.per_kv.div(static_cast<uint32_t>(min(it.rho0 + TM, it.rows) - 1)))) : prefix_keys(p, it.owner);
-  if (static_cast<int64_t>(chunk) * sp.chunk >= keys) return;
+  if (!WHOLE && static_cast<int64_t>(chunk) * sp.chunk >= keys) return;
   const int key0 = chunk * sp.chunk;
   keys = static_cast<int>(min(static_cast<int64_t>(keys), static_cast<int64_t>(key0) + sp.chunk));
+  int group = -1, shared_keys = 0;
+  if (WHOLE && length >= 0) {
+    group = group_of(p, it.owner);
+    shared_keys = prefix_keys(p, group);
+  }
+  const int shared = (shared_keys + 15) / 16;
   const PagedTable& table = own ? p.rows.table : p.prefix;
   const int blocks = it.rows - it.rho0 > 8 ? RB : 1;  // that have rows
 
   // The warp's units, in its turn: unit i of them begins with key key0 + 16 (rank + i warps).  They are looked up 32 at a time, a lane each, one
   // turn ahead; the lane that has a unit issues its copies.
-  const int units = (keys - key0 + 15) / 16, mine = units > rank ? (units - rank - 1) / warps + 1 : 0;
+  const int units = shared + (keys - key0 + 15) / 16, mine = units > rank ? (units - rank - 1) / warps + 1 : 0;
   const int64_t head_at = static_cast<int64_t>(head) * p.fp4.page_units.d * UNIT;
   const uint32_t ring = smem_u32(smem) + warp * Shape::kRing;
   auto look_up = [&](int i, uint32_t& rest) {
     rest = 0;
     if (i >= mine) return -1;
     uint32_t index;
-    p.fp4.page_units.divmod(static_cast<uint32_t>(key0 / 16 + rank + i * warps), index, rest);
-    return page_of(table, it.owner, index, p.cache.pages);
+    const int unit = rank + i * warps - shared;
+    const bool in_prefix = WHOLE && unit < 0;
+    p.fp4.page_units.divmod(static_cast<uint32_t>(in_prefix ? unit + shared : key0 / 16 + unit), index, rest);
+    return page_of(in_prefix ? p.prefix : table, in_prefix ? group : it.owner, index, p.cache.pages);
   };
   uint32_t rest, rest_next;
   int page = look_up(lane, rest), page_next = look_up(32 + lane, rest_next);
@@ -173,7 +191,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows4_ctas(RB, D)) prefix_rows_
     if (lane == at) {
       uint64_t* const bar = &full_s[warp][write];
       uint8_t* const dst = smem + warp * Shape::kRing + write * 2 * UNIT;
-      first_s[warp][write] = key0 + 16 * (rank + (turn + at) * warps);
+      first_s[warp][write] = key0 + 16 * (rank + (turn + at) * warps - shared);  // (of the prefix: as far in front)
       mbar_expect_tx(bar, 2 * UNIT);
       const int64_t off = head_at + static_cast<int64_t>(rest) * UNIT;
       bulk_load(dst, p.fp4.k + page * p.fp4.k_page + off, UNIT, bar);
@@ -273,7 +291,16 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows4_ctas(RB, D)) prefix_rows_
     for (int r = 0; r < RB; ++r)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[r][e] *= factor[r][e & 1];
-    if (j0 + 16 > min_limit) {
+    if (WHOLE && j0 < 0) {  // of the prefix (key0 is 0): its last unit may end early
+      const int end = shared_keys - 16 * shared;
+      if (j0 + 16 > end) {
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j0 + 8 * (e >> 1) + g >= end) s[r][e] = NEG_INF;
+      }
+    } else if (j0 + 16 > min_limit) {
 #pragma unroll
       for (int r = 0; r < RB; ++r)
 #pragma unroll
@@ -402,24 +429,37 @@ __global__ void __launch_bounds__(PR_WARPS * 32, rows4_ctas(RB, D)) prefix_rows_
     uint32_t tok, hq;
     p.per_kv.divmod(static_cast<uint32_t>(rho), tok, hq);
     const int64_t row = it.row0 + static_cast<int>(tok), qh = head * static_cast<int64_t>(p.per_kv.d) + hq;
+    if (WHOLE) {
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(p.out + row * p.o_row + qh * p.o_head + col) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      continue;
+    }
     const int64_t at = (static_cast<int64_t>(sp.part0 + chunk) * p.rows.rows + row) * p.q_heads + qh;
     if (col == 0) p.part_ml[at] = make_float2(m, sum);
     *reinterpret_cast<float4*>(p.part_o + at * D + col) = acc;
   }
 }
 
-template <int D, int RB>
+template <int D, int RB, int WARPS, bool WHOLE>
 int launch(const RowsParams& rp, int64_t blocks, cudaStream_t st) {
+  constexpr int kSmem = WARPS * Rows4Shape<D>::kRing;
   int dev = 0;
   VX_CUDA_OK(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_done{0};
   const bool cached = dev >= 0 && dev < 64;
   if (!cached || !(attr_done.load(std::memory_order_acquire) & (1ull << dev))) {
-    VX_CUDA_OK(cudaFuncSetAttribute(prefix_rows_fp4_kernel<D, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows4Shape<D>::kSmem));
+    VX_CUDA_OK(cudaFuncSetAttribute(prefix_rows_fp4_kernel<D, RB, WARPS, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     if (cached) attr_done.fetch_or(1ull << dev, std::memory_order_release);
   }
-  VX_CUDA_OK(launch_dependent(prefix_rows_fp4_kernel<D, RB>, dim3(static_cast<unsigned>(blocks)), dim3(PR_WARPS * 32), Rows4Shape<D>::kSmem, st, rp));
+  VX_CUDA_OK(launch_dependent(prefix_rows_fp4_kernel<D, RB, WARPS, WHOLE>, dim3(static_cast<unsigned>(blocks)), dim3(WARPS * 32), kSmem, st, rp));
   return 0;
+}
+template <int D>
+int launch(const RowsParams& rp, int rb, int64_t blocks, cudaStream_t st) {
+  if (rp.span[0].part0 < 0)
+    return rp.warps[0] == 16 ? launch<D, 1, 16, true>(rp, blocks, st) : rp.warps[0] == 8 ? launch<D, 1, 8, true>(rp, blocks, st) : launch<D, 1, PR_WARPS, true>(rp, blocks, st);
+  return rb == 2 ? launch<D, 2, PR_WARPS, false>(rp, blocks, st) : launch<D, 1, PR_WARPS, false>(rp, blocks, st);
 }
 
 }  // namespace
@@ -428,8 +468,7 @@ int rows_fp4_ctas(int rb, int head_dim) { return rows4_ctas(rb, head_dim); }
 
 int launch_rows_fp4(const RowsParams& rp, int head_dim, int rb, int64_t blocks, void* stream) {
   const auto st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 64) return rb == 2 ? launch<64, 2>(rp, blocks, st) : launch<64, 1>(rp, blocks, st);
-  return rb == 2 ? launch<128, 2>(rp, blocks, st) : launch<128, 1>(rp, blocks, st);
+  return head_dim == 64 ? launch<64>(rp, rb, blocks, st) : launch<128>(rp, rb, blocks, st);
 }
 
 }  // namespace vx
