@@ -1317,6 +1317,7 @@ PyObject* py_kv_append(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
   }
   {
     NoGil nogil;
+    const c10::cuda::CUDAGuard on(dev);
     if (q && !out.defined()) out = empty(q->sizes(), at::kBFloat16, dev);
     if (q) { d.q_out = out.data_ptr(); d.qo_row = step(out, 0); d.qo_head = step(out, 1); }
     if (cache.fp4) check(g.vx_kv_append_fp4(&cache.b4, &rows, &d, stream()), "vx_kv_append_fp4");
@@ -1364,6 +1365,7 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
   }
   {
     NoGil nogil;
+    const c10::cuda::CUDAGuard on(dev);
     if (!out.defined()) out = empty(q->sizes(), at::kBFloat16, dev);
     d.out = out.data_ptr(); d.o_row = step(out, 0); d.o_head = step(out, 1);
     const char* const what = cache.fp4 ? "vx_prefix_attention_fp4" : "vx_prefix_attention";
@@ -1392,6 +1394,7 @@ PyObject* py_kv_values(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
   at::Tensor out;
   {
     NoGil nogil;
+    const c10::cuda::CUDAGuard on(x->device());
     const int64_t D = x->size(3) / 9;
     out = empty({x->size(0), 16 * x->size(2), x->size(1), D}, at::kBFloat16, x->device());
     check(g.vx_kv_values_fp4(x->data_ptr(), x->size(0), step(*x, 0), static_cast<int>(16 * x->size(2)), static_cast<int>(x->size(1)), static_cast<int>(D), static_cast<float>(s), out.data_ptr(),

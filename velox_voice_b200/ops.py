@@ -906,7 +906,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
         starts = _int32_on(starts, "starts", (r.sequences,), dev)
         d.starts = starts.data_ptr()
     name = "vx_kv_append_fp4" if isinstance(cache, _lib.KvCacheFp4) else "vx_kv_append"
-    _lib.check(getattr(_lib.load(), name)(C.byref(cache), C.byref(r), C.byref(d), _stream()), name)
+    with torch.cuda.device(dev):
+        _lib.check(getattr(_lib.load(), name)(C.byref(cache), C.byref(r), C.byref(d), _stream()), name)
     _count(1 if rows else 0)
     del keep
     return q_out
@@ -928,7 +929,9 @@ def kv_values(pages: torch.Tensor, scale: float = 1.0, *, out: Optional[torch.Te
         _require_cuda(out, "out")
         if out.dtype != torch.bfloat16 or tuple(out.shape) != shape or out.device != pages.device or not out.is_contiguous() or out.data_ptr() % 16 != 0:
             raise ValueError(f"out must be contiguous bfloat16 {list(shape)} at a 16-byte aligned address")
-    _lib.check(_lib.load().vx_kv_values_fp4(pages.data_ptr(), n, _step(pages, 0), 16 * units, heads, unit // 9, scale, out.data_ptr(), _stream()), "vx_kv_values_fp4")
+    with torch.cuda.device(pages.device):
+        rc = _lib.load().vx_kv_values_fp4(pages.data_ptr(), n, _step(pages, 0), 16 * units, heads, unit // 9, scale, out.data_ptr(), _stream())
+    _lib.check(rc, "vx_kv_values_fp4")
     _count(1 if n else 0)
     return out
 
@@ -987,13 +990,14 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     d.out, d.o_row, d.o_head = out.data_ptr(), _step(out, 0), _step(out, 1)
     lib = _lib.load()
     name = "vx_prefix_attention_fp4" if isinstance(cache, _lib.KvCacheFp4) else "vx_prefix_attention"
-    size = int(getattr(lib, name + "_scratch")(C.byref(cache), C.byref(r), C.byref(d)))
-    if size < 0:
-        _lib.check(size, name)
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    d.scratch, d.scratch_bytes = _ptr(scratch), size
-    _lib.check(getattr(lib, name)(C.byref(cache), C.byref(r), C.byref(d), _stream()), name)
-    _count(int(getattr(lib, name + "_launches")(C.byref(cache), C.byref(r), C.byref(d))))
+    with torch.cuda.device(dev):
+        size = int(getattr(lib, name + "_scratch")(C.byref(cache), C.byref(r), C.byref(d)))
+        if size < 0:
+            _lib.check(size, name)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        d.scratch, d.scratch_bytes = _ptr(scratch), size
+        _lib.check(getattr(lib, name)(C.byref(cache), C.byref(r), C.byref(d), _stream()), name)
+        _count(int(getattr(lib, name + "_launches")(C.byref(cache), C.byref(r), C.byref(d))))
     del keep, prefix_table, prefix_lengths, group_offsets
     return out
 
