@@ -76,7 +76,9 @@ struct TileShape {
   static constexpr int kStagesK = FP4 ? (D == 128 ? 2 : 3) : (D == 128 ? 3 : 5);  // of a stream
   static constexpr int kStagesV = FP4 ? (D == 128 ? (PAIRED ? 2 : 1) : 3) : (D == 128 ? 2 : 5);
   // FP4: keys and values of tiles of a stream that are on their way as they lie in the cache
-  static constexpr int kRawK = FP4 ? (D == 128 ? (PAIRED ? 2 : 3) : (PAIRED ? 3 : 6)) : 1, kRawV = FP4 && D == 128 && PAIRED ? 1 : kRawK;
+  static constexpr int kRawK = FP4 ? (D == 128 ? (PAIRED ? 2 : 3) : (PAIRED ? 3 : 6)) : 1, kRawV = FP4 && D == 128 ? (PAIRED ? 1 : 3) : kRawK;
+  static_assert(kRawV <= kRawK, "barriers are counted by kRawK");
+  static constexpr bool kBox = FP4 && !PAIRED && D == 64;  // rows of a slot twice, see the softmax
   static constexpr int kUnits = kKeys / 16, kRawHalf = FP4 ? kUnits * kFp4Unit * D : 0;  // units of a tile's keys, bytes
   static constexpr int kSmem = 2 * kQ + kStreams * (kStagesK + kStagesV) * kTile + kStreams * (kRawK + kRawV) * kRawHalf + 1024;
 };
@@ -109,6 +111,8 @@ struct TileBarriers {
     uint64_t full[Shape::kRawK], empty[Shape::kRawK];
     uint32_t there[Shape::kRawK];  // which units of a tile there are; kRawEnd: no tile, the stream ends
   } raw[2][2];
+  uint64_t box_full[2], box_empty[2];  // FP4, not PAIRED: what the upper half of a slot hands to the lower
+  float2 box_ml[Shape::kBox ? 2 : 1][Shape::kBox ? kSlotRows / 2 : 1];
   alignas(16) uint16_t mask[2][PT_MASKS][Shape::kKeys / 16];
   TileItem item[2][PT_ITEMS];
   uint32_t tmem_base;
@@ -411,6 +415,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       mbar_init(&bar.q_full[s], (FP4 ? 256 : 64) / STREAMS);  // threads that load queries
       mbar_init(&bar.q_empty[s], 1);
       mbar_init(&bar.p_half[s], 4);
+      mbar_init(&bar.box_full[s], 2);
+      mbar_init(&bar.box_empty[s], 2);
     }
     if (FP4 && s < STREAMS && lane < 2 * Shape::kRawK) {
       auto& raw = bar.raw[s][lane & 1];
@@ -606,10 +612,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       auto desc = [&](uint32_t lo) { return (static_cast<uint64_t>(desc_hi) << 32) | lo; };
       const uint32_t q_lo = smem_u32(q_s) >> 4, k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
       bool ok = true;
-      // (the copies are writes of the generic proxy: the fence orders them before the products that read them)
+      // (the copies are writes of the generic proxy: the fence orders them before the products that read them; FP4: whoever wrote has fenced)
       auto landed = [&](uint64_t* full, int stage, int phase) {
         const bool there = __all_sync(ALL, mbar_wait_spin(&full[stage], phase & 1, p.status, 42));
-        if (leader) fence_proxy_async_smem();
+        if (!FP4 && leader) fence_proxy_async_smem();
         return there;
       };
       auto issue_s = [&](int slot, int buffer, int stage) {
@@ -639,7 +645,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       auto wait_q = [&](int i) {
         const bool there = __all_sync(ALL, mbar_wait_spin(&bar.q_full[i], q_phase, p.status, 41));
         q_phase ^= 1;
-        if (leader) fence_proxy_async_smem();
+        if (!FP4 && leader) fence_proxy_async_smem();
         return there;
       };
       if (PAIRED) {
@@ -893,11 +899,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
     int masks = 0;                          // tiles of the stream up to this item
     [[maybe_unused]] uint32_t q_phase = 0;
     uint32_t units = 0, mine_done = 0;      // tiles of the slot so far: unit n has buffer n % NB, phase n / NB; its items so far
+    [[maybe_unused]] uint32_t splits = 0;   // items of the slot so far that were split
     bool ok = true;
     while (true) {
       ok = next_item(stream, items, t);
       if (!ok || t.tiles == 0) break;
-      const int rho = t.rho0 + (PAIRED ? slot * kSlotRows : 0) + quad * 32 + lane;
+      // kBox, up to 64 rows: rows 64 to 127 of the slot are the same rows again, and take the second half of each tile's keys.  A thread has half of the
+      // exponentials of a tile, which is what a tile waits for; the two sums of a row are joined behind the last tile.  (16 groups of 50 rows over 3,750 keys, head_dim 64: a
+      // call of 56 us without, 52 with; at head_dim 128 a tile waits for its values then, which have one place, and nothing is gained.)
+      const bool split = Shape::kBox && t.rows - t.rho0 <= kSlotRows / 2;
+      const int half = split ? quad >> 1 : 0;
+      const int rho = t.rho0 + (PAIRED ? slot * kSlotRows : 0) + (split ? quad & 1 : quad) * 32 + lane;
       uint32_t tok, hq;
       p.per_kv.divmod(static_cast<uint32_t>(rho), tok, hq);
       const bool there = rho < t.rows;
@@ -909,6 +921,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         // The thread's query, in fp16 by a power of two, which puts its largest value in [1, 2) (queries between 2^-100 and 2^100).  (By the warps that hand
         // out items 15,000 cycles ahead of the first product, by these 3,000, of which none pass under the item before.)
         ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
+        if (Shape::kBox && ok && splits > 0) ok = __all_sync(ALL, mbar_wait(&bar.box_empty[slot], (splits - 1) & 1, p.status, 51));  // (the box is where the queries are)
         if (!ok) break;
         q_phase ^= 1;
         if (!idle) {
@@ -941,9 +954,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       float o_apart[D];    // O behind the tile before, where that was formed apart (in local memory)
       bool apart = false;
       const int mine = PAIRED ? (slot ? t.n[1] : t.n[0]) : t.tiles;
-      // One tile.  LATE: it has own tokens that rows of the warp see and others do not.
-      auto do_tile = [&](auto late, int u) {
-        constexpr bool LATE = decltype(late)::value;
+      // One tile.  LATE: it has own tokens that rows of the warp see and others do not (kBox: `own_late` says so, the code is the same).
+      auto do_tile = [&](auto late, auto halves, int u, bool own_late) {
+        constexpr bool LATE = decltype(late)::value && !FP4, SPLIT = decltype(halves)::value;
+        const bool is_late = Shape::kBox ? own_late : decltype(late)::value;
         const uint32_t buffer = units % NB, parity = (units / NB) & 1;
         const uint32_t tb = tm + buffer * BN;
         if (idle) {
@@ -969,7 +983,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           both &= seen[i];
         }
         bool masked = both != 0xffffffffu;
-        if (LATE) {
+        if (is_late) {
           masked = true;
 #pragma unroll
           for (int i = 0; i < W; ++i) seen[i] &= low_bits(limit - (v - t.p128) - 32 * i);
@@ -989,16 +1003,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 #pragma unroll
           for (int e = 0; e < 32; e += 2) m4[(e >> 1) & 3] = max3(m4[(e >> 1) & 3], __uint_as_float(sc[i][e]), __uint_as_float(sc[i][e + 1]));
         };
-        tc_ld_32x32b_x32(tb, sc[0]);
-        if (W == 4) tc_ld_32x32b_x32(tb + 32, sc[1]);
-        tc_wait_ld();
+        if constexpr (SPLIT) {  // words 0 and 1 of the tile, of which this warp has one
+          seen[0] = half ? seen[1] : seen[0];
+          tc_ld_32x32b_x32(tb + 32 * half, sc[0]);
+          tc_wait_ld();
+          largest(0);
+        } else {
+          tc_ld_32x32b_x32(tb, sc[0]);
+          if (W == 4) tc_ld_32x32b_x32(tb + 32, sc[1]);
+          tc_wait_ld();
 #pragma unroll
-        for (int i = W / 2; i < W; ++i) tc_ld_32x32b_x32(tb + 32 * i, sc[i]);
+          for (int i = W / 2; i < W; ++i) tc_ld_32x32b_x32(tb + 32 * i, sc[i]);
 #pragma unroll
-        for (int i = 0; i < W / 2; ++i) largest(i);
-        tc_wait_ld();
+          for (int i = 0; i < W / 2; ++i) largest(i);
+          tc_wait_ld();
 #pragma unroll
-        for (int i = W / 2; i < W; ++i) largest(i);
+          for (int i = W / 2; i < W; ++i) largest(i);
+        }
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         const float m_tile = mx * factor;
         const bool moves = m_tile > m_ref + 8.0f;
@@ -1040,7 +1061,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         const uint64_t k2 = pack_f32x2(factor, factor), n2 = pack_f32x2(-ref, -ref);
         uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
+        for (int i = 0; i < (SPLIT ? 1 : W); ++i) {
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
@@ -1052,7 +1073,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], pack_f32x2(x0, x1));
             pk[e >> 1] = FP4 ? pack_f16(x0, x1) : pack_bf16(x0, x1);
           }
-          tc_st_x16(tb + 16 * i, pk);  // over S, which is in registers
+          tc_st_x16(tb + 16 * (SPLIT ? half : i), pk);  // over S, which is in registers
+          if (SPLIT) {
+            const uint32_t none[16] = {};
+            tc_st_x16(tb + 16 * (half ^ 1), none);
+          }
           if (Shape::kHalves && !LATE && i == W / 2 - 1) {
             tc_wait_st_all();
             tc_fence_before();
@@ -1088,8 +1113,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       // that they have come here.
       if (PAIRED && mine > 0 && !idle) ok = __all_sync(ALL, mbar_wait(&bar.s_full[slot][units % NB], (units / NB) & 1, p.status, 55));
       int u = 0;
-      for (; ok && u < first_late; ++u, ++units) do_tile(std::false_type{}, u);
-      for (; ok && u < mine; ++u, ++units) do_tile(std::true_type{}, u);
+      if constexpr (Shape::kBox) {
+        if (split)
+          for (; ok && u < mine; ++u, ++units) do_tile(std::false_type{}, std::true_type{}, u, u >= first_late);
+        for (; ok && u < mine; ++u, ++units) do_tile(std::false_type{}, std::false_type{}, u, u >= first_late);
+      } else {
+        for (; ok && u < first_late; ++u, ++units) do_tile(std::false_type{}, std::false_type{}, u, false);
+        for (; ok && u < mine; ++u, ++units) do_tile(std::true_type{}, std::false_type{}, u, true);
+      }
       masks += t.tiles;
       if (!ok) break;
       if (mine == 0) continue;
@@ -1097,6 +1128,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       ok = __all_sync(ALL, mbar_wait(&bar.pv_done[slot][(units - 1) % NB], (PAIRED ? mine_done : (units - 1) / NB) & 1, p.status, 46));
       if (!ok) break;
       ++mine_done;
+      if constexpr (Shape::kBox) {
+        if (split) {
+          // The upper half hands its sums over where the queries were (a row of D floats, its 16-byte pieces in an order of its own), the lower half joins them.
+          tc_fence_after();
+          const int r = (quad & 1) * 32 + lane;
+          const uint32_t box = smem_u32(q_s) + slot * Shape::kQ + r * (D * 4);
+          auto piece = [&](int c) { return box + ((c ^ (r & 7)) << 4); };
+          if (half == 1) {
+            if (!idle) {
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) {
+                uint32_t o[32];
+                tc_ld_32x32b_x32(tm + PT_TM_O + 32 * i, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t x[4] = {o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]};
+                  st_shared16(piece(8 * i + e), x);
+                }
+              }
+              bar.box_ml[slot][r] = make_float2(in_log2(m_ref, factor, scale2), l);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.box_full[slot]);
+          } else {
+            ok = __all_sync(ALL, mbar_wait(&bar.box_full[slot], splits & 1, p.status, 52));
+            if (!ok) break;
+            if (!idle) {
+              const float2 other = bar.box_ml[slot][r];
+              const float own_m = in_log2(m_ref, factor, scale2), m = fmaxf(own_m, other.x), ref = m == NEG_INF ? 0.0f : m;
+              const float a = ex2(own_m - ref), b = ex2(other.x - ref);
+              const int64_t row = t.row0 + static_cast<int>(tok), qh = t.head * static_cast<int64_t>(p.per_kv.d) + hq;
+              const int64_t at = (static_cast<int64_t>(t.part) * p.rows.rows + row) * p.q_heads + qh;
+              if (there) p.part_ml[at] = make_float2(m, a * l + b * other.y);
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) {
+                uint32_t o[32];
+                tc_ld_32x32b_x32(tm + PT_TM_O + 32 * i, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  float4 x;
+                  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(piece(8 * i + e)) : "memory");
+                  const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) o[4 * e + k] = __float_as_uint((a * __uint_as_float(o[4 * e + k]) + b * y[k]) * p.v_factor);
+                }
+                if (there) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) store32(p.part_o + at * D + 32 * i + 8 * e, &o[8 * e]);
+                }
+              }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.box_empty[slot]);
+          }
+          ++splits;
+          continue;
+        }
+      }
       if (idle) continue;
       tc_fence_after();
       if (apart) put_back<D>(o_apart, tm + PT_TM_O);
