@@ -16,6 +16,7 @@
 // too, so that no thread waits for another's maximum (a second load of the same bytes, from L1).
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -404,37 +405,47 @@ struct ValuesParams {
   int64_t page_bytes, total;  // total: scales
   float scale;
   int32_t head_dim;
-  FastDiv per_head, heads, tokens;
+  FastDiv per_head, per_token, tokens;
   __nv_bfloat16* out;
 };
-__global__ void __launch_bounds__(256) kv_values_kernel(const ValuesParams p) {
+// WIDE: more than 2^31 scales, with divisions of 64 bits.
+template <bool WIDE>
+__global__ void __launch_bounds__(256) kv_values_kernel(const __grid_constant__ ValuesParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int D = p.head_dim;
   for (int64_t n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; n < p.total; n += static_cast<int64_t>(gridDim.x) * 256) {
     // page, token, head, scale of the head
-    const uint32_t per_token = p.per_head.d * p.heads.d;
-    const int64_t place = n / per_token;
-    uint32_t head, u, token;
-    p.per_head.divmod(static_cast<uint32_t>(n - place * per_token), head, u);
-    const int64_t page = place / p.tokens.d;
-    token = static_cast<uint32_t>(place - page * p.tokens.d);
+    const uint32_t per_token = p.per_token.d;
+    int64_t page;
+    uint32_t head, u, token, in_token;
+    if (WIDE) {
+      const int64_t place = n / per_token;
+      in_token = static_cast<uint32_t>(n - place * per_token);
+      page = place / p.tokens.d;
+      token = static_cast<uint32_t>(place - page * p.tokens.d);
+    } else {
+      uint32_t place, page32;
+      p.per_token.divmod(static_cast<uint32_t>(n), place, in_token);
+      p.tokens.divmod(place, page32, token);
+      page = page32;
+    }
+    p.per_head.divmod(in_token, head, u);
     const uint8_t* const unit = p.pages + page * p.page_bytes + (static_cast<int64_t>(head) * (p.tokens.d / kFp4Tokens) + token / kFp4Tokens) * (kFp4Unit * D);
     token %= kFp4Tokens;
     const uint2 codes = *reinterpret_cast<const uint2*>(unit + token * (D / 2) + u * 8);
     const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(e4m3_as_half(unit[8 * D + token * (D / 16) + u])))) * 256.0f * p.scale;
     uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t two = (j < 4 ? codes.x : codes.y) >> (8 * (j & 3)) & 0xffu;
-      float v[2];
+    for (int j = 0; j < 2; ++j) {
+      uint32_t h[4];
+      e2m1_as_half(j ? codes.y : codes.x, h);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // (sign, two bits of exponent, one of significand: as fp16 bits the value over 2^14)
-        const uint32_t c = two >> (4 * e);
-        v[e] = __half2float(__ushort_as_half(static_cast<unsigned short>((c & 8) << 12 | (c & 7) << 9))) * 16384.0f * s;
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+        const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * s, f.y * s);
+        w[4 * j + e] = *reinterpret_cast<const uint32_t*>(&b);
       }
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
-      w[j] = *reinterpret_cast<const uint32_t*>(&b);
     }
     uint4* const dst = reinterpret_cast<uint4*>(p.out + n * 16);
     dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -479,8 +490,8 @@ extern "C" int vx_kv_values_fp4(const void* pages, int64_t n_pages, int64_t page
   if (n_pages == 0) return 0;
   if (!out || !aligned16(out)) return fail(-1, "out must be 16-byte aligned");
   ValuesParams p{c.k, page_bytes, n_pages * page_size * kv_heads * (head_dim / 16), scale, head_dim, FastDiv(static_cast<uint32_t>(head_dim / 16)),
-                 FastDiv(static_cast<uint32_t>(kv_heads)), FastDiv(static_cast<uint32_t>(page_size)), static_cast<__nv_bfloat16*>(out)};
-  const int64_t blocks = (p.total + 255) / 256, most = 16 * static_cast<int64_t>(sm_count());
-  VX_CUDA_OK(launch_dependent(kv_values_kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
+                 FastDiv(static_cast<uint32_t>(kv_heads * (head_dim / 16))), FastDiv(static_cast<uint32_t>(page_size)), static_cast<__nv_bfloat16*>(out)};
+  const int64_t blocks = (p.total + 255) / 256, most = 64 * static_cast<int64_t>(sm_count());
+  VX_CUDA_OK(launch_dependent(p.total < (1ll << 31) ? kv_values_kernel<false> : kv_values_kernel<true>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
   return 0;
 }

@@ -119,6 +119,17 @@ constexpr int kFp4Tokens = 16, kFp4Unit = 9;  // of a unit; bytes per value of a
 // included.  The sign bit is dropped; 0x7f gives 480 / 256.
 __device__ __forceinline__ uint32_t e4m3_as_half(uint32_t byte) { return (byte & 0x7fu) << 7; }
 
+// The eight codes of a word as fp16, byte by byte.
+__device__ __forceinline__ void e2m1_as_half(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
 // Checks of the descriptors that both entry points make; 0 or an error code.
 int check_paged(const vx_kv_cache* cache, const vx_kv_rows* rows, PagedCache& c, KvRows& r);
 int check_paged(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, Fp4Cache& c, KvRows& r);

@@ -159,14 +159,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 // Eight codes times their scale (fp16 twice, over 256), exactly
 __device__ __forceinline__ void codes_as_half(uint32_t w, uint32_t scale, uint32_t (&h)[4]) {
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(w));
+  e2m1_as_half(w, h);
 #pragma unroll
   for (int j = 0; j < 4; ++j) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(scale));
 }

@@ -24,12 +24,8 @@ namespace {
 
 constexpr int VR_THREADS = 256;
 constexpr int VN_THREADS = 512;
-#ifndef VR_LEAST
-#define VR_LEAST 4096
-#endif
-#ifndef VN_LEAST
-#define VN_LEAST 4096
-#endif
+constexpr int VR_CTAS = 4;     // per SM at least, of rows: eight loads of 16 bytes a thread are on their way (64 sequences of six rows of 131,071, both sides: 144 us, six CTAs 145)
+constexpr int VR_LEAST = 4096, VN_LEAST = 4096;  // values of a CTA, where a row is cut
 constexpr unsigned ALL = 0xffffffffu;
 
 enum Draft : int32_t { kFalls = 0, kStands = 1, kOpen = 2 };
@@ -88,11 +84,13 @@ __device__ __forceinline__ V ld_cluster(const V* p, uint32_t rank) {  // of the 
 // Maximum and sum of a part of a row, of this thread; and, for temperature 0, the first place of the maximum.
 struct Running {
   float m = -INFINITY, sum = 0.0f;
+  float off = 0.0f;  // -m c, 0 for -infinity
   int at = 0x7fffffff;
 };
 
-template <bool GREEDY, int N>
-__device__ __forceinline__ void take(Running& r, const float (&x)[N], int at, float c) {
+// N values, in ascending order; `at`: place of the first, the next PIECE follow it, those behind are `step` further
+template <bool GREEDY, int PIECE, int N>
+__device__ __forceinline__ void take(Running& r, const float (&x)[N], int at, int step, float c) {
   float m = x[0];
 #pragma unroll
   for (int j = 1; j < N; ++j) m = fmaxf(m, x[j]);
@@ -104,16 +102,18 @@ __device__ __forceinline__ void take(Running& r, const float (&x)[N], int at, fl
       r.m = m;
 #pragma unroll
       for (int j = N - 1; j >= 0; --j)
-        if (x[j] == m) r.at = at + j;
+        if (x[j] == m) r.at = at + j / PIECE * step + j % PIECE;
     }
   } else {
     if (m > r.m) {
       r.sum *= ex2((r.m - m) * c);
       r.m = m;
+      r.off = -m * c;
     }
-    const float ref = r.m == -INFINITY ? 0.0f : r.m;
+    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < N; ++j) r.sum += ex2((x[j] - ref) * c);
+    for (int j = 0; j < N; ++j) sum[j & 1] += ex2(fmaf(x[j], c, r.off));
+    r.sum += sum[0] + sum[1];
   }
 }
 template <bool GREEDY>
@@ -130,12 +130,21 @@ __device__ __forceinline__ void join(Running& a, float m, float sum, int at, flo
 }
 
 // 16-byte pieces of a row from the first aligned one on, values in front and behind one by one; pieces first, first + step, ...
-template <typename T, bool GREEDY>
-__device__ __forceinline__ void walk(Running& r, const T* row, int n, int first, int step, float c) {
-  constexpr int N = 16 / sizeof(T), AHEAD = 4;
-  const int head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T)), n);
-  const int pieces = (n - head) / N;
-  auto convert = [](const uint4& u, float (&x)[N]) {
+template <typename T>
+struct RowPieces {
+  static constexpr int N = 16 / sizeof(T);
+  const T* row;
+  int head, pieces, rest;  // values in front of the pieces, pieces, values around them
+  __device__ __forceinline__ RowPieces(const T* r, int n) : row(r) {
+    head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / static_cast<int>(sizeof(T)), n);
+    pieces = (n - head) / N;
+    rest = n - pieces * N;
+  }
+  __device__ __forceinline__ uint4 load(int i) const {  // behind the end: -infinity
+    constexpr uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+    return i < pieces ? reinterpret_cast<const uint4*>(row + head)[i] : make_uint4(none, none, none, none);
+  }
+  __device__ __forceinline__ static void convert(const uint4& u, float* x) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -146,36 +155,49 @@ __device__ __forceinline__ void walk(Running& r, const T* row, int n, int first,
         x[j] = __uint_as_float(w[j]);
       }
     }
-  };
-  const uint4* const src = reinterpret_cast<const uint4*>(row + head);
-  int i = first;
-  for (; i + (AHEAD - 1) * step < pieces; i += AHEAD * step) {
-    uint4 u[AHEAD];
+  }
+  __device__ __forceinline__ int rest_at(int i) const { return i < head ? i : pieces * N + i; }  // where the i-th value around the pieces is
+};
+
+// One or two rows (SIDES) together: all that is loaded of a turn is on its way before any of it is used.
+template <typename T, bool GREEDY, int SIDES>
+__device__ __forceinline__ void walk(Running (&r)[2], const T* const (&rows)[2], int n, int first, int step, float c) {
+  using Pieces = RowPieces<T>;
+  constexpr int AHEAD = 4;
+  const Pieces p[2] = {Pieces(rows[0], n), Pieces(rows[SIDES - 1], n)};
+  const int most = SIDES == 2 ? max(p[0].pieces, p[1].pieces) : p[0].pieces;
+  float edge[2];
+  bool has[2] = {};
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) u[a] = src[i + a * step];
+  for (int e = 0; e < SIDES; ++e) {  // (fewer than 2 N values)
+    has[e] = first < p[e].rest;
+    edge[e] = has[e] ? to_float(rows[e][p[e].rest_at(first)]) : -INFINITY;
+  }
+#pragma unroll 1
+  for (int i = first; i < most; i += AHEAD * step) {
+    uint4 u[SIDES][AHEAD];
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      float x[N];
-      convert(u[a], x);
-      take<GREEDY>(r, x, head + (i + a * step) * N, c);
+    for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+      for (int e = 0; e < SIDES; ++e) u[e][a] = p[e].load(i + a * step);
+#pragma unroll
+    for (int e = 0; e < SIDES; ++e) {
+      float x[AHEAD * Pieces::N];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) Pieces::convert(u[e][a], x + a * Pieces::N);
+      take<GREEDY, Pieces::N>(r[e], x, p[e].head + i * Pieces::N, step * Pieces::N, c);
     }
   }
-  for (; i < pieces; i += step) {
-    float x[N];
-    convert(src[i], x);
-    take<GREEDY>(r, x, head + i * N, c);
-  }
-  // the values around the pieces, of which there are fewer than 2 N
-  const int rest = head + (n - head - pieces * N);
-  if (first < rest) {
-    const int at = first < head ? first : head + pieces * N + first - head;
-    const float x[1] = {to_float(row[at])};
-    take<GREEDY>(r, x, at, c);
-  }
+#pragma unroll
+  for (int e = 0; e < SIDES; ++e)
+    if (has[e]) {
+      const float x[1] = {edge[e]};
+      take<GREEDY, 1>(r[e], x, p[e].rest_at(first), 0, c);
+    }
 }
 
 template <typename T, bool GREEDY>
-__global__ void __launch_bounds__(VR_THREADS) verify_rows_kernel(const __grid_constant__ VerifyParams p, int ctas) {
+__global__ void __launch_bounds__(VR_THREADS, VR_CTAS) verify_rows_kernel(const __grid_constant__ VerifyParams p, int ctas) {
   pdl_launch_dependents();
   __shared__ float m_s[2][VR_THREADS / 32], sum_s[2][VR_THREADS / 32];
   __shared__ int at_s[VR_THREADS / 32];
@@ -198,11 +220,17 @@ __global__ void __launch_bounds__(VR_THREADS) verify_rows_kernel(const __grid_co
   const T* const row_t = static_cast<const T*>(p.logits) + row * p.ld;
   const bool drafter = !GREEDY && p.draft_logits && !last;
   const T* const row_d = drafter ? static_cast<const T*>(p.draft_logits) + row * p.ld_draft : row_t;
+  // (of the draft, for the end: on its way with the rows)
+  const int64_t draft = last ? -1 : id_at(p, row + 1);
+  const bool known = draft >= 0 && draft < p.vocab;
+  const float u = p.uniforms[row].x, draft_t = known ? to_float(row_t[draft]) : 0.0f, draft_d = known ? to_float(row_d[draft]) : 0.0f;
   Running r[2];
+  const T* const rows[2] = {row_t, row_d};
+  if (drafter) walk<T, GREEDY, 2>(r, rows, p.vocab, rank * VR_THREADS + threadIdx.x, ctas * VR_THREADS, c);
+  else walk<T, GREEDY, 1>(r, rows, p.vocab, rank * VR_THREADS + threadIdx.x, ctas * VR_THREADS, c);
 #pragma unroll
   for (int e = 0; e < (GREEDY ? 1 : 2); ++e) {
     if (e == 1 && !drafter) break;
-    walk<T, GREEDY>(r[e], e ? row_d : row_t, p.vocab, rank * VR_THREADS + threadIdx.x, ctas * VR_THREADS, c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float m = __shfl_xor_sync(ALL, r[e].m, o), sum = __shfl_xor_sync(ALL, r[e].sum, o);
@@ -239,15 +267,13 @@ __global__ void __launch_bounds__(VR_THREADS) verify_rows_kernel(const __grid_co
     RowFinding f{a[0].m, a[1].m, kFalls, -1};
     auto sound = [](const Running& r) { return r.sum > 0.0f && r.sum < INFINITY && fabsf(r.m) < INFINITY; };  // (NaN among the logits: the sum is)
     if (!GREEDY && !(sound(a[0]) && (!drafter || sound(a[1])))) f.most = NAN;  // nothing is drawn from this row
-    const int64_t d = last ? -1 : id_at(p, row + 1);
-    const bool known = d >= 0 && d < p.vocab;
     if (GREEDY) {
       // (a maximum that is not finite, or NaN among the logits: none)
       f.best = a[0].sum == 0.0f && fabsf(a[0].m) < INFINITY ? a[0].at : -1;
-      if (known && f.best == d) f.draft = kStands;
+      if (known && f.best == draft) f.draft = kStands;
     } else if (known && f.most == f.most) {
-      const float pt = ex2((to_float(row_t[d]) - a[0].m) * c), qd = drafter ? ex2((to_float(row_d[d]) - a[1].m) * c) : 1.0f;
-      const float left = p.uniforms[row].x * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * 0x1p-12f;
+      const float pt = ex2((draft_t - a[0].m) * c), qd = drafter ? ex2((draft_d - a[1].m) * c) : 1.0f;
+      const float left = u * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * 0x1p-12f;
       // (anything near the end of the range is open)
       if (!(left > 1e-30f && right > 1e-30f && left < 1e30f && right < 1e30f) || fabsf(left - right) <= gap) f.draft = kOpen;
       else f.draft = left < right ? kStands : kFalls;
