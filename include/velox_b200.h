@@ -491,7 +491,7 @@ int vx_prefix_attention_fp4(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows
  * temperature 0: a draft stands where it is the first of the largest logits, next is that of its row.
  * accepted i32 [sequences]: drafts that stand; next i32 [sequences], -1 where the row has no finite logit, or one that is NaN or +infinity, or the
  * drafter's row where it counts (such a row's draft does not stand either), or where the sequence has no row.  An id outside [0, vocab) does not stand.  Logits of -infinity have probability 0.
- * What decides is computed in 64 bits, or in 32 where a bound of their error leaves no doubt; probabilities below 2^-1020 count as 0.  Rows behind the last
+ * What decides is computed in 64 bits, or in 32 where a bound of their error leaves no doubt; probabilities below 2^-1000 count as 0.  Rows behind the last
  * sequence are not looked at. */
 typedef struct {
   int32_t struct_size; /* sizeof(vx_verify_desc) */

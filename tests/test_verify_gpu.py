@@ -223,3 +223,32 @@ def test_refusals_and_launches(ops):
     ops.reset_launch_count()
     ops.verify_drafts(x, ids, u, row_offsets=off, temperature=1)
     assert ops.launch_count() == 2
+
+
+@pytest.mark.parametrize("temperature,level", [(0.01, 500.0), (0.01, -500.0), (2.0 ** -10, 64.0), (1.0, 30000.0), (2.0 ** -20, 0.25), (2.0 ** -20, -1.0)])
+@pytest.mark.parametrize("drafter", [True, False])
+def test_logits_that_are_large_for_their_temperature(ops, temperature, level, drafter):
+    """The largest logit over the temperature is 30,000 to 1,000,000, and the uniform numbers are 2^-11 from where a draft falls."""
+    x, y, ids, u = make(120, 3000, torch.float32, 21, True, gain=1.0)
+    x, y = level + temperature * x, level + temperature * y
+    p, q = (torch.softmax(t.double() / temperature, 1)[:-1].gather(1, ids[1:, None])[:, 0] for t in (x, y))
+    side = torch.where(torch.arange(119, device="cuda") % 7 < 5, -1.0, 1.0)  # (five that stand, then two that fall)
+    ratio = p / q if drafter else p
+    u[:-1, 0] = (ratio * (1 + side * 2.0 ** -11)).clamp(0, 1 - 2.0 ** -24).float()
+    check(ops, x, y if drafter else None, ids, u, [6 * i for i in range(21)], temperature)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 2.0 ** -20, 2.0 ** 20, 0.0])
+def test_lowest_and_largest_logits(ops, dtype, temperature):
+    """Tokens that are masked with the type's lowest value have no probability beside others, and one like another where they are all there is.
+    (A masked draft has 0 on both sides of its comparison, of any rounding: no margin is asked for.)"""
+    x, y, ids, u = make(32, 517, dtype, 22, True)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x[:8, 100:], y[:8, 90:] = low, low
+    x[8:16], y[9] = low, low
+    x[16:20, 5], x[20:24], y[21] = high, high, high
+    x[24:28, 3:], x[24:28, :3] = low, -float("inf")
+    off = [4 * i for i in range(9)]
+    check(ops, x, y, ids, u, off, temperature, margin=False)
+    check(ops, x, None, ids, u, off, temperature, margin=False)

@@ -1,13 +1,17 @@
 // Drafted tokens against the target's probabilities (vx_verify_drafts), in two launches:
 //
 //   verify_rows_kernel   a cluster per row: the row's largest logit and the sum of 2^((x - max) c), c = log2(e) / T, of the target and of the drafter, in
-//                        one pass in fp32; from them whether the row's draft stands.  p(d) and q(d) come out within 2^-17 (2^-24 of the exponent, up to 128,
-//                        in each of the two exponentials; sums of positive terms, the exponents of those that count small), so where u q(d) and
-//                        p(d) are 2^-12 of each other apart the comparison is settled; the others, some 1 of 4,000, are left open.
+//                        one pass in fp32; from them whether the row's draft stands.  The exponentials come out within 2^-16 (a difference and a product, 2^-24 each of an
+//                        exponent up to 128), their sums, 16 of a thread at a time, within vocab 2^-36 more at worst, so where u q(d) and p(d) are 2^-12 +
+//                        vocab 2^-34 of each other apart the comparison is settled; the others, some 1 of 4,000, are left open.
 //   verify_next_kernel   a cluster per sequence: the first row whose draft falls (open rows settled in fp64), and the token drawn from what is left there:
-//                        sums of both rows, then of max(p - q, 0) in ascending order -- CTA, thread, token -- in fp64, since a token stands or falls with
-//                        one comparison of a sum over the vocabulary: with 131,071 tokens and fp32 sums one draw of ten would be near a border.
+//                        sums of both rows, then of max(p - q, 0) in ascending order -- CTA, warp, group of 32, lane -- in fp64, since a token stands or falls
+//                        with one comparison of a sum over the vocabulary: with 131,071 tokens and fp32 sums one draw of ten would be near a border.
 //
+// What bounds them: the first, HBM (384 rows of 131,071 in fp32 and 320 of the drafter's, 369 MB in 68 us, 5.4 TB/s); the second the barriers between its
+// passes, the loads of few clusters and fp64 (nine operations a logit and walk, 20 % of that pipe in 80 us); small calls the round trips to memory: 50 rows of 5,538
+// take 12.5 us in both together.
+
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -84,7 +88,7 @@ __device__ __forceinline__ V ld_cluster(const V* p, uint32_t rank) {  // of the 
 // Maximum and sum of a part of a row, of this thread; and, for temperature 0, the first place of the maximum.
 struct Running {
   float m = -INFINITY, sum = 0.0f;
-  float off = 0.0f;  // -m c, 0 for -infinity
+  float ref = 0.0f;  // m, 0 for -infinity
   int at = 0x7fffffff;
 };
 
@@ -108,11 +112,11 @@ __device__ __forceinline__ void take(Running& r, const float (&x)[N], int at, in
     if (m > r.m) {
       r.sum *= ex2((r.m - m) * c);
       r.m = m;
-      r.off = -m * c;
+      r.ref = m;
     }
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum[j & 1] += ex2(fmaf(x[j], c, r.off));
+    for (int j = 0; j < N; ++j) sum[j & 1] += ex2((x[j] - r.ref) * c);  // (x c - m c in one operation is off by 2^-24 of m c, and m c is not bounded)
     r.sum += sum[0] + sum[1];
   }
 }
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(VR_THREADS, VR_CTAS) verify_rows_kernel(const 
       if (known && f.best == draft) f.draft = kStands;
     } else if (known && f.most == f.most) {
       const float pt = ex2((draft_t - a[0].m) * c), qd = drafter ? ex2((draft_d - a[1].m) * c) : 1.0f;
-      const float left = u * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * 0x1p-12f;
+      const float left = u * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * (0x1p-12f + 0x1p-34f * static_cast<float>(p.vocab));
       // (anything near the end of the range is open)
       if (!(left > 1e-30f && right > 1e-30f && left < 1e30f && right < 1e30f) || fabsf(left - right) <= gap) f.draft = kOpen;
       else f.draft = left < right ? kStands : kFalls;
@@ -299,18 +303,18 @@ __device__ const double kFine[32] = {  // 2^(k / 1024)
     1.0108892860517005, 1.011573790214578, 1.0122587578762337, 1.0129441893505169, 1.0136300849514894, 1.0143164449934257, 1.0150032697908125, 1.0156905596583505,
     1.016378314910953, 1.0170665358637463, 1.0177552228320703, 1.0184443761314785, 1.019133996077738, 1.0198240829868295, 1.0205146371749483, 1.0212056589585028};
 
-// 2^((x - at) c) for x <= at; 0 below 2^-1000
+// 2^((x - at) c) for x <= at; 0 below 2^-1000.  (The difference first: it is exact, or as near as its own size asks for; x c and at c are not bounded.)
 struct Weight {
-  double c, from;  // from: at c
-  float c32, at;
+  double c, at;
+  float c32, at32;
   __device__ __forceinline__ double operator()(const double* tab, float x) const {
     constexpr double big = 6755399441055744.0 / kExpTable;  // 1.5 2^52 / 1024: the last bit of a sum is 1 / 1024
-    const double y = fma(static_cast<double>(x), c, -from), t = y + big, r = y - (t - big);
+    const double y = static_cast<double>(x) - at, t = fma(y, c, big), r = fma(y, c, -(t - big));
     const int n = __double2loint(t);
     constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3;
     const double s = tab[n & (kExpTable - 1)], v = fma(s, fma(fma(c3, r, c2), r, c1) * r, s);
     const int high = __double2hiint(v) + ((n >> 10) << 20);
-    return (x - at) * c32 >= -1000.0f ? __hiloint2double(high, __double2loint(v)) : 0.0;
+    return (x - at32) * c32 >= -1000.0f ? __hiloint2double(high, __double2loint(v)) : 0.0;
   }
 };
 
@@ -418,8 +422,8 @@ __global__ void __launch_bounds__(VN_THREADS, 2) verify_next_kernel(const __grid
     const int row = row0 + i;
     t = static_cast<const T*>(p.logits) + row * p.ld;
     d = i < drafts && p.draft_logits ? static_cast<const T*>(p.draft_logits) + row * p.ld_draft : nullptr;
-    wt = {c, static_cast<double>(found.most) * c, static_cast<float>(c), found.most};
-    wd = {c, static_cast<double>(found.draft_most) * c, static_cast<float>(c), found.draft_most};
+    wt = {c, found.most, static_cast<float>(c), found.most};
+    wd = {c, found.draft_most, static_cast<float>(c), found.draft_most};
     sure = -1;
     if (i < drafts && !p.draft_logits) {
       const int64_t id = id_at(p, row + 1);
