@@ -252,3 +252,13 @@ def test_lowest_and_largest_logits(ops, dtype, temperature):
     off = [4 * i for i in range(9)]
     check(ops, x, y, ids, u, off, temperature, margin=False)
     check(ops, x, None, ids, u, off, temperature, margin=False)
+
+
+@pytest.mark.parametrize("seqs,vocab", [(2, 2 ** 22 + 5), (150, 40001), (40, 70003)])
+def test_draws_from_long_rows(ops, seqs, vocab):
+    """Rows that a cluster or a block has alone, drawn from at their ends and between.  (A number of 0 asks for the first token that has a weight: tokens in front of it
+    have none, at any rounding, so no margin is asked for.)"""
+    x, y, ids, u = make(2 * seqs, vocab, torch.bfloat16, 23, True, peaks=0)
+    u[0::2, 0] = 1 - 2.0 ** -24
+    u[0::3, 1], u[1::5, 1] = 0.0, 1 - 2.0 ** -24
+    check(ops, x, y, ids, u, [2 * i for i in range(seqs + 1)], margin=False)

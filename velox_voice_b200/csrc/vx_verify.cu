@@ -334,7 +334,8 @@ __device__ __forceinline__ double warp_scan(double x) {  // the sum up to this l
 }
 
 // The tokens of a CTA are a run of the vocabulary, those of its warps runs of that, and a warp takes 32 neighbours at a time: sums by warps are sums in
-// ascending order, whose first to pass a number tells the warp that has the token.
+// ascending order, whose first to pass a number tells the warp that has the token.  (That warp's run, 2,048 of 131,071 tokens in a cluster of four, walked by the
+// warp alone took some 10 us.)
 template <typename T>
 __global__ void __launch_bounds__(VN_THREADS, 2) verify_next_kernel(const __grid_constant__ VerifyParams p, int ctas) {
   pdl_launch_dependents();
@@ -386,31 +387,33 @@ __global__ void __launch_bounds__(VN_THREADS, 2) verify_next_kernel(const __grid
   const int each = ((p.vocab + ctas * WARPS - 1) / (ctas * WARPS) + 31) / 32 * 32;
   const int v0 = min((rank * WARPS + warp) * each, p.vocab), v1 = min(v0 + each, p.vocab);
   int turn = 0;
-  // a and b, the warps' own, summed over the cluster; the sums of a in front of this warp in `before`
-  auto sum_all = [&](double& a, double& b, double& before) {
+  // a and b, the warps' own, summed over the cluster; what lane w keeps: a of warp w and of those up to it, in this CTA; lane k: of CTA k and of those up to it
+  double warp_own, warp_up, cta_own, cta_up;
+  auto sums_of_warps = [&](double a) {
     turn ^= 1;
-    if (lane == 0) {
-      warp_s[turn][0][warp] = a;
-      warp_s[turn][1][warp] = b;
-    }
+    if (lane == 0) warp_s[turn][0][warp] = a;
     __syncthreads();
-    const double up = warp_scan(lane < WARPS ? warp_s[turn][0][lane] : 0.0);
-    a = __shfl_sync(ALL, up, 31);
-    before = __shfl_sync(ALL, up, (warp + 31) & 31);
-    if (warp == 0) before = 0.0;
+    warp_own = lane < WARPS ? warp_s[turn][0][lane] : 0.0;
+    warp_up = warp_scan(warp_own);
+  };
+  auto sum_all = [&](double& a, double& b) {
+    if (lane == 0) warp_s[turn ^ 1][1][warp] = b;
+    sums_of_warps(a);
+    a = __shfl_sync(ALL, warp_up, 31);
     b = warp_sum(lane < WARPS ? warp_s[turn][1][lane] : 0.0);
+    cta_own = cta_up = a;
     if (ctas > 1) {
       if (threadIdx.x == 0) {
         cta_s[turn][0] = a;
         cta_s[turn][1] = b;
       }
       cluster_sync_all();
-      a = b = 0.0;
-      for (int k = 0; k < ctas; ++k) {
-        if (k == rank) before += a;
-        a += ld_cluster(&cta_s[turn][0], k);
-        b += ld_cluster(&cta_s[turn][1], k);
-      }
+      cta_own = lane < ctas ? ld_cluster(&cta_s[turn][0], lane) : 0.0;
+      b = warp_sum(lane < ctas ? ld_cluster(&cta_s[turn][1], lane) : 0.0);
+      cta_up = warp_scan(cta_own);
+      a = __shfl_sync(ALL, cta_up, 31);
+    } else if (lane > 0) {
+      cta_own = 0.0;
     }
   };
   // The row that is looked at: weights of its tokens, times 2^(largest logit c); the drafter's
@@ -477,16 +480,14 @@ __global__ void __launch_bounds__(VN_THREADS, 2) verify_next_kernel(const __grid
   };
   __syncthreads();  // (the table)
   int i = first_doubt(0), chosen = -1;
-  bool mine = false;                            // this warp has the token
   enum { kSums, kRest, kAll } what = kSums;     // what is summed up
   if (found.most == found.most) begin_row(i);
 #pragma unroll 1
   while (found.most == found.most) {            // (uniform over the cluster; NaN: nothing is drawn from the row)
-    double own, all, others, before;
-    if (d) walk_row(std::true_type{}, own, others);
-    else walk_row(std::false_type{}, own, others);
-    all = own;
-    sum_all(all, others, before);
+    double all, others;
+    if (d) walk_row(std::true_type{}, all, others);
+    else walk_row(std::false_type{}, all, others);
+    sum_all(all, others);
     if (what == kSums) {
       if (i < drafts && found.draft == kOpen) {
         const int64_t id = id_at(p, row0 + i + 1);
@@ -513,64 +514,54 @@ __global__ void __launch_bounds__(VN_THREADS, 2) verify_next_kernel(const __grid
       continue;
     }
     const double target = static_cast<double>(p.uniforms[row0 + i].y) * all;
-    // The first warp whose sum passes the target has the token; a number that is not below 1 (or rounding) can leave none: then the last with a weight.
-    __shared__ int first_s[2], seen_s[2];
-    if (threadIdx.x == 0) first_s[0] = 0x7fffffff, first_s[1] = -1;
-    __syncthreads();
-    if (lane == 0 && own > 0.0) {
-      if (before + own > target) atomicMin(&first_s[0], warp);
-      atomicMax(&first_s[1], warp);
-    }
-    __syncthreads();
-    int from = first_s[0], owner = from != 0x7fffffff ? rank : -1;
-    if (ctas > 1) {
-      if (threadIdx.x < 2) seen_s[threadIdx.x] = first_s[threadIdx.x];
-      cluster_sync_all();
-      owner = -1;
-      int fallback = -1;
-      for (int k = ctas - 1; k >= 0; --k) {
-        if (ld_cluster(&seen_s[0], k) != 0x7fffffff) owner = k;
-        if (fallback < 0 && ld_cluster(&seen_s[1], k) >= 0) fallback = k;
-      }
-      if (owner < 0) {
-        owner = fallback;
-        from = 0x7fffffff;
-      }
-    } else {
-      owner = 0;
-    }
-    const bool exact = from != 0x7fffffff;
-    mine = owner == rank && warp == (exact ? from : first_s[1]);
-    if (mine) {
-      // groups of 32 neighbours, four at a time: their sums, the first that passes the target, its lanes
-      double sum = before;
-      int pick = -1, heavy = -1;
+    // The first part whose sum passes the target has the token; a number that is not below 1 (or rounding) can leave none: then the last with a weight.
+    double before = 0.0;
+    bool exact = true;
+    auto holder_of = [&](double part, double up) {  // of a lane's part and those up to it; `before` moves on to what is in front of it
+      const unsigned has = __ballot_sync(ALL, part > 0.0), over = exact ? __ballot_sync(ALL, before + up > target) & has : 0;
+      exact = over != 0;
+      const int at = over ? __ffs(over) - 1 : 31 - __clz(has);
+      const double front = __shfl_sync(ALL, up, max(at - 1, 0));
+      if (at > 0) before += front;
+      return at;
+    };
+    if (holder_of(cta_own, cta_up) != rank) break;
+    // The run of the CTA's warp that has it, walked again by all of the CTA's, and of that the warp's that has it, until a warp's part is what it holds.
+    int holder = holder_of(warp_own, warp_up), run0 = min((rank * WARPS + max(holder, 0)) * each, p.vocab), run1 = min(run0 + each, p.vocab);
+    while (true) {
+      const int part = ((run1 - run0 + WARPS - 1) / WARPS + 31) / 32 * 32, w0 = min(run0 + warp * part, run1), w1 = min(w0 + part, run1);
+      double x[AHEAD] = {}, sum = 0.0;
 #pragma unroll 1
-      for (int v = v0; v < v1 && pick < 0; v += 32 * AHEAD) {
-        double x[AHEAD], group[AHEAD];
+      for (int v = w0; v < w1; v += 32 * AHEAD) {
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e) {
           const int at = v + 32 * e + lane;
           double drafter;
-          const float l = at < v1 ? to_float(t[at]) : -INFINITY;
-          x[e] = d ? left_of(std::true_type{}, at, l, at < v1 ? to_float(d[at]) : -INFINITY, drafter) : left_of(std::false_type{}, at, l, 0.0f, drafter);
+          const float l = at < w1 ? to_float(t[at]) : -INFINITY;
+          x[e] = d ? left_of(std::true_type{}, at, l, at < w1 ? to_float(d[at]) : -INFINITY, drafter) : left_of(std::false_type{}, at, l, 0.0f, drafter);
         }
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-          const unsigned has = __ballot_sync(ALL, x[e] > 0.0);
-          if (has) heavy = v + 32 * e + 31 - __clz(has);
-          group[e] = warp_sum(x[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-          if (exact && pick < 0 && sum + group[e] > target) {
-            const unsigned has = __ballot_sync(ALL, x[e] > 0.0), over = __ballot_sync(ALL, sum + warp_scan(x[e]) > target) & has;
-            pick = v + 32 * e + (over ? __ffs(over) - 1 : 31 - __clz(has));  // (a group of no weight does not pass)
-          }
-          sum += group[e];
-        }
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
       }
-      chosen = pick >= 0 ? pick : heavy;
+      sums_of_warps(warp_sum(sum));
+      holder = max(holder_of(warp_own, warp_up), 0);
+      if (part <= 32 * AHEAD) {
+        if (warp == holder) {
+#pragma unroll
+          for (int e = 0; e < AHEAD; ++e) {  // groups of 32 neighbours
+            const double up = warp_scan(x[e]);
+            const unsigned has = __ballot_sync(ALL, x[e] > 0.0), over = exact ? __ballot_sync(ALL, before + up > target) & has : 0;
+            if (over) {
+              chosen = w0 + 32 * e + __ffs(over) - 1;
+              break;
+            }
+            if (has) chosen = w0 + 32 * e + 31 - __clz(has);
+            before += __shfl_sync(ALL, up, 31);
+          }
+        }
+        break;
+      }
+      run0 = min(run0 + holder * part, run1);
+      run1 = min(run0 + part, run1);
     }
     break;
   }
