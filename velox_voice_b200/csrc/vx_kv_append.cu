@@ -13,7 +13,8 @@
 
 //
 // Into a cache in 4 bits (FP4): a thread takes the 16 values of one scale of a key or value; for a rotated key it loads the partners of its values
-// too, so that no thread waits for another's maximum (a second load of the same bytes, from L1).
+// too, so that no thread waits for another's maximum (a second load of the same bytes, from L1).  The size above takes 384 us, 1.9 GB at 4.9 TB/s: issue slots 56 % busy,
+// loads in flight of five blocks an SM (queries by a launch of their own, of six blocks: 410); 10 tokens 5 us, the call.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

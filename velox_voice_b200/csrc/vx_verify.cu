@@ -8,9 +8,9 @@
 //                        sums of both rows, then of max(p - q, 0) in ascending order -- CTA, warp, group of 32, lane -- in fp64, since a token stands or falls
 //                        with one comparison of a sum over the vocabulary: with 131,071 tokens and fp32 sums one draw of ten would be near a border.
 //
-// What bounds them: the first, HBM (384 rows of 131,071 in fp32 and 320 of the drafter's, 369 MB in 68 us, 5.4 TB/s); the second the barriers between its
-// passes, the loads of few clusters and fp64 (nine operations a logit and walk, 20 % of that pipe in 80 us); small calls the round trips to memory: 50 rows of 5,538
-// take 12.5 us in both together.
+// What bounds them: the first, HBM (384 rows of 131,071 in fp32 and 320 of the drafter's, 369 MB in 68 us, 5.4 TB/s); the second, 60 us there, latency: two walks in
+// fp64, nine operations a logit, that keep half of the issue slots busy, and the clusters' barriers between them; small calls the round trips to memory: 50 rows of
+// 5,538 take 11.5 us in both together.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
