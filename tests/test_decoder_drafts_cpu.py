@@ -45,6 +45,19 @@ def test_verify_keeps_the_drafts_that_stand(dec, monkeypatch):
         dec.settle(hyp)
 
 
+def test_a_refused_call_keeps_nothing(dec, monkeypatch):
+    def refuse(*a, **k):
+        raise ValueError("uniforms")
+
+    monkeypatch.setattr(D.ops, "verify_drafts", refuse)
+    hyp = dec.begin(dec.read(torch.zeros(10, 64), [4, 6]), 2, 12)
+    hyp.lengths.copy_(torch.tensor([3, 0, -1, 5], dtype=torch.int32))
+    hyp.tokens = [3, 0, 2, 5]
+    with pytest.raises(ValueError, match="uniforms"):
+        dec.verify(hyp, torch.arange(10), [4, 2, 4, 0], torch.rand(3, 2))
+    assert hyp.lengths.tolist() == [3, 0, -1, 5] and hyp.tokens == [3, 0, 2, 5]
+
+
 def test_unknown_caches_and_page_sizes_are_refused():
     for kw, text in ((dict(cache="fp5"), "cache"), (dict(cache="fp4", page_size=24), "16 n")):
         cfg = D.DecoderConfig(blocks=0, **kw)

@@ -229,8 +229,14 @@ class HypothesisDecoder:
         """Drafts: ids [sum(counts)] are, hypothesis after hypothesis, the token that :meth:`step` or this gave last and the drafts behind it; arguments and
         results (accepted, next) of :func:`ops.verify_drafts`.  The cache keeps the first token of a hypothesis and its drafts that stand.  (A hypothesis of
         no ids, or one that has finished, stays as it is, whatever the results say.)  `hyp.tokens` counts all drafts: :meth:`settle` after some calls."""
+        kept = hyp.tokens
         logits, offsets, n = self._score(hyp, ids, counts)
-        accepted, following = ops.verify_drafts(logits, ids, uniforms, draft_logits=draft_logits, row_offsets=offsets, temperature=temperature)
+        try:
+            accepted, following = ops.verify_drafts(logits, ids, uniforms, draft_logits=draft_logits, row_offsets=offsets, temperature=temperature)
+        except Exception:  # (refused: nothing of it is kept)
+            hyp.lengths.sub_(torch.where(hyp.lengths >= 0, n, 0))
+            hyp.tokens = kept
+            raise
         hyp.lengths.sub_(torch.where((hyp.lengths >= 0) & (n > 0), n - 1 - accepted, 0))
         return accepted, following
 
