@@ -2,8 +2,8 @@
 //
 //   verify_rows_kernel   a cluster per row: the row's largest logit and the sum of 2^((x - max) c), c = log2(e) / T, of the target and of the drafter, in
 //                        one pass in fp32; from them whether the row's draft stands.  The exponentials come out within 2^-16 (a difference and a product, 2^-24 each of an
-//                        exponent up to 128), their sums, 16 of a thread at a time, within vocab 2^-36 more at worst, so where u q(d) and p(d) are 2^-12 +
-//                        vocab 2^-34 of each other apart the comparison is settled; the others, some 1 of 4,000, are left open.
+//                        exponent up to 128), their sums, 16 of a thread at a time, within vocab 2^-35 more at worst, so where u q(d) and p(d) are 2^-12 +
+//                        vocab 2^-33 of each other apart the comparison is settled; the others, some 1 of 4,000, are left open.
 //   verify_next_kernel   a cluster per sequence: the first row whose draft falls (open rows settled in fp64), and the token drawn from what is left there:
 //                        sums of both rows, then of max(p - q, 0) in ascending order -- CTA, warp, group of 32, lane -- in fp64, since a token stands or falls
 //                        with one comparison of a sum over the vocabulary: with 131,071 tokens and fp32 sums one draw of ten would be near a border.
@@ -26,9 +26,9 @@
 namespace vx {
 namespace {
 
-constexpr int VR_THREADS = 256;
+constexpr int VR_THREADS = 128;  // rows of 5,538 have three pieces of 16 bytes a thread: 256 threads, of which an SM holds half as many rows, take 27.8 us for 26.5 with 1,038 rows
 constexpr int VN_THREADS = 512;
-constexpr int VR_CTAS = 4;     // per SM at least, of rows: eight loads of 16 bytes a thread are on their way (64 sequences of six rows of 131,071, both sides: 144 us, six CTAs 145)
+constexpr int VR_CTAS = 8;     // per SM at least, of rows: eight loads of 16 bytes a thread are on their way (more CTAs gain nothing, 144 : 145 us at 64 sequences of six rows of 131,071)
 constexpr int VR_LEAST = 4096, VN_LEAST = 4096;  // values of a CTA, where a row is cut
 constexpr unsigned ALL = 0xffffffffu;
 
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(VR_THREADS, VR_CTAS) verify_rows_kernel(const 
       if (known && f.best == draft) f.draft = kStands;
     } else if (known && f.most == f.most) {
       const float pt = ex2((draft_t - a[0].m) * c), qd = drafter ? ex2((draft_d - a[1].m) * c) : 1.0f;
-      const float left = u * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * (0x1p-12f + 0x1p-34f * static_cast<float>(p.vocab));
+      const float left = u * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * (0x1p-12f + 0x1p-33f * static_cast<float>(p.vocab));
       // (anything near the end of the range is open)
       if (!(left > 1e-30f && right > 1e-30f && left < 1e30f && right < 1e30f) || fabsf(left - right) <= gap) f.draft = kOpen;
       else f.draft = left < right ? kStands : kFalls;
@@ -645,7 +645,7 @@ extern "C" int vx_verify_drafts(const vx_verify_desc* d, void* stream) {
   const auto st = static_cast<cudaStream_t>(stream);
   const bool f32 = d->dtype == VX_F32;
   if (d->rows > 0) {
-    const int ctas = cluster_size(d->rows, 12 * static_cast<int64_t>(sm_count()), d->vocab, VR_LEAST);
+    const int ctas = cluster_size(d->rows, 24 * static_cast<int64_t>(sm_count()), d->vocab, VR_LEAST);
     auto kernel = p.greedy ? (f32 ? verify_rows_kernel<float, true> : verify_rows_kernel<__nv_bfloat16, true>)
                            : (f32 ? verify_rows_kernel<float, false> : verify_rows_kernel<__nv_bfloat16, false>);
     VX_CUDA_OK(launch_clusters(kernel, d->rows, ctas, VR_THREADS, st, p));
