@@ -403,3 +403,27 @@ def test_launches_are_counted(ops):
     assert ops.launch_count() == 3  # (few keys: attention is one launch)
     ops.prefix_attention(q, kp, vp, t.expand(2, 1).repeat(1, 900), n)
     assert ops.launch_count() == 5
+
+
+@pytest.mark.parametrize("rows,length", [(1, 90), (3, 2000), (70, 700)])
+def test_pages_beyond_four_gigabytes(ops, rows, length):
+    """The last of 480,000 pages (4.4 GB of keys and of values): what is appended and read is what a small cache of the same pages gives, bit for bit."""
+    many, ps, kv, d, seqs = 480_000, 16, 8, 128, 3
+    per = -(-(length + rows) // ps)
+    g = torch.Generator(device="cuda").manual_seed(31)
+    big = [ops.fp4_pages(many, ps, kv, d) for _ in range(2)]
+    small = [torch.randint(256, (seqs * per, kv, 1, 9 * d), generator=g, device="cuda", dtype=torch.uint8) for _ in range(2)]
+    for s, b in zip(small, big):
+        b[many - seqs * per:] = s
+    table = torch.arange(seqs * per, dtype=torch.int32, device="cuda").view(seqs, per)
+    offsets = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * rows
+    lengths = torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(seqs * rows, h, d, generator=g, device="cuda").bfloat16() for h in (32, kv, kv))
+    outs = []
+    for pages, at in ((big, table + (many - seqs * per)), (small, table)):
+        ops.kv_append(k, v, *pages, at, lengths, row_offsets=offsets)
+        outs.append(ops.prefix_attention(q, *pages, at, lengths, row_offsets=offsets))
+    assert torch.equal(*outs)
+    for s, b in zip(small, big):
+        assert torch.equal(b[many - seqs * per:], s) and not b[:1000].any()
+        assert torch.equal(ops.kv_values(b)[many - seqs * per:], ops.kv_values(s))
