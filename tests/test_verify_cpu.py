@@ -29,7 +29,7 @@ def test_definition_is_the_targets_distribution():
 
 
 def _desc(**kw):
-    d = _lib.VerifyDesc(C.sizeof(_lib.VerifyDesc), _lib.DT_BF16, 6, 100, 2, 4096, 100, 8192, 100, 256, 8, 0, 512, 1024, 1.0, 2048, 2064, 3072, 1 << 20)
+    d = _lib.VerifyDesc(C.sizeof(_lib.VerifyDesc), _lib.DT_BF16, 6, 100, 2, 4096, 100, 8192, 100, 256, 8, 0, 512, 1024, 1.0, 2048, 2064, 8448, 1 << 20)
     for k, v in kw.items():
         setattr(d, k, v)
     return _lib.load().vx_verify_drafts(C.byref(d), None)
