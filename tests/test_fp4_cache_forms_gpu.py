@@ -1,0 +1,98 @@
+"""prefix_attention over a cache in 4 bits, in each form that a call can take: few rows in one launch and in parts, tiles of the
+prefix and of own tokens, tiles of up to 64 rows, pairs of tiles with one result and with parts.  In each: scales of the cache, bytes of any kind, queries of all
+sizes, scores beyond what fp32 holds to the unit, rows of zeros under tiny scales, probabilities far below the largest.
+
+Tolerances by the number formats, as in test_fp4_cache_gpu.py, but for probabilities far below the row's largest: fp16 holds them to 2^-25 where the largest is
+2^7 or more, so they are off by 2^-32 of that, n of them by n 2^-32 of the largest value."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as P
+from test_fp4_cache_gpu import ints, host, ops, pages_of, tables  # noqa: F401  (ops: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+# (heads 4 on 2: two rows per token and key head.)  What decides: rows per owner and key head, how many keys the tables have place for.
+FORMS = {
+    "whole": dict(rows_of=[1, 2, 1, 3], lengths=[50, 7, 0, 90], prefix=[300]),                       # one launch
+    "rows": dict(rows_of=[1, 2, 1, 3], lengths=[1500, 7, 0, 900], prefix=[300]),                     # few rows, in parts
+    "rows16": dict(rows_of=[8, 5, 7], lengths=[1500, 7, 900], prefix=[300]),                         # two blocks of eight
+    "tiles": dict(rows_of=[5] * 10, lengths=[3 * i for i in range(10)], prefix=[1500]),              # 100 rows over a prefix
+    "own": dict(rows_of=[50, 40], lengths=[300, 9]),                                                 # 90 rows over own tokens
+    "halves": dict(rows_of=[25, 20, 17], lengths=[400, 30, 0]),                                      # up to 64 rows
+    "pairs": dict(rows_of=[100, 70], lengths=[0, 30]),                                               # more than 128, one part
+    "parts": dict(rows_of=[100, 70], lengths=[3000, 200], prefix=[100]),                             # in several
+    "shared": dict(rows_of=[30] * 10, lengths=[2 * i for i in range(10)], prefix=[900]),             # 600 rows over a prefix
+}
+EACH = [(f, d) for f in FORMS for d in (64, 128)]
+
+
+class Call:
+    def __init__(self, form, d, *, ps=16, seed=0, heads=4, kv=2, k_scale=1.0, v_scale=1.0, scale=None, pages=None, units=(0x18, 0x31)):
+        self.rows_of, self.lengths, prefix = FORMS[form]["rows_of"], FORMS[form]["lengths"], FORMS[form].get("prefix")
+        own = [-(-(l + t) // ps) for l, t in zip(self.lengths, self.rows_of)]
+        shared = [-(-p // ps) for p in prefix] if prefix else []
+        total = sum(own) + sum(shared) + 2
+        t, _ = tables(shared + own, total, seed)
+        self.pt, self.table = (t[:len(shared)], t[len(shared):]) if shared else (None, t)
+        if shared:
+            self.pt, self.table = self.pt[:, :max(shared)], self.table[:, :max(own)]
+        self.prefix, self.scale, self.k_scale, self.v_scale, self.heads, self.kv, self.d = prefix, scale, k_scale, v_scale, heads, kv, d
+        self.kp, self.vp = pages(total, ps, kv, d) if pages else (pages_of(total, ps, kv, d, seed + i, *units) for i in range(2))
+        self.off = np.cumsum([0] + self.rows_of)
+        self.rows = int(self.off[-1])
+        self.q = torch.randn(self.rows, heads, d, generator=torch.Generator().manual_seed(seed))
+
+    def run(self, ops):  # noqa: F811
+        from velox_voice_b200 import _lib
+
+        self.q16 = self.q.bfloat16().cuda()
+        shared = () if self.pt is None else (ints(self.pt), ints(self.prefix))
+        out = ops.prefix_attention(self.q16, torch.from_numpy(self.kp).cuda(), torch.from_numpy(self.vp).cuda(), ints(self.table), ints(self.lengths), *shared,
+                                   row_offsets=ints(self.off), scale=self.scale, k_scale=self.k_scale, v_scale=self.v_scale)
+        torch.cuda.synchronize()
+        assert _lib.device_status() == 0
+        return host(out.double())
+
+    def want(self):
+        k, v = P.fp4_values(self.kp, self.k_scale), P.fp4_values(self.vp, self.v_scale)
+        self.most = np.abs(v).max()
+        return P.prefix_attention_ref(host(self.q16.double()), k, v, self.table, np.array(self.lengths), self.pt, None if self.prefix is None else np.array(self.prefix),
+                                      self.off, None, self.scale)
+
+    def check(self, ops, small=None):  # noqa: F811
+        """`small`: what the rounding of small probabilities can take of a result."""
+        out = self.run(ops)
+        want, spread = self.want()
+        keys = max(l + t for l, t in zip(self.lengths, self.rows_of)) + (max(self.prefix) if self.prefix else 0)
+        small = 2.0 ** -32 * keys * self.most if small is None else small
+        err = np.abs(out - want)
+        bound = 2.0 ** -8 * (np.abs(want) + 2.0 ** -9 * spread) + (2.0 ** -11 + 2.0 ** -13) * spread + small
+        assert (err <= bound).all(), f"worst {np.nanmax(err / np.maximum(bound, 1e-300)):.3g} of the tolerance, {(~(err <= bound)).sum()} of {err.size} values, {(~np.isfinite(out)).sum()} not finite"
+
+
+@pytest.mark.parametrize("form,d", EACH)
+@pytest.mark.parametrize("k_scale,v_scale", [(2.0 ** -12, 2.0 ** 9), (2.0 ** 20, 2.0 ** -30)])
+def test_scales_of_the_cache(ops, form, d, k_scale, v_scale):  # noqa: F811
+    c = Call(form, d, seed=1, k_scale=k_scale, v_scale=v_scale)
+    c.q /= k_scale
+    c.check(ops)
+
+
+@pytest.mark.parametrize("form,d", EACH)
+def test_any_bytes_are_finite_values(ops, form, d):  # noqa: F811
+    c = Call(form, d, seed=2, ps=32, units=(0, 256))
+    c.q *= 2.0 ** -9
+    c.check(ops)
+
+
+@pytest.mark.parametrize("form,d", EACH)
+def test_queries_of_all_sizes(ops, form, d):  # noqa: F811
+    """Rows whose largest values are 2^60 apart, heads of different sizes beside each other, values 2^20 apart in a row, a row of zeros."""
+    c = Call(form, d, seed=3)
+    c.q *= torch.exp2(torch.linspace(-58, 2, c.rows).round())[:, None, None] * torch.exp2(torch.tensor([0.0, -3.0, -40.0, 0.0]))[:, None]
+    c.q[..., ::7] *= 2.0 ** -20
+    c.q[c.rows // 2] = 0
+    c.check(ops)
