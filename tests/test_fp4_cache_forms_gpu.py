@@ -5,6 +5,8 @@ sizes, scores beyond what fp32 holds to the unit, rows of zeros under tiny scale
 Tolerances by the number formats, as in test_fp4_cache_gpu.py, but for probabilities far below the row's largest: fp16 holds them to 2^-25 where the largest is
 2^7 or more, so they are off by 2^-32 of that, n of them by n 2^-32 of the largest value."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -96,3 +98,27 @@ def test_queries_of_all_sizes(ops, form, d):  # noqa: F811
     c.q[..., ::7] *= 2.0 ** -20
     c.q[c.rows // 2] = 0
     c.check(ops)
+
+
+@pytest.mark.parametrize("form,d", EACH)
+@pytest.mark.parametrize("low", [18, 25, 95])
+def test_large_scores(ops, form, d, low):  # noqa: F811
+    """One key takes all of the weight; largest scores from 2^18 to 2^110 in units of log2, all sizes between 2^18 and 2^34 among them.  A score in fp32 is off by some
+    2^-22 of the largest; rows whose two largest scores are nearer than 2^-18 of that are left out."""
+    c = Call(form, d, seed=low)
+    c.q *= torch.exp2(low + torch.arange(c.rows) % 11 + 0.15 * torch.arange(4)[:, None] * torch.ones(1, c.rows)).t()[..., None]
+    out = c.run(ops)
+    assert np.isfinite(out).all()
+    k, v, q = P.fp4_values(c.kp), P.fp4_values(c.vp), host(c.q16.double())
+    prefix = P._run(c.pt[0], c.prefix[0], k, v)[:2] if c.prefix else (np.zeros((0, 2, d)),) * 2
+    compared = 0
+    for r, (s, i) in enumerate(P.row_owner(c.rows, len(c.lengths), c.off)):
+        ks, vs, _ = P._run(c.table[s], c.lengths[s] + i + 1, k, v)
+        ks, vs = np.concatenate([prefix[0], ks]), np.concatenate([prefix[1], vs])
+        for h in range(4):
+            x = ks[:, h // 2] @ q[r, h] / math.sqrt(d) * math.log2(math.e)
+            top = np.sort(x)[-2:]
+            if top.size == 1 or top[1] - top[0] > 2.0 ** -18 * np.abs(x).max() + 60:
+                compared += 1
+                assert np.allclose(out[r, h], vs[x.argmax(), h // 2], rtol=2.0 ** -8, atol=2.0 ** -20), (r, h, np.log2(np.abs(top)), out[r, h], vs[x.argmax(), h // 2])
+    assert compared > 3 * c.rows
