@@ -122,3 +122,12 @@ def test_large_scores(ops, form, d, low):  # noqa: F811
                 compared += 1
                 assert np.allclose(out[r, h], vs[x.argmax(), h // 2], rtol=2.0 ** -8, atol=2.0 ** -20), (r, h, np.log2(np.abs(top)), out[r, h], vs[x.argmax(), h // 2])
     assert compared > 3 * c.rows
+
+
+@pytest.mark.parametrize("form,d", EACH)
+@pytest.mark.parametrize("scale,k_scale", [(2.0 ** -60, 1.0), (2.0 ** -30, 2.0 ** -32), (2.0 ** -126, 2.0 ** -32)])
+def test_rows_of_zeros_under_a_tiny_scale(ops, form, d, scale, k_scale):  # noqa: F811
+    """All scores are 0, more or less: rows are the means of what they see.  (The factor of a row of zeros is below what fp32 holds.)"""
+    c = Call(form, d, seed=5, scale=scale, k_scale=k_scale)
+    c.q[::3] = 0
+    c.check(ops)

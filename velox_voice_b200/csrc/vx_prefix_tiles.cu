@@ -935,7 +935,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
             most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu), __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu)));
           const int e = static_cast<int>(min(max(max(most >> 16, most & 0xffffu) >> 7, 27u), 227u));
           const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-          scale2 = fminf(scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f);
+          // (a factor of 0 times -infinity, a key that is not seen, would be NaN; below 2^-126 all scores are 0 either way)
+          scale2 = fmaxf(fminf(scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f), 0x1p-126f);
           const int r = quad * 32 + lane;
           const uint32_t row = smem_u32(q_s) + slot * Shape::kQ + r * 128;
 #pragma unroll
