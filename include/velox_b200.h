@@ -476,7 +476,8 @@ int vx_prefix_attention_launches(const vx_kv_cache* cache, const vx_kv_rows* row
 int vx_prefix_attention(const vx_kv_cache* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc, void* stream);
 
 /* The same over a cache in 4 bits.  Queries and probabilities as fp16 operands (a query by a power of two of its own, so that its largest value is in
- * [1, 2): below 2^115), keys and values exactly; fp32 scores, statistics and sums. */
+ * [1, 2): below 2^115), keys and values exactly; fp32 scores, statistics and sums.  A probability is off by 2^-11 of itself or 2^-32 of the row's largest,
+ * whichever is more: n keys that are less likely than that count as nothing, where exactly they had n 2^-32 of the weight at most. */
 int64_t vx_prefix_attention_fp4_scratch(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
 int vx_prefix_attention_fp4_launches(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc);
 int vx_prefix_attention_fp4(const vx_kv_cache_fp4* cache, const vx_kv_rows* rows, const vx_prefix_attention_desc* desc, void* stream);

@@ -131,3 +131,46 @@ def test_rows_of_zeros_under_a_tiny_scale(ops, form, d, scale, k_scale):  # noqa
     c = Call(form, d, seed=5, scale=scale, k_scale=k_scale)
     c.q[::3] = 0
     c.check(ops)
+
+
+def falling(total, ps, kv, d):
+    """Units whose first key alone has a score, and a value of 0; the others random values."""
+    kp, vp = np.zeros((total, kv, ps // 16, 9 * d), dtype=np.uint8), pages_of(total, ps, kv, d, 6)
+    kp[..., 0] = 7                                  # 6 at the first place of the first key
+    kp[..., 8 * d:] = 0x38                          # times 1
+    vp[..., :d // 2] = 0
+    return kp, vp
+
+
+@pytest.mark.parametrize("form,d", EACH)
+@pytest.mark.parametrize("below", [20.0, 24.3, 27.1, 29.0, 31.5])
+def test_probabilities_far_below_the_largest(ops, form, d, below):  # noqa: F811
+    """Every unit has a key with the row's largest score and a value of 0; the others, which alone have values, are `below` powers of two less likely.  A row that
+    sees n keys sees n / 16 of the former or more, so the largest share is 16 / n, and what is lost 16 2^-32 of the largest value at most."""
+    c = Call(form, d, seed=7, pages=falling, scale=below * math.log(2) / 6)
+    c.q[:] = 0
+    c.q[..., 0] = 1
+    c.check(ops, small=16 * 2.0 ** -32 * np.abs(P.fp4_values(c.vp)).max())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [90_000, 1_000_000])
+@pytest.mark.parametrize("below", [20.1, 25.1, 28.1, 31.0])
+@pytest.mark.parametrize("rows", [1, 50, 100, 200])
+def test_one_key_in_front_of_a_long_tail(ops, d, n, below, rows):  # noqa: F811
+    """The first key has a value of 0, n others, each `below` powers of two less likely, a value of 1.  (The rows are one sequence's, whose own tokens are of the tail.)  fp32
+    sums of up to n equal numbers, some 2^14 of them one after another: 2^-10 of the result."""
+    ps = 16
+    kp, vp = np.zeros((2, 1, 1, 9 * d), dtype=np.uint8), np.full((2, 1, 1, 9 * d), 0x22, dtype=np.uint8)
+    kp[..., 8 * d:] = vp[..., 8 * d:] = 0x38
+    kp[0, ..., 0] = 7
+    vp[0, ..., :d // 2] = 0
+    q = torch.zeros(rows, 1, d, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 1
+    table = torch.ones(1, n // ps, dtype=torch.int32, device="cuda")
+    table[0, 0] = 0
+    out = ops.prefix_attention(q, torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), ints([[1] * -(-rows // ps)]), ints([0]), table, ints([n]), row_offsets=ints([0, rows]),
+                               scale=below * math.log(2) / 6)
+    tail = (n - 1 + 1 + np.arange(rows)) * 2.0 ** -below
+    want = (tail / (1 + tail))[:, None, None]
+    assert (np.abs(host(out.double()) - want) <= want * (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -13) + 2.0 ** -32 * n).all(), (host(out.double()).min() / want.min(), host(out.double()).max() / want.max())

@@ -4,8 +4,8 @@
 // A SPAN is one kind of keys: those of the groups' prefixes, the sequences' own tokens, or both in a row (joint).  Its owners (groups,
 // sequences, sequences) have runs of rows; row rho of an owner and a key head stands for token rho / per_kv of its run and query head
 // rho % per_kv, so that all query heads that share a key head read its keys together.  Rows are cut into tiles, keys into chunks.  An
-// item is one tile, one chunk and one key head; it leaves (m, l, O) of its rows -- maximum, sum of 2^(x - m), sum of 2^(x - m) v, with
-// x = scale log2(e) q.k -- as part `part0 + chunk` in scratch, from which a last kernel joins the parts of a row:
+// item is one tile, one chunk and one key head; it leaves (m, l, O) of its rows -- a maximum or a number near it, sum of 2^(x - m), sum of
+// 2^(x - m) v, with x = scale log2(e) q.k -- as part `part0 + chunk` in scratch, from which a last kernel joins the parts of a row:
 //   out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c,  m = max_c m_c.
 // The number of chunks is fixed on the host from the width of the tables; how many of them hold keys is known on the device only, and
 // both sides derive it from the same lengths, so empty parts are neither written nor read.
@@ -214,6 +214,9 @@ __device__ __forceinline__ bool find_tile(const PrefixParams& p, const Span& sp,
 // Not 0 if one of the two bf16 values of a word is an infinity or NaN, gathered in `sum` (0 x is 0 or NaN).
 __device__ __forceinline__ void note_not_finite(uint32_t& sum, uint32_t two) { asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(two), "r"(0u)); }
 __device__ __forceinline__ bool any_not_finite(uint32_t sum) { return (sum & 0x7fff7fffu) != 0; }
+
+// A cache in 4 bits: probabilities are formed in fp16 as 2^(x - reference), the reference this far below a maximum (see vx_prefix_fp4.cu).
+constexpr float kFp4Below = 7.0f;
 
 // What the kernels for few rows walk.
 struct RowsParams {

@@ -1,6 +1,6 @@
 // Attention over a cache in 4 bits, for few rows per owner and key head (the cut of the work: vx_prefix.cuh; what it is: vx_prefix_attn.cu, whose
 // kernel for few rows this one follows: up to 16 rows against one chunk of keys, by one, two or four warps, keys and values on the m16 side of
-// m16n8k16 products, a reference maximum that moves when exceeded by 2^8).  What is its own:
+// m16n8k16 products).  What is its own:
 //
 // A unit of 16 keys (vx_paged.cuh) is one bulk copy of 9 D bytes, for the keys and for the values; a warp has a ring of them.  Units whose page is not
 // there are left out of the ring, so that a step has 16 keys or the end of a run.
@@ -8,6 +8,10 @@
 // Products are fp16: a code is 0 to 6 in halves, a scale of 4 significant bits over 256 at most 1.875 and 2^-17 at least, so code times scale is exact.
 // Queries are multiplied by a power of two of their row, which puts the largest in [1, 2): from 2^-17 of it on bf16 values stay exact, smaller
 // ones are off by 2^-25 of it at most.  Whatever bytes a cache holds are finite values, so what a row does not see needs a probability of 0 only.
+//
+// Probabilities are 2^(x - reference).  fp16 goes from 2^-24 to 2^16, so the reference is a maximum less 7 and moves when exceeded by 15: the largest is between 2^7 and 2^15,
+// and the others are off by 2^-11 or by 2^-32 of the largest (2^-25 of it with the maximum itself as reference: a key in front of 90,000 that are 2^25 times less likely took a
+// part of their weight from the result, though not from the row's sum, which is fp32).
 //
 // Where the values come from, lane = 4 g + c:
 //   S^T = K Q^T: a lane has D / 4 values of keys g and g + 8, those at (D / 4) c: their scales are its own.  Two values of a byte are one register of
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(WARPS * 32, rows4_ctas(RB, D) * PR_WARPS / WAR
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         mx[r][e] = fmaxf(s[r][e], s[r][2 + e]);
-        moves = moves || mx[r][e] > m_ref[r][e] + 8.0f;
+        moves = moves || mx[r][e] - m_ref[r][e] > kFp4Below + 8.0f;  // (the difference: a sum can be rounded up)
       }
     if (__any_sync(ALL, moves)) {
 #pragma unroll
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(WARPS * 32, rows4_ctas(RB, D) * PR_WARPS / WAR
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) mx[r][e] = fmaxf(mx[r][e], __shfl_xor_sync(ALL, mx[r][e], x));
-          const float m_new = fmaxf(m_ref[r][e], mx[r][e]);
+          const float m_new = fmaxf(m_ref[r][e], mx[r][e] - kFp4Below);
           const float alpha = m_new == NEG_INF ? 1.0f : ex2(m_ref[r][e] - m_new);
           m_ref[r][e] = m_new;
           l[r][e] *= alpha;

@@ -179,10 +179,19 @@ __device__ __forceinline__ void store32(float* dst, const uint32_t* v) {
 // the same for all keys of the row and in its sum, which leaves the range where m is 2^31 or more.  From 2^30 on scale2 without its mantissa
 // stands in, and products are exact: two different scores are 64 or more in log2 apart there, 32 with the smaller factor, so that the
 // largest takes all of the weight either way.
-// FP4: P is fp16, which ends at 2^16, so from 2^27 on, where half a unit of m is 8.  Below, P is at most 2^(8 + 4).  (Two different scores are 8 or more apart there, 4 with
-// the smaller factor; a sum of products in fp32 is off by half of that itself.)
+// FP4: P is fp16, which ends at 2^16, so from 2^27 on, where half a unit of m is 8.  (Two different scores are 8 or more apart there, 4 with the smaller
+// factor; a sum of products in fp32 is off by half of that itself.)
 template <bool FP4>
 constexpr float PT_LARGE = FP4 ? 134217728.0f : 1073741824.0f;
+// Where the reference is put below the maximum, and how far above it scores may be before it moves.  FP4: fp16 ends at 2^-24 below, so the reference is 2^7 less than the
+// maximum (see vx_prefix_fp4.cu); a score's exponent is off by half a unit of it, 8 at 2^27, so 15 less that keep P below 2^16.
+template <bool FP4>
+constexpr float PT_BELOW = FP4 ? kFp4Below : 0.0f;
+template <bool FP4>
+__device__ __forceinline__ bool reference_moves(float m_tile, float m_ref) {
+  if (FP4) return m_tile - m_ref > fmaxf(fmaf(fabsf(m_tile), -0x1p-24f, kFp4Below + 8.0f), kFp4Below);
+  return m_tile > m_ref + 8.0f;
+}
 __device__ __forceinline__ float without_mantissa(float x) { return __uint_as_float(__float_as_uint(x) & 0x7f800000u); }
 // such a reference maximum in units of log2, for the parts of a row and where it moves
 __device__ __forceinline__ float in_log2(float m, float factor, float scale2) {
@@ -1023,7 +1032,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         }
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         const float m_tile = mx * factor;
-        const bool moves = FP4 ? m_tile - m_ref > 8.0f : m_tile > m_ref + 8.0f;  // (fp16 has no room for a sum that is rounded up)
+        const bool moves = reference_moves<FP4>(m_tile, m_ref);
         // P V of the tile before has to be complete before O is touched (with one buffer this tile's S was issued behind it)
         auto o_is_there = [&] {
           if (NB > 1) ok = __all_sync(ALL, mbar_wait(&bar.pv_done[slot][(units - 1) % NB], ((units - 1) / NB) & 1, p.status, 46));
@@ -1035,11 +1044,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
           if (moves) {
             const float before = in_log2(m_ref, factor, scale2);
             factor = scale2;
-            m_ref = mx * factor;
+            m_ref = mx * factor - PT_BELOW<FP4>;
             alpha = ex2(before - m_ref);  // 0 for -inf
             if (fabsf(m_ref) >= PT_LARGE<FP4>) {
               factor = without_mantissa(factor);
-              m_ref = mx * factor;
+              m_ref = mx * factor - PT_BELOW<FP4>;
             }
           }
           l *= alpha;

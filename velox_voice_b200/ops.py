@@ -951,7 +951,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     that are not there (entries outside [0, pages)) are not attended; a row that has no key, or whose sequence has a negative
     length, gets zeros.  ``scale``: positive, head_dim ** -0.5 unless given.
 
-    Pages in 4 bits (:func:`fp4_pages`, ``k_scale`` and ``v_scale`` those of :func:`kv_append`) are read as they are (``vx_prefix_attention_fp4``)."""
+    Pages in 4 bits (:func:`fp4_pages`, ``k_scale`` and ``v_scale`` those of :func:`kv_append`) are read as they are (``vx_prefix_attention_fp4``): queries
+    below 2^115, keys with less than 2^-32 of the weight of a row's largest count as nothing."""
     r = (_native or _host()).prefix_attention(q, k_pages, v_pages, page_table, lengths, prefix_table, prefix_lengths, row_offsets, group_offsets,
                                               scale, out, k_scale, v_scale)
     if r is not None:
