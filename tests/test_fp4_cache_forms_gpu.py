@@ -174,3 +174,11 @@ def test_one_key_in_front_of_a_long_tail(ops, d, n, below, rows):  # noqa: F811
     tail = (n - 1 + 1 + np.arange(rows)) * 2.0 ** -below
     want = (tail / (1 + tail))[:, None, None]
     assert (np.abs(host(out.double()) - want) <= want * (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -13) + 2.0 ** -32 * n).all(), (host(out.double()).min() / want.min(), host(out.double()).max() / want.max())
+
+
+def test_a_scale_below_the_normal_numbers(ops):  # noqa: F811
+    """scale 2^-149 with k_scale 2^32: their product with log2(e) is formed before it is rounded."""
+    d, ps = 64, 16
+    c = Call("whole", d, seed=8, scale=2.0 ** -149, k_scale=2.0 ** 32)
+    c.q *= 2.0 ** 112
+    c.check(ops)

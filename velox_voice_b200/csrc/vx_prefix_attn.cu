@@ -639,7 +639,7 @@ int check_prefix(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_att
       return fail(-1, "prefix_lengths or prefix_table is NULL, or its rows are too short");
   }
   p.scale2 = d->scale * 1.4426950408889634f;
-  if (FP4) p.scale2 *= 256.0f * p.fp4.k_scale;
+  if (FP4) p.scale2 = static_cast<float>(static_cast<double>(d->scale) * 1.4426950408889634 * 256.0 * static_cast<double>(p.fp4.k_scale));  // (rounded once: a scale may be subnormal and k_scale 2^32)
   p.v_factor = FP4 ? 256.0f * p.fp4.v_scale : 1.0f;
   if (!(d->scale > 0.0f) || !(p.scale2 < INFINITY)) return fail(-1, FP4 ? "scale must be positive and finite, 256 scale k_scale log2(e) too" : "scale must be positive and finite, scale log2(e) too");
   const int per = d->q_heads / cache->kv_heads;
