@@ -207,9 +207,12 @@ __device__ __forceinline__ uint2 quantize16(const float (&a)[8], const float (&b
       const uint64_t x = mul_f32x2(e ? pack_f32x2(b[j], b[j + 1]) : pack_f32x2(a[j], a[j + 1]), g2), q0 = mul_f32x2(x, r2);
       unpack_f32x2(fma_f32x2(fma_f32x2(q0, s2, x), r2, q0), q[j], q[j + 1]);
     }
-    if (!(most < 1e30f)) {  // (infinities: to the largest codes of their signs)
+    if (!(most < INFINITY)) {  // (infinities, which have no remainder: to the largest codes of their signs)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = __fmul_rn(e ? b[j] : a[j], inv_g) * r;
+      for (int j = 0; j < 8; ++j) {
+        const float x = __fmul_rn(e ? b[j] : a[j], inv_g);
+        if (!(fabsf(x) < INFINITY)) q[j] = x;
+      }
     }
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
