@@ -369,20 +369,27 @@ __global__ void __launch_bounds__(WARPS * 32, rows4_ctas(RB, D) * PR_WARPS / WAR
           if (r < blocks) mma_f16_16816(o[r][b][j], even[0][j], odd[0][j], even[1][j], odd[1][j], pt[r][0], pt[r][1]);
     }
   };
-  int stage = 0;
+  int stage = 0, done = 0;
   uint32_t phase = 0;
-  bool ok = true;
-#pragma unroll 1
-  for (int done = 0; done < issued; ++done) {
-    ok = __all_sync(ALL, mbar_wait(&full_s[warp][stage], phase, p.status, 60));
-    if (!ok) break;
-    step(ring + stage * 2 * UNIT, first_s[warp][stage]);
-    __syncwarp();  // every lane has read the stage: it is filled again
-    fetch();
+  auto next_stage = [&] {
     if (++stage == NS) {
       stage = 0;
       phase ^= 1;
     }
+  };
+#pragma unroll 1
+  for (; done < issued; ++done) {
+    if (!__all_sync(ALL, mbar_wait(&full_s[warp][stage], phase, p.status, 60))) break;
+    step(ring + stage * 2 * UNIT, first_s[warp][stage]);
+    __syncwarp();  // every lane has read the stage: it is filled again
+    fetch();
+    next_stage();
+  }
+  // Copies on their way after a limit ran out: each is waited for, with a limit, before its place is used for something else.
+#pragma unroll 1
+  for (; done < issued; ++done) {
+    __all_sync(ALL, mbar_wait(&full_s[warp][stage], phase, p.status, 60));
+    next_stage();
   }
   named_bar_sync(1 + team, 32 * warps);  // every warp of the item is done with its ring: the sums go there
 
