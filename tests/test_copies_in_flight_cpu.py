@@ -51,3 +51,41 @@ def test_the_kernel_for_few_rows_over_4_bit_pages_waits_for_what_it_issued():
     assert not re.search(r"\b(done|stage|phase) ?=(?!=)", text[first:second + len(body)].replace("for (; done", ""))
     assert text[second + len(body):].lstrip("\n }").startswith("named_bar_sync(")
     assert text.index("bulk_load(") < first and "bulk_load(" not in text[second:]
+
+
+def walked_back(slots, calls, fetched):
+    """The end of the warp that fetches units for the tiles: the slots and phases that it waits for."""
+    slot, phase = 0, 0
+    armed = []
+    for _ in range(calls):
+        armed.append((slot, phase))
+        slot += 1
+        if slot == slots:
+            slot, phase = 0, phase ^ 1
+    waits = []
+    i = 0
+    while i < slots and i <= fetched:
+        if slot == 0:
+            phase ^= 1
+        slot = (slots if slot == 0 else slot) - 1
+        waits.append((slot, phase))
+        i += 1
+    return armed, waits
+
+
+@pytest.mark.parametrize("slots", [1, 2, 3, 6])
+@pytest.mark.parametrize("fetched", range(9))
+def test_the_last_units_of_the_tiles_are_waited_for(slots, fetched):
+    """Ended as it should (a slot for the end behind those of the tiles), or given up with or without a slot asked for in vain."""
+    for calls in (fetched, fetched + 1):
+        armed, waits = walked_back(slots, calls, fetched)
+        assert set(armed[-slots:]) <= set(waits)
+
+
+def test_the_warp_that_fetches_for_the_tiles_waits_whether_it_gave_up_or_not():
+    """It can have issued all of its copies before a loader's wait runs out."""
+    text = source("vx_prefix_tiles.cu")
+    text = text[text.index("next_raw(e, kRawEnd, 0)"):]
+    text = text[:text.index("cp_async_wait_all()")]
+    assert re.search(r"for \(int e = 0; e < 2; \+\+e\)\s*for \(int i = 0; i < \(e \? Shape::kRawV : Shape::kRawK\) && i <= fetched; \+\+i\) {", text)
+    assert "mbar_wait(&bar.raw[stream][e].full[raw_slot[e]], raw_phase[e], p.status" in text and "if (!ok)" not in text

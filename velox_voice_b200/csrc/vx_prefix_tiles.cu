@@ -885,9 +885,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
         if (ok) hand_out(end, lane == 0);
         if constexpr (FP4) {
           for (int e = 0; e < 2 && ok; ++e) next_raw(e, kRawEnd, 0);
-          // (copies on their way after a limit ran out: each is waited for, with a limit)
-          for (int e = 0; e < 2 && !ok; ++e)
-            for (int i = 0; i < (e ? Shape::kRawV : Shape::kRawK) && i < fetched; ++i) {
+          // The copies of the last tiles are waited for, each with a limit: where one of the loaders' waits ran out, nobody else does.  (`fetched` slots and one more: the end's,
+          // or one that was asked for in vain.)
+          for (int e = 0; e < 2; ++e)
+            for (int i = 0; i < (e ? Shape::kRawV : Shape::kRawK) && i <= fetched; ++i) {
               if (raw_slot[e] == 0) raw_phase[e] ^= 1;
               raw_slot[e] = (raw_slot[e] == 0 ? (e ? Shape::kRawV : Shape::kRawK) : raw_slot[e]) - 1;
               mbar_wait(&bar.raw[stream][e].full[raw_slot[e]], raw_phase[e], p.status, 59);
