@@ -779,6 +779,8 @@ def _fp4_tensor(t, name: str) -> None:
     _require_cuda(t, name)
     if t.dtype != torch.uint8 or t.dim() != 4 or t.shape[3] % 144 != 0 or not 144 <= t.shape[3] <= 2304 or t.shape[1] < 1 or t.shape[2] < 1:
         raise ValueError(f"{name} must be uint8 [pages, kv_heads, page_size / 16, 9 head_dim], got {t.dtype} {tuple(t.shape)}")
+    if t.shape[2] >= 2 ** 27:
+        raise ValueError(f"{name} must have pages of fewer than 2^31 tokens, got {16 * t.shape[2]}")
     page = t[0].numel() if t.shape[0] else 0
     if t.data_ptr() % 16 != 0 or (t.shape[0] and not t[0].is_contiguous()) or _step(t, 0) % 16 != 0 or (t.shape[0] > 1 and t.stride(0) < page):
         raise ValueError(f"{name} must have contiguous pages at 16-byte aligned addresses (strides {t.stride()})")
