@@ -182,3 +182,13 @@ def test_a_scale_below_the_normal_numbers(ops):  # noqa: F811
     c = Call("whole", d, seed=8, scale=2.0 ** -149, k_scale=2.0 ** 32)
     c.q *= 2.0 ** 112
     c.check(ops)
+
+
+@pytest.mark.parametrize("form,d", EACH)
+@pytest.mark.parametrize("low", [-100, -118, -124])
+def test_queries_below_2_to_the_minus_100(ops, form, d, low):  # noqa: F811
+    """Down to the smallest numbers of bf16, under a scale that makes scores of them (2^84 log2(e) times 256 times k_scale is the largest that is taken)."""
+    c = Call(form, d, seed=9, scale=2.0 ** min(-low - 34, 84), k_scale=2.0 ** 32, units=(0x18, 0x31) if low > -120 else (0x40, 0x51))
+    c.q *= 2.0 ** low
+    c.q[1::5] *= 2.0 ** -6
+    c.check(ops)

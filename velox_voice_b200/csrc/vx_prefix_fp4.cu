@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(WARPS * 32, rows4_ctas(RB, D) * PR_WARPS / WAR
     }
     most = max(most, __shfl_xor_sync(ALL, most, 1));
     most = max(most, __shfl_xor_sync(ALL, most, 2));
-    const int e = min(max(static_cast<int>(most >> 23), 27), 227);  // (2^-100 to 2^100)
+    const int e = min(max(static_cast<int>(most >> 23), 1), 227);  // (to 2^100; what is above, to 2^115, fp16 holds as it is)
     const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23), up = fminf(p.scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f);
 #pragma unroll
     for (int i = 0; i < KW; ++i)

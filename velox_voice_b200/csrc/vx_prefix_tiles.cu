@@ -928,7 +928,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
       const int warp_limit = __shfl_sync(ALL, limit, 0);  // limits ascend with the rows
       float scale2 = p.scale2;
       if constexpr (FP4) {
-        // The thread's query, in fp16 by a power of two, which puts its largest value in [1, 2) (queries between 2^-100 and 2^100).  (By the warps that hand
+        // The thread's query, in fp16 by a power of two, which puts its largest value in [1, 2) (up to 2^100; from there to 2^115 fp16 holds it as it is).  (By the warps that hand
         // out items 15,000 cycles ahead of the first product, by these 3,000, of which none pass under the item before.)
         ok = __all_sync(ALL, mbar_wait(&bar.q_empty[stream], q_phase ^ 1, p.status, 50));
         if (Shape::kBox && ok && splits > 0) ok = __all_sync(ALL, mbar_wait(&bar.box_empty[slot], (splits - 1) & 1, p.status, 51));  // (the box is where the queries are)
@@ -943,7 +943,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefix_tiles_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < D / 8; ++i)
             most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu), __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu)));
-          const int e = static_cast<int>(min(max(max(most >> 16, most & 0xffffu) >> 7, 27u), 227u));
+          const int e = static_cast<int>(min(max(max(most >> 16, most & 0xffffu) >> 7, 1u), 227u));
           const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
           // (a factor of 0 times -infinity, a key that is not seen, would be NaN; below 2^-126 all scores are 0 either way)
           scale2 = fmaxf(fminf(scale2 * __uint_as_float(static_cast<uint32_t>(e) << 23), 3.0e38f), 0x1p-126f);
