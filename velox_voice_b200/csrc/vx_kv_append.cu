@@ -97,7 +97,7 @@ namespace {
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_BLOCKS = 6;     // per SM, at 40 registers a thread: five of 46 take 375 us at the size above, seven or eight, which spill, 507
-constexpr int AP_BLOCKS_FP4 = 5;  // at 48 registers: 384 us for four of 62 389, six 399 (and with 17 divisions for 16 values, four of them, 418)
+constexpr int AP_BLOCKS_FP4 = 5;  // at 48 registers (bf16 rows spill 28 bytes, fp32 rows 8): 384 us for four of 62 389, six 399 (and with 17 divisions for 16 values, four of them, 418)
 constexpr int AP_UNITS = 16;     // of a thread in large calls, since a block looks its rows up before it moves any: 4 take 422 us there, 8 391, 16 375 (of five blocks)
 constexpr int AP_MAX_ROWS = 32;  // rows of a block at most
 

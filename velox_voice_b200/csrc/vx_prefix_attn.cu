@@ -659,7 +659,7 @@ int check_prefix(const Cache* cache, const vx_kv_rows* rows, const vx_prefix_att
   const int64_t cap_p = G > 0 ? d->prefix_pages * cache->page_size : 0, cap_o = rows->table_pages * cache->page_size;
   if (cap_p + cap_o > (1ll << 31) - 1024) return fail(-1, "prefix and own tokens of a sequence may be 2^31 - 1024 together");  // (indexes of keys are 32 bits)
   // The kernel of a span goes by its rows per owner and key head, on the average, and its keys, as many as the tables have place for (which
-  // kernel takes a row changes no result beyond rounding).
+  // kernel takes a row changes no result beyond rounding).  Where it does not say 4 bits, a rule was measured over bf16 pages and is taken for both.
   const bool single = !rows->row_offsets;
   const int64_t rows_p = cap_p > 0 ? R * per / G : 0, rows_o = cap_o > 0 ? R * per / S : 0;
   auto cut = [&](Span& sp, SpanKind kind, Plan::Kernel kernel, int64_t owners, int64_t cap, int64_t equal_rows) {

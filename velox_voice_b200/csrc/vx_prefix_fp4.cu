@@ -18,8 +18,8 @@
 //     a product; q is read in the same order.
 //   O^T += V^T P^T: a lane has the D / 8 values at (D / 8) g of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9.  The halves of two keys' bytes are put together
 //     (key 2 c low), so that a converted byte is one register: columns 2 t and 2 t + 1 of a word are rows g and g + 8 of product t.
-// What bounds it: issue slots.  A unit takes a warp some 400 instructions at head_dim 128, 163 of them in the ALU pipe; 64 sequences of 4,000 to 8,000 tokens, 32 query heads on 8 key
-// heads of 128 (269 MB), take 87 us, 3.1 TB/s, issue slots 62 % busy (bf16 pages: 171).  Few keys: round trips to memory; ten sequences of 400 tokens, 8 heads of 64, 6.5 us.
+// What bounds it: issue slots.  A unit takes a warp some 410 instructions at head_dim 128, 163 of them in the ALU pipe; 64 sequences of 4,000 to 8,000 tokens, 32 query heads on 8 key
+// heads of 128 (269 MB), take 86 to 91 us, 3.1 TB/s, issue slots 63 % busy (bf16 pages: 171).  Few keys: round trips to memory; ten sequences of 400 tokens, 8 heads of 64, 6.5 us.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,7 +35,8 @@
 namespace vx {
 namespace {
 
-// CTAs of four warps per SM; those of eight or sixteen, which take an item each, have as many warps together.
+// CTAs of four warps per SM; those of eight or sixteen, which take an item each, have as many warps together.  (Two blocks of rows at head_dim 128 spill 48 bytes, at 168
+// registers, the others none.)
 constexpr int rows4_ctas(int rb, int head_dim) { return head_dim == 64 ? 4 : (rb == 2 ? 3 : 4); }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -38,8 +38,8 @@
 // rows, and what a CTA costs to begin and end where an SM has a few tiles only (16 groups of 100 rows over 64 keys, one tile each: 11 us at head_dim 64).
 // FP4: a cache in 4 bits.  The warps that hand out items fetch its units into rings of their own, as they lie in the cache (a bulk copy each, the table read a tile ahead); the loaders turn
 // them into fp16 tiles, one warp per stream and tensor (PAIRED two); the threads of the softmax load the query of their row, in fp16 by a power of two.  128 rows a head over 90,000
-// keys: 77 us, bounded by the softmax's chain (2,250 cycles a tile of 64 keys: 480 to the maximum, 1,200 exponentials and what belongs to them, 400 to the next wait); 3,000 tokens of two
-// prompts behind 8,192, 32 heads on 8 of 128: 543 us, 0.85 PFLOP/s, 4,350 cycles a tile of a pair.
+// keys: 79 us, bounded by the softmax's chain (2,250 cycles a tile of 64 keys: 480 to the maximum, 1,200 exponentials and what belongs to them, 400 to the next wait); 3,000 tokens of two
+// prompts behind 8,192, 32 heads on 8 of 128: 541 us, 0.86 PFLOP/s, 4,350 cycles a tile of a pair.  (Spills, at 128 registers: 8 to 16 bytes, pairs 24 to 28.)
 // Every wait on a barrier is bounded.
 
 #include <cuda_bf16.h>

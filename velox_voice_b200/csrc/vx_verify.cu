@@ -8,7 +8,7 @@
 //                        sums of both rows, then of max(p - q, 0) in ascending order -- CTA, warp, group of 32, lane -- in fp64, since a token stands or falls
 //                        with one comparison of a sum over the vocabulary: with 131,071 tokens and fp32 sums one draw of ten would be near a border.
 //
-// What bounds them: the first, HBM (384 rows of 131,071 in fp32 and 320 of the drafter's, 369 MB in 68 us, 5.4 TB/s); the second, 60 us there, latency: two walks in
+// What bounds them: the first, HBM (384 rows of 131,071 in fp32 and 320 of the drafter's, 369 MB in 71 us by ncu, 5.2 TB/s); the second, 66 us there (127 both, in a call), latency: two walks in
 // fp64, nine operations a logit, that keep half of the issue slots busy, and the clusters' barriers between them; small calls the round trips to memory: 50 rows of
 // 5,538 take 11.5 us in both together.
 
@@ -28,7 +28,8 @@ namespace {
 
 constexpr int VR_THREADS = 128;  // rows of 5,538 have three pieces of 16 bytes a thread: 256 threads, of which an SM holds half as many rows, take 27.8 us for 26.5 with 1,038 rows
 constexpr int VN_THREADS = 512;
-constexpr int VR_CTAS = 8;     // per SM at least, of rows: eight loads of 16 bytes a thread are on their way (more CTAs gain nothing, 144 : 145 us at 64 sequences of six rows of 131,071)
+constexpr int VR_CTAS = 8;     // per SM at least, of rows, at 64 registers: eight loads of 16 bytes a thread are on their way.  Ten and twelve, at 48 and 40, where bf16 rows spill, take 131 and 136 us for the
+                               // 127 of a call with 64 sequences of six rows of 131,071 in fp32, 30.2 and 33.9 for 26.6 with 1,038 rows of 5,538 in bf16
 constexpr int VR_LEAST = 4096, VN_LEAST = 4096;  // values of a CTA, where a row is cut
 constexpr unsigned ALL = 0xffffffffu;
 
