@@ -1,9 +1,10 @@
 // Drafted tokens against the target's probabilities (vx_verify_drafts), in two launches:
 //
 //   verify_rows_kernel   a cluster per row: the row's largest logit and the sum of 2^((x - max) c), c = log2(e) / T, of the target and of the drafter, in
-//                        one pass in fp32; from them whether the row's draft stands.  The exponentials come out within 2^-16 (a difference and a product, 2^-24 each of an
-//                        exponent up to 128), their sums, 16 of a thread at a time, within vocab 2^-35 more at worst, so where u q(d) and p(d) are 2^-12 +
-//                        vocab 2^-33 of each other apart the comparison is settled; the others, some 1 of 4,000, are left open.
+//                        one pass in fp32; from them whether the row's draft stands.  The exponentials come out within 2^-16 (a difference, c and a product, 2^-24 each of an
+//                        exponent up to 128), their sums, 16 or more of a thread at a time, each time rounded and, where the maximum moves, multiplied by an exponential (2^-22),
+//                        within 2^-16 + vocab 1.25 2^-33 more at worst, so where u q(d) and p(d) are 2^-12 + vocab 2^-31 of each other apart the comparison is settled; the
+//                        others, some 1 of 4,000, are left open.
 //   verify_next_kernel   a cluster per sequence: the first row whose draft falls (open rows settled in fp64), and the token drawn from what is left there:
 //                        sums of both rows, then of max(p - q, 0) in ascending order -- CTA, warp, group of 32, lane -- in fp64, since a token stands or falls
 //                        with one comparison of a sum over the vocabulary: with 131,071 tokens and fp32 sums one draw of ten would be near a border.
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(VR_THREADS, VR_CTAS) verify_rows_kernel(const 
       if (known && f.best == draft) f.draft = kStands;
     } else if (known && f.most == f.most) {
       const float pt = ex2((draft_t - a[0].m) * c), qd = drafter ? ex2((draft_d - a[1].m) * c) : 1.0f;
-      const float left = u * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * (0x1p-12f + 0x1p-33f * static_cast<float>(p.vocab));
+      const float left = u * qd * a[0].sum, right = pt * (drafter ? a[1].sum : 1.0f), gap = fmaxf(left, right) * (0x1p-12f + 0x1p-31f * static_cast<float>(p.vocab));
       // (anything near the end of the range is open)
       if (!(left > 1e-30f && right > 1e-30f && left < 1e30f && right < 1e30f) || fabsf(left - right) <= gap) f.draft = kOpen;
       else f.draft = left < right ? kStands : kFalls;
